@@ -128,14 +128,19 @@ def _to_8_bits(x):
     mant, exp = torch.frexp(b.abs().amax(-1))            # max|x| = mant 2^exp, mant in [0.5, 1); 448 = 0.875 2^9
     top = 8 if x.dtype == torch.float16 else 120         # there 256 2^E is past the type's largest value
     e = torch.where(mant <= 0.875, exp - 9, exp - 8).clamp(min=-117)
-    y = torch.ldexp(b, -e[..., None])
+    y = b * _power(-e)[..., None]
     y = torch.where((e == top)[..., None], y.clamp(-240, 240), y)
     codes = y.to(torch.float8_e4m3fn).view(x.shape[0], -1)[:, :x.shape[1]].contiguous()
     return codes, (e + 127).to(torch.uint8)
 
 
+def _power(e):
+    """2^e in fp32, exactly."""
+    return ((e.int() + 127) << 23).view(torch.float32)
+
+
 def _from_8_bits(codes, exponents):
-    scale = torch.exp2(exponents.float() - 127)
+    scale = _power(exponents.int() - 127)
     return (_blocks(codes.float()) * scale[..., None]).view(codes.shape[0], -1)[:, :codes.shape[1]]
 
 
@@ -221,6 +226,11 @@ def exact(case, seed):
     """The definitions in 64 bits."""
     s = prepare(case, seed)
     f64 = torch.float64
+
+    def power(e):
+        # torch.exp2 may be off by a bit in 64 bits: an exponent field is not
+        return ((e.long() + 1023) << 52).view(f64)
+
     if case['op'] == 'checkpoint':
         x = s['x'].to(f64)
         m, k = x.shape
@@ -230,11 +240,13 @@ def exact(case, seed):
         peak.scatter_reduce_(1, index.expand(m, k), x.abs(), 'amax')
         e = torch.ceil(torch.log2(peak / 448)).clamp(min=-117)
         # the logarithm is rounded: move to the least exponent that holds the peak
-        e = torch.where(448 * torch.exp2(e - 1) >= peak, e - 1, e).clamp(min=-117)
-        e = torch.where(448 * torch.exp2(e) < peak, e + 1, e)
-        scale = torch.exp2(e)[:, index]
+        e = torch.where(448 * power(e - 1) >= peak, e - 1, e).clamp(min=-117)
+        e = torch.where(448 * power(e) < peak, e + 1, e)
+        scale = power(e)[:, index]
         v = x / scale
-        step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+        step = torch.ones_like(v) * 2.0 ** -9
+        for exponent in range(-5, 9):                    # e4m3's binades
+            step = torch.where(v.abs() >= 2.0 ** exponent, 2.0 ** (exponent - 3), step)
         r = torch.round(v / step) * step
         lim = torch.where(scale == 2.0 ** (8 if case['dtype'] == 'float16' else 120), 240.0, 448.0)
         r = torch.minimum(torch.maximum(r, -lim), lim)
@@ -261,5 +273,5 @@ def exact(case, seed):
         x = s['x'].to(f64)
     else:
         index = torch.arange(case['k'], device=dp.device) // BLOCK
-        x = s['codes'].to(f64) * torch.exp2(s['exponents'].to(f64) - 127)[:, index]
+        x = s['codes'].to(f64) * power(s['exponents'].long() - 127)[:, index]
     return {'x': torch.mm(dp, w.t()), 'kernel': torch.mm(x.t(), dp), 'bias': torch.sum(dp, 0)}
