@@ -115,6 +115,36 @@ SYMBOLS += [
 ]
 
 
+class PetdenseForwardArgs(C.Structure):
+    _fields_ = [('x', C.c_void_p), ('kernel', C.c_void_p), ('bias', C.c_void_p), ('residual', C.c_void_p),
+                ('y', C.c_void_p), ('pre', C.c_void_p), ('ldx', C.c_int64), ('ldk', C.c_int64), ('ldr', C.c_int64),
+                ('ldy', C.c_int64), ('ldp', C.c_int64), ('m', C.c_int64), ('k', C.c_int64), ('n', C.c_int64),
+                ('dtype', C.c_int), ('activation', C.c_int), ('bias_f32', C.c_int), ('out_f32', C.c_int)]
+
+
+class PetdenseBackwardArgs(C.Structure):
+    _fields_ = [('dy', C.c_void_p), ('x', C.c_void_p), ('x_exponents', C.c_void_p), ('kernel', C.c_void_p),
+                ('saved', C.c_void_p), ('dx', C.c_void_p), ('dkernel', C.c_void_p), ('dbias', C.c_void_p),
+                ('dresidual', C.c_void_p), ('lddy', C.c_int64), ('ldx', C.c_int64), ('lde', C.c_int64),
+                ('ldk', C.c_int64), ('lds', C.c_int64), ('lddx', C.c_int64), ('lddk', C.c_int64),
+                ('lddr', C.c_int64), ('m', C.c_int64), ('k', C.c_int64), ('n', C.c_int64), ('dtype', C.c_int),
+                ('activation', C.c_int), ('grad_f32', C.c_int)]
+
+
+SYMBOLS += [
+    # dense layer: products with epilogue, backward pass, 8-bit activation checkpoints (include/petdense.h)
+    ('petdense_forward_workspace', C.c_size_t, [C.POINTER(PetdenseForwardArgs)]),
+    ('petdense_forward', C.c_int, [C.POINTER(PetdenseForwardArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    ('petdense_backward_workspace', C.c_size_t, [C.POINTER(PetdenseBackwardArgs)]),
+    ('petdense_backward', C.c_int, [C.POINTER(PetdenseBackwardArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    ('petdense_checkpoint', C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_int64,
+                                      C.c_void_p, C.c_int64, C.c_void_p]),
+    ('petdense_restore', C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int,
+                                   C.c_void_p, C.c_int64, C.c_void_p]),
+    ('petdense_last_error', C.c_char_p, []),
+]
+
+
 class PetsimPrior(C.Structure):
     _fields_ = [('n_roi', C.c_int), ('n_frames', C.c_int), ('time_vector', C.c_void_p), ('dt', C.c_void_p),
                 ('mu_DVR', C.c_void_p), ('cov_DVR', C.c_void_p), ('mu_R1', C.c_void_p), ('cov_R1', C.c_void_p),

@@ -1,0 +1,336 @@
+// C-ABI implementation of the dense layer's operators (include/petdense.h): checks, the choice of tile and split for
+// each product, and the launches.
+#include "petdense.h"
+#include "dense_internal.h"
+
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+using namespace petdense_k;
+
+namespace {
+
+thread_local std::string g_err;
+
+int fail(int code, const char* what) noexcept {
+  try {
+    g_err = what;
+  } catch (...) {
+  }
+  return code;
+}
+
+#define HIPC(expr)                                                                         \
+  do {                                                                                     \
+    hipError_t e_ = (expr);                                                                \
+    if (e_ != hipSuccess) return fail(PETDIFF_ERR_HIP, hipGetErrorString(e_));             \
+  } while (0)
+#define NEED(cond, what) \
+  do {                   \
+    if (!(cond)) return fail(PETDIFF_ERR_INVALID, what); \
+  } while (0)
+
+constexpr int64_t kMaxDim = 0x7fffffff - 256;
+constexpr size_t kAlign = 256;
+
+size_t up(size_t b) { return (b + kAlign - 1) / kAlign * kAlign; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int size_of(int dtype) { return dtype == PETDENSE_F32 ? 4 : 2; }
+
+struct Plan {
+  int tile = kSmall, splits = 1, c_per = 0;
+  size_t part_bytes = 0;
+};
+
+// Tile and split of a product, by an estimate of its time in clocks of a compute unit.
+Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
+  struct Kind { int t, b, slots; double step; } kinds[] = {
+      // slots: workgroups of a compute unit at once (LDS and registers); step: clocks of one step of all of them
+      {kLarge, 256, 1, 2600}, {kMid, 128, 2, 1500}, {kSmall, 64, 4, 1000}};
+  const int bc = type == kF32 ? 32 : 64;
+  const double slow = type == kF32 ? 8.0 : 1.0;
+  const int64_t steps = ceil_div(C, bc);
+  Plan best;
+  double best_t = 0;
+  for (const Kind& k : kinds) {
+    if (k.t == kLarge && loader != kDma) continue;
+    const int64_t tiles = ceil_div(I, k.b) * ceil_div(J, k.b);
+    for (int64_t s = 1; s <= 64 && s <= steps; s = s < 4 ? s + 1 : s * 5 / 4) {
+      const int64_t per = ceil_div(steps, s), parts = ceil_div(steps, per);
+      if (parts != s) continue;
+      const int64_t waves = ceil_div(tiles * s, 256 * k.slots);
+      // a last, partly filled wave of workgroups shares its compute units with fewer others
+      const double fill = waves > 1 ? 1.0 : std::min(1.0, 0.35 + 0.65 * (double)tiles * s / (256.0 * k.slots));
+      double t = (double)waves * ((double)per * k.step * slow * fill + 3000);
+      if (s > 1) t += 9000 + (double)I * J * (s + 1) * 4 / 1600;
+      if (best.c_per == 0 || t < best_t) {
+        best_t = t;
+        best.tile = k.t;
+        best.splits = (int)s;
+        best.c_per = (int)std::min<int64_t>(per * bc, kMaxDim);
+      }
+    }
+  }
+  best.part_bytes = best.splits > 1 ? up((size_t)best.splits * I * J * 4) : 0;
+  return best;
+}
+
+bool dma_ok(const void* p, int64_t ld, int64_t contiguous, int size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0 && (contiguous * size) % 16 == 0 &&
+         ld * size < (int64_t)0x7fffffff / 256;          // a tile's offsets fit 31 bits
+}
+
+bool vec_ok(const void* p, int64_t ld, int size) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && ld % 4 == 0);
+}
+
+int run_product(Product p, int layout, int loader, int type, int q8, const Plan& pl, void* part, hipStream_t s) {
+  p.splits = pl.splits;
+  p.c_per = pl.c_per;
+  p.part = static_cast<float*>(part);
+  HIPC(type == kF32    ? product_f32(p, layout, loader, pl.tile, q8, s)
+       : type == kBF16 ? product_bf16(p, layout, loader, pl.tile, q8, s)
+                       : product_f16(p, layout, loader, pl.tile, q8, s));
+  if (pl.splits > 1) HIPC(join(p, type, s));
+  return PETDIFF_OK;
+}
+
+bool type_ok(int t) { return t >= PETDENSE_F32 && t <= PETDENSE_F16; }
+bool act_ok(int a) { return a >= PETDENSE_NONE && a <= PETDENSE_SILU; }
+bool work_ok(const void* w, size_t have, size_t need) {
+  return need == 0 || (w && have >= need && reinterpret_cast<uintptr_t>(w) % kAlign == 0);
+}
+
+// ---------------------------------------------------------------- forward
+int check_forward(const petdense_forward_args* a) {
+  NEED(a, "null arguments");
+  NEED(type_ok(a->dtype), "dtype must be PETDENSE_F32, PETDENSE_BF16 or PETDENSE_F16");
+  NEED(act_ok(a->activation), "unknown activation");
+  NEED(a->m >= 0 && a->k >= 1 && a->n >= 1, "m must be >= 0, k and n >= 1");
+  NEED(a->m < kMaxDim && a->k < kMaxDim && a->n < kMaxDim, "a dimension is too large");
+  if (a->m == 0) return PETDIFF_OK;
+  NEED(a->x && a->kernel && a->y, "x, kernel and y must be given");
+  NEED(a->ldx >= a->k && a->ldk >= a->n && a->ldy >= a->n, "a row stride is shorter than its row");
+  NEED(!a->residual || a->ldr >= a->n, "the residual's row stride is shorter than its row");
+  NEED(!a->pre || a->ldp >= a->n, "the pre-activation's row stride is shorter than its row");
+  NEED(a->y != a->x && a->y != a->kernel && (!a->pre || (a->pre != a->y && a->pre != a->x)),
+       "outputs must not alias inputs");
+  NEED(a->y != a->residual || (a->ldy == a->ldr && (!a->out_f32 || a->dtype == PETDENSE_F32)),
+       "y may be the residual only with its stride and type");
+  NEED(ceil_div(a->m, 64) * ceil_div(a->n, 64) < (int64_t)1 << 23, "too many outputs in one call");
+  return PETDIFF_OK;
+}
+
+struct ForwardPlan {
+  Plan p;
+  int loader;
+  bool rows;
+};
+
+ForwardPlan plan_forward(const petdense_forward_args* a) {
+  ForwardPlan f{};
+  const int sz = size_of(a->dtype);
+  f.loader = dma_ok(a->x, a->ldx, a->k, sz) && dma_ok(a->kernel, a->ldk, a->n, sz) ? kDma : kReg;
+  f.rows = a->m <= kMaxRows;
+  if (!f.rows && a->m > 0) f.p = plan(a->m, a->n, a->k, a->dtype, f.loader);
+  return f;
+}
+
+// ---------------------------------------------------------------- backward
+int check_backward(const petdense_backward_args* a) {
+  NEED(a, "null arguments");
+  NEED(type_ok(a->dtype), "dtype must be PETDENSE_F32, PETDENSE_BF16 or PETDENSE_F16");
+  NEED(act_ok(a->activation), "unknown activation");
+  NEED(a->m >= 0 && a->k >= 1 && a->n >= 1, "m must be >= 0, k and n >= 1");
+  NEED(a->m < kMaxDim && a->k < kMaxDim && a->n < kMaxDim, "a dimension is too large");
+  NEED(!a->dkernel || a->lddk >= a->n, "dkernel's row stride is shorter than its row");
+  if (a->m > 0) {
+    NEED(a->dy && a->lddy >= a->n, "dy must be given, with a row stride of at least n");
+    NEED(a->activation == PETDENSE_NONE || (a->saved && a->lds >= a->n),
+         "an activation's backward pass needs what the forward pass saved, with a row stride of at least n");
+    NEED(!a->dx || (a->kernel && a->ldk >= a->n && a->lddx >= a->k), "dx needs the kernel, and row strides of the rows");
+    NEED(!a->dkernel || (a->x && a->ldx >= a->k), "dkernel needs x, with a row stride of at least k");
+    NEED(!a->dkernel || !a->x_exponents || a->lde >= ceil_div(a->k, PETDENSE_BLOCK),
+         "the exponents' row stride is shorter than a row's blocks");
+    NEED(!a->dresidual || a->lddr >= a->n, "dresidual's row stride is shorter than its row");
+    const void* outs[] = {a->dx, a->dkernel, a->dbias, a->dresidual};
+    for (const void* o : outs)
+      NEED(!o || (o != a->dy && o != a->x && o != a->kernel && o != a->saved), "outputs must not alias inputs");
+  }
+  NEED(ceil_div(a->m, 64) * ceil_div(a->k, 64) < (int64_t)1 << 23 &&
+           ceil_div(a->k, 64) * ceil_div(a->n, 64) < (int64_t)1 << 23,
+       "too many outputs in one call");
+  return PETDIFF_OK;
+}
+
+struct BackwardPlan {
+  const void* dp;          // what the products read: dy, dresidual or the workspace
+  int64_t lddp;
+  bool make_dp;            // dp is made by act_grad
+  bool sums;               // column sums wanted
+  int chunks;
+  Plan px, pk;
+  int load_x, load_k;
+  size_t o_dp, o_sums, o_part, bytes;
+};
+
+BackwardPlan plan_backward(const petdense_backward_args* a, void* work) {
+  BackwardPlan b{};
+  const int sz = size_of(a->dtype);
+  char* w = static_cast<char*>(work);
+  size_t o = 0;
+  b.make_dp = a->activation != PETDENSE_NONE || a->dresidual;
+  b.sums = a->dbias != nullptr;
+  b.dp = a->dy;
+  b.lddp = a->lddy;
+  if (b.make_dp) {
+    if (a->dresidual) {
+      b.dp = a->dresidual;
+      b.lddp = a->lddr;
+    } else {
+      b.lddp = ceil_div(a->n, 64) * 64;
+      b.o_dp = o;
+      b.dp = w + o;
+      o += up((size_t)a->m * b.lddp * sz);
+    }
+  }
+  if (b.sums) {
+    const int64_t blocks = ceil_div(a->n, 256);
+    b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(a->m, 16), std::max<int64_t>(1, std::min<int64_t>(256, 1024 / blocks))));
+    b.o_sums = o;
+    o += up((size_t)b.chunks * a->n * 4);
+  } else {
+    b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(a->m, 16), 1024));
+  }
+  const void* base = work ? b.dp : (b.make_dp && !a->dresidual ? nullptr : b.dp);
+  if (a->dx) {
+    b.load_x = dma_ok(base, b.lddp, a->n, sz) && dma_ok(a->kernel, a->ldk, a->n, sz) ? kDma : kReg;
+    b.px = plan(a->m, a->k, a->n, a->dtype, b.load_x);
+  }
+  if (a->dkernel) {
+    // 8-bit inputs go through registers whatever their alignment: `loader` is dp's
+    b.load_k = dma_ok(base, b.lddp, a->n, sz) && (a->x_exponents || dma_ok(a->x, a->ldx, a->k, sz)) ? kDma : kReg;
+    b.pk = plan(a->k, a->n, a->m, a->dtype, b.load_k);
+  }
+  b.o_part = o;
+  b.bytes = o + std::max(b.px.part_bytes, b.pk.part_bytes);
+  return b;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* petdense_last_error(void) { return g_err.c_str(); }
+
+size_t petdense_forward_workspace(const petdense_forward_args* a) {
+  if (check_forward(a) != PETDIFF_OK || a->m == 0) return 0;
+  return plan_forward(a).p.part_bytes;
+}
+
+int petdense_forward(const petdense_forward_args* a, void* work, size_t work_bytes, void* stream) {
+  if (int r = check_forward(a)) return r;
+  if (a->m == 0) return PETDIFF_OK;
+  const ForwardPlan f = plan_forward(a);
+  NEED(work_ok(work, work_bytes, f.p.part_bytes), "the workspace is missing, too small or not 256-byte aligned");
+  const int sz = size_of(a->dtype), out = a->out_f32 ? 4 : sz;
+  Product p{};
+  p.A = a->x;
+  p.lda = a->ldx;
+  p.B = a->kernel;
+  p.ldb = a->ldk;
+  p.I = (int)a->m;
+  p.J = (int)a->n;
+  p.C = (int)a->k;
+  p.e = Epilogue{a->bias, a->residual, a->y, a->pre, a->ldr, a->ldy, a->ldp, a->activation, a->bias_f32, a->out_f32, 0};
+  p.e.vec = vec_ok(a->bias, 4, a->bias_f32 ? 4 : sz) && vec_ok(a->residual, a->ldr, sz) && vec_ok(a->y, a->ldy, out) &&
+            vec_ok(a->pre, a->ldp, out);
+  if (f.rows) {
+    HIPC(rows(p, a->dtype, (hipStream_t)stream));
+    return PETDIFF_OK;
+  }
+  return run_product(p, kForward, f.loader, a->dtype, 0, f.p, work, (hipStream_t)stream);
+}
+
+size_t petdense_backward_workspace(const petdense_backward_args* a) {
+  if (check_backward(a) != PETDIFF_OK || a->m == 0) return 0;
+  return plan_backward(a, nullptr).bytes;
+}
+
+int petdense_backward(const petdense_backward_args* a, void* work, size_t work_bytes, void* stream) {
+  if (int r = check_backward(a)) return r;
+  hipStream_t s = (hipStream_t)stream;
+  const int sz = size_of(a->dtype), gsz = a->grad_f32 ? 4 : sz;
+  if (a->m == 0) {                                     // no rows: the sums over them are zero
+    if (a->dkernel) HIPC(fill_zero(a->dkernel, a->k, a->n, a->lddk, gsz, s));
+    if (a->dbias) HIPC(fill_zero(a->dbias, 1, a->n, a->n, gsz, s));
+    return PETDIFF_OK;
+  }
+  const BackwardPlan b = plan_backward(a, work);
+  NEED(work_ok(work, work_bytes, b.bytes), "the workspace is missing, too small or not 256-byte aligned");
+  char* w = static_cast<char*>(work);
+  float* sums = b.sums ? reinterpret_cast<float*>(w + b.o_sums) : nullptr;
+  if (b.make_dp || b.sums)
+    HIPC(act_grad(a->dy, a->lddy, a->activation == PETDENSE_NONE ? nullptr : a->saved, a->lds,
+                  b.make_dp ? const_cast<void*>(b.dp) : nullptr, b.lddp, sums, b.chunks, (int)a->m, (int)a->n, a->dtype,
+                  a->activation, s));
+  if (b.sums) HIPC(join_columns(sums, b.chunks, (int)a->n, a->dbias, a->grad_f32 ? kF32 : a->dtype, s));
+  if (a->dx) {
+    Product p{};
+    p.A = b.dp;
+    p.lda = b.lddp;
+    p.B = a->kernel;
+    p.ldb = a->ldk;
+    p.I = (int)a->m;
+    p.J = (int)a->k;
+    p.C = (int)a->n;
+    p.e.out = a->dx;
+    p.e.ldo = a->lddx;
+    p.e.vec = vec_ok(a->dx, a->lddx, sz);
+    if (int r = run_product(p, kInputGrad, b.load_x, a->dtype, 0, b.px, w + b.o_part, s)) return r;
+  }
+  if (a->dkernel) {
+    Product p{};
+    p.A = a->x;
+    p.lda = a->ldx;
+    p.exps = a->x_exponents;
+    p.lde = a->lde;
+    p.B = b.dp;
+    p.ldb = b.lddp;
+    p.I = (int)a->k;
+    p.J = (int)a->n;
+    p.C = (int)a->m;
+    p.e.out = a->dkernel;
+    p.e.ldo = a->lddk;
+    p.e.out_f32 = a->grad_f32;
+    p.e.vec = vec_ok(a->dkernel, a->lddk, gsz);
+    if (int r = run_product(p, kKernelGrad, b.load_k, a->dtype, a->x_exponents != nullptr, b.pk, w + b.o_part, s))
+      return r;
+  }
+  return PETDIFF_OK;
+}
+
+int petdense_checkpoint(const void* x, int64_t ldx, int64_t m, int64_t k, int dtype, uint8_t* codes, int64_t ldc,
+                        uint8_t* exponents, int64_t lde, void* stream) {
+  NEED(type_ok(dtype), "dtype must be PETDENSE_F32, PETDENSE_BF16 or PETDENSE_F16");
+  NEED(m >= 0 && k >= 1 && m < kMaxDim && k < kMaxDim, "m must be >= 0, k >= 1, both < 2^31 - 256");
+  if (m == 0) return PETDIFF_OK;
+  NEED(x && codes && exponents, "x, codes and exponents must be given");
+  NEED(ldx >= k && ldc >= k && lde >= ceil_div(k, PETDENSE_BLOCK), "a row stride is shorter than its row");
+  HIPC(quantize(x, ldx, m, (int)k, dtype, codes, ldc, exponents, lde, (hipStream_t)stream));
+  return PETDIFF_OK;
+}
+
+int petdense_restore(const uint8_t* codes, int64_t ldc, const uint8_t* exponents, int64_t lde, int64_t m, int64_t k,
+                     int dtype, void* x, int64_t ldx, void* stream) {
+  NEED(type_ok(dtype), "dtype must be PETDENSE_F32, PETDENSE_BF16 or PETDENSE_F16");
+  NEED(m >= 0 && k >= 1 && m < kMaxDim && k < kMaxDim, "m must be >= 0, k >= 1, both < 2^31 - 256");
+  if (m == 0) return PETDIFF_OK;
+  NEED(x && codes && exponents, "x, codes and exponents must be given");
+  NEED(ldx >= k && ldc >= k && lde >= ceil_div(k, PETDENSE_BLOCK), "a row stride is shorter than its row");
+  HIPC(restore(codes, ldc, exponents, lde, m, (int)k, dtype, x, ldx, (hipStream_t)stream));
+  return PETDIFF_OK;
+}
+
+}  // extern "C"

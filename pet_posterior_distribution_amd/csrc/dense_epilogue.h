@@ -1,0 +1,132 @@
+// Scalar pieces shared by the dense layer's kernels: types, activations and their derivatives, the epilogue.
+#pragma once
+#include "dense_internal.h"
+
+namespace petdense_k {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Vec4 {
+  typedef T type __attribute__((ext_vector_type(4)));
+};
+
+// Phi(x) = (1 + erf(x / sqrt 2)) / 2.
+// 16-bit outputs: Abramowitz & Stegun 7.1.26, |error of erf| <= 1.5e-7, i.e. 2^-22.7 beside the 2^-9 and 2^-12
+// of a rounded output; about a third of erff's instructions, and the epilogue pays them once per output.
+template <bool EXACT>
+__device__ __forceinline__ float normal_cdf(float x) {
+  const float z = x * 0.70710678118654752f;
+  if constexpr (EXACT) {
+    return 0.5f * (1.0f + erff(z));
+  } else {
+    const float a = fabsf(z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float q = 0.5f * p * t * __expf(-a * a);          // 1 - Phi(|x|)
+    return x < 0.f ? q : 1.0f - q;
+  }
+}
+
+template <bool EXACT>
+__device__ __forceinline__ float sigmoid(float x) {
+  if constexpr (EXACT) return 1.0f / (1.0f + expf(-x));
+  return __builtin_amdgcn_rcpf(1.0f + __expf(-x));
+}
+
+template <bool EXACT>
+__device__ __forceinline__ float activate(float v, int act) {
+  if (act == kRelu) return v < 0.f ? 0.f : v;               // a NaN stays
+  if (act == kGelu) return v * normal_cdf<EXACT>(v);
+  if (act == kSilu) return v * sigmoid<EXACT>(v);
+  return v;
+}
+
+// act'(v); for ReLU v may be the output as well as the pre-activation
+template <bool EXACT>
+__device__ __forceinline__ float activate_grad(float g, float v, int act) {
+  if (act == kRelu) return v <= 0.f ? 0.f : g;
+  if (act == kGelu) {
+    const float pdf = 0.39894228040143268f * (EXACT ? expf(-0.5f * v * v) : __expf(-0.5f * v * v));
+    return g * fmaf(v, pdf, normal_cdf<EXACT>(v));
+  }
+  if (act == kSilu) {
+    const float s = sigmoid<EXACT>(v);
+    return g * s * fmaf(v, 1.0f - s, 1.0f);
+  }
+  return g;
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const void* p, int64_t o) {
+  typename Vec4<T>::type v = *reinterpret_cast<const typename Vec4<T>::type*>(static_cast<const T*>(p) + o);
+  return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+template <typename T>
+__device__ __forceinline__ void store4(void* p, int64_t o, f32x4 v) {
+  typename Vec4<T>::type r = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+  *reinterpret_cast<typename Vec4<T>::type*>(static_cast<T*>(p) + o) = r;
+}
+
+// Four outputs (i, j .. j + 3) of which `n` exist.
+template <typename T>
+__device__ __forceinline__ void epilogue4(const Epilogue& e, int64_t i, int64_t j, int n, f32x4 v) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  if (e.vec && n >= 4) {
+    if (e.bias) v += e.bias_f32 ? load4<float>(e.bias, j) : load4<T>(e.bias, j);
+    if (e.res) v += load4<T>(e.res, i * e.ldr + j);
+    if (e.pre) {
+      if (e.out_f32) store4<float>(e.pre, i * e.ldp + j, v);
+      else store4<T>(e.pre, i * e.ldp + j, v);
+    }
+    if (e.act != kNone) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = activate<EXACT>(v[q], e.act);
+    }
+    if (e.out_f32) store4<float>(e.out, i * e.ldo + j, v);
+    else store4<T>(e.out, i * e.ldo + j, v);
+    return;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (q >= n) continue;
+    float x = v[q];
+    if (e.bias) x += e.bias_f32 ? static_cast<const float*>(e.bias)[j + q] : (float)static_cast<const T*>(e.bias)[j + q];
+    if (e.res) x += (float)static_cast<const T*>(e.res)[i * e.ldr + j + q];
+    if (e.pre) {
+      if (e.out_f32) static_cast<float*>(e.pre)[i * e.ldp + j + q] = x;
+      else static_cast<T*>(e.pre)[i * e.ldp + j + q] = (T)x;
+    }
+    x = activate<EXACT>(x, e.act);
+    if (e.out_f32) static_cast<float*>(e.out)[i * e.ldo + j + q] = x;
+    else static_cast<T*>(e.out)[i * e.ldo + j + q] = (T)x;
+  }
+}
+
+// e4m3 codes of a word's four bytes times 2^E (`scale`) as two packed words of T; exact for the blocks the checkpoint
+// writes (four significant bits, E >= -117, no value past T's largest), except that fp16 rounds what is below 2^-14.
+template <typename T>
+__device__ __forceinline__ void restore4(unsigned w, float scale, T* out) {
+  if constexpr (sizeof(T) == 4) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, false);
+    const f2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, true);
+    out[0] = a[0]; out[1] = a[1]; out[2] = b[0]; out[3] = b[1];
+  } else if constexpr (__is_same(T, __bf16)) {
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
+    out[0] = a[0]; out[1] = a[1]; out[2] = b[0]; out[3] = b[1];
+  } else {
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true);
+    out[0] = a[0]; out[1] = a[1]; out[2] = b[0]; out[3] = b[1];
+  }
+}
+
+// 2^(byte - 127): an exponent byte as a float's exponent field (the checkpoint writes 10 .. 247)
+__device__ __forceinline__ float exponent_scale(unsigned byte) { return __uint_as_float(byte << 23); }
+
+}  // namespace petdense_k

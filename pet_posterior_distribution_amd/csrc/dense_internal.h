@@ -1,0 +1,68 @@
+// Internal declarations of the dense layer's operators (dense_*.hip <-> dense_api.cpp, include/petdense.h).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <cstddef>
+#include <cstdint>
+
+namespace petdense_k {
+
+enum Type { kF32 = 0, kBF16 = 1, kF16 = 2 };
+enum Act { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
+
+// What a product's accumulators go through: v + bias[j] + res[i][j], stored as `pre` if asked, then the activation.
+struct Epilogue {
+  const void* bias;      // [J] or null
+  const void* res;       // [I][J] (row stride ldr) in the operands' type, or null
+  void* out;             // [I][J] (row stride ldo)
+  void* pre;             // [I][J] (row stride ldp) or null
+  int64_t ldr, ldo, ldp;
+  int act;
+  int bias_f32, out_f32; // these are fp32 (else: the operands' type); `pre` has out's type
+  int vec;               // rows and bias take four values at a time (alignment and strides allow it)
+};
+
+// C[i][j] = sum over c of A(i, c) B(c, j).  A is stored [I][C] or, with free-contiguous operands, [C][I];
+// B likewise [J][C] or [C][J].
+struct Product {
+  const void* A;
+  const void* B;
+  int64_t lda, ldb;
+  const uint8_t* exps;   // A held in 8 bits: exponent bytes [C][I / 32] (row stride lde)
+  int64_t lde;
+  int I, J, C;
+  int splits, c_per;     // contraction split into `splits` parts of c_per (a multiple of the k-step)
+  float* part;           // [splits][I][J] fp32 when splits > 1 (the epilogue is then the joining kernel's)
+  Epilogue e;
+};
+
+enum Layout { kForward = 0, kInputGrad = 1, kKernelGrad = 2 };   // (A, B): (c-, j-), (c-, c-), (i-, j-contiguous)
+enum Loader { kDma = 0, kReg = 1 };
+enum Tile { kLarge = 0, kMid = 1, kSmall = 2 };
+
+// One launch of the tiled product: `q8`: A is e4m3 codes with exponent bytes (kKernelGrad only).
+hipError_t product_f32(const Product& p, int layout, int loader, int tile, int q8, hipStream_t s);
+hipError_t product_bf16(const Product& p, int layout, int loader, int tile, int q8, hipStream_t s);
+hipError_t product_f16(const Product& p, int layout, int loader, int tile, int q8, hipStream_t s);
+
+// Joins split products: the sum of p.part over the splits, in order, through the epilogue.
+hipError_t join(const Product& p, int type, hipStream_t s);
+
+// Few rows: one pass over B ([C][J], j-contiguous), I <= kMaxRows.
+constexpr int kMaxRows = 8;
+hipError_t rows(const Product& p, int type, hipStream_t s);
+
+// dp = dy act'(saved) (dp may be null), part[chunk][n] = column sums of dp over the chunk's rows (may be null)
+hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, float* part,
+                    int chunks, int M, int N, int type, int act, hipStream_t s);
+// out[n] = sum over chunks of part[chunk][n], in order
+hipError_t join_columns(const float* part, int chunks, int N, void* out, int out_type, hipStream_t s);
+
+// rows x n values of `size` bytes (row stride ld) become zero; a kernel, so that a graph can hold it
+hipError_t fill_zero(void* p, int64_t rows, int n, int64_t ld, int size, hipStream_t s);
+
+hipError_t quantize(const void* x, int64_t ldx, int64_t M, int K, int type, uint8_t* codes, int64_t ldc, uint8_t* exps,
+                    int64_t lde, hipStream_t s);
+hipError_t restore(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int64_t lde, int64_t M, int K, int type,
+                   void* x, int64_t ldx, hipStream_t s);
+
+}  // namespace petdense_k

@@ -1,0 +1,382 @@
+// The dense layer's kernels around its tiled product: the join of split products, few-row products, the activation's
+// gradient with the bias gradient's column sums, and the 8-bit activation checkpoint.
+#include "dense_epilogue.h"
+
+#include <algorithm>
+
+namespace petdense_k {
+
+namespace {
+
+constexpr int64_t kSlab = (int64_t)1 << 29;     // threads of one launch (a grid holds fewer than 2^32)
+
+inline unsigned blocks_for(int64_t n, int per) { return (unsigned)((n + per - 1) / per); }
+
+// ---------------------------------------------------------------------------------------------------------------
+// join: out = epilogue(sum over splits, in order).  Bound by reading the parts; a thread takes four columns.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(Product p, int64_t quads, int qrow) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= quads) return;
+  const int64_t i = t / qrow;
+  const int j = (int)(t - i * qrow) * 4, n = p.J - j;
+  const int64_t o = i * p.J + j, plane = (int64_t)p.I * p.J;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (p.J % 4 == 0) {
+    for (int s = 0; s < p.splits; ++s) v += *reinterpret_cast<const f32x4*>(p.part + s * plane + o);
+  } else {
+    for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < n) v[q] += p.part[s * plane + o + q];
+  }
+  epilogue4<T>(p.e, i, j, n, v);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows (decoding, a single sample): every value of B is read once by one workgroup, which owns COLS columns and
+// the whole contraction, so that one launch ends the call.  4 lanes share a row's 8-column pieces; the other lanes
+// and waves take other rows; their sums meet by shuffles and then in LDS, in a fixed order.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kRowThreads = 1024, kRowCols = 32;
+
+template <typename T, int ROWS>
+__global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p, int vec) {
+  constexpr int W = 8, LANES = kRowCols / W, GROUPS = kRowThreads / LANES;   // 4 lanes a row, 256 rows at a time
+  __shared__ float red[kRowThreads / 64][ROWS][kRowCols];
+  const int tid = threadIdx.x, l = tid % LANES, grp = tid / LANES;
+  const int j0 = blockIdx.x * kRowCols, j = j0 + l * W;
+  const T* A = static_cast<const T*>(p.A);
+  const T* B = static_cast<const T*>(p.B);
+  float acc[ROWS][W];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int q = 0; q < W; ++q) acc[r][q] = 0.f;
+  const int n = p.J - j;
+  if (n > 0) {
+#pragma unroll 4
+    for (int c = grp; c < p.C; c += GROUPS) {
+      T w[W];
+      const T* src = B + (int64_t)c * p.ldb + j;
+      if (vec && n >= W) {
+        __builtin_memcpy(w, __builtin_assume_aligned(src, W * sizeof(T) >= 16 ? 16 : W * sizeof(T)), sizeof(w));
+      } else {
+#pragma unroll
+        for (int q = 0; q < W; ++q) w[q] = q < n ? src[q] : (T)0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const float x = r < p.I ? (float)A[r * p.lda + c] : 0.f;
+#pragma unroll
+        for (int q = 0; q < W; ++q) acc[r][q] = fmaf(x, (float)w[q], acc[r][q]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+#pragma unroll
+      for (int o = LANES; o < 64; o *= 2) acc[r][q] += __shfl_xor(acc[r][q], o);
+      if ((tid & 63) < LANES) red[tid >> 6][r][l * W + q] = acc[r][q];
+    }
+  __syncthreads();
+  // thread t: row t / 8, columns 4 (t % 8) ..
+  constexpr int Q = kRowCols / 4;
+  if (tid < ROWS * Q) {
+    const int r = tid / Q, c = (tid % Q) * 4;
+    if (r < p.I && j0 + c < p.J) {
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < kRowThreads / 64; ++w)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += red[w][r][c + q];
+      epilogue4<T>(p.e, r, j0 + c, p.J - j0 - c, v);
+    }
+  }
+}
+
+template <typename T>
+hipError_t rows_t(const Product& p, hipStream_t s) {
+  const int vec = (reinterpret_cast<uintptr_t>(p.B) | (uintptr_t)(p.ldb * (int64_t)sizeof(T))) % 16 == 0;
+  const dim3 grid(blocks_for(p.J, kRowCols)), block(kRowThreads);
+  if (p.I == 1) hipLaunchKernelGGL((rows_kernel<T, 1>), grid, block, 0, s, p, vec);
+  else if (p.I == 2) hipLaunchKernelGGL((rows_kernel<T, 2>), grid, block, 0, s, p, vec);
+  else if (p.I <= 4) hipLaunchKernelGGL((rows_kernel<T, 4>), grid, block, 0, s, p, vec);
+  else hipLaunchKernelGGL((rows_kernel<T, 8>), grid, block, 0, s, p, vec);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// dp = dy act'(saved), and column sums of the unrounded dp over a chunk of rows.  One pass, memory bound: a wave
+// takes 4 columns a lane (256 columns), the block's 4 waves take every fourth row of the chunk.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void act_grad_kernel(const T* dy, int64_t ldy, const T* saved, int64_t lds, T* dp,
+                                                       int64_t ldd, float* part, int rows_per, int M, int N, int act,
+                                                       int vec) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  __shared__ f32x4 red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int j = blockIdx.x * 256 + lane * 4, n = N - j;
+  const int64_t m0 = (int64_t)blockIdx.y * rows_per, m1 = min(m0 + rows_per, (int64_t)M);
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (n > 0) {
+#pragma unroll 4
+    for (int64_t m = m0 + wave; m < m1; m += 4) {
+      f32x4 g, v = {0.f, 0.f, 0.f, 0.f};
+      if (vec && n >= 4) {
+        g = load4<T>(dy, m * ldy + j);
+        if (act != kNone) v = load4<T>(saved, m * lds + j);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          g[q] = q < n ? (float)dy[m * ldy + j + q] : 0.f;
+          if (act != kNone && q < n) v[q] = (float)saved[m * lds + j + q];
+        }
+      }
+      if (act != kNone) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], act);
+      }
+      sum += g;
+      if (dp) {
+        if (vec && n >= 4) {
+          store4<T>(dp, m * ldd + j, g);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q < n) dp[m * ldd + j + q] = (T)g[q];
+        }
+      }
+    }
+  }
+  if (!part) return;
+  red[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && n > 0) {
+    const f32x4 v = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < n) part[(int64_t)blockIdx.y * N + j + q] = v[q];
+  }
+}
+
+template <typename T>
+hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, float* part,
+                      int chunks, int M, int N, int act, hipStream_t s) {
+  const int rows_per = (M + chunks - 1) / chunks;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(saved) |
+                      reinterpret_cast<uintptr_t>(dp) | (uintptr_t)((ldy | (saved ? lds : 0) | (dp ? ldd : 0)) * (int64_t)sizeof(T));
+  hipLaunchKernelGGL((act_grad_kernel<T>), dim3(blocks_for(N, 256), chunks), dim3(256), 0, s,
+                     static_cast<const T*>(dy), ldy, static_cast<const T*>(saved), lds, static_cast<T*>(dp), ldd, part,
+                     rows_per, M, N, act, (int)(a % (4 * sizeof(T)) == 0));
+  return hipGetLastError();
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void join_columns_kernel(const float* part, int chunks, int N, T* out) {
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= N) return;
+  float v = 0.f;
+  for (int c = 0; c < chunks; ++c) v += part[(int64_t)c * N + j];
+  out[j] = (T)v;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// 8-bit checkpoint.  A lane takes 8 neighbouring values, 4 lanes a block of 32; the block's largest finite magnitude
+// meets over the 4 lanes by two shuffles.  Memory bound both ways.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void load_values(const T* src, int n, int vec, float* v) {
+  if (n >= 8) {
+    T w[8];
+    if (vec) __builtin_memcpy(w, __builtin_assume_aligned(src, 16), sizeof(w));
+    else __builtin_memcpy(w, src, sizeof(w));
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = (float)w[q];
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = q < n ? (float)src[q] : 0.f;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, int64_t octets, int orow, int K,
+                                                       uint8_t* codes, int64_t ldc, uint8_t* exps, int64_t lde,
+                                                       int vec_x, int vec_c) {
+  // orow: octets of a row, rounded up to whole blocks (a multiple of 4), so the 4 lanes of a block stay together
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t m = t / orow;
+  const int k = (int)(t - m * orow) * 8;
+  const bool live = t < octets;
+  const int n = live ? K - k : 0;                       // may be <= 0 in a row's last block
+  float v[8];
+  load_values<T>(live ? x + m * ldx + k : x, n, vec_x, v);
+  float top = 0.f;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float a = fabsf(v[q]);
+    top = fmaxf(top, a < __builtin_inff() ? a : 0.f);   // NaN and infinities do not count
+  }
+  top = fmaxf(top, __shfl_xor(top, 1));
+  top = fmaxf(top, __shfl_xor(top, 2));
+  // least E with top <= 448 2^E (448 = 1.75 2^8): top = 1.f 2^p gives E = p - 8, one more past a fraction of 0.75.
+  // A subnormal top has exponent field 0 and ends at the least E as it should.
+  const unsigned b = __float_as_uint(top);
+  int byte = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  byte = max(byte, 127 - 117);
+  const float inv = __uint_as_float((unsigned)(254 - byte) << 23);      // 2^-E, exact
+  const float lim = byte == (sizeof(T) == 2 && __is_same(T, _Float16) ? 127 + 8 : 127 + 120) ? 240.f : 448.f;
+  unsigned w[2] = {0, 0};
+#pragma unroll
+  for (int q = 0; q < 8; q += 2) {
+    const float y0 = fminf(fmaxf(v[q] * inv, -lim), lim), y1 = fminf(fmaxf(v[q + 1] * inv, -lim), lim);
+    const int c = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false) & 0xffff;
+    w[q >> 2] |= (unsigned)c << ((q & 2) * 8);
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    if (!(fabsf(v[q]) < __builtin_inff())) w[q >> 2] |= 0x7fu << ((q & 3) * 8);   // no infinities: they become NaN
+  if (n <= 0) return;
+  uint8_t* dst = codes + m * ldc + k;
+  if (n >= 8) {
+    if (vec_c) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else __builtin_memcpy(dst, w, 8);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < n) dst[q] = (uint8_t)(w[q >> 2] >> ((q & 3) * 8));
+  }
+  if ((k & 31) == 0) exps[m * lde + k / 32] = (uint8_t)byte;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void restore_kernel(const uint8_t* codes, int64_t ldc, const uint8_t* exps,
+                                                      int64_t lde, int64_t octets, int orow, int K, T* x, int64_t ldx,
+                                                      int vec_x, int vec_c) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= octets) return;
+  const int64_t m = t / orow;
+  const int k = (int)(t - m * orow) * 8, n = K - k;
+  const uint8_t* src = codes + m * ldc + k;
+  unsigned w[2] = {0, 0};
+  if (n >= 8) {
+    if (vec_c) {
+      const uint2 u = *reinterpret_cast<const uint2*>(src);
+      w[0] = u.x;
+      w[1] = u.y;
+    } else {
+      __builtin_memcpy(w, src, 8);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < n) w[q >> 2] |= (unsigned)src[q] << ((q & 3) * 8);
+  }
+  const float sc = exponent_scale(exps[m * lde + k / 32]);
+  T v[8];
+  restore4<T>(w[0], sc, v);
+  restore4<T>(w[1], sc, v + 4);
+  T* dst = x + m * ldx + k;
+  if (n >= 8) {
+    if (vec_x) __builtin_memcpy(__builtin_assume_aligned(dst, 16), v, sizeof(v));
+    else __builtin_memcpy(dst, v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < n) dst[q] = v[q];
+  }
+}
+
+template <typename T>
+hipError_t quantize_t(const void* x, int64_t ldx, int64_t M, int K, uint8_t* codes, int64_t ldc, uint8_t* exps, int64_t lde,
+                      hipStream_t s) {
+  const int orow = (K + 31) / 32 * 4;
+  const int vx = (reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * (int64_t)sizeof(T))) % 16 == 0;
+  const int vc = (reinterpret_cast<uintptr_t>(codes) | (uintptr_t)ldc) % 8 == 0;
+  const int64_t slab = std::max<int64_t>(1, kSlab / orow);
+  for (int64_t m = 0; m < M; m += slab) {
+    const int64_t octets = std::min(slab, M - m) * orow;
+    hipLaunchKernelGGL((quantize_kernel<T>), dim3(blocks_for(octets, 256)), dim3(256), 0, s,
+                       static_cast<const T*>(x) + m * ldx, ldx, octets, orow, K, codes + m * ldc, ldc, exps + m * lde,
+                       lde, vx, vc);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
+
+template <typename T>
+hipError_t restore_t(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int64_t lde, int64_t M, int K, void* x,
+                     int64_t ldx, hipStream_t s) {
+  const int orow = (K + 7) / 8;
+  const int vx = (reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * (int64_t)sizeof(T))) % 16 == 0;
+  const int vc = (reinterpret_cast<uintptr_t>(codes) | (uintptr_t)ldc) % 8 == 0;
+  const int64_t slab = std::max<int64_t>(1, kSlab / orow);
+  for (int64_t m = 0; m < M; m += slab) {
+    const int64_t octets = std::min(slab, M - m) * orow;
+    hipLaunchKernelGGL((restore_kernel<T>), dim3(blocks_for(octets, 256)), dim3(256), 0, s, codes + m * ldc, ldc,
+                       exps + m * lde, lde, octets, orow, K, static_cast<T*>(x) + m * ldx, ldx, vx, vc);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+#define PETDENSE_BY_TYPE(type, call)         \
+  switch (type) {                            \
+    case kF32: { using T = float; call; }    \
+    case kBF16: { using T = __bf16; call; }  \
+    default: { using T = _Float16; call; }   \
+  }
+
+hipError_t join(const Product& p, int type, hipStream_t s) {
+  const int qrow = (p.J + 3) / 4;
+  const int64_t quads = (int64_t)p.I * qrow;
+  PETDENSE_BY_TYPE(type, hipLaunchKernelGGL((join_kernel<T>), dim3(blocks_for(quads, 256)), dim3(256), 0, s, p, quads,
+                                            qrow);
+                   return hipGetLastError())
+}
+
+hipError_t rows(const Product& p, int type, hipStream_t s) { PETDENSE_BY_TYPE(type, return rows_t<T>(p, s)) }
+
+hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, float* part,
+                    int chunks, int M, int N, int type, int act, hipStream_t s) {
+  PETDENSE_BY_TYPE(type, return act_grad_t<T>(dy, ldy, saved, lds, dp, ldd, part, chunks, M, N, act, s))
+}
+
+hipError_t join_columns(const float* part, int chunks, int N, void* out, int out_type, hipStream_t s) {
+  PETDENSE_BY_TYPE(out_type, hipLaunchKernelGGL((join_columns_kernel<T>), dim3(blocks_for(N, 256)), dim3(256), 0, s,
+                                                part, chunks, N, static_cast<T*>(out));
+                   return hipGetLastError())
+}
+
+__global__ __launch_bounds__(256) void fill_zero_kernel(char* p, int64_t total, int n, int64_t ld, int size) {
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int64_t r = t / n;
+    char* d = p + (r * ld + (t - r * n)) * size;
+    if (size == 4) *reinterpret_cast<float*>(d) = 0.f;
+    else *reinterpret_cast<uint16_t*>(d) = 0;
+  }
+}
+
+hipError_t fill_zero(void* p, int64_t rows, int n, int64_t ld, int size, hipStream_t s) {
+  const int64_t total = rows * n;
+  hipLaunchKernelGGL(fill_zero_kernel, dim3((unsigned)std::min<int64_t>(4096, (total + 255) / 256)), dim3(256), 0, s,
+                     static_cast<char*>(p), total, n, ld, size);
+  return hipGetLastError();
+}
+
+hipError_t quantize(const void* x, int64_t ldx, int64_t M, int K, int type, uint8_t* codes, int64_t ldc, uint8_t* exps,
+                    int64_t lde, hipStream_t s) {
+  PETDENSE_BY_TYPE(type, return quantize_t<T>(x, ldx, M, K, codes, ldc, exps, lde, s))
+}
+
+hipError_t restore(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int64_t lde, int64_t M, int K, int type, void* x,
+                   int64_t ldx, hipStream_t s) {
+  PETDENSE_BY_TYPE(type, return restore_t<T>(codes, ldc, exps, lde, M, K, x, ldx, s))
+}
+
+}  // namespace petdense_k

@@ -1,0 +1,515 @@
+"""GPU tests of the dense layer's operators (petdense_*, layers.py) against their formulas in 64 bits.
+
+Tolerances, elementwise and derived, with u = eps / 2 of the output's type and S = the sum of the magnitudes of the
+terms of an output (from the 64-bit reference):
+* a product of C terms in fp32: every addition is off by at most 2^-23 of a partial sum that S bounds, the terms
+  themselves by 2^-24: (C + 4) 2^-23 S covers the sum, a split's join, bias and residual;
+* activations have slope at most 1.13 (GELU) and are evaluated to 4e-7 (|v| + 1): A = 1.13 P + 4e-7 (|v| + 1);
+* rounding the output: u |y|, and 2^-25 for fp16 outputs below its normal range;
+* a 16-bit layer's dP is rounded once more before the products: u |dP| through |W| and |X|.
+"""
+import ctypes as C
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = [BF16, F16, F32]
+ACTS = [None, 'relu', 'gelu', 'silu']
+E23 = 2.0 ** -23
+
+# one row and value, a few rows, odd sizes, sizes of whole tiles, a long contraction that is split, narrow outputs
+SHAPES = [(1, 1, 1), (1, 54, 256), (2, 300, 33), (7, 129, 64), (8, 64, 6), (9, 65, 33), (64, 64, 64), (77, 40, 136),
+          (130, 129, 257), (256, 256, 256), (257, 312, 128), (49 * 3, 33, 48), (40, 4100, 64), (24, 8000, 16),
+          (300, 72, 6)]
+# outputs of many tiles
+WIDE = [(2048, 128, 2048), (2040, 72, 4104)]
+
+
+def rand(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device='cuda') * scale).to(dtype)
+
+
+def act64(p, act):
+    if act == 'relu':
+        return torch.where(p < 0, torch.zeros_like(p), p)
+    if act == 'gelu':
+        return p * torch.special.ndtr(p)
+    if act == 'silu':
+        return p * torch.sigmoid(p)
+    return p
+
+
+def act_grad64(v, act):
+    if act == 'relu':
+        return torch.where(v <= 0, torch.zeros_like(v), torch.ones_like(v))
+    if act == 'gelu':
+        return torch.special.ndtr(v) + v * torch.exp(-v * v / 2) / (2 * torch.pi) ** 0.5
+    if act == 'silu':
+        s = torch.sigmoid(v)
+        return s * (1 + v * (1 - s))
+    return torch.ones_like(v)
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def close(got, ref, tol, what):
+    tol = tol + half_step(got.dtype) * (ref.abs() + tol) + (2.0 ** -25 if got.dtype == F16 else 1e-37)
+    err = (got.double() - ref).abs()
+    worst = (err / tol).max().item() if err.numel() else 0.0
+    assert worst <= 1.0, f'{what}: {worst:.3g} of its tolerance, max error {err.max().item():.3g}'
+
+
+def check_forward(x, w, b, act, r, pre, out_dtype=None):
+    from pet_posterior_distribution_amd import dense
+    got = dense(x, w, b, activation=act, residual=r, return_preactivation=pre, out_dtype=out_dtype)
+    y, p_got = got if pre else (got, None)
+    x64, w64 = x.double().reshape(-1, x.shape[-1]), w.double()
+    n, k = w.shape[1], w.shape[0]
+    p, s = x64 @ w64, x64.abs() @ w64.abs()
+    for extra in (b, r):
+        if extra is not None:
+            e = extra.double().reshape(-1, n) if extra.dim() > 1 else extra.double()
+            p, s = p + e, s + e.abs()
+    lead = tuple(x.shape[:-1]) + (n,)
+    assert tuple(y.shape) == lead and y.dtype == (out_dtype or x.dtype)
+    tol = (k + 4) * E23 * s
+    if pre:
+        close(p_got.reshape(-1, n), p, tol, 'pre-activation')
+    if act:
+        tol = 1.13 * tol + 4e-7 * (p.abs() + 1)
+    close(y.reshape(-1, n), act64(p, act), tol, 'output')
+    return y
+
+
+def reference_backward(dy, x64, w, act, saved):
+    """(dX, dW, db, dP) in 64 bits, and the tolerances of each before the last rounding."""
+    t = dy.dtype
+    n = dy.shape[-1]
+    d = dy.double().reshape(-1, n)
+    m, k = x64.shape
+    w64 = w.double()
+    e_dp = torch.zeros_like(d)
+    dp = d
+    if act:
+        v = saved.double().reshape(-1, n)
+        dp = d * act_grad64(v, act)
+        if act != 'relu':
+            e_dp = d.abs() * 1e-6 * (v.abs() + 1)
+    e_in = e_dp if act in (None, 'relu') or t == F32 else e_dp + half_step(t) * dp.abs() * 1.01 + \
+        (2.0 ** -25 if t == F16 else 0)
+    mag = dp.abs() + e_in
+    t_x = e_in @ w64.abs().T + (n + 4) * E23 * (mag @ w64.abs().T)
+    t_w = x64.abs().T @ e_in + (m + 4) * E23 * (x64.abs().T @ mag)
+    t_b = e_dp.sum(0) + (m + 260) * E23 * dp.abs().sum(0)
+    return (dp @ w64.T, x64.T @ dp, dp.sum(0), dp), (t_x, t_w, t_b, e_dp)
+
+
+def check_backward(dy, x, w, act, saved, grad_dtype=None, residual=True, x64=None):
+    from pet_posterior_distribution_amd import dense_backward
+    g = dense_backward(dy, x, w, activation=act, saved=saved, need_residual=residual, grad_dtype=grad_dtype)
+    n, k = w.shape[1], w.shape[0]
+    x64 = x.double().reshape(-1, k) if x64 is None else x64
+    ref, tol = reference_backward(dy, x64, w, act, saved)
+    assert g.x.dtype == dy.dtype and g.kernel.dtype == g.bias.dtype == (grad_dtype or dy.dtype)
+    assert tuple(g.x.shape) == tuple(dy.shape[:-1]) + (k,)
+    close(g.x.reshape(-1, k), ref[0], tol[0], 'dx')
+    close(g.kernel, ref[1], tol[1], 'dkernel')
+    close(g.bias, ref[2], tol[2], 'dbias')
+    if residual:
+        assert g.residual.dtype == dy.dtype and g.residual.shape == dy.shape
+        close(g.residual.reshape(-1, n), ref[3], tol[3], 'dresidual')
+    else:
+        assert g.residual is None
+    return g
+
+
+def inputs(m, k, n, t, seed=1):
+    return (rand((m, k), t, seed), rand((k, n), t, seed + 1, k ** -0.5), rand((n,), t, seed + 2),
+            rand((m, n), t, seed + 3), rand((m, n), t, seed + 4))
+
+
+@pytest.mark.parametrize('t', TYPES, ids=str)
+@pytest.mark.parametrize('m,k,n', SHAPES + WIDE)
+def test_forward(m, k, n, t):
+    x, w, b, r, _ = inputs(m, k, n, t)
+    i = SHAPES.index((m, k, n)) if (m, k, n) in SHAPES else 0
+    for j, act in enumerate(ACTS):
+        # every activation meets every mix of bias and residual over the shapes
+        check_forward(x, w, b if (i + j) % 3 else None, act, r if (i + j) % 2 else None, pre=(i + j) % 4 < 2)
+
+
+@pytest.mark.parametrize('t', [BF16, F16], ids=str)
+def test_forward_fp32_outputs_and_bias(t):
+    x, w, b, r, _ = inputs(150, 96, 72, t)
+    for act in ACTS:
+        y = check_forward(x, w, b.float() * 1.001, act, r, True, out_dtype=F32)
+        assert y.dtype == F32
+    check_forward(x[:3], w, b.float() * 1.001, 'gelu', r[:3], True, out_dtype=F32)
+
+
+@pytest.mark.parametrize('t', TYPES, ids=str)
+@pytest.mark.parametrize('m,k,n', SHAPES + WIDE)
+def test_backward(m, k, n, t):
+    x, w, _, p, dy = inputs(m, k, n, t)
+    for act in ACTS:
+        saved = None if act is None else (p.clamp(min=0) if act == 'relu' else p)
+        check_backward(dy, x, w, act, saved, residual=act in ('relu', 'gelu'))
+
+
+@pytest.mark.parametrize('act', [None, 'relu', 'gelu'])
+def test_backward_long_sums_and_fp32_gradients(act):
+    """Many rows into few gradients: the rows are split, and the parts joined in fp32."""
+    for t in (BF16, F16):
+        x, w, _, p, dy = inputs(20011, 48, 56, t)
+        check_backward(dy, x, w, act, None if act is None else p, grad_dtype=F32)
+
+
+def test_gradients_against_differences():
+    """dX, dW, db and dR are the derivatives of sum(dense(...) * dy): fp32, central differences of the 64-bit formula
+    along random directions (the difference quotient is off by about h^2 = 1e-8 of third derivatives)."""
+    from pet_posterior_distribution_amd import dense, dense_backward
+    for act in ACTS:
+        x, w, b, r, dy = inputs(33, 20, 17, F32, seed=40)
+        _, pre = dense(x, w, b, activation=act, residual=r, return_preactivation=True)
+        g = dense_backward(dy, x, w, activation=act, saved=pre, need_residual=True)
+        args = [v.double() for v in (x, w, b, r)]
+
+        def loss(a):
+            return (act64(a[0] @ a[1] + a[2] + a[3], act) * dy.double()).sum()
+
+        for i, gi in enumerate((g.x, g.kernel, g.bias, g.residual)):
+            d = rand(tuple(args[i].shape), F32, 50 + i).double()
+            h = 1e-4
+            if act == 'relu':      # no kink between the two points: only where every |P| is past the step
+                base = args[0] @ args[1] + args[2] + args[3]
+                step = [torch.zeros_like(a) for a in args]
+                step[i] = d * h
+                move = step[0] @ args[1] + args[0] @ step[1] + step[2] + step[3]
+                h *= min(1.0, 0.5 * (base.abs() / (move.abs() + 1e-30)).min().item())
+            up = [a + d * h if j == i else a for j, a in enumerate(args)]
+            dn = [a - d * h if j == i else a for j, a in enumerate(args)]
+            num = ((loss(up) - loss(dn)) / (2 * h)).item()
+            ana = (gi.double() * d).sum().item()
+            scale = (gi.double().abs() * d.abs()).sum().item()
+            assert abs(num - ana) <= 2e-5 * scale, (act, i, num, ana)
+
+
+def test_views_strides_and_leading_dimensions():
+    """Row strides (aligned and odd), merged and unmergeable leading dimensions, transposed kernels, broadcast
+    residuals and gradients: NaN in the gaps stays where it is."""
+    for t in (BF16, F32):
+        for gap in (8, 3):
+            wide = torch.full((66, 64 + gap), float('nan'), dtype=t, device='cuda')
+            wide[:, :64] = rand((66, 64), t, 1)
+            x = wide[:, :64]
+            wk = torch.full((64, 40 + gap), float('nan'), dtype=t, device='cuda')
+            wk[:, :40] = rand((64, 40), t, 2, 0.125)
+            w = wk[:, :40]
+            p = torch.full((66, 40 + gap), float('nan'), dtype=t, device='cuda')
+            p[:, :40] = rand((66, 40), t, 3)
+            p = p[:, :40]
+            check_forward(x, w, None, 'gelu', p, True)
+            check_backward(p, x, w, 'silu', p)
+            check_forward(x[5:11], w, None, None, p[5:11], False)
+        x3 = rand((4, 48, 24), t, 4)
+        w = rand((32, 24), t, 5).T
+        check_forward(x3, w, None, 'relu', rand((4, 48, 32), t, 6), False)
+        check_forward(x3.transpose(0, 1), w, None, 'relu', None, False)
+        check_forward(x3[:, 3:20], w, None, 'silu', None, True)
+        dy = rand((1, 32), t, 7).expand(4 * 48, 32)                       # the gradient of a sum over rows
+        check_backward(dy, x3.reshape(192, 24), w, None, None)
+        check_forward(rand((24,), t, 8), w, rand((32,), t, 9), None, None, False)
+        check_forward(x3.reshape(192, 24), w, None, None, rand((32,), t, 9).expand(192, 32), False)
+
+
+def test_a_contraction_longer_than_a_tile_row_reads_no_neighbour():
+    """Rows end inside a tile's row of 64 values: what lies behind them (the next row, NaN) must not enter."""
+    for t in TYPES:
+        for k in (1, 8, 31, 56, 63, 65, 72, 120):
+            buf = torch.full((140 * (k + 8),), float('nan'), dtype=t, device='cuda')
+            x = buf.view(140, k + 8)[:, :k]
+            x.copy_(rand((140, k), t, k))
+            w = rand((k, 24), t, k + 1, k ** -0.5)
+            check_forward(x, w, None, None, None, False)
+            check_backward(rand((140, 24), t, 3), x, w, None, None)
+
+
+def test_not_finite_values_stay_in_their_rows_and_columns():
+    from pet_posterior_distribution_amd import dense, dense_backward
+    for t in TYPES:
+        for m, k, n in ((200, 64, 72), (5, 33, 17)):
+            x, w, b, _, dy = inputs(m, k, n, t)
+            x[2, 5] = float('nan')
+            x[4, 6] = float('inf')
+            y = dense(x, w, b, activation='relu')
+            ref = act64(x.double() @ w.double() + b.double(), 'relu')
+            assert torch.equal(torch.isnan(y), torch.isnan(ref))
+            assert torch.equal(torch.isinf(y), torch.isinf(ref))
+            assert torch.isnan(y[2]).all() and torch.isfinite(y[[0, 1, 3]]).all()
+            dy[1, 3] = float('nan')
+            g = dense_backward(dy, inputs(m, k, n, t)[0], w, need_residual=True)
+            assert torch.isnan(g.x[1]).all() and torch.isfinite(g.x[2:]).all() and torch.isfinite(g.x[0]).all()
+            bad = torch.zeros(n, dtype=torch.bool, device='cuda')
+            bad[3] = True
+            assert torch.equal(torch.isnan(g.bias), bad) and torch.isnan(g.kernel[:, 3]).all()
+            assert torch.isfinite(g.kernel[:, ~bad]).all()
+
+
+def test_saved_values_of_relu_may_be_input_or_output():
+    from pet_posterior_distribution_amd import dense, dense_backward
+    x, w, b, _, dy = inputs(90, 40, 50, BF16)
+    y, pre = dense(x, w, b, activation='relu', return_preactivation=True)
+    one = dense_backward(dy, x, w, activation='relu', saved=y)
+    two = dense_backward(dy, x, w, activation='relu', saved=pre)
+    for a, c in zip(one[:3], two[:3]):
+        assert torch.equal(a, c)
+
+
+def test_no_rows():
+    from pet_posterior_distribution_amd import checkpoint_activations, dense, dense_backward
+    for t in TYPES:
+        w = rand((24, 16), t, 1)
+        x = torch.empty(0, 24, dtype=t, device='cuda')
+        y, p = dense(x, w, activation='gelu', return_preactivation=True)
+        assert y.shape == p.shape == (0, 16)
+        g = dense_backward(torch.empty(0, 16, dtype=t, device='cuda'), x, w, activation='relu', saved=y,
+                           need_residual=True, grad_dtype=F32)
+        assert g.x.shape == (0, 24) and g.residual.shape == (0, 16)
+        assert not g.kernel.any() and not g.bias.any() and g.kernel.shape == (24, 16)
+        c = checkpoint_activations(x)
+        assert c.restore().shape == (0, 24) and c.exponents.shape == (0, 1)
+
+
+def test_only_what_is_asked_for():
+    from pet_posterior_distribution_amd import dense_backward
+    x, w, _, p, dy = inputs(130, 72, 40, BF16)
+    full = dense_backward(dy, x, w, activation='gelu', saved=p, need_residual=True)
+    for i in range(4):
+        need = [j == i for j in range(4)]
+        g = dense_backward(dy, x, w, activation='gelu', saved=p, need_x=need[0], need_kernel=need[1],
+                           need_bias=need[2], need_residual=need[3])
+        for j in range(4):
+            assert (g[j] is not None) == need[j]
+        assert torch.equal(g[i], full[i])
+
+
+def test_rows_between_and_behind_the_outputs_are_left_as_they_were():
+    """C entry with output strides wider than the rows, and spare rows behind them."""
+    from pet_posterior_distribution_amd import _lib
+    from pet_posterior_distribution_amd.layers import _check, _stream
+    L = _lib.lib()
+    dev = torch.device('cuda', 0)
+    for t, code in ((BF16, 1), (F32, 0)):
+        for m, k, n in ((37, 40, 56), (130, 24, 30), (5, 24, 30)):
+            x, w, _, _, dy = inputs(m, k, n, t)
+            y = torch.full((m + 3, n + 5), 7.0, dtype=t, device=dev)
+            a = _lib.PetdenseForwardArgs(x.data_ptr(), w.data_ptr(), None, None, y.data_ptr(), None, k, n, 0, n + 5, 0,
+                                         m, k, n, code, 0, 0, 0)
+            nb = L.petdense_forward_workspace(C.byref(a))
+            ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+            _check(L.petdense_forward(C.byref(a), ws.data_ptr(), nb, _stream(dev)), 'dense')
+            assert (y[m:] == 7).all() and (y[:, n:] == 7).all()
+            close(y[:m, :n], x.double() @ w.double(), (k + 4) * E23 * (x.double().abs() @ w.double().abs()), 'output')
+            gx = torch.full((m + 3, k + 5), 7.0, dtype=t, device=dev)
+            gk = torch.full((k + 3, n + 5), 7.0, dtype=t, device=dev)
+            gb = torch.full((n + 3,), 7.0, dtype=t, device=dev)
+            bw = _lib.PetdenseBackwardArgs(dy.data_ptr(), x.data_ptr(), None, w.data_ptr(), None, gx.data_ptr(),
+                                           gk.data_ptr(), gb.data_ptr(), None, n, k, 0, n, 0, k + 5, n + 5, 0, m, k, n,
+                                           code, 0, 0)
+            nb = L.petdense_backward_workspace(C.byref(bw))
+            ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+            _check(L.petdense_backward(C.byref(bw), ws.data_ptr(), nb, _stream(dev)), 'dense_backward')
+            assert (gx[m:] == 7).all() and (gx[:, k:] == 7).all() and (gb[n:] == 7).all()
+            assert (gk[k:] == 7).all() and (gk[:, n:] == 7).all()
+            ref, tol = reference_backward(dy, x.double(), w, None, None)
+            close(gx[:m, :k], ref[0], tol[0], 'dx')
+            close(gk[:k, :n], ref[1], tol[1], 'dkernel')
+            close(gb[:n], ref[2], tol[2], 'dbias')
+
+
+# ---------------------------------------------------------------------------------------------------- checkpoints
+def power(e):
+    """2^e in 64 bits, exactly (torch.exp2 and torch.ldexp of 64-bit GPU tensors may be off by a bit)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def quantize64(x):
+    """(restored values in 64 bits, exponent bytes) by the definition."""
+    m, k = x.shape
+    nb = -(-k // 32)
+    x64 = x.double()
+    pad = torch.zeros(m, nb * 32, dtype=torch.float64, device=x.device)
+    pad[:, :k] = x64
+    b = pad.view(m, nb, 32)
+    fin = torch.isfinite(b)
+    top = torch.where(fin, b.abs(), torch.zeros_like(b)).amax(-1)
+    mant, e = torch.frexp(top)
+    big = torch.where(mant <= 0.875, e - 9, e - 8).clamp(min=-117)
+    big = torch.where(top == 0, torch.full_like(big, -117), big)
+    v = b * power(-big)[..., None]
+    step = torch.full_like(v, 2.0 ** -9)
+    for e in range(-5, 9):                                    # e4m3's binades
+        step = torch.where(v.abs() >= 2.0 ** e, 2.0 ** (e - 3), step)
+    q = torch.round(v / step) * step
+    lim = torch.where(big == (8 if x.dtype == F16 else 120), 240.0, 448.0)[..., None]
+    q = torch.where(fin, q.clamp(-lim, lim), torch.full_like(q, float('nan')))
+    return (q * power(big)[..., None]).view(m, -1)[:, :k], (big + 127).to(torch.uint8)
+
+
+def check_checkpoint(x):
+    from pet_posterior_distribution_amd import checkpoint_activations
+    c = checkpoint_activations(x)
+    ref, e = quantize64(x.reshape(-1, x.shape[-1]))
+    assert c.codes.shape == x.shape and c.dtype == x.dtype
+    assert torch.equal(c.exponents.reshape(e.shape), e)
+    back = c.restore()
+    assert back.shape == x.shape and back.dtype == x.dtype
+    got = back.double().reshape(ref.shape)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    ok = ~torch.isnan(ref)
+    # exact, but for fp16 below its normal range: half of 2^-24
+    assert ((got - ref).abs()[ok] <= (2.0 ** -25 if x.dtype == F16 else 0.0)).all()
+    assert torch.isfinite(back[torch.isfinite(x)]).all()
+    return c
+
+
+@pytest.mark.parametrize('t', TYPES, ids=str)
+@pytest.mark.parametrize('m,k', [(1, 1), (1, 31), (3, 32), (5, 33), (257, 615), (64, 256), (33, 1537), (2, 40000)])
+def test_checkpoint(m, k, t):
+    x = rand((m, k), F32, k) * torch.exp(rand((m, 1), F32, m) * 3)
+    x[0, 0] = 0
+    check_checkpoint(x.clamp(-6e4, 6e4).to(t))
+
+
+@pytest.mark.parametrize('t', TYPES, ids=str)
+def test_checkpoint_extremes(t):
+    f = torch.finfo(t)
+    x = torch.zeros(16, 64, dtype=t, device='cuda')
+    x[1, 3], x[1, 4] = f.max, -f.max                                    # restored as finite values
+    x[2] = f.tiny
+    x[3, :8] = torch.tensor([1, 1.75, 1.7500001, 2, 448, 449, 3.5, -3.5], device='cuda').to(t)
+    x[4, 0] = 448
+    x[5, 0] = 450 if t != BF16 else 452                                  # just past 448: the next exponent
+    x[6, 0], x[6, 1], x[6, 2], x[6, 40] = float('nan'), float('inf'), 1.0, float('-inf')
+    x[7] = float('nan')
+    x[8, 0], x[8, 1] = f.max, f.smallest_normal
+    x[9, :32] = rand((32,), t, 1) * f.max / 8
+    x[10, 0], x[10, 1] = f.max / 2, f.max / 4
+    x[11] = torch.linspace(-1, 1, 64, device='cuda').to(t)               # ties and subnormal codes
+    x[12, :] = torch.exp2(-torch.arange(64, device='cuda').float() / 3).to(t)
+    x[13, 0] = f.smallest_normal / 4                                     # a subnormal
+    check_checkpoint(x)
+
+
+def test_checkpoint_views():
+    wide = torch.full((40, 80), float('nan'), dtype=BF16, device='cuda')
+    wide[:, 3:75] = rand((40, 72), BF16, 1)
+    check_checkpoint(wide[:, 3:75])
+    check_checkpoint(rand((3, 5, 7, 40), F16, 2))
+    check_checkpoint(rand((64, 20), F32, 3).T)
+
+
+@pytest.mark.parametrize('t', TYPES, ids=str)
+@pytest.mark.parametrize('m,k,n', SHAPES + [(2048, 2048, 256)])
+def test_backward_from_checkpoint(m, k, n, t):
+    """dX and db are those of the layer; dW is the product with the restored activations, which it reads as they lie
+    (fp16 restores values below 2^-14 to a multiple of 2^-24: half of it times |dP|)."""
+    from pet_posterior_distribution_amd import checkpoint_activations, dense_backward
+    x, w, _, p, dy = inputs(m, k, n, t)
+    x = x * torch.exp2(torch.arange(m, device='cuda') % 9 - 4).to(t)[:, None]
+    c = checkpoint_activations(x)
+    for act in (None, 'relu', 'silu'):
+        saved = None if act is None else p
+        g = check_backward(dy, c, w, act, saved, residual=False, x64=c.restore().double(),
+                           grad_dtype=F32 if act == 'relu' else None)
+        whole = dense_backward(dy, x, w, activation=act, saved=saved, grad_dtype=F32 if act == 'relu' else None)
+        assert torch.equal(g.x, whole.x) and torch.equal(g.bias, whole.bias)
+
+
+# ------------------------------------------------------------------------------------------- streams and graphs
+def chain(x, ws, bs, dy):
+    """Two layers forward, the first one's input kept in 8 bits, and their backward passes."""
+    from pet_posterior_distribution_amd import checkpoint_activations, dense, dense_backward
+    c = checkpoint_activations(x)
+    h, p1 = dense(x, ws[0], bs[0], activation='gelu', return_preactivation=True)
+    y = dense(h, ws[1], bs[1], activation='relu', residual=x)
+    g2 = dense_backward(dy, h, ws[1], activation='relu', saved=y, need_residual=True)
+    g1 = dense_backward(g2.x, c, ws[0], activation='gelu', saved=p1, grad_dtype=F32)
+    return [h, y, g2.x, g2.kernel, g2.bias, g2.residual, g1.x, g1.kernel, g1.bias, c.restore()]
+
+
+def chain_inputs(seed, m=333, t=BF16):
+    x = rand((m, 96), t, seed)
+    ws = [rand((96, 200), t, seed + 1, 0.1), rand((200, 96), t, seed + 2, 0.07)]
+    bs = [rand((200,), t, seed + 3), rand((96,), F32, seed + 4)]
+    return x, ws, bs, rand((m, 96), t, seed + 5)
+
+
+def test_a_run_of_the_operators_against_64_bits():
+    """The chain of two layers as it is used.  Each stage is checked from the stages before it by the tests above; the
+    run as a whole by its distance in the 2-norm: about a dozen independent roundings of at most 2^-9 to its inputs,
+    sqrt(12) 2^-9 = 0.7 %, and the checkpoint's 2^-4 / sqrt 3 = 3.6 % in the first kernel's gradient alone."""
+    x, ws, bs, dy = chain_inputs(7)
+    got = chain(x, ws, bs, dy)
+    x6, w0, w1, b0, b1, d6 = (v.double() for v in (x, ws[0], ws[1], bs[0], bs[1], dy))
+    p1 = x6 @ w0 + b0
+    h = act64(p1, 'gelu')
+    y = act64(h @ w1 + b1 + x6, 'relu')
+    dp2 = d6 * (got[1] > 0)                       # the run's own mask: a pre-activation next to zero may go either way
+    gh = dp2 @ w1.T
+    dp1 = gh * act_grad64(p1, 'gelu')
+    ref = [h, y, gh, h.T @ dp2, dp2.sum(0), dp2, dp1 @ w0.T, x6.T @ dp1, dp1.sum(0), x6]
+    for i, (a, r) in enumerate(zip(got, ref)):
+        far = ((a.double() - r).norm() / r.norm()).item()
+        assert far < (0.036 if i in (7, 9) else 0.007), (i, far)
+
+
+def test_results_repeat_bit_by_bit_and_on_another_stream():
+    x, ws, bs, dy = chain_inputs(11)
+    one = chain(x, ws, bs, dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        two = chain(x, ws, bs, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    three = chain(x, ws, bs, dy)
+    torch.cuda.synchronize()
+    for a, b, c in zip(one, two, three):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_two_captured_graphs_replay_like_eager_runs():
+    sets = [chain_inputs(21), chain_inputs(31, m=40)]
+    eager = [chain(*s) for s in sets]
+    graphs, outs = [], []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(chain(*s))
+        graphs.append(g)
+    for rep in range(4):
+        for o in outs:
+            for v in o:
+                v.zero_()
+        other = chain(*chain_inputs(41 + rep))        # eager work between the replays
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for o, e in zip(outs, eager):
+            for a, b in zip(o, e):
+                assert torch.equal(a, b), rep
+        del other
+    # new inputs in the captured tensors' place
+    fresh = chain_inputs(61)
+    for dst, src in zip([sets[0][0], *sets[0][1], *sets[0][2], sets[0][3]], [fresh[0], *fresh[1], *fresh[2], fresh[3]]):
+        dst.copy_(src)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    for a, b in zip(outs[0], chain(*fresh)):
+        assert torch.equal(a, b)
