@@ -81,10 +81,6 @@ bool dma_ok(const void* p, int64_t ld, int64_t contiguous, int size) {
          ld * size < (int64_t)0x7fffffff / 256;          // a tile's offsets fit 31 bits
 }
 
-bool vec_ok(const void* p, int64_t ld, int size) {
-  return !p || (reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && ld % 4 == 0);
-}
-
 int run_product(Product p, int layout, int loader, int type, int q8, const Plan& pl, void* part, hipStream_t s) {
   p.splits = pl.splits;
   p.c_per = pl.c_per;
@@ -234,7 +230,6 @@ int petdense_forward(const petdense_forward_args* a, void* work, size_t work_byt
   if (a->m == 0) return PETDIFF_OK;
   const ForwardPlan f = plan_forward(a);
   NEED(work_ok(work, work_bytes, f.p.part_bytes), "the workspace is missing, too small or not 256-byte aligned");
-  const int sz = size_of(a->dtype), out = a->out_f32 ? 4 : sz;
   Product p{};
   p.A = a->x;
   p.lda = a->ldx;
@@ -243,9 +238,7 @@ int petdense_forward(const petdense_forward_args* a, void* work, size_t work_byt
   p.I = (int)a->m;
   p.J = (int)a->n;
   p.C = (int)a->k;
-  p.e = Epilogue{a->bias, a->residual, a->y, a->pre, a->ldr, a->ldy, a->ldp, a->activation, a->bias_f32, a->out_f32, 0};
-  p.e.vec = vec_ok(a->bias, 4, a->bias_f32 ? 4 : sz) && vec_ok(a->residual, a->ldr, sz) && vec_ok(a->y, a->ldy, out) &&
-            vec_ok(a->pre, a->ldp, out);
+  p.e = Epilogue{a->bias, a->residual, a->y, a->pre, a->ldr, a->ldy, a->ldp, a->activation, a->bias_f32, a->out_f32};
   if (f.rows) {
     HIPC(rows(p, a->dtype, (hipStream_t)stream));
     return PETDIFF_OK;
@@ -261,7 +254,7 @@ size_t petdense_backward_workspace(const petdense_backward_args* a) {
 int petdense_backward(const petdense_backward_args* a, void* work, size_t work_bytes, void* stream) {
   if (int r = check_backward(a)) return r;
   hipStream_t s = (hipStream_t)stream;
-  const int sz = size_of(a->dtype), gsz = a->grad_f32 ? 4 : sz;
+  const int gsz = a->grad_f32 ? 4 : size_of(a->dtype);
   if (a->m == 0) {                                     // no rows: the sums over them are zero
     if (a->dkernel) HIPC(fill_zero(a->dkernel, a->k, a->n, a->lddk, gsz, s));
     if (a->dbias) HIPC(fill_zero(a->dbias, 1, a->n, a->n, gsz, s));
@@ -287,7 +280,6 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     p.C = (int)a->n;
     p.e.out = a->dx;
     p.e.ldo = a->lddx;
-    p.e.vec = vec_ok(a->dx, a->lddx, sz);
     if (int r = run_product(p, kInputGrad, b.load_x, a->dtype, 0, b.px, w + b.o_part, s)) return r;
   }
   if (a->dkernel) {
@@ -304,7 +296,6 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     p.e.out = a->dkernel;
     p.e.ldo = a->lddk;
     p.e.out_f32 = a->grad_f32;
-    p.e.vec = vec_ok(a->dkernel, a->lddk, gsz);
     if (int r = run_product(p, kKernelGrad, b.load_k, a->dtype, a->x_exponents != nullptr, b.pk, w + b.o_part, s))
       return r;
   }

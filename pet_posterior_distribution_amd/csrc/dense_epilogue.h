@@ -71,39 +71,66 @@ __device__ __forceinline__ void store4(void* p, int64_t o, f32x4 v) {
   *reinterpret_cast<typename Vec4<T>::type*>(static_cast<T*>(p) + o) = r;
 }
 
-// Four outputs (i, j .. j + 3) of which `n` exist.
+// W neighbouring values of a row, of which n exist (the others read as zero).  Whole groups are one access of any
+// alignment.
+template <typename T, int W>
+__device__ __forceinline__ void load_row(const T* src, int n, float* v) {
+  if (n >= W) {
+    T w[W];
+    __builtin_memcpy(w, src, sizeof(w));
+#pragma unroll
+    for (int q = 0; q < W; ++q) v[q] = (float)w[q];
+  } else {
+#pragma unroll
+    for (int q = 0; q < W; ++q) v[q] = q < n ? (float)src[q] : 0.f;
+  }
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_row(T* dst, int n, const float* v) {
+  if (n >= W) {
+    T w[W];
+#pragma unroll
+    for (int q = 0; q < W; ++q) w[q] = (T)v[q];
+    __builtin_memcpy(dst, w, sizeof(w));
+  } else {
+#pragma unroll
+    for (int q = 0; q < W; ++q)
+      if (q < n) dst[q] = (T)v[q];
+  }
+}
+
+// Eight outputs (i, j .. j + 7) of which `n` exist.
 template <typename T>
-__device__ __forceinline__ void epilogue4(const Epilogue& e, int64_t i, int64_t j, int n, f32x4 v) {
+__device__ __forceinline__ void epilogue8(const Epilogue& e, int64_t i, int64_t j, int n, float* v) {
   constexpr bool EXACT = sizeof(T) == 4;
-  if (e.vec && n >= 4) {
-    if (e.bias) v += e.bias_f32 ? load4<float>(e.bias, j) : load4<T>(e.bias, j);
-    if (e.res) v += load4<T>(e.res, i * e.ldr + j);
-    if (e.pre) {
-      if (e.out_f32) store4<float>(e.pre, i * e.ldp + j, v);
-      else store4<T>(e.pre, i * e.ldp + j, v);
-    }
-    if (e.act != kNone) {
+  float w[8];
+  if (e.bias) {
+    if (e.bias_f32) load_row<float, 8>(static_cast<const float*>(e.bias) + j, n, w);
+    else load_row<T, 8>(static_cast<const T*>(e.bias) + j, n, w);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = activate<EXACT>(v[q], e.act);
-    }
-    if (e.out_f32) store4<float>(e.out, i * e.ldo + j, v);
-    else store4<T>(e.out, i * e.ldo + j, v);
-    return;
+    for (int q = 0; q < 8; ++q) v[q] += w[q];
   }
+  if (e.res) {
+    load_row<T, 8>(static_cast<const T*>(e.res) + i * e.ldr + j, n, w);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (q >= n) continue;
-    float x = v[q];
-    if (e.bias) x += e.bias_f32 ? static_cast<const float*>(e.bias)[j + q] : (float)static_cast<const T*>(e.bias)[j + q];
-    if (e.res) x += (float)static_cast<const T*>(e.res)[i * e.ldr + j + q];
-    if (e.pre) {
-      if (e.out_f32) static_cast<float*>(e.pre)[i * e.ldp + j + q] = x;
-      else static_cast<T*>(e.pre)[i * e.ldp + j + q] = (T)x;
-    }
-    x = activate<EXACT>(x, e.act);
-    if (e.out_f32) static_cast<float*>(e.out)[i * e.ldo + j + q] = x;
-    else static_cast<T*>(e.out)[i * e.ldo + j + q] = (T)x;
+    for (int q = 0; q < 8; ++q) v[q] += w[q];
   }
+  if (e.pre) {
+    if (e.out_f32) store_row<float, 8>(static_cast<float*>(e.pre) + i * e.ldp + j, n, v);
+    else store_row<T, 8>(static_cast<T*>(e.pre) + i * e.ldp + j, n, v);
+  }
+  if (e.act == kRelu) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = activate<EXACT>(v[q], kRelu);
+  } else if (e.act == kGelu) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = activate<EXACT>(v[q], kGelu);
+  } else if (e.act == kSilu) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = activate<EXACT>(v[q], kSilu);
+  }
+  if (e.out_f32) store_row<float, 8>(static_cast<float*>(e.out) + i * e.ldo + j, n, v);
+  else store_row<T, 8>(static_cast<T*>(e.out) + i * e.ldo + j, n, v);
 }
 
 // e4m3 codes of a word's four bytes times 2^E (`scale`) as two packed words of T; exact for the blocks the checkpoint

@@ -18,7 +18,6 @@ struct Epilogue {
   int64_t ldr, ldo, ldp;
   int act;
   int bias_f32, out_f32; // these are fp32 (else: the operands' type); `pre` has out's type
-  int vec;               // rows and bias take four values at a time (alignment and strides allow it)
 };
 
 // C[i][j] = sum over c of A(i, c) B(c, j).  A is stored [I][C] or, with free-contiguous operands, [C][I];

@@ -13,25 +13,25 @@ constexpr int64_t kSlab = (int64_t)1 << 29;     // threads of one launch (a grid
 inline unsigned blocks_for(int64_t n, int per) { return (unsigned)((n + per - 1) / per); }
 
 // ---------------------------------------------------------------------------------------------------------------
-// join: out = epilogue(sum over splits, in order).  Bound by reading the parts; a thread takes four columns.
+// join: out = epilogue(sum over splits, in order).  Bound by reading the parts; a thread takes eight columns.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(Product p, int64_t quads, int qrow) {
+__global__ __launch_bounds__(256) void join_kernel(Product p, int64_t octets, int orow) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= quads) return;
-  const int64_t i = t / qrow;
-  const int j = (int)(t - i * qrow) * 4, n = p.J - j;
-  const int64_t o = i * p.J + j, plane = (int64_t)p.I * p.J;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (p.J % 4 == 0) {
-    for (int s = 0; s < p.splits; ++s) v += *reinterpret_cast<const f32x4*>(p.part + s * plane + o);
-  } else {
-    for (int s = 0; s < p.splits; ++s)
+  if (t >= octets) return;
+  const int64_t i = t / orow;
+  const int j = (int)(t - i * orow) * 8, n = p.J - j;
+  const float* src = p.part + i * p.J + j;
+  const int64_t plane = (int64_t)p.I * p.J;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    float w[8];
+    load_row<float, 8>(src + s * plane, n, w);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (q < n) v[q] += p.part[s * plane + o + q];
+    for (int q = 0; q < 8; ++q) v[q] += w[q];
   }
-  epilogue4<T>(p.e, i, j, n, v);
+  epilogue8<T>(p.e, i, j, n, v);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -42,36 +42,53 @@ __global__ __launch_bounds__(256) void join_kernel(Product p, int64_t quads, int
 constexpr int kRowThreads = 1024, kRowCols = 32;
 
 template <typename T, int ROWS>
-__global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p, int vec) {
+__global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
   constexpr int W = 8, LANES = kRowCols / W, GROUPS = kRowThreads / LANES;   // 4 lanes a row, 256 rows at a time
+  constexpr int AHEAD = ROWS <= 4 ? 4 : 2;                                  // rows of a lane in flight
   __shared__ float red[kRowThreads / 64][ROWS][kRowCols];
   const int tid = threadIdx.x, l = tid % LANES, grp = tid / LANES;
-  const int j0 = blockIdx.x * kRowCols, j = j0 + l * W;
+  const int j0 = blockIdx.x * kRowCols, j = j0 + l * W, n = p.J - j;
   const T* A = static_cast<const T*>(p.A);
-  const T* B = static_cast<const T*>(p.B);
+  const T* B = static_cast<const T*>(p.B) + j;
   float acc[ROWS][W];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int q = 0; q < W; ++q) acc[r][q] = 0.f;
-  const int n = p.J - j;
-  if (n > 0) {
-#pragma unroll 4
-    for (int c = grp; c < p.C; c += GROUPS) {
-      T w[W];
-      const T* src = B + (int64_t)c * p.ldb + j;
-      if (vec && n >= W) {
-        __builtin_memcpy(w, __builtin_assume_aligned(src, W * sizeof(T) >= 16 ? 16 : W * sizeof(T)), sizeof(w));
-      } else {
+  auto add = [&](const T* w, const T* x) {
 #pragma unroll
-        for (int q = 0; q < W; ++q) w[q] = q < n ? src[q] : (T)0.f;
-      }
+    for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        const float x = r < p.I ? (float)A[r * p.lda + c] : 0.f;
+      for (int q = 0; q < W; ++q) acc[r][q] = fmaf((float)x[r], (float)w[q], acc[r][q]);
+  };
+  auto xs = [&](int c, T* x) {
 #pragma unroll
-        for (int q = 0; q < W; ++q) acc[r][q] = fmaf(x, (float)w[q], acc[r][q]);
-      }
+    for (int r = 0; r < ROWS; ++r) x[r] = A[(r < p.I ? r : 0) * p.lda + c];      // rows past the last are not stored
+  };
+  int c = grp;
+  if (n >= W) {
+    for (; c + (AHEAD - 1) * GROUPS < p.C; c += AHEAD * GROUPS) {
+      T w[AHEAD][W], x[AHEAD][ROWS];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) __builtin_memcpy(w[u], B + (int64_t)(c + u * GROUPS) * p.ldb, sizeof(w[u]));
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) xs(c + u * GROUPS, x[u]);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) add(w[u], x[u]);
+    }
+    for (; c < p.C; c += GROUPS) {
+      T w[W], x[ROWS];
+      __builtin_memcpy(w, B + (int64_t)c * p.ldb, sizeof(w));
+      xs(c, x);
+      add(w, x);
+    }
+  } else if (n > 0) {
+    for (; c < p.C; c += GROUPS) {
+      T w[W], x[ROWS];
+#pragma unroll
+      for (int q = 0; q < W; ++q) w[q] = q < n ? B[(int64_t)c * p.ldb + q] : (T)0.f;
+      xs(c, x);
+      add(w, x);
     }
   }
 #pragma unroll
@@ -83,28 +100,26 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p, int vec) {
       if ((tid & 63) < LANES) red[tid >> 6][r][l * W + q] = acc[r][q];
     }
   __syncthreads();
-  // thread t: row t / 8, columns 4 (t % 8) ..
-  constexpr int Q = kRowCols / 4;
-  if (tid < ROWS * Q) {
-    const int r = tid / Q, c = (tid % Q) * 4;
+  // thread t: row t / 4, columns 8 (t % 4) ..
+  if (tid < ROWS * LANES) {
+    const int r = tid / LANES, c = (tid % LANES) * W;
     if (r < p.I && j0 + c < p.J) {
-      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      float v[W] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       for (int w = 0; w < kRowThreads / 64; ++w)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] += red[w][r][c + q];
-      epilogue4<T>(p.e, r, j0 + c, p.J - j0 - c, v);
+        for (int q = 0; q < W; ++q) v[q] += red[w][r][c + q];
+      epilogue8<T>(p.e, r, j0 + c, p.J - j0 - c, v);
     }
   }
 }
 
 template <typename T>
 hipError_t rows_t(const Product& p, hipStream_t s) {
-  const int vec = (reinterpret_cast<uintptr_t>(p.B) | (uintptr_t)(p.ldb * (int64_t)sizeof(T))) % 16 == 0;
   const dim3 grid(blocks_for(p.J, kRowCols)), block(kRowThreads);
-  if (p.I == 1) hipLaunchKernelGGL((rows_kernel<T, 1>), grid, block, 0, s, p, vec);
-  else if (p.I == 2) hipLaunchKernelGGL((rows_kernel<T, 2>), grid, block, 0, s, p, vec);
-  else if (p.I <= 4) hipLaunchKernelGGL((rows_kernel<T, 4>), grid, block, 0, s, p, vec);
-  else hipLaunchKernelGGL((rows_kernel<T, 8>), grid, block, 0, s, p, vec);
+  if (p.I == 1) hipLaunchKernelGGL((rows_kernel<T, 1>), grid, block, 0, s, p);
+  else if (p.I == 2) hipLaunchKernelGGL((rows_kernel<T, 2>), grid, block, 0, s, p);
+  else if (p.I <= 4) hipLaunchKernelGGL((rows_kernel<T, 4>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((rows_kernel<T, 8>), grid, block, 0, s, p);
   return hipGetLastError();
 }
 
@@ -175,13 +190,24 @@ hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t ld
   return hipGetLastError();
 }
 
+// 16 columns by 16 groups of chunks a block: group g sums chunks g, g + 16, ..; the groups meet in LDS, in order.
 template <typename T>
 __global__ __launch_bounds__(256) void join_columns_kernel(const float* part, int chunks, int N, T* out) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= N) return;
+  __shared__ float red[16][16];
+  const int c = threadIdx.x & 15, g = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
   float v = 0.f;
-  for (int c = 0; c < chunks; ++c) v += part[(int64_t)c * N + j];
-  out[j] = (T)v;
+  if (j < N) {
+#pragma unroll 8
+    for (int k = g; k < chunks; k += 16) v += part[(int64_t)k * N + j];
+  }
+  red[g][c] = v;
+  __syncthreads();
+  if (g == 0 && j < N) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += red[k][c];
+    out[j] = (T)s;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -189,23 +215,8 @@ __global__ __launch_bounds__(256) void join_columns_kernel(const float* part, in
 // meets over the 4 lanes by two shuffles.  Memory bound both ways.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ void load_values(const T* src, int n, int vec, float* v) {
-  if (n >= 8) {
-    T w[8];
-    if (vec) __builtin_memcpy(w, __builtin_assume_aligned(src, 16), sizeof(w));
-    else __builtin_memcpy(w, src, sizeof(w));
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = (float)w[q];
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = q < n ? (float)src[q] : 0.f;
-  }
-}
-
-template <typename T>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, int64_t octets, int orow, int K,
-                                                       uint8_t* codes, int64_t ldc, uint8_t* exps, int64_t lde,
-                                                       int vec_x, int vec_c) {
+                                                       uint8_t* codes, int64_t ldc, uint8_t* exps, int64_t lde) {
   // orow: octets of a row, rounded up to whole blocks (a multiple of 4), so the 4 lanes of a block stay together
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t m = t / orow;
@@ -213,7 +224,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, 
   const bool live = t < octets;
   const int n = live ? K - k : 0;                       // may be <= 0 in a row's last block
   float v[8];
-  load_values<T>(live ? x + m * ldx + k : x, n, vec_x, v);
+  load_row<T, 8>(live ? x + m * ldx + k : x, n, v);
   float top = 0.f;
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
@@ -242,8 +253,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, 
   if (n <= 0) return;
   uint8_t* dst = codes + m * ldc + k;
   if (n >= 8) {
-    if (vec_c) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-    else __builtin_memcpy(dst, w, 8);
+    __builtin_memcpy(dst, w, 8);
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
@@ -254,8 +264,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* x, int64_t ldx, 
 
 template <typename T>
 __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* codes, int64_t ldc, const uint8_t* exps,
-                                                      int64_t lde, int64_t octets, int orow, int K, T* x, int64_t ldx,
-                                                      int vec_x, int vec_c) {
+                                                      int64_t lde, int64_t octets, int orow, int K, T* x, int64_t ldx) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (t >= octets) return;
   const int64_t m = t / orow;
@@ -263,13 +272,7 @@ __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* codes, int6
   const uint8_t* src = codes + m * ldc + k;
   unsigned w[2] = {0, 0};
   if (n >= 8) {
-    if (vec_c) {
-      const uint2 u = *reinterpret_cast<const uint2*>(src);
-      w[0] = u.x;
-      w[1] = u.y;
-    } else {
-      __builtin_memcpy(w, src, 8);
-    }
+    __builtin_memcpy(w, src, 8);
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
@@ -281,8 +284,7 @@ __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* codes, int6
   restore4<T>(w[1], sc, v + 4);
   T* dst = x + m * ldx + k;
   if (n >= 8) {
-    if (vec_x) __builtin_memcpy(__builtin_assume_aligned(dst, 16), v, sizeof(v));
-    else __builtin_memcpy(dst, v, sizeof(v));
+    __builtin_memcpy(dst, v, sizeof(v));
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
@@ -294,14 +296,12 @@ template <typename T>
 hipError_t quantize_t(const void* x, int64_t ldx, int64_t M, int K, uint8_t* codes, int64_t ldc, uint8_t* exps, int64_t lde,
                       hipStream_t s) {
   const int orow = (K + 31) / 32 * 4;
-  const int vx = (reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * (int64_t)sizeof(T))) % 16 == 0;
-  const int vc = (reinterpret_cast<uintptr_t>(codes) | (uintptr_t)ldc) % 8 == 0;
   const int64_t slab = std::max<int64_t>(1, kSlab / orow);
   for (int64_t m = 0; m < M; m += slab) {
     const int64_t octets = std::min(slab, M - m) * orow;
     hipLaunchKernelGGL((quantize_kernel<T>), dim3(blocks_for(octets, 256)), dim3(256), 0, s,
                        static_cast<const T*>(x) + m * ldx, ldx, octets, orow, K, codes + m * ldc, ldc, exps + m * lde,
-                       lde, vx, vc);
+                       lde);
     if (hipError_t e = hipGetLastError()) return e;
   }
   return hipSuccess;
@@ -311,13 +311,11 @@ template <typename T>
 hipError_t restore_t(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int64_t lde, int64_t M, int K, void* x,
                      int64_t ldx, hipStream_t s) {
   const int orow = (K + 7) / 8;
-  const int vx = (reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * (int64_t)sizeof(T))) % 16 == 0;
-  const int vc = (reinterpret_cast<uintptr_t>(codes) | (uintptr_t)ldc) % 8 == 0;
   const int64_t slab = std::max<int64_t>(1, kSlab / orow);
   for (int64_t m = 0; m < M; m += slab) {
     const int64_t octets = std::min(slab, M - m) * orow;
     hipLaunchKernelGGL((restore_kernel<T>), dim3(blocks_for(octets, 256)), dim3(256), 0, s, codes + m * ldc, ldc,
-                       exps + m * lde, lde, octets, orow, K, static_cast<T*>(x) + m * ldx, ldx, vx, vc);
+                       exps + m * lde, lde, octets, orow, K, static_cast<T*>(x) + m * ldx, ldx);
     if (hipError_t e = hipGetLastError()) return e;
   }
   return hipSuccess;
@@ -333,10 +331,10 @@ hipError_t restore_t(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int
   }
 
 hipError_t join(const Product& p, int type, hipStream_t s) {
-  const int qrow = (p.J + 3) / 4;
-  const int64_t quads = (int64_t)p.I * qrow;
-  PETDENSE_BY_TYPE(type, hipLaunchKernelGGL((join_kernel<T>), dim3(blocks_for(quads, 256)), dim3(256), 0, s, p, quads,
-                                            qrow);
+  const int orow = (p.J + 7) / 8;
+  const int64_t octets = (int64_t)p.I * orow;
+  PETDENSE_BY_TYPE(type, hipLaunchKernelGGL((join_kernel<T>), dim3(blocks_for(octets, 256)), dim3(256), 0, s, p,
+                                            octets, orow);
                    return hipGetLastError())
 }
 
@@ -348,7 +346,7 @@ hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds,
 }
 
 hipError_t join_columns(const float* part, int chunks, int N, void* out, int out_type, hipStream_t s) {
-  PETDENSE_BY_TYPE(out_type, hipLaunchKernelGGL((join_columns_kernel<T>), dim3(blocks_for(N, 256)), dim3(256), 0, s,
+  PETDENSE_BY_TYPE(out_type, hipLaunchKernelGGL((join_columns_kernel<T>), dim3(blocks_for(N, 16)), dim3(256), 0, s,
                                                 part, chunks, N, static_cast<T*>(out));
                    return hipGetLastError())
 }

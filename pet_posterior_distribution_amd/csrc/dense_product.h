@@ -4,8 +4,13 @@
 //
 // A workgroup owns a BI x BJ tile of C; its waves split the tile, each holding its part in fp32 accumulators.  Per
 // step the workgroup stages BC contraction values of both operands in LDS (128 bytes of each operand's row or
-// BC rows), two stages deep: the loads of step t + 1 are in flight while step t is multiplied, one barrier a step.
-// 16-bit operands go through v_mfma_f32_16x16x32, fp32 through v_mfma_f32_16x16x4.
+// BC rows), two stages deep.  16-bit operands go through v_mfma_f32_16x16x32, fp32 through v_mfma_f32_16x16x4.
+// A step is two groups of products (KS = 2), and every read is one group ahead of its use:
+//   group 0: read group 1's fragments while group 0 is multiplied
+//   wait: group 1's fragments are in registers, the next stage has landed; barrier: so it is for every wave
+//   group 1: the load of the stage after the next goes into the stage just read; read the next stage's group 0
+//            fragments while group 1 is multiplied
+// so neither a barrier nor LDS latency stands before a product, and a load has a whole step to land.
 //
 // Operands are taken as they lie in memory:
 //  - contraction-contiguous ([free][c]): a lane's fragment is 16 bytes of its row, one ds_read_b128;
@@ -18,6 +23,8 @@
 #pragma once
 #include "dense_epilogue.h"
 
+#include <type_traits>
+
 namespace petdense_k {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -29,8 +36,14 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 
 #define PETDENSE_LDS __attribute__((address_space(3)))
 
-__device__ void raw_buffer_load_lds(i32x4 rsrc, PETDENSE_LDS void* lds, int size, int voffset, int soffset,
-                                    int offset, int aux) __asm("llvm.amdgcn.raw.buffer.load.lds");
+// One wave's buffer load of 64 x 16 bytes straight into LDS at `lds` (wave-uniform) + 16 lane.  In assembly, because
+// the compiler would put a wait for it before every LDS read that follows; the kernel waits for it itself, before the
+// barrier that publishes a stage.  (No output register: nothing the compiler could reuse early.)
+__device__ __forceinline__ void load_to_lds(i32x4 rsrc, unsigned lds, int voffset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset),
+               "s"(rsrc)
+               : "memory", "m0");
+}
 
 // A stage of one operand: ROWS rows of CPR 16-byte pieces.  Piece c of row r lies at place c ^ key(r) of the row, so
 // that the lanes of one LDS read, which take the same piece of several rows, meet every bank once.
@@ -141,66 +154,69 @@ struct Filler {
     }
   }
 
-  // the first bytes of step t
-  __device__ const char* step(int t) const {
-    return base + (FREE ? (int64_t)t * BC * ld : (int64_t)t * BC * (int64_t)sizeof(T));
+  // what every piece of step t needs
+  struct Step {
+    i32x4 rs;            // kDma: the buffer that begins at the step
+    const char* p;
+    int t, left;         // contraction values of the step that exist (<= 0: a step past the end loads nothing)
+  };
+  __device__ __forceinline__ Step at(int t) const {
+    Step u;
+    u.t = t;
+    u.left = clen - t * BC;
+    u.p = base + (FREE ? (int64_t)t * BC * ld : (int64_t)t * BC * (int64_t)sizeof(T));
+    if constexpr (LOADER == kDma) {
+      const unsigned long long a = reinterpret_cast<unsigned long long>(u.p);
+      u.rs[0] = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffull));
+      u.rs[1] = __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffffull));
+      u.rs[2] = (int)0x80000000;
+      u.rs[3] = 0x00020000;
+    }
+    return u;
   }
 
-  // begins the loads of step t (kDma: into `st`)
-  __device__ __forceinline__ void begin(char* st, int t, int tid) {
-    const int left = clen - t * BC;                                  // contraction values of this step that exist
+  // begins the load of the thread's piece q of a step (kDma: into `st`)
+  __device__ __forceinline__ void begin(char* st, const Step& u, int q, int tid) {
+    const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
     if constexpr (LOADER == kDma) {
-      const unsigned long long a = reinterpret_cast<unsigned long long>(step(t));
-      i32x4 rs;
-      rs[0] = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffull));
-      rs[1] = __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffffull));
-      rs[2] = (int)0x80000000;
-      rs[3] = 0x00020000;
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-#pragma unroll
-      for (int q = 0; q < N; ++q) {
-        int o = voff[q];
-        if (left < BC) {
-          const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
-          if (FREE ? r >= left : c * S::EPC >= left) o = (int)0x80000000;
-        }
-        raw_buffer_load_lds(rs, (PETDENSE_LDS void*)(st + (q * THREADS + wave * 64) * 16), 16, o, 0, 0, 0);
-      }
+      const int o = (FREE ? r >= u.left : c * S::EPC >= u.left) ? (int)0x80000000 : voff[q];
+      load_to_lds(u.rs, (unsigned)(uintptr_t)(PETDENSE_LDS char*)st + (q * THREADS + wave * 64) * 16, o);
     } else {
-      const char* p = step(t);
+      // values of the piece that exist
+      const int n = FREE ? (r < u.left ? limit - c * S::EPC : 0) : (r < limit ? u.left - c * S::EPC : 0);
+      reg[q] = u32x4{0, 0, 0, 0};
+      if constexpr (Q8) {
+        const char* s = u.p + r * ld + c * S::EPC;
+        unsigned w[2] = {0, 0};
+        if (n >= S::EPC) __builtin_memcpy(w, s, S::EPC);
+        else
+          for (int v = 0; v < n; ++v) w[v >> 2] |= (unsigned)(uint8_t)s[v] << ((v & 3) * 8);
+        // a piece past the end keeps no exponent: its codes are zero
+        const unsigned b = n > 0 ? exps[((int64_t)u.t * BC + r) * lde + (c * S::EPC) / 32] : 127;
+        reg[q][0] = w[0];
+        reg[q][1] = w[1];
+        reg[q][2] = b;
+      } else {
+        const char* s = u.p + r * ld + c * 16;
+        if (n >= S::EPC) {
+          __builtin_memcpy(&reg[q], s, 16);
+        } else if (n > 0) {
+          T v[S::EPC];
 #pragma unroll
-      for (int q = 0; q < N; ++q) {
-        const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
-        // values of the piece that exist
-        const int n = FREE ? (r < left ? limit - c * S::EPC : 0) : (r < limit ? left - c * S::EPC : 0);
-        reg[q] = u32x4{0, 0, 0, 0};
-        if constexpr (Q8) {
-          const char* s = p + r * ld + c * S::EPC;
-          unsigned w[2] = {0, 0};
-          if (n >= S::EPC) __builtin_memcpy(w, s, S::EPC);
-          else
-            for (int v = 0; v < n; ++v) w[v >> 2] |= (unsigned)(uint8_t)s[v] << ((v & 3) * 8);
-          // a step past the end keeps no exponent: its codes are zero
-          const unsigned b = n > 0 ? exps[((int64_t)t * BC + r) * lde + (c * S::EPC) / 32] : 127;
-          reg[q][0] = w[0];
-          reg[q][1] = w[1];
-          reg[q][2] = b;
-        } else {
-          const char* s = p + r * ld + c * 16;
-          if (n >= S::EPC) {
-            __builtin_memcpy(&reg[q], s, 16);
-          } else if (n > 0) {
-            T v[S::EPC];
-#pragma unroll
-            for (int x = 0; x < S::EPC; ++x) {
-              v[x] = (T)0.f;
-              if (x < n) __builtin_memcpy(&v[x], s + x * sizeof(T), sizeof(T));
-            }
-            __builtin_memcpy(&reg[q], v, 16);
+          for (int x = 0; x < S::EPC; ++x) {
+            v[x] = (T)0.f;
+            if (x < n) __builtin_memcpy(&v[x], s + x * sizeof(T), sizeof(T));
           }
+          __builtin_memcpy(&reg[q], v, 16);
         }
       }
     }
+  }
+  __device__ __forceinline__ void begin_all(char* st, int t, int tid) {
+    const Step u = at(t);
+#pragma unroll
+    for (int q = 0; q < N; ++q) begin(st, u, q, tid);
   }
 
   // ends them: kReg: writes the registers to `st`
@@ -222,11 +238,10 @@ struct Filler {
   }
 };
 
-// Own loads and LDS accesses done, then a bare barrier.
+// All but the last N of this wave's loads have landed, its LDS accesses are done; then a bare barrier.
+template <int N>
 __device__ __forceinline__ void step_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 template <typename T, int BI, int BJ, int WI, int WJ, bool FA, bool FB, int LA, int LB, bool Q8>
@@ -278,60 +293,111 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(Product p) {
 #pragma unroll
     for (int y = 0; y < FJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  fa.begin(lds, 0, tid);
-  fb.begin(lds + SA::BYTES, 0, tid);
+  typename Frag<T>::type a[KS][FI], b[KS][FJ];
+  const int ra = wi * (BI / WI), rb = wj * (BJ / WJ);
+  // fragment f of a group: the FJ of B, then the FI of A
+  auto read = [&](const char* st, int ks, int f) {
+    if (f < FJ) b[ks][f] = fragment<T, FB, BJ, BC>(st + SA::BYTES, rb + f * 16, ks, lane);
+    else a[ks][f - FJ] = fragment<T, FA, BI, BC>(st, ra + (f - FJ) * 16, ks, lane);
+  };
+  // Multiplies group ks row by row of A's fragments while it reads group kn of stage `rd` and, with LOAD, begins the
+  // pieces of step `ua` / `ub` into `ld`.  A row's fragment is dead after its row, and the reads are spread so that
+  // two more than FI are live at once; the last row reads nothing, which covers the last read's latency.
+  constexpr int READS = FI + FJ, ROWS = FI > 1 ? FI - 1 : 1;
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
+  constexpr int NA = decltype(fa)::N, NB = decltype(fb)::N;
+  auto group = [&](int ks, int kn, auto reads, const char* rd, auto loads, char* ld, const auto& ua, const auto& ub) {
+#pragma unroll
+    for (int x = 0; x < FI; ++x) {
+      if constexpr (decltype(loads)::value) {
+#pragma unroll
+        for (int q = 0; q < NA; ++q)
+          if (q * FI / NA == x) fa.begin(ld, ua, q, tid);
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+          if (q * FI / NB == x) fb.begin(ld + SA::BYTES, ub, q, tid);
+      }
+      if constexpr (decltype(reads)::value) {
+#pragma unroll
+        for (int f = 0; f < READS; ++f)
+          if (f * ROWS / READS == x) read(rd, kn, f);
+      }
+#pragma unroll
+      for (int y = 0; y < FJ; ++y) acc[x][y] = multiply<T>(b[ks][y], a[ks][x], acc[x][y]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  fa.begin_all(lds, 0, tid);
+  fb.begin_all(lds + SA::BYTES, 0, tid);
   fa.end(lds, tid);
   fb.end(lds + SA::BYTES, tid);
-  for (int t = 0; t < steps; ++t) {
-    char* cur = lds + (t & 1) * STAGE;
-    char* nxt = lds + ((t & 1) ^ 1) * STAGE;
-    step_barrier();             // step t has landed, and every wave is done with step t - 1's stage
-    if (t + 1 < steps) {
-      fa.begin(nxt, t + 1, tid);
-      fb.begin(nxt + SA::BYTES, t + 1, tid);
-    }
+  fa.begin_all(lds + STAGE, 1, tid);
+  fb.begin_all(lds + STAGE + SA::BYTES, 1, tid);
+  step_barrier<(LA == kDma ? NA : 0) + (LB == kDma ? NB : 0)>();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      typename Frag<T>::type a[FI], b[FJ];
-#pragma unroll
-      for (int y = 0; y < FJ; ++y)
-        b[y] = fragment<T, FB, BJ, BC>(cur + SA::BYTES, wj * (BJ / WJ) + y * 16, ks, lane);
-#pragma unroll
-      for (int x = 0; x < FI; ++x) a[x] = fragment<T, FA, BI, BC>(cur, wi * (BI / WI) + x * 16, ks, lane);
-#pragma unroll
-      for (int x = 0; x < FI; ++x)
-#pragma unroll
-        for (int y = 0; y < FJ; ++y) acc[x][y] = multiply<T>(b[y], a[x], acc[x][y]);
-    }
-    if (t + 1 < steps) {
-      fa.end(nxt, tid);
-      fb.end(nxt + SA::BYTES, tid);
-    }
+  for (int f = 0; f < READS; ++f) read(lds, 0, f);
+  char* cur = lds;
+  char* nxt = lds + STAGE;
+  for (int t = 0; t + 1 < steps; ++t) {
+    const auto ua = fa.at(t + 2);
+    const auto ub = fb.at(t + 2);
+    group(0, 1, yes, cur, no, nullptr, ua, ub);
+    fa.end(nxt, tid);
+    fb.end(nxt + SA::BYTES, tid);
+    step_barrier<0>();
+    group(1, 0, yes, nxt, yes, cur, ua, ub);
+    char* s = cur;
+    cur = nxt;
+    nxt = s;
   }
+  {
+    const auto ua = fa.at(steps);
+    const auto ub = fb.at(steps);
+    group(0, 1, yes, cur, no, nullptr, ua, ub);
+    group(1, 0, no, nullptr, no, nullptr, ua, ub);
+  }
+  // loads into LDS past the last step (of zeros) end before the workgroup's LDS is given away
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
+  // Epilogue.  A wave turns its accumulators, ROWS_AT x 16 rows at a time, through its own part of LDS (16-byte piece
+  // c of row r at place c ^ r), so that a lane gets eight neighbouring outputs of a row and a row's lanes touch whole
+  // cache lines.
+  __syncthreads();
+  constexpr int TJ = BJ / WJ, PIECES = TJ / 4, MASK = PIECES < 16 ? PIECES - 1 : 15;
+  constexpr int ROWS_FIT = STAGE * 2 / (WI * WJ) / (16 * TJ * 4);
+  constexpr int ROWS_AT = ROWS_FIT < FI ? ROWS_FIT : FI;
+  static_assert(ROWS_FIT >= 1 && FI % ROWS_AT == 0, "the tile's rows pass through LDS in equal parts");
+  Epilogue e = p.e;
+  if (p.splits > 1) {
+    e = Epilogue{};
+    e.out = p.part + (int64_t)blockIdx.y * p.I * p.J;
+    e.ldo = p.J;
+    e.out_f32 = 1;
+  }
+  char* own = lds + wave * (ROWS_AT * 16 * TJ * 4);
   const int g = lane >> 4, il = lane & 15;
 #pragma unroll
-  for (int x = 0; x < FI; ++x) {
-    const int i = i0 + wi * (BI / WI) + x * 16 + il;
-    if (i >= p.I) continue;
+  for (int x0 = 0; x0 < FI; x0 += ROWS_AT) {
 #pragma unroll
-    for (int y = 0; y < FJ; ++y) {
-      const int j = j0 + wj * (BJ / WJ) + y * 16 + g * 4;
-      const int n = p.J - j;
-      if (n <= 0) continue;
-      if (p.splits > 1) {
-        float* o = p.part + ((int64_t)blockIdx.y * p.I + i) * p.J + j;
-        if (n >= 4 && p.J % 4 == 0) {
-          *reinterpret_cast<f32x4*>(o) = acc[x][y];
-        } else {
+    for (int x = 0; x < ROWS_AT; ++x)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q < n) o[q] = acc[x][y][q];
-        }
-      } else {
-        epilogue4<T>(p.e, i, j, n, acc[x][y]);
+      for (int y = 0; y < FJ; ++y)
+        *reinterpret_cast<f32x4*>(own + ((x * 16 + il) * PIECES + ((y * 4 + g) ^ (il & MASK))) * 16) = acc[x0 + x][y];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // other lanes of the wave read what this one wrote
+#pragma unroll 1
+    for (int k = lane; k < ROWS_AT * 16 * (TJ / 8); k += 64) {
+      const int r = k / (TJ / 8), c = (k % (TJ / 8)) * 2, key = r & MASK;
+      const int i = i0 + ra + x0 * 16 + r, j = j0 + rb + c * 4;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(own + (r * PIECES + (c ^ key)) * 16);
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(own + (r * PIECES + ((c + 1) ^ key)) * 16);
+      if (i < p.I && j < p.J) {
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        epilogue8<T>(e, i, j, p.J - j, v);
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
