@@ -133,10 +133,11 @@ class PetdenseBackwardArgs(C.Structure):
 
 SYMBOLS += [
     # dense layer: products with epilogue, backward pass, 8-bit activation checkpoints (include/petdense.h)
-    ('petdense_forward_workspace', C.c_size_t, [C.POINTER(PetdenseForwardArgs)]),
-    ('petdense_forward', C.c_int, [C.POINTER(PetdenseForwardArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
-    ('petdense_backward_workspace', C.c_size_t, [C.POINTER(PetdenseBackwardArgs)]),
-    ('petdense_backward', C.c_int, [C.POINTER(PetdenseBackwardArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    # the arguments: byref of the struct, or its bytes
+    ('petdense_forward_workspace', C.c_size_t, [C.c_void_p]),
+    ('petdense_forward', C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    ('petdense_backward_workspace', C.c_size_t, [C.c_void_p]),
+    ('petdense_backward', C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     ('petdense_checkpoint', C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_int64,
                                       C.c_void_p, C.c_int64, C.c_void_p]),
     ('petdense_restore', C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int,

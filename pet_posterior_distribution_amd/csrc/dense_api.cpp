@@ -41,38 +41,100 @@ int size_of(int dtype) { return dtype == PETDENSE_F32 ? 4 : 2; }
 struct Plan {
   int tile = kSmall, splits = 1, c_per = 0;
   size_t part_bytes = 0;
+  double us = 0;           // estimate
 };
 
-// Tile and split of a product, by an estimate of its time in clocks of a compute unit.
+// What a kind of tile costs, in microseconds, as measured on products of 64 .. 12288 rows.  A step (128 bytes of
+// contraction) takes `wait` when its workgroup has a compute unit to itself, and `share` per workgroup when several
+// fill it; `ends` is a workgroup's first load and its epilogue.  [operands by DMA, operands through registers]
+struct Cost {
+  int tile, b, slots, k;   // b: rows and columns of the tile; slots: workgroups of a compute unit; k: steps at a time
+  double wait[2], share[2], ends;
+};
+constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.45, 1.45}, {1.45, 1.45}, 8.0},
+                             {kMid, 128, 2, 1, {0.65, 1.0}, {0.46, 0.8}, 3.5},
+                             {kSmall, 64, 4, 1, {0.28, 0.5}, {0.19, 0.3}, 2.0},
+                             {kSlice, 32, 1, 8, {0.7, 0.9}, {0.7, 0.9}, 2.5}};
+constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 6.9}, {6.9, 6.9}, 10.0},
+                             {kMid, 128, 2, 1, {2.3, 2.5}, {2.1, 2.3}, 4.0},
+                             {kSmall, 64, 4, 1, {0.65, 0.8}, {0.53, 0.65}, 2.0},
+                             {kSlice, 32, 1, 8, {1.2, 1.4}, {1.2, 1.4}, 2.5}};
+constexpr double kLaunch = 2.5;      // a launch behind another
+constexpr int kUnits = 256;
+
+double step_us(const Cost& c, double per_unit, int loader) {
+  return std::max(c.wait[loader], c.share[loader] * per_unit);
+}
+
+double product_us(const Cost& c, int64_t groups, int64_t steps, int loader) {
+  const double per = (double)ceil_div(steps, c.k);
+  const int64_t whole = groups / (kUnits * c.slots), rest = groups % (kUnits * c.slots);
+  double t = kLaunch + whole * (per * step_us(c, c.slots, loader) + c.ends);
+  if (rest) t += per * step_us(c, (double)ceil_div(rest, kUnits), loader) + c.ends;
+  return t;
+}
+
+double join_us(int64_t I, int64_t J, int64_t splits) {
+  return splits > 1 ? kLaunch + 1.0 + (double)I * J * (splits + 1) * 4 / 3.5e6 : 0.0;
+}
+
+// Splits of `steps` into equal parts (the last may be shorter), few to many.
+template <typename F>
+void for_splits(int64_t steps, int64_t most, F f) {
+  for (int64_t s = 1; s <= most && s <= steps; s = s < 4 ? s + 1 : s * 5 / 4) {
+    const int64_t per = ceil_div(steps, s);
+    if (ceil_div(steps, per) == s) f(s, per);
+  }
+}
+
+void set_plan(Plan& p, const Cost& c, int64_t splits, int64_t per, int bc, int64_t I, int64_t J) {
+  p.tile = c.tile;
+  p.splits = (int)splits;
+  p.c_per = (int)std::min<int64_t>(per * bc, kMaxDim);
+  p.part_bytes = splits > 1 ? up((size_t)splits * I * J * 4) : 0;
+}
+
+// Tile and split of a product by their estimated time.
 Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
-  struct Kind { int t, b, slots; double step; } kinds[] = {
-      // slots: workgroups of a compute unit at once (LDS and registers); step: clocks of one step of all of them
-      {kLarge, 256, 1, 2600}, {kMid, 128, 2, 1500}, {kSmall, 64, 4, 1000}};
   const int bc = type == kF32 ? 32 : 64;
-  const double slow = type == kF32 ? 8.0 : 1.0;
   const int64_t steps = ceil_div(C, bc);
   Plan best;
-  double best_t = 0;
-  for (const Kind& k : kinds) {
-    if (k.t == kLarge && loader != kDma) continue;
-    const int64_t tiles = ceil_div(I, k.b) * ceil_div(J, k.b);
-    for (int64_t s = 1; s <= 64 && s <= steps; s = s < 4 ? s + 1 : s * 5 / 4) {
-      const int64_t per = ceil_div(steps, s), parts = ceil_div(steps, per);
-      if (parts != s) continue;
-      const int64_t waves = ceil_div(tiles * s, 256 * k.slots);
-      // a last, partly filled wave of workgroups shares its compute units with fewer others
-      const double fill = waves > 1 ? 1.0 : std::min(1.0, 0.35 + 0.65 * (double)tiles * s / (256.0 * k.slots));
-      double t = (double)waves * ((double)per * k.step * slow * fill + 3000);
-      if (s > 1) t += 9000 + (double)I * J * (s + 1) * 4 / 1600;
-      if (best.c_per == 0 || t < best_t) {
-        best_t = t;
-        best.tile = k.t;
-        best.splits = (int)s;
-        best.c_per = (int)std::min<int64_t>(per * bc, kMaxDim);
-      }
-    }
+  for (const Cost& c : type == kF32 ? kCosts32 : kCosts16) {
+    if (c.tile == kLarge && loader != kDma) continue;
+    const int64_t tiles = ceil_div(I, c.b) * ceil_div(J, c.b);
+    for_splits(steps, 64, [&](int64_t s, int64_t per) {
+      const double t = product_us(c, tiles * s, per, loader) + join_us(I, J, s);
+      if (best.c_per && t >= best.us) return;
+      best.us = t;
+      set_plan(best, c, s, per, bc, I, J);
+    });
   }
-  best.part_bytes = best.splits > 1 ? up((size_t)best.splits * I * J * 4) : 0;
+  return best;
+}
+
+// The backward pass's two products as one launch (x: I = m, J = k, C = n; k: I = k, J = n, C = m), both with the same
+// kind of tile; only the kernel gradient's contraction is split.
+double plan_pair(int64_t m, int64_t k, int64_t n, int type, int lx, int lk, Plan& px, Plan& pk) {
+  const int bc = type == kF32 ? 32 : 64;
+  const int64_t sx = ceil_div(n, bc), sk = ceil_div(m, bc);
+  double best = -1;
+  for (const Cost& c : type == kF32 ? kCosts32 : kCosts16) {
+    if (c.tile != kSmall && c.tile != kSlice) continue;
+    const int64_t tx = ceil_div(m, c.b) * ceil_div(k, c.b), tk = ceil_div(k, c.b) * ceil_div(n, c.b);
+    if (tx > 16384 || tk > 16384) continue;
+    for_splits(sk, 64, [&](int64_t s, int64_t per) {
+      const double wx = (double)ceil_div(sx, c.k), wk = (double)ceil_div(per, c.k);
+      const double groups = (double)(tx + tk * s);
+      const double share = ((double)tx * (wx * c.share[lx] + c.ends / c.slots) +
+                            (double)tk * s * (wk * c.share[lk] + c.ends / c.slots)) / kUnits;
+      const double longest = std::max(wx * c.wait[lx], wk * c.wait[lk]) + c.ends;
+      const double t = kLaunch + std::max(longest, share * (groups > kUnits * c.slots ? 1.1 : 1.0)) + join_us(k, n, s);
+      if (best >= 0 && t >= best) return;
+      best = t;
+      set_plan(px, c, 1, sx, bc, m, k);
+      set_plan(pk, c, s, per, bc, k, n);
+    });
+  }
   return best;
 }
 
@@ -81,10 +143,16 @@ bool dma_ok(const void* p, int64_t ld, int64_t contiguous, int size) {
          ld * size < (int64_t)0x7fffffff / 256;          // a tile's offsets fit 31 bits
 }
 
-int run_product(Product p, int layout, int loader, int type, int q8, const Plan& pl, void* part, hipStream_t s) {
+Product placed(Product p, const Plan& pl, void* part) {
   p.splits = pl.splits;
   p.c_per = pl.c_per;
   p.part = static_cast<float*>(part);
+  return p;
+}
+
+int run_product(const Product& of, int layout, int loader, int type, int q8, const Plan& pl, void* part,
+                hipStream_t s) {
+  const Product p = placed(of, pl, part);
   HIPC(type == kF32    ? product_f32(p, layout, loader, pl.tile, q8, s)
        : type == kBF16 ? product_bf16(p, layout, loader, pl.tile, q8, s)
                        : product_f16(p, layout, loader, pl.tile, q8, s));
@@ -167,6 +235,7 @@ struct BackwardPlan {
   bool sums;               // column sums wanted
   int chunks;
   Plan px, pk;
+  bool pair;               // one launch for both products and the bias gradient's join
   int load_x, load_k;
   size_t o_dp, o_sums, o_part, bytes;
 };
@@ -208,6 +277,15 @@ BackwardPlan plan_backward(const petdense_backward_args* a, void* work) {
     // 8-bit inputs go through registers whatever their alignment: `loader` is dp's
     b.load_k = dma_ok(base, b.lddp, a->n, sz) && (a->x_exponents || dma_ok(a->x, a->ldx, a->k, sz)) ? kDma : kReg;
     b.pk = plan(a->k, a->n, a->m, a->dtype, b.load_k);
+  }
+  if (a->dx && a->dkernel) {
+    Plan px, pk;
+    const double t = plan_pair(a->m, a->k, a->n, a->dtype, b.load_x, b.load_k, px, pk);
+    if (t >= 0 && t < b.px.us + b.pk.us + (b.sums ? kLaunch : 0.0)) {
+      b.pair = true;
+      b.px = px;
+      b.pk = pk;
+    }
   }
   b.o_part = o;
   b.bytes = o + std::max(b.px.part_bytes, b.pk.part_bytes);
@@ -268,37 +346,50 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     HIPC(act_grad(a->dy, a->lddy, a->activation == PETDENSE_NONE ? nullptr : a->saved, a->lds,
                   b.make_dp ? const_cast<void*>(b.dp) : nullptr, b.lddp, sums, b.chunks, (int)a->m, (int)a->n, a->dtype,
                   a->activation, s));
-  if (b.sums) HIPC(join_columns(sums, b.chunks, (int)a->n, a->dbias, a->grad_f32 ? kF32 : a->dtype, s));
+  const ColumnJoin cols{sums, a->dbias, b.chunks, b.sums ? (int)a->n : 0, a->grad_f32 ? kF32 : a->dtype};
+  Product x{}, k{};
   if (a->dx) {
-    Product p{};
-    p.A = b.dp;
-    p.lda = b.lddp;
-    p.B = a->kernel;
-    p.ldb = a->ldk;
-    p.I = (int)a->m;
-    p.J = (int)a->k;
-    p.C = (int)a->n;
-    p.e.out = a->dx;
-    p.e.ldo = a->lddx;
-    if (int r = run_product(p, kInputGrad, b.load_x, a->dtype, 0, b.px, w + b.o_part, s)) return r;
+    x.A = b.dp;
+    x.lda = b.lddp;
+    x.B = a->kernel;
+    x.ldb = a->ldk;
+    x.I = (int)a->m;
+    x.J = (int)a->k;
+    x.C = (int)a->n;
+    x.e.out = a->dx;
+    x.e.ldo = a->lddx;
   }
   if (a->dkernel) {
-    Product p{};
-    p.A = a->x;
-    p.lda = a->ldx;
-    p.exps = a->x_exponents;
-    p.lde = a->lde;
-    p.B = b.dp;
-    p.ldb = b.lddp;
-    p.I = (int)a->k;
-    p.J = (int)a->n;
-    p.C = (int)a->m;
-    p.e.out = a->dkernel;
-    p.e.ldo = a->lddk;
-    p.e.out_f32 = a->grad_f32;
-    if (int r = run_product(p, kKernelGrad, b.load_k, a->dtype, a->x_exponents != nullptr, b.pk, w + b.o_part, s))
-      return r;
+    k.A = a->x;
+    k.lda = a->ldx;
+    k.exps = a->x_exponents;
+    k.lde = a->lde;
+    k.B = b.dp;
+    k.ldb = b.lddp;
+    k.I = (int)a->k;
+    k.J = (int)a->n;
+    k.C = (int)a->m;
+    k.e.out = a->dkernel;
+    k.e.ldo = a->lddk;
+    k.e.out_f32 = a->grad_f32;
   }
+  const int q8 = a->x_exponents != nullptr;
+  if (b.pair) {
+    Pair p{};
+    p.x = placed(x, b.px, nullptr);
+    p.k = placed(k, b.pk, w + b.o_part);
+    p.cols = cols;
+    HIPC(a->dtype == kF32    ? pair_f32(p, b.load_x, b.load_k, b.px.tile, q8, s)
+         : a->dtype == kBF16 ? pair_bf16(p, b.load_x, b.load_k, b.px.tile, q8, s)
+                             : pair_f16(p, b.load_x, b.load_k, b.px.tile, q8, s));
+    if (b.pk.splits > 1) HIPC(join(p.k, a->dtype, s));
+    return PETDIFF_OK;
+  }
+  if (b.sums) HIPC(join_columns(cols, s));
+  if (a->dx)
+    if (int r = run_product(x, kInputGrad, b.load_x, a->dtype, 0, b.px, w + b.o_part, s)) return r;
+  if (a->dkernel)
+    if (int r = run_product(k, kKernelGrad, b.load_k, a->dtype, q8, b.pk, w + b.o_part, s)) return r;
   return PETDIFF_OK;
 }
 

@@ -133,6 +133,27 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, int64_t i, int64_t 
   else store_row<T, 8>(static_cast<T*>(e.out) + i * e.ldo + j, n, v);
 }
 
+// Sums 16 columns of a column join: thread t < 256 takes column t % 16 of the chunks t / 16, t / 16 + 16, ..; the 16
+// groups meet in LDS, in order.  Every thread of the workgroup comes here.
+__device__ __forceinline__ void join_columns16(const ColumnJoin& p, int block, int t, float* red) {
+  const int c = t & 15, g = t >> 4, j = block * 16 + c;
+  float v = 0.f;
+  if (t < 256 && j < p.N) {
+#pragma unroll 8
+    for (int k = g; k < p.chunks; k += 16) v += p.part[(int64_t)k * p.N + j];
+  }
+  if (t < 256) red[t] = v;
+  __syncthreads();
+  if (g == 0 && j < p.N) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += red[k * 16 + c];
+    if (p.out_type == kF32) static_cast<float*>(p.out)[j] = s;
+    else if (p.out_type == kBF16) static_cast<__bf16*>(p.out)[j] = (__bf16)s;
+    else static_cast<_Float16*>(p.out)[j] = (_Float16)s;
+  }
+}
+
 // e4m3 codes of a word's four bytes times 2^E (`scale`) as two packed words of T; exact for the blocks the checkpoint
 // writes (four significant bits, E >= -117, no value past T's largest), except that fp16 rounds what is below 2^-14.
 template <typename T>

@@ -36,12 +36,31 @@ struct Product {
 
 enum Layout { kForward = 0, kInputGrad = 1, kKernelGrad = 2 };   // (A, B): (c-, j-), (c-, c-), (i-, j-contiguous)
 enum Loader { kDma = 0, kReg = 1 };
-enum Tile { kLarge = 0, kMid = 1, kSmall = 2 };
+enum Tile { kLarge = 0, kMid = 1, kSmall = 2, kSlice = 3 };
+
+// out[n] = sum over chunks of part[chunk][n], in order
+struct ColumnJoin {
+  const float* part;
+  void* out;
+  int chunks, N;         // N = 0: nothing to join
+  int out_type;
+};
+
+// The backward pass's products and its bias gradient as one launch (kSmall, kSlice).
+struct Pair {
+  Product x, k;
+  ColumnJoin cols;
+  int tx, tk, nx, nk;    // tiles and workgroups of each (the launcher's)
+};
 
 // One launch of the tiled product: `q8`: A is e4m3 codes with exponent bytes (kKernelGrad only).
 hipError_t product_f32(const Product& p, int layout, int loader, int tile, int q8, hipStream_t s);
 hipError_t product_bf16(const Product& p, int layout, int loader, int tile, int q8, hipStream_t s);
 hipError_t product_f16(const Product& p, int layout, int loader, int tile, int q8, hipStream_t s);
+
+hipError_t pair_f32(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s);
+hipError_t pair_bf16(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s);
+hipError_t pair_f16(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s);
 
 // Joins split products: the sum of p.part over the splits, in order, through the epilogue.
 hipError_t join(const Product& p, int type, hipStream_t s);
@@ -53,8 +72,7 @@ hipError_t rows(const Product& p, int type, hipStream_t s);
 // dp = dy act'(saved) (dp may be null), part[chunk][n] = column sums of dp over the chunk's rows (may be null)
 hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, float* part,
                     int chunks, int M, int N, int type, int act, hipStream_t s);
-// out[n] = sum over chunks of part[chunk][n], in order
-hipError_t join_columns(const float* part, int chunks, int N, void* out, int out_type, hipStream_t s);
+hipError_t join_columns(const ColumnJoin& c, hipStream_t s);
 
 // rows x n values of `size` bytes (row stride ld) become zero; a kernel, so that a graph can hold it
 hipError_t fill_zero(void* p, int64_t rows, int n, int64_t ld, int size, hipStream_t s);

@@ -190,24 +190,9 @@ hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t ld
   return hipGetLastError();
 }
 
-// 16 columns by 16 groups of chunks a block: group g sums chunks g, g + 16, ..; the groups meet in LDS, in order.
-template <typename T>
-__global__ __launch_bounds__(256) void join_columns_kernel(const float* part, int chunks, int N, T* out) {
-  __shared__ float red[16][16];
-  const int c = threadIdx.x & 15, g = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
-  float v = 0.f;
-  if (j < N) {
-#pragma unroll 8
-    for (int k = g; k < chunks; k += 16) v += part[(int64_t)k * N + j];
-  }
-  red[g][c] = v;
-  __syncthreads();
-  if (g == 0 && j < N) {
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) s += red[k][c];
-    out[j] = (T)s;
-  }
+__global__ __launch_bounds__(256) void join_columns_kernel(ColumnJoin p) {
+  __shared__ float red[256];
+  join_columns16(p, blockIdx.x, threadIdx.x, red);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -345,10 +330,9 @@ hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds,
   PETDENSE_BY_TYPE(type, return act_grad_t<T>(dy, ldy, saved, lds, dp, ldd, part, chunks, M, N, act, s))
 }
 
-hipError_t join_columns(const float* part, int chunks, int N, void* out, int out_type, hipStream_t s) {
-  PETDENSE_BY_TYPE(out_type, hipLaunchKernelGGL((join_columns_kernel<T>), dim3(blocks_for(N, 16)), dim3(256), 0, s,
-                                                part, chunks, N, static_cast<T*>(out));
-                   return hipGetLastError())
+hipError_t join_columns(const ColumnJoin& c, hipStream_t s) {
+  hipLaunchKernelGGL(join_columns_kernel, dim3(blocks_for(c.N, 16)), dim3(256), 0, s, c);
+  return hipGetLastError();
 }
 
 __global__ __launch_bounds__(256) void fill_zero_kernel(char* p, int64_t total, int n, int64_t ld, int size) {

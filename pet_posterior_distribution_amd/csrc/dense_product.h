@@ -23,6 +23,7 @@
 #pragma once
 #include "dense_epilogue.h"
 
+#include <atomic>
 #include <type_traits>
 
 namespace petdense_k {
@@ -72,14 +73,21 @@ struct Frag<_Float16> { typedef f16x8 type; };
 template <>
 struct Frag<float> { typedef f32x4 type; };
 
-template <typename T>
-__device__ __forceinline__ f32x4 multiply(typename Frag<T>::type a, typename Frag<T>::type b, f32x4 c) {
-  if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  else if constexpr (__is_same(T, _Float16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  else {
+// acc[y] += b[y] a: one row of a wave's 16 x 16 tiles.  fp32: the four instructions of a product are spread over the
+// row, so that none waits for the one before it.
+template <typename T, int N>
+__device__ __forceinline__ void multiply_row(const typename Frag<T>::type* b, typename Frag<T>::type a, f32x4* acc) {
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[q], b[q], c, 0, 0, 0);
-    return c;
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int y = 0; y < N; ++y) acc[y] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[y][q], a[q], acc[y], 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int y = 0; y < N; ++y) {
+      if constexpr (__is_same(T, __bf16)) acc[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[y], a, acc[y], 0, 0, 0);
+      else acc[y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b[y], a, acc[y], 0, 0, 0);
+    }
   }
 }
 
@@ -118,9 +126,10 @@ __device__ __forceinline__ typename Frag<T>::type fragment(const char* st, int r
 // Fills stages of one operand.  `c0` is the operand's first contraction value, `clen` the values of this part.
 // LOADER kDma: rows and row starts are multiples of 16 bytes: buffer loads that write LDS themselves; a piece outside
 //   the operand gets an offset past the buffer's end, and the hardware writes zeros for it.
-// LOADER kReg: any alignment: through registers, loaded before the step's products and stored after them.
+// LOADER kReg: any alignment: through registers, loaded a step ahead and stored after the step's first group.
 // Q8: the operand is e4m3 codes with exponent bytes, free-contiguous: through registers, restored to T on the way.
-template <typename T, bool FREE, int R, int BC, int THREADS, int LOADER, bool Q8>
+// KW > 1: the filler's wave takes every KW-th step, from step `kw`.
+template <typename T, bool FREE, int R, int BC, int THREADS, int KW, int LOADER, bool Q8>
 struct Filler {
   using S = Stage<T, FREE, R, BC>;
   static constexpr int N = (S::PIECES + THREADS - 1) / THREADS;      // pieces of a thread
@@ -129,14 +138,15 @@ struct Filler {
   const char* base;      // the tile's first value at contraction value 0 of this part
   int64_t ld;            // bytes from row to row
   int limit;             // free values of the tile that exist
-  int clen;
+  int clen, kw;
   const uint8_t* exps;   // Q8: exponent byte of the tile's first block at the part's first row
   int64_t lde;
   int voff[LOADER == kDma ? N : 1];
   u32x4 reg[LOADER == kDma ? 1 : N];
 
   __device__ void init(const void* p, int64_t ld_values, int f0, int f_limit, int64_t c0, int clen_,
-                       const uint8_t* ex, int64_t lde_, int tid) {
+                       const uint8_t* ex, int64_t lde_, int kw_, int tid) {
+    kw = kw_;
     constexpr int SZ = Q8 ? 1 : (int)sizeof(T);
     ld = ld_values * SZ;
     base = static_cast<const char*>(p) + (FREE ? c0 * ld + (int64_t)f0 * SZ : f0 * ld + c0 * SZ);
@@ -154,17 +164,20 @@ struct Filler {
     }
   }
 
-  // what every piece of step t needs
+  // what every piece of the t-th step needs
   struct Step {
     i32x4 rs;            // kDma: the buffer that begins at the step
     const char* p;
     int t, left;         // contraction values of the step that exist (<= 0: a step past the end loads nothing)
+    bool whole;          // kReg: no piece has to be cut
   };
   __device__ __forceinline__ Step at(int t) const {
     Step u;
-    u.t = t;
-    u.left = clen - t * BC;
-    u.p = base + (FREE ? (int64_t)t * BC * ld : (int64_t)t * BC * (int64_t)sizeof(T));
+    u.t = KW > 1 ? t * KW + kw : t;
+    u.left = clen - u.t * BC;
+    u.p = base + (FREE ? (int64_t)u.t * BC * ld : (int64_t)u.t * BC * (int64_t)sizeof(T));
+    // free-contiguous: 16 bytes from a piece's first value may run into the next row, which then has to exist
+    u.whole = FREE ? u.left > BC && ld >= 16 : u.left >= BC;
     if constexpr (LOADER == kDma) {
       const unsigned long long a = reinterpret_cast<unsigned long long>(u.p);
       u.rs[0] = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffull));
@@ -175,33 +188,54 @@ struct Filler {
     return u;
   }
 
-  // begins the load of the thread's piece q of a step (kDma: into `st`)
+  // begins the load of the thread's piece q of a step into LDS at `st`
   __device__ __forceinline__ void begin(char* st, const Step& u, int q, int tid) {
-    const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
     if constexpr (LOADER == kDma) {
+      const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
       const int o = (FREE ? r >= u.left : c * S::EPC >= u.left) ? (int)0x80000000 : voff[q];
       load_to_lds(u.rs, (unsigned)(uintptr_t)(PETDENSE_LDS char*)st + (q * THREADS + wave * 64) * 16, o);
-    } else {
-      // values of the piece that exist
-      const int n = FREE ? (r < u.left ? limit - c * S::EPC : 0) : (r < limit ? u.left - c * S::EPC : 0);
-      reg[q] = u32x4{0, 0, 0, 0};
-      if constexpr (Q8) {
-        const char* s = u.p + r * ld + c * S::EPC;
-        unsigned w[2] = {0, 0};
-        if (n >= S::EPC) __builtin_memcpy(w, s, S::EPC);
-        else
-          for (int v = 0; v < n; ++v) w[v >> 2] |= (unsigned)(uint8_t)s[v] << ((v & 3) * 8);
-        // a piece past the end keeps no exponent: its codes are zero
-        const unsigned b = n > 0 ? exps[((int64_t)u.t * BC + r) * lde + (c * S::EPC) / 32] : 127;
-        reg[q][0] = w[0];
-        reg[q][1] = w[1];
-        reg[q][2] = b;
-      } else {
-        const char* s = u.p + r * ld + c * 16;
-        if (n >= S::EPC) {
-          __builtin_memcpy(&reg[q], s, 16);
-        } else if (n > 0) {
+    }
+  }
+
+  // begins the loads of a step into registers.  Whole steps load without a branch: pieces past the operand's free
+  // end read its first value instead (they feed outputs that are not stored).
+  __device__ __forceinline__ void begin_reg(const Step& u, int tid) {
+    if constexpr (LOADER == kReg) {
+      constexpr int PB = Q8 ? S::EPC : 16;              // bytes of a piece in memory
+      if (u.whole) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+          const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
+          const int rr = FREE ? r : min(r, limit - 1), cc = FREE && c * S::EPC >= limit ? 0 : c;
+          const char* s = u.p + (int64_t)rr * ld + cc * PB;
+          if constexpr (Q8) {
+            unsigned w[2] = {0, 0};
+            __builtin_memcpy(w, s, PB);
+            reg[q][0] = w[0];
+            reg[q][1] = w[1];
+            reg[q][2] = exps[((int64_t)u.t * BC + r) * lde + (cc * S::EPC) / 32];
+          } else {
+            __builtin_memcpy(&reg[q], s, 16);
+          }
+        }
+        return;
+      }
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
+        // values of the piece that exist
+        const int n = FREE ? (r < u.left ? limit - c * S::EPC : 0) : (r < limit ? u.left - c * S::EPC : 0);
+        const char* s = u.p + (int64_t)r * ld + c * PB;
+        if constexpr (Q8) {
+          unsigned w[2] = {0, 0};
+#pragma unroll
+          for (int v = 0; v < S::EPC; ++v)
+            if (v < n) w[v >> 2] |= (unsigned)(uint8_t)s[v] << ((v & 3) * 8);
+          reg[q][0] = w[0];
+          reg[q][1] = w[1];
+          reg[q][2] = n > 0 ? exps[((int64_t)u.t * BC + r) * lde + (c * S::EPC) / 32] : 127;
+        } else {
           T v[S::EPC];
 #pragma unroll
           for (int x = 0; x < S::EPC; ++x) {
@@ -213,10 +247,12 @@ struct Filler {
       }
     }
   }
+
   __device__ __forceinline__ void begin_all(char* st, int t, int tid) {
     const Step u = at(t);
 #pragma unroll
     for (int q = 0; q < N; ++q) begin(st, u, q, tid);
+    begin_reg(u, tid);
   }
 
   // ends them: kReg: writes the registers to `st`
@@ -238,18 +274,28 @@ struct Filler {
   }
 };
 
-// All but the last N of this wave's loads have landed, its LDS accesses are done; then a bare barrier.
-template <int N>
+// All but the last N of this wave's loads have landed, its LDS accesses are done; then, where waves share stages, a
+// bare barrier.
+template <int N, bool SHARED>
 __device__ __forceinline__ void step_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+  if constexpr (SHARED) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+  else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ, bool FA, bool FB, int LA, int LB, bool Q8>
-struct Shape {
-  static constexpr int BC = 128 / (int)sizeof(T);
-  static constexpr int THREADS = WI * WJ * 64;
-  static constexpr int LDS = 2 * (Stage<T, FA, BI, BC>::BYTES + Stage<T, FB, BJ, BC>::BYTES);
+// A kind of tile: BI x BJ outputs, by WI x WJ waves that share the stages; or (KW > 1) by KW waves that each multiply
+// the whole tile over every KW-th step, from stages of their own, and meet at the end: for few outputs with a long
+// contraction, where one wave after another would wait for memory.
+template <int BI_, int BJ_, int WI_, int WJ_, int KW_>
+struct Kind {
+  static constexpr int BI = BI_, BJ = BJ_, WI = WI_, WJ = WJ_, KW = KW_;
+  static constexpr int THREADS = WI * WJ * KW * 64;
+  static constexpr int LDS = 2 * KW * (BI + BJ) * 128;
+  static_assert(KW == 1 || WI * WJ == 1, "");
 };
+typedef Kind<256, 256, 2, 4, 1> Large;
+typedef Kind<128, 128, 2, 2, 1> Mid;
+typedef Kind<64, 64, 2, 2, 1> Small;
+typedef Kind<32, 32, 1, 1, 8> Slice;
 
 // Workgroup -> tile.  Neighbouring workgroup numbers go to different XCDs, each with its own L2: every XCD gets a
 // contiguous run of tiles, and a run walks bands of 4 tile rows, so that the workgroups an XCD runs together share
@@ -264,28 +310,34 @@ __device__ __forceinline__ void tile_of(int b, int ti, int tj, int& i, int& j) {
   j = r / h;
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ, bool FA, bool FB, int LA, int LB, bool Q8>
-__global__ __launch_bounds__(WI* WJ * 64) void product_kernel(Product p) {
-  using SH = Shape<T, BI, BJ, WI, WJ, FA, FB, LA, LB, Q8>;
-  constexpr int BC = SH::BC, THREADS = SH::THREADS;
+template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8>
+__device__ __forceinline__ void product_body(const Product& p, int block, int split, char* lds) {
+  constexpr int BI = K::BI, BJ = K::BJ, WI = K::WI, WJ = K::WJ, KW = K::KW;
+  constexpr int BC = 128 / (int)sizeof(T);
+  constexpr bool SHARED = KW == 1;
+  constexpr int THREADS = WI * WJ * 64;                 // that share a stage
   using SA = Stage<T, FA, BI, BC>;
   using SB = Stage<T, FB, BJ, BC>;
   constexpr int STAGE = SA::BYTES + SB::BYTES;
+  static_assert(2 * KW * STAGE == K::LDS, "");
   constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16, KS = 2;
-  extern __shared__ char lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wi = wave / WJ, wj = wave % WJ;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tid = SHARED ? threadIdx.x : lane;
+  const int wi = SHARED ? wave / WJ : 0, wj = SHARED ? wave % WJ : 0;
+  const int kw = SHARED ? 0 : __builtin_amdgcn_readfirstlane(wave);
+  char* mine = lds + kw * 2 * STAGE;
   int ti, tj;
-  tile_of(blockIdx.x, (p.I + BI - 1) / BI, (p.J + BJ - 1) / BJ, ti, tj);
+  tile_of(block, (p.I + BI - 1) / BI, (p.J + BJ - 1) / BJ, ti, tj);
   const int i0 = ti * BI, j0 = tj * BJ;
-  const int64_t c0 = (int64_t)blockIdx.y * p.c_per;
+  const int64_t c0 = (int64_t)split * p.c_per;
   const int clen = (int)min((int64_t)p.c_per, p.C - c0);
-  const int steps = (clen + BC - 1) / BC;
+  // steps of this wave; one at least, which finds nothing past the end
+  const int steps = SHARED ? (clen + BC - 1) / BC : max(1, ((clen + BC - 1) / BC - kw + KW - 1) / KW);
 
-  Filler<T, FA, BI, BC, THREADS, LA, Q8> fa;
-  Filler<T, FB, BJ, BC, THREADS, LB, false> fb;
-  fa.init(p.A, p.lda, i0, p.I, c0, clen, p.exps, p.lde, tid);
-  fb.init(p.B, p.ldb, j0, p.J, c0, clen, nullptr, 0, tid);
+  Filler<T, FA, BI, BC, THREADS, KW, LA, Q8> fa;
+  Filler<T, FB, BJ, BC, THREADS, KW, LB, false> fb;
+  fa.init(p.A, p.lda, i0, p.I, c0, clen, p.exps, p.lde, kw, tid);
+  fb.init(p.B, p.ldb, j0, p.J, c0, clen, nullptr, 0, kw, tid);
 
   f32x4 acc[FI][FJ];
 #pragma unroll
@@ -311,6 +363,10 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(Product p) {
 #pragma unroll
     for (int x = 0; x < FI; ++x) {
       if constexpr (decltype(loads)::value) {
+        if (x == 0) {
+          fa.begin_reg(ua, tid);
+          fb.begin_reg(ub, tid);
+        }
 #pragma unroll
         for (int q = 0; q < NA; ++q)
           if (q * FI / NA == x) fa.begin(ld, ua, q, tid);
@@ -323,30 +379,29 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(Product p) {
         for (int f = 0; f < READS; ++f)
           if (f * ROWS / READS == x) read(rd, kn, f);
       }
-#pragma unroll
-      for (int y = 0; y < FJ; ++y) acc[x][y] = multiply<T>(b[ks][y], a[ks][x], acc[x][y]);
+      multiply_row<T, FJ>(b[ks], a[ks][x], acc[x]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  fa.begin_all(lds, 0, tid);
-  fb.begin_all(lds + SA::BYTES, 0, tid);
-  fa.end(lds, tid);
-  fb.end(lds + SA::BYTES, tid);
-  fa.begin_all(lds + STAGE, 1, tid);
-  fb.begin_all(lds + STAGE + SA::BYTES, 1, tid);
-  step_barrier<(LA == kDma ? NA : 0) + (LB == kDma ? NB : 0)>();
+  fa.begin_all(mine, 0, tid);
+  fb.begin_all(mine + SA::BYTES, 0, tid);
+  fa.end(mine, tid);
+  fb.end(mine + SA::BYTES, tid);
+  fa.begin_all(mine + STAGE, 1, tid);
+  fb.begin_all(mine + STAGE + SA::BYTES, 1, tid);
+  step_barrier<(LA == kDma ? NA : 0) + (LB == kDma ? NB : 0), SHARED>();
 #pragma unroll
-  for (int f = 0; f < READS; ++f) read(lds, 0, f);
-  char* cur = lds;
-  char* nxt = lds + STAGE;
+  for (int f = 0; f < READS; ++f) read(mine, 0, f);
+  char* cur = mine;
+  char* nxt = mine + STAGE;
   for (int t = 0; t + 1 < steps; ++t) {
     const auto ua = fa.at(t + 2);
     const auto ub = fb.at(t + 2);
     group(0, 1, yes, cur, no, nullptr, ua, ub);
     fa.end(nxt, tid);
     fb.end(nxt + SA::BYTES, tid);
-    step_barrier<0>();
+    step_barrier<0, SHARED>();
     group(1, 0, yes, nxt, yes, cur, ua, ub);
     char* s = cur;
     cur = nxt;
@@ -365,19 +420,44 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(Product p) {
   // c of row r at place c ^ r), so that a lane gets eight neighbouring outputs of a row and a row's lanes touch whole
   // cache lines.
   __syncthreads();
+  Epilogue e = p.e;
+  if (p.splits > 1) {
+    e = Epilogue{};
+    e.out = p.part + (int64_t)split * p.I * p.J;
+    e.ldo = p.J;
+    e.out_f32 = 1;
+  }
+  const int g = lane >> 4, il = lane & 15;
+  if constexpr (!SHARED) {
+    // every wave's sums of the whole tile, then one octet of outputs a thread: the waves' parts added in order
+    constexpr int PIECES = BJ / 4, MASK = PIECES < 16 ? PIECES - 1 : 15, PLANE = BI * BJ * 4;
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+      for (int y = 0; y < FJ; ++y)
+        *reinterpret_cast<f32x4*>(lds + kw * PLANE + ((x * 16 + il) * PIECES + ((y * 4 + g) ^ (il & MASK))) * 16) =
+            acc[x][y];
+    __syncthreads();
+    for (int k = threadIdx.x; k < BI * (BJ / 8); k += K::THREADS) {
+      const int r = k / (BJ / 8), c = (k % (BJ / 8)) * 2, key = r & MASK, i = i0 + r, j = j0 + c * 4;
+      f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        lo += *reinterpret_cast<const f32x4*>(lds + w * PLANE + (r * PIECES + (c ^ key)) * 16);
+        hi += *reinterpret_cast<const f32x4*>(lds + w * PLANE + (r * PIECES + ((c + 1) ^ key)) * 16);
+      }
+      if (i < p.I && j < p.J) {
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        epilogue8<T>(e, i, j, p.J - j, v);
+      }
+    }
+    return;
+  } else {
   constexpr int TJ = BJ / WJ, PIECES = TJ / 4, MASK = PIECES < 16 ? PIECES - 1 : 15;
   constexpr int ROWS_FIT = STAGE * 2 / (WI * WJ) / (16 * TJ * 4);
   constexpr int ROWS_AT = ROWS_FIT < FI ? ROWS_FIT : FI;
   static_assert(ROWS_FIT >= 1 && FI % ROWS_AT == 0, "the tile's rows pass through LDS in equal parts");
-  Epilogue e = p.e;
-  if (p.splits > 1) {
-    e = Epilogue{};
-    e.out = p.part + (int64_t)blockIdx.y * p.I * p.J;
-    e.ldo = p.J;
-    e.out_f32 = 1;
-  }
   char* own = lds + wave * (ROWS_AT * 16 * TJ * 4);
-  const int g = lane >> 4, il = lane & 15;
 #pragma unroll
   for (int x0 = 0; x0 < FI; x0 += ROWS_AT) {
 #pragma unroll
@@ -399,48 +479,113 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(Product p) {
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
+  }
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ, bool FA, bool FB, int LA, int LB, bool Q8>
+template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8>
+__global__ __launch_bounds__(K::THREADS) void product_kernel(Product p) {
+  extern __shared__ char lds[];
+  product_body<T, K, FA, FB, LA, LB, Q8>(p, blockIdx.x, blockIdx.y, lds);
+}
+
+// The backward pass's two products and the join of its column sums as one launch: workgroups [0, nx) multiply the
+// input gradient, the next nk the kernel gradient, the others join 16 columns each.
+template <typename T, typename K, int LX, int LK, bool Q8>
+__global__ __launch_bounds__(K::THREADS) void pair_kernel(Pair p) {
+  extern __shared__ char lds[];
+  const int b = blockIdx.x;
+  if (b < p.nx) {
+    product_body<T, K, false, false, LX, LX, false>(p.x, b % p.tx, b / p.tx, lds);
+  } else if (b < p.nx + p.nk) {
+    const int d = b - p.nx;
+    product_body<T, K, true, true, Q8 ? kReg : LK, LK, Q8>(p.k, d % p.tk, d / p.tk, lds);
+  } else {
+    join_columns16(p.cols, b - p.nx - p.nk, threadIdx.x, reinterpret_cast<float*>(lds));
+  }
+}
+
+// Marks a kernel's use of more LDS than the default, once per device.
+inline hipError_t allow_lds(const void* k, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev)) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return hipSuccess;
+  if (hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  done.fetch_or(bit, std::memory_order_release);
+  return hipSuccess;
+}
+
+inline int64_t tiles_of(const Product& p, int bi, int bj) {
+  return (int64_t)((p.I + bi - 1) / bi) * ((p.J + bj - 1) / bj);
+}
+
+template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8>
 hipError_t launch(const Product& p, hipStream_t s) {
-  using SH = Shape<T, BI, BJ, WI, WJ, FA, FB, LA, LB, Q8>;
-  auto k = product_kernel<T, BI, BJ, WI, WJ, FA, FB, LA, LB, Q8>;
-  hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                     SH::LDS);
-  if (e != hipSuccess) return e;
-  const int64_t tiles = (int64_t)((p.I + BI - 1) / BI) * ((p.J + BJ - 1) / BJ);
-  hipLaunchKernelGGL(k, dim3((unsigned)tiles, (unsigned)p.splits), dim3(SH::THREADS), SH::LDS, s, p);
+  static std::atomic<uint64_t> done{0};
+  auto k = product_kernel<T, K, FA, FB, LA, LB, Q8>;
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
+  hipLaunchKernelGGL(k, dim3((unsigned)tiles_of(p, K::BI, K::BJ), (unsigned)p.splits), dim3(K::THREADS), K::LDS, s, p);
   return hipGetLastError();
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ>
-hipError_t product_tile(const Product& p, int layout, int loader, int q8, hipStream_t s) {
-  if constexpr (BI == 256) {      // the plan takes the largest tile only for operands that DMA can stage
+template <typename T, typename K, int LX, int LK, bool Q8>
+hipError_t launch_pair(Pair p, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  auto k = pair_kernel<T, K, LX, LK, Q8>;
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
+  p.tx = (int)tiles_of(p.x, K::BI, K::BJ);
+  p.tk = (int)tiles_of(p.k, K::BI, K::BJ);
+  p.nx = p.tx * p.x.splits;
+  p.nk = p.tk * p.k.splits;
+  hipLaunchKernelGGL(k, dim3((unsigned)(p.nx + p.nk + (p.cols.N + 15) / 16)), dim3(K::THREADS), K::LDS, s, p);
+  return hipGetLastError();
+}
+
+template <typename T, typename K>
+hipError_t product_kind(const Product& p, int layout, int loader, int q8, hipStream_t s) {
+  if constexpr (K::BI == 256) {      // the plan takes the largest tile only for operands that DMA can stage
     if (loader != kDma) return hipErrorInvalidValue;
-    if (layout == kForward) return launch<T, BI, BJ, WI, WJ, false, true, kDma, kDma, false>(p, s);
-    if (layout == kInputGrad) return launch<T, BI, BJ, WI, WJ, false, false, kDma, kDma, false>(p, s);
-    return q8 ? launch<T, BI, BJ, WI, WJ, true, true, kReg, kDma, true>(p, s)
-              : launch<T, BI, BJ, WI, WJ, true, true, kDma, kDma, false>(p, s);
+    if (layout == kForward) return launch<T, K, false, true, kDma, kDma, false>(p, s);
+    if (layout == kInputGrad) return launch<T, K, false, false, kDma, kDma, false>(p, s);
+    return q8 ? launch<T, K, true, true, kReg, kDma, true>(p, s) : launch<T, K, true, true, kDma, kDma, false>(p, s);
   } else {
-  if (layout == kForward)
-    return loader == kDma ? launch<T, BI, BJ, WI, WJ, false, true, kDma, kDma, false>(p, s)
-                          : launch<T, BI, BJ, WI, WJ, false, true, kReg, kReg, false>(p, s);
-  if (layout == kInputGrad)
-    return loader == kDma ? launch<T, BI, BJ, WI, WJ, false, false, kDma, kDma, false>(p, s)
-                          : launch<T, BI, BJ, WI, WJ, false, false, kReg, kReg, false>(p, s);
-  if (q8)
-    return loader == kDma ? launch<T, BI, BJ, WI, WJ, true, true, kReg, kDma, true>(p, s)
-                          : launch<T, BI, BJ, WI, WJ, true, true, kReg, kReg, true>(p, s);
-  return loader == kDma ? launch<T, BI, BJ, WI, WJ, true, true, kDma, kDma, false>(p, s)
-                        : launch<T, BI, BJ, WI, WJ, true, true, kReg, kReg, false>(p, s);
+    if (layout == kForward)
+      return loader == kDma ? launch<T, K, false, true, kDma, kDma, false>(p, s)
+                            : launch<T, K, false, true, kReg, kReg, false>(p, s);
+    if (layout == kInputGrad)
+      return loader == kDma ? launch<T, K, false, false, kDma, kDma, false>(p, s)
+                            : launch<T, K, false, false, kReg, kReg, false>(p, s);
+    if (q8)
+      return loader == kDma ? launch<T, K, true, true, kReg, kDma, true>(p, s)
+                            : launch<T, K, true, true, kReg, kReg, true>(p, s);
+    return loader == kDma ? launch<T, K, true, true, kDma, kDma, false>(p, s)
+                          : launch<T, K, true, true, kReg, kReg, false>(p, s);
   }
 }
 
 template <typename T>
 hipError_t product(const Product& p, int layout, int loader, int tile, int q8, hipStream_t s) {
-  if (tile == kLarge) return product_tile<T, 256, 256, 2, 4>(p, layout, loader, q8, s);
-  if (tile == kMid) return product_tile<T, 128, 128, 2, 2>(p, layout, loader, q8, s);
-  return product_tile<T, 64, 64, 2, 2>(p, layout, loader, q8, s);
+  if (tile == kLarge) return product_kind<T, Large>(p, layout, loader, q8, s);
+  if (tile == kMid) return product_kind<T, Mid>(p, layout, loader, q8, s);
+  if (tile == kSmall) return product_kind<T, Small>(p, layout, loader, q8, s);
+  return product_kind<T, Slice>(p, layout, loader, q8, s);
+}
+
+template <typename T, typename K>
+hipError_t pair_kind(const Pair& p, int lx, int lk, int q8, hipStream_t s) {
+  if (q8) {
+    if (lx == kDma && lk == kDma) return launch_pair<T, K, kDma, kDma, true>(p, s);
+    if (lx != kDma && lk != kDma) return launch_pair<T, K, kReg, kReg, true>(p, s);
+    return lx == kDma ? launch_pair<T, K, kDma, kReg, true>(p, s) : launch_pair<T, K, kReg, kDma, true>(p, s);
+  }
+  if (lx == kDma && lk == kDma) return launch_pair<T, K, kDma, kDma, false>(p, s);
+  if (lx != kDma && lk != kDma) return launch_pair<T, K, kReg, kReg, false>(p, s);
+  return lx == kDma ? launch_pair<T, K, kDma, kReg, false>(p, s) : launch_pair<T, K, kReg, kDma, false>(p, s);
+}
+
+template <typename T>
+hipError_t pair(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s) {
+  return tile == kSmall ? pair_kind<T, Small>(p, lx, lk, q8, s) : pair_kind<T, Slice>(p, lx, lk, q8, s);
 }
 
 }  // namespace petdense_k

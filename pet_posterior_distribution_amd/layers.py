@@ -22,7 +22,7 @@ tape.gradient of both  diffusion_model.py:580     ``dense_backward``
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -73,28 +73,20 @@ def _on(t, device, what):
 
 
 def _rows(t, what):
-    """(..., n) as (rows, n) with contiguous rows that do not overlap, copied if it has to be, and its row stride."""
-    if t.dim() < 1:
-        raise ValueError(f'{what} must have at least one dimension')
+    """(..., n) as rows that are contiguous and do not overlap (copied if they have to be), and their stride."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     n = t.shape[-1]
-    if t.dim() == 1:
-        v = t.reshape(1, n)
-    elif t.dim() == 2:
-        v = t
-    else:
-        m = 1
-        for d in t.shape[:-1]:
-            m *= d
-        v = t.reshape(m, n)                    # a view where the leading dimensions can be merged
-    if n > 0 and v.shape[0] > 0 and ((n > 1 and v.stride(1) != 1) or (v.shape[0] > 1 and v.stride(0) < n)):
-        v = v.contiguous()
-    return v, (v.stride(0) if v.shape[0] > 1 else n)
+    v = t if t.dim() <= 2 else t.reshape(-1, n)      # a view where the leading dimensions can be merged
+    if v.dim() == 2 and (n == 1 or v.stride(1) == 1) and v.stride(0) >= n:
+        return v, v.stride(0)
+    return v.contiguous(), n
 
 
-def _same_rows(t, lead, n, dtype, device, what):
+def _same_rows(t, shape, dtype, device, what):
     _on(t, device, what)
-    if tuple(t.shape) != tuple(lead) + (n,):
-        raise ValueError(f'{what} must have shape {tuple(lead) + (n,)}, got {tuple(t.shape)}')
+    if t.shape != shape:
+        raise ValueError(f'{what} must have shape {tuple(shape)}, got {tuple(t.shape)}')
     if t.dtype != dtype:
         raise ValueError(f'{what} must be {dtype}, got {t.dtype}')
     return _rows(t, what)
@@ -102,26 +94,40 @@ def _same_rows(t, lead, n, dtype, device, what):
 
 def _kernel(kernel, k, dtype, device):
     _on(kernel, device, 'kernel')
-    if kernel.dim() != 2 or (k is not None and kernel.shape[0] != k):
-        raise ValueError(f'kernel must be (k, n){f" with k = {k}" if k is not None else ""}, got {tuple(kernel.shape)}')
+    shape = kernel.shape
+    if len(shape) != 2 or shape[0] != k:
+        raise ValueError(f'kernel must be (k, n) with k = {k}, got {tuple(shape)}')
     if kernel.dtype != dtype:
         raise ValueError(f'kernel must be {dtype}, got {kernel.dtype}')
-    if kernel.shape[1] < 1 or kernel.shape[0] < 1:
+    if shape[1] < 1:
         raise ValueError('kernel must not be empty')
     return _rows(kernel, 'kernel')
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
-def _stream(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+# the C structs' bytes (petdense_forward_args, petdense_backward_args): packing them is quicker than filling fields
+_FORWARD = struct.Struct('@6P8q4i')
+_BACKWARD = struct.Struct('@9P11q3i4x')
 
 
-def _workspace(nbytes, device):
+def _run(entry, workspace, args, dev, what):
+    """One call of the library on the current stream of `dev`, with its workspace."""
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _run(entry, workspace, args, dev, what)
+    nb = workspace(args)
     # from the allocator of the current stream: two streams, and two captured graphs, never share one
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    rc = entry(args, _ptr(ws), nb, _stream(dev))
+    if rc:
+        _check(rc, what)
+
+
+def _stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
 def dense(x, kernel, bias=None, activation=None, residual=None, return_preactivation=False, out_dtype=None):
@@ -135,9 +141,12 @@ def dense(x, kernel, bias=None, activation=None, residual=None, return_preactiva
     dev = x.device
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError('x must be (..., k) with k >= 1')
-    lead, k = x.shape[:-1], x.shape[-1]
+    shape = x.shape
+    k = shape[-1]
     w, ldk = _kernel(kernel, k, x.dtype, dev)
-    n = w.shape[1]
+    n = kernel.shape[1]
+    m = x.numel() // k
+    out = (*shape[:-1], n)
     act = _activation(activation)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in (x.dtype, torch.float32):
@@ -148,17 +157,13 @@ def dense(x, kernel, bias=None, activation=None, residual=None, return_preactiva
             raise ValueError(f'bias must be ({n},) of {x.dtype} or float32, got {tuple(bias.shape)} of {bias.dtype}')
         bias = bias.contiguous()
     x2, ldx = _rows(x, 'x')
-    r2, ldr = (None, 0) if residual is None else _same_rows(residual, lead, n, x.dtype, dev, 'residual')
-    y = torch.empty((*lead, n), dtype=out_dtype, device=dev)
-    pre = torch.empty((*lead, n), dtype=out_dtype, device=dev) if return_preactivation else None
-    a = _lib.PetdenseForwardArgs(
-        _ptr(x2), _ptr(w), _ptr(bias), _ptr(r2), _ptr(y), _ptr(pre), ldx, ldk, ldr, n, n, x2.shape[0], k, n, dt, act,
-        int(bias is not None and bias.dtype == torch.float32), int(out_dtype == torch.float32))
+    r2, ldr = (None, 0) if residual is None else _same_rows(residual, out, x.dtype, dev, 'residual')
+    y = torch.empty(out, dtype=out_dtype, device=dev)
+    pre = torch.empty(out, dtype=out_dtype, device=dev) if return_preactivation else None
     L = _lib.lib()
-    with torch.cuda.device(dev):
-        nb = int(L.petdense_forward_workspace(C.byref(a)))
-        ws = _workspace(nb, dev)
-        _check(L.petdense_forward(C.byref(a), _ptr(ws), nb, _stream(dev)), 'dense')
+    _run(L.petdense_forward, L.petdense_forward_workspace, _FORWARD.pack(
+        _ptr(x2), _ptr(w), _ptr(bias), _ptr(r2), _ptr(y), _ptr(pre), ldx, ldk, ldr, n, n, m, k, n, dt, act,
+        bias is not None and bias.dtype == torch.float32, out_dtype == torch.float32), dev, 'dense')
     return (y, pre) if return_preactivation else y
 
 
@@ -175,7 +180,8 @@ def dense_backward(dy, x, kernel, activation=None, saved=None, need_x=True, need
     dev = dy.device
     if dy.dim() < 1 or dy.shape[-1] < 1:
         raise ValueError('dy must be (..., n) with n >= 1')
-    lead, n = dy.shape[:-1], dy.shape[-1]
+    shape = dy.shape
+    lead, n = shape[:-1], shape[-1]
     act = _activation(activation)
     grad_dtype = dy.dtype if grad_dtype is None else grad_dtype
     if grad_dtype not in (dy.dtype, torch.float32):
@@ -185,41 +191,34 @@ def dense_backward(dy, x, kernel, activation=None, saved=None, need_x=True, need
         if x.dtype != dy.dtype:
             raise ValueError(f'the checkpoint is of {x.dtype} activations, dy is {dy.dtype}')
         k = x.shape[-1]
-        if tuple(x.shape[:-1]) != tuple(lead):
-            raise ValueError(f'the checkpoint must have shape {tuple(lead) + (k,)}, got {tuple(x.shape)}')
+        if x.shape[:-1] != lead:
+            raise ValueError(f'the checkpoint must have shape {(*lead, k)}, got {tuple(x.shape)}')
         _on(x.codes, dev, 'the checkpoint')
         x2, ldx = _rows(x.codes, 'codes')
         exps, lde = _rows(x.exponents, 'exponents')
     else:
         k = x.shape[-1] if isinstance(x, torch.Tensor) and x.dim() else 0
-        x2, ldx = _same_rows(x, lead, k, dy.dtype, dev, 'x')
+        x2, ldx = _same_rows(x, (*lead, k), dy.dtype, dev, 'x')
         if k < 1:
             raise ValueError('x must be (..., k) with k >= 1')
     w, ldk = _kernel(kernel, k, dy.dtype, dev)
-    if w.shape[1] != n:
+    if kernel.shape[1] != n:
         raise ValueError(f'kernel must be ({k}, {n}), got {tuple(kernel.shape)}')
     s2, lds = None, 0
     if act:
         if saved is None:
             raise ValueError(f'activation {activation!r} needs saved=')
-        s2, lds = _same_rows(saved, lead, n, dy.dtype, dev, 'saved')
+        s2, lds = _same_rows(saved, shape, dy.dtype, dev, 'saved')
     d2, ldd = _rows(dy, 'dy')
 
-    def out(need, shape, dtype):
-        return torch.empty(shape, dtype=dtype, device=dev) if need else None
-
-    gx = out(need_x, (*lead, k), dy.dtype)
-    gk = out(need_kernel, (k, n), grad_dtype)
-    gb = out(need_bias, (n,), grad_dtype)
-    gr = out(need_residual, (*lead, n), dy.dtype)
-    a = _lib.PetdenseBackwardArgs(
-        _ptr(d2), _ptr(x2), _ptr(exps), _ptr(w), _ptr(s2), _ptr(gx), _ptr(gk), _ptr(gb), _ptr(gr), ldd, ldx, lde, ldk,
-        lds, k, n, n, d2.shape[0], k, n, dt, act, int(grad_dtype == torch.float32))
+    gx = torch.empty((*lead, k), dtype=dy.dtype, device=dev) if need_x else None
+    gk = torch.empty((k, n), dtype=grad_dtype, device=dev) if need_kernel else None
+    gb = torch.empty((n,), dtype=grad_dtype, device=dev) if need_bias else None
+    gr = torch.empty(shape, dtype=dy.dtype, device=dev) if need_residual else None
     L = _lib.lib()
-    with torch.cuda.device(dev):
-        nb = int(L.petdense_backward_workspace(C.byref(a)))
-        ws = _workspace(nb, dev)
-        _check(L.petdense_backward(C.byref(a), _ptr(ws), nb, _stream(dev)), 'dense_backward')
+    _run(L.petdense_backward, L.petdense_backward_workspace, _BACKWARD.pack(
+        _ptr(d2), _ptr(x2), _ptr(exps), _ptr(w), _ptr(s2), _ptr(gx), _ptr(gk), _ptr(gb), _ptr(gr), ldd, ldx, lde, ldk,
+        lds, k, n, n, dy.numel() // n, k, n, dt, act, grad_dtype == torch.float32), dev, 'dense_backward')
     return DenseGradients(gx, gk, gb, gr)
 
 
@@ -256,11 +255,11 @@ class ActivationCheckpoint:
         """The activations that the codes stand for (..., k), in ``dtype``."""
         c2, ldc = _rows(self.codes, 'codes')
         e2, lde = _rows(self.exponents, 'exponents')
-        m, k = c2.shape
-        x = torch.empty(self.codes.shape, dtype=self.dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _check(_lib.lib().petdense_restore(_ptr(c2), ldc, _ptr(e2), lde, m, k, _TYPES[self.dtype], _ptr(x), k,
-                                               _stream(self.device)), 'restore')
+        dev, k = self.codes.device, self.codes.shape[-1]
+        x = torch.empty(self.codes.shape, dtype=self.dtype, device=dev)
+        with torch.cuda.device(dev):
+            _check(_lib.lib().petdense_restore(_ptr(c2), ldc, _ptr(e2), lde, x.numel() // k, k, _TYPES[self.dtype],
+                                               _ptr(x), k, _stream(dev)), 'restore')
         return x
 
 
@@ -271,11 +270,11 @@ def checkpoint_activations(x):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError('x must be (..., k) with k >= 1')
     x2, ldx = _rows(x, 'x')
-    m, k = x2.shape
+    k = x.shape[-1]
     nb = -(-k // BLOCK)
     codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     exps = torch.empty((*x.shape[:-1], nb), dtype=torch.uint8, device=x.device)
     with torch.cuda.device(x.device):
-        _check(_lib.lib().petdense_checkpoint(_ptr(x2), ldx, m, k, dt, _ptr(codes), k, _ptr(exps), nb,
+        _check(_lib.lib().petdense_checkpoint(_ptr(x2), ldx, x.numel() // k, k, dt, _ptr(codes), k, _ptr(exps), nb,
                                               _stream(x.device)), 'checkpoint_activations')
     return ActivationCheckpoint(codes, exps, x.dtype)

@@ -114,17 +114,28 @@ def test_the_layers_refuse_cpu_tensors():
             call()
 
 
+def test_packed_arguments_are_the_structs():
+    f = _lib.PetdenseForwardArgs(*range(1, 19))
+    assert bytes(f) == layers._FORWARD.pack(*range(1, 19))
+    b = _lib.PetdenseBackwardArgs(*range(1, 24))
+    assert bytes(b) == layers._BACKWARD.pack(*range(1, 24))
+
+
 def test_row_views():
-    rows = layers._rows
+    def rows(t, what):
+        return layers._rows(t, what)
+
     x = torch.zeros(6, 10)
     assert rows(x, 'x')[1] == 10 and rows(x[:, :4], 'x')[1] == 10 and rows(x[::2, :4], 'x')[1] == 20
     v, ld = rows(x.T, 'x')
     assert v.is_contiguous() and ld == 6
     v, ld = rows(torch.zeros(1, 4).expand(6, 4), 'x')          # rows that overlap are copied
     assert v.is_contiguous() and ld == 4
-    v, ld = rows(torch.zeros(2, 3, 4), 'x')
+    assert rows(torch.zeros(2, 3, 4), 'x')[1] == 4 and rows(torch.zeros(5), 'x')[1] == 5
+    v, ld = rows(torch.zeros(2, 3, 8)[:, :, :4], 'x')          # merged leading dimensions keep the row stride
+    assert tuple(v.shape) == (6, 4) and ld == 8
+    v, ld = rows(torch.zeros(2, 3, 4).transpose(0, 1), 'x')    # unmergeable ones are copied, in order
     assert tuple(v.shape) == (6, 4) and ld == 4
-    v, ld = rows(torch.zeros(5), 'x')
-    assert tuple(v.shape) == (1, 5) and ld == 5
-    v, ld = rows(torch.zeros(0, 5), 'x')
-    assert tuple(v.shape) == (0, 5) and ld == 5
+    v, ld = rows(torch.zeros(10)[::2], 'x')
+    assert v.is_contiguous() and ld == 5
+    assert rows(torch.zeros(0, 5), 'x')[1] == 5
