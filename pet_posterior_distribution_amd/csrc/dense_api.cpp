@@ -95,12 +95,12 @@ void set_plan(Plan& p, const Cost& c, int64_t splits, int64_t per, int bc, int64
 }
 
 // Tile and split of a product by their estimated time.
-Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
+Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader, bool q8 = false) {
   const int bc = type == kF32 ? 32 : 64;
   const int64_t steps = ceil_div(C, bc);
   Plan best;
   for (const Cost& c : type == kF32 ? kCosts32 : kCosts16) {
-    if (c.tile == kLarge && loader != kDma) continue;
+    if (c.tile == kLarge && (loader != kDma || q8)) continue;
     const int64_t tiles = ceil_div(I, c.b) * ceil_div(J, c.b);
     for_splits(steps, 64, [&](int64_t s, int64_t per) {
       const double t = product_us(c, tiles * s, per, loader) + join_us(I, J, s);
@@ -260,13 +260,13 @@ BackwardPlan plan_backward(const petdense_backward_args* a, void* work) {
       o += up((size_t)a->m * b.lddp * sz);
     }
   }
+  // row chunks of the activation's gradient: about 1024 workgroups, each of two rounds of its rows at least
+  const int lanes = act_grad_lanes((int)a->n);
+  const int64_t most = std::max<int64_t>(1, 1024 / ceil_div(a->n, lanes * 8));
+  b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, ceil_div(a->m, 2 * 256 / lanes)));
   if (b.sums) {
-    const int64_t blocks = ceil_div(a->n, 256);
-    b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(a->m, 16), std::max<int64_t>(1, std::min<int64_t>(256, 1024 / blocks))));
     b.o_sums = o;
     o += up((size_t)b.chunks * a->n * 4);
-  } else {
-    b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(a->m, 16), 1024));
   }
   const void* base = work ? b.dp : (b.make_dp && !a->dresidual ? nullptr : b.dp);
   if (a->dx) {
@@ -276,7 +276,7 @@ BackwardPlan plan_backward(const petdense_backward_args* a, void* work) {
   if (a->dkernel) {
     // 8-bit inputs go through registers whatever their alignment: `loader` is dp's
     b.load_k = dma_ok(base, b.lddp, a->n, sz) && (a->x_exponents || dma_ok(a->x, a->ldx, a->k, sz)) ? kDma : kReg;
-    b.pk = plan(a->k, a->n, a->m, a->dtype, b.load_k);
+    b.pk = plan(a->k, a->n, a->m, a->dtype, b.load_k, a->x_exponents != nullptr);
   }
   if (a->dx && a->dkernel) {
     Plan px, pk;

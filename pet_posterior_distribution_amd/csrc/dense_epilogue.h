@@ -6,11 +6,6 @@ namespace petdense_k {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-template <typename T>
-struct Vec4 {
-  typedef T type __attribute__((ext_vector_type(4)));
-};
-
 // Phi(x) = (1 + erf(x / sqrt 2)) / 2.
 // 16-bit outputs: Abramowitz & Stegun 7.1.26, |error of erf| <= 1.5e-7, i.e. 2^-22.7 beside the 2^-9 and 2^-12
 // of a rounded output; about a third of erff's instructions, and the epilogue pays them once per output.
@@ -58,17 +53,6 @@ __device__ __forceinline__ float activate_grad(float g, float v, int act) {
     return g * s * fmaf(v, 1.0f - s, 1.0f);
   }
   return g;
-}
-
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const void* p, int64_t o) {
-  typename Vec4<T>::type v = *reinterpret_cast<const typename Vec4<T>::type*>(static_cast<const T*>(p) + o);
-  return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
-}
-template <typename T>
-__device__ __forceinline__ void store4(void* p, int64_t o, f32x4 v) {
-  typename Vec4<T>::type r = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-  *reinterpret_cast<typename Vec4<T>::type*>(static_cast<T*>(p) + o) = r;
 }
 
 // W neighbouring values of a row, of which n exist (the others read as zero).  Whole groups are one access of any

@@ -50,7 +50,7 @@ struct ColumnJoin {
 struct Pair {
   Product x, k;
   ColumnJoin cols;
-  int tx, tk, nx, nk;    // tiles and workgroups of each (the launcher's)
+  int nx, nk;            // workgroups of each (the launcher's)
 };
 
 // One launch of the tiled product: `q8`: A is e4m3 codes with exponent bytes (kKernelGrad only).
@@ -68,6 +68,13 @@ hipError_t join(const Product& p, int type, hipStream_t s);
 // Few rows: one pass over B ([C][J], j-contiguous), I <= kMaxRows.
 constexpr int kMaxRows = 8;
 hipError_t rows(const Product& p, int type, hipStream_t s);
+
+// lanes that share a row of N columns in act_grad: a power of two
+inline int act_grad_lanes(int N) {
+  int l = 1;
+  while (l < 64 && l * 8 < N) l *= 2;
+  return l;
+}
 
 // dp = dy act'(saved) (dp may be null), part[chunk][n] = column sums of dp over the chunk's rows (may be null)
 hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, float* part,

@@ -124,69 +124,86 @@ hipError_t rows_t(const Product& p, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// dp = dy act'(saved), and column sums of the unrounded dp over a chunk of rows.  One pass, memory bound: a wave
-// takes 4 columns a lane (256 columns), the block's 4 waves take every fourth row of the chunk.
+// dp = dy act'(saved), and column sums of the unrounded dp over a chunk of rows.  One pass, memory bound: a lane takes
+// 8 columns, LPR lanes a row (a power of two, so that narrow layers fill the wave with rows); the wave's rows meet by
+// shuffles, the block's waves in LDS, in a fixed order.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* dy, int64_t ldy, const T* saved, int64_t lds, T* dp,
                                                        int64_t ldd, float* part, int rows_per, int M, int N, int act,
-                                                       int vec) {
+                                                       int lpr) {
   constexpr bool EXACT = sizeof(T) == 4;
-  __shared__ f32x4 red[4][64];
+  constexpr int W = 8;
+  __shared__ float red[4][64 * W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int j = blockIdx.x * 256 + lane * 4, n = N - j;
+  const int l = lane & (lpr - 1), rows = 256 / lpr;             // rows the block takes at a time
+  const int j = (blockIdx.x * lpr + l) * W, n = N - j;
   const int64_t m0 = (int64_t)blockIdx.y * rows_per, m1 = min(m0 + rows_per, (int64_t)M);
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  float sum[W];
+#pragma unroll
+  for (int q = 0; q < W; ++q) sum[q] = 0.f;
+  auto row = [&](const float* g0, const float* v, int64_t m) {
+    float g[W];
+#pragma unroll
+    for (int q = 0; q < W; ++q) g[q] = g0[q];
+    if (act == kRelu) {
+#pragma unroll
+      for (int q = 0; q < W; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], kRelu);
+    } else if (act == kGelu) {
+#pragma unroll
+      for (int q = 0; q < W; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], kGelu);
+    } else if (act == kSilu) {
+#pragma unroll
+      for (int q = 0; q < W; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], kSilu);
+    }
+#pragma unroll
+    for (int q = 0; q < W; ++q) sum[q] += g[q];
+    if (dp) store_row<T, W>(dp + m * ldd + j, n, g);
+  };
   if (n > 0) {
-#pragma unroll 4
-    for (int64_t m = m0 + wave; m < m1; m += 4) {
-      f32x4 g, v = {0.f, 0.f, 0.f, 0.f};
-      if (vec && n >= 4) {
-        g = load4<T>(dy, m * ldy + j);
-        if (act != kNone) v = load4<T>(saved, m * lds + j);
-      } else {
+    int64_t m = m0 + threadIdx.x / lpr;
+    if (n >= W) {
+      // two rows in flight
+      for (; m + rows < m1; m += 2 * rows) {
+        float g[2][W], v[2][W];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          g[q] = q < n ? (float)dy[m * ldy + j + q] : 0.f;
-          if (act != kNone && q < n) v[q] = (float)saved[m * lds + j + q];
+        for (int u = 0; u < 2; ++u) {
+          load_row<T, W>(dy + (m + u * rows) * ldy + j, W, g[u]);
+          if (act != kNone) load_row<T, W>(saved + (m + u * rows) * lds + j, W, v[u]);
         }
-      }
-      if (act != kNone) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], act);
+        for (int u = 0; u < 2; ++u) row(g[u], v[u], m + u * rows);
       }
-      sum += g;
-      if (dp) {
-        if (vec && n >= 4) {
-          store4<T>(dp, m * ldd + j, g);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q < n) dp[m * ldd + j + q] = (T)g[q];
-        }
-      }
+    }
+    for (; m < m1; m += rows) {
+      float g[W], v[W];
+      load_row<T, W>(dy + m * ldy + j, n, g);
+      if (act != kNone) load_row<T, W>(saved + m * lds + j, n, v);
+      row(g, v, m);
     }
   }
   if (!part) return;
-  red[wave][lane] = sum;
-  __syncthreads();
-  if (wave == 0 && n > 0) {
-    const f32x4 v = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q < n) part[(int64_t)blockIdx.y * N + j + q] = v[q];
+  for (int q = 0; q < W; ++q)
+    for (int o = lpr; o < 64; o *= 2) sum[q] += __shfl_xor(sum[q], o);
+  if (lane < lpr) {
+#pragma unroll
+    for (int q = 0; q < W; ++q) red[wave][lane * W + q] = sum[q];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < lpr * W; c += 256) {
+    const int k = blockIdx.x * lpr * W + c;
+    if (k < N) part[(int64_t)blockIdx.y * N + k] = ((red[0][c] + red[1][c]) + red[2][c]) + red[3][c];
   }
 }
 
 template <typename T>
 hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, float* part,
                       int chunks, int M, int N, int act, hipStream_t s) {
-  const int rows_per = (M + chunks - 1) / chunks;
-  const uintptr_t a = reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(saved) |
-                      reinterpret_cast<uintptr_t>(dp) | (uintptr_t)((ldy | (saved ? lds : 0) | (dp ? ldd : 0)) * (int64_t)sizeof(T));
-  hipLaunchKernelGGL((act_grad_kernel<T>), dim3(blocks_for(N, 256), chunks), dim3(256), 0, s,
+  const int rows_per = (M + chunks - 1) / chunks, lpr = act_grad_lanes(N);
+  hipLaunchKernelGGL((act_grad_kernel<T>), dim3(blocks_for(N, lpr * 8), chunks), dim3(256), 0, s,
                      static_cast<const T*>(dy), ldy, static_cast<const T*>(saved), lds, static_cast<T*>(dp), ldd, part,
-                     rows_per, M, N, act, (int)(a % (4 * sizeof(T)) == 0));
+                     rows_per, M, N, act, lpr);
   return hipGetLastError();
 }
 

@@ -138,15 +138,17 @@ struct Filler {
   const char* base;      // the tile's first value at contraction value 0 of this part
   int64_t ld;            // bytes from row to row
   int limit;             // free values of the tile that exist
+  bool brief;            // kReg: the operand's rows are shorter than a piece
   int clen, kw;
   const uint8_t* exps;   // Q8: exponent byte of the tile's first block at the part's first row
   int64_t lde;
   int voff[LOADER == kDma ? N : 1];
   u32x4 reg[LOADER == kDma ? 1 : N];
 
-  __device__ void init(const void* p, int64_t ld_values, int f0, int f_limit, int64_t c0, int clen_,
+  __device__ void init(const void* p, int64_t ld_values, int f0, int f_limit, int64_t c0, int clen_, int c_all,
                        const uint8_t* ex, int64_t lde_, int kw_, int tid) {
     kw = kw_;
+    brief = (FREE ? f_limit : c_all) < S::EPC;
     constexpr int SZ = Q8 ? 1 : (int)sizeof(T);
     ld = ld_values * SZ;
     base = static_cast<const char*>(p) + (FREE ? c0 * ld + (int64_t)f0 * SZ : f0 * ld + c0 * SZ);
@@ -177,7 +179,8 @@ struct Filler {
     u.left = clen - u.t * BC;
     u.p = base + (FREE ? (int64_t)u.t * BC * ld : (int64_t)u.t * BC * (int64_t)sizeof(T));
     // free-contiguous: 16 bytes from a piece's first value may run into the next row, which then has to exist
-    u.whole = FREE ? u.left > BC && ld >= 16 : u.left >= BC;
+    // (offsets within a step fit 31 bits)
+    u.whole = !brief && (FREE ? u.left > BC && ld >= 16 : u.left >= BC) && ld < 0x7fffffff / 256;
     if constexpr (LOADER == kDma) {
       const unsigned long long a = reinterpret_cast<unsigned long long>(u.p);
       u.rs[0] = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffull));
@@ -198,53 +201,91 @@ struct Filler {
     }
   }
 
-  // begins the loads of a step into registers.  Whole steps load without a branch: pieces past the operand's free
-  // end read its first value instead (they feed outputs that are not stored).
+  // Begins the loads of a step into registers, each a whole piece of any alignment, with no branch on the lane:
+  //  - whole steps: pieces past the operand's free end read its first value instead (they feed outputs that are not
+  //    stored);
+  //  - cut steps: a piece that ends past its row is read so that it ends with it, and shifted; what does not exist
+  //    becomes zero;
+  //  - rows shorter than a piece: value by value.
   __device__ __forceinline__ void begin_reg(const Step& u, int tid) {
     if constexpr (LOADER == kReg) {
-      constexpr int PB = Q8 ? S::EPC : 16;              // bytes of a piece in memory
+      constexpr int SZ = Q8 ? 1 : (int)sizeof(T), PB = SZ * S::EPC;        // bytes of a value and a piece in memory
       if (u.whole) {
 #pragma unroll
         for (int q = 0; q < N; ++q) {
           const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
           const int rr = FREE ? r : min(r, limit - 1), cc = FREE && c * S::EPC >= limit ? 0 : c;
-          const char* s = u.p + (int64_t)rr * ld + cc * PB;
-          if constexpr (Q8) {
-            unsigned w[2] = {0, 0};
-            __builtin_memcpy(w, s, PB);
-            reg[q][0] = w[0];
-            reg[q][1] = w[1];
-            reg[q][2] = exps[((int64_t)u.t * BC + r) * lde + (cc * S::EPC) / 32];
-          } else {
-            __builtin_memcpy(&reg[q], s, 16);
-          }
+          load_piece(q, u.p + (unsigned)(rr * (int)ld + cc * PB));
+          if constexpr (Q8)
+            reg[q][2] = (exps + (int64_t)u.t * BC * lde)[(unsigned)(r * (int)lde + (cc * S::EPC) / 32)];
         }
         return;
       }
+      // cut steps are rare: nothing of theirs is worth a register across the others
+      asm volatile("" : "+v"(tid));
 #pragma unroll
       for (int q = 0; q < N; ++q) {
         const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
-        // values of the piece that exist
-        const int n = FREE ? (r < u.left ? limit - c * S::EPC : 0) : (r < limit ? u.left - c * S::EPC : 0);
-        const char* s = u.p + (int64_t)r * ld + c * PB;
-        if constexpr (Q8) {
-          unsigned w[2] = {0, 0};
-#pragma unroll
-          for (int v = 0; v < S::EPC; ++v)
-            if (v < n) w[v >> 2] |= (unsigned)(uint8_t)s[v] << ((v & 3) * 8);
-          reg[q][0] = w[0];
-          reg[q][1] = w[1];
-          reg[q][2] = n > 0 ? exps[((int64_t)u.t * BC + r) * lde + (c * S::EPC) / 32] : 127;
-        } else {
-          T v[S::EPC];
-#pragma unroll
-          for (int x = 0; x < S::EPC; ++x) {
-            v[x] = (T)0.f;
-            if (x < n) __builtin_memcpy(&v[x], s + x * sizeof(T), sizeof(T));
+        // the piece's row (clamped to one that exists), its first value in it, and the values that follow
+        const int64_t row = FREE ? min((int64_t)u.t * BC + r, (int64_t)clen - 1) : min(r, limit - 1);
+        const int64_t first = (FREE ? 0 : (int64_t)u.t * BC) + c * S::EPC;
+        const int64_t after = (FREE ? limit : clen) - first;
+        const bool in = FREE ? r < u.left : r < limit;
+        const int n = !in || after <= 0 ? 0 : after < S::EPC ? (int)after : S::EPC;
+        const char* p = base + row * ld;
+        if (brief) {
+#pragma unroll 1
+          for (int x = S::EPC - 1; x >= 0; --x) {
+            // the values come in from the last to the first, each moving those behind it up
+            const char* s = p + min(first + x, (int64_t)(FREE ? limit : clen) - 1) * SZ;
+            unsigned one = 0;
+            __builtin_memcpy(&one, s, SZ);
+            push_value(q, x < n ? one : 0u);
           }
-          __builtin_memcpy(&reg[q], v, 16);
+        } else {
+          const int64_t at = after >= S::EPC ? first : (int64_t)(FREE ? limit : clen) - S::EPC;
+          load_piece(q, p + at * SZ);
+          shift_piece(q, (after >= S::EPC && in ? 0 : S::EPC - n) * SZ * 8);
         }
+        if constexpr (Q8) reg[q][2] = exps[row * lde + min(first, (int64_t)limit - 1) / 32];
       }
+    }
+  }
+
+  __device__ __forceinline__ void load_piece(int q, const char* s) {
+    if constexpr (Q8) {
+      unsigned w[2] = {0, 0};
+      __builtin_memcpy(w, s, S::EPC);
+      reg[q][0] = w[0];
+      reg[q][1] = w[1];
+    } else {
+      __builtin_memcpy(&reg[q], s, 16);
+    }
+  }
+  // moves the piece's values up by one and puts `v` in front
+  __device__ __forceinline__ void push_value(int q, unsigned v) {
+    constexpr int BITS = Q8 ? 8 : 8 * (int)sizeof(T);
+#pragma unroll
+    for (int w = Q8 ? 1 : 3; w >= 0; --w) {
+      const unsigned below = w ? reg[q][w - 1] : 0;
+      if constexpr (BITS == 32) reg[q][w] = w ? below : v;
+      else reg[q][w] = reg[q][w] << BITS | (w ? below >> (32 - BITS) : v);
+    }
+  }
+  // moves the piece's values down by `bits`, zeros behind them
+  __device__ __forceinline__ void shift_piece(int q, int bits) {
+    const uint64_t lo = reg[q][0] | (uint64_t)reg[q][1] << 32;
+    if constexpr (Q8) {
+      constexpr int ALL = S::EPC * 8;
+      const uint64_t v = bits >= ALL ? 0 : lo >> bits;
+      reg[q][0] = (unsigned)v;
+      reg[q][1] = (unsigned)(v >> 32);
+    } else {
+      const uint64_t hi = reg[q][2] | (uint64_t)reg[q][3] << 32;
+      const int b = bits & 63;
+      const uint64_t lo1 = (lo >> b) | (b ? hi << (64 - b) : 0), hi1 = hi >> b;
+      const uint64_t l = bits >= 128 ? 0 : bits >= 64 ? hi1 : lo1, h = bits >= 64 ? 0 : hi1;
+      reg[q] = u32x4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
     }
   }
 
@@ -297,13 +338,15 @@ typedef Kind<128, 128, 2, 2, 1> Mid;
 typedef Kind<64, 64, 2, 2, 1> Small;
 typedef Kind<32, 32, 1, 1, 8> Slice;
 
-// Workgroup -> tile.  Neighbouring workgroup numbers go to different XCDs, each with its own L2: every XCD gets a
-// contiguous run of tiles, and a run walks bands of 4 tile rows, so that the workgroups an XCD runs together share
-// rows of A and columns of B.
-__device__ __forceinline__ void tile_of(int b, int ti, int tj, int& i, int& j) {
-  const int n = ti * tj;
+// Workgroup -> part of the contraction and tile.  Neighbouring workgroup numbers go to different XCDs, each with its
+// own L2: every XCD gets a contiguous run of (part, tile), so that a part's rows are fetched by one XCD, and the tiles
+// of a part run in bands of 4 tile rows, so that the workgroups an XCD runs together share rows of A and columns of B.
+__device__ __forceinline__ void place_of(int b, int ti, int tj, int splits, int& split, int& i, int& j) {
+  const int tiles = ti * tj, n = tiles * splits;
   const int per = n / 8, rest = n % 8, x = b % 8;
-  const int t = x * per + min(x, rest) + b / 8;
+  const int u = x * per + min(x, rest) + b / 8;
+  split = u / tiles;
+  const int t = u - split * tiles;
   constexpr int BAND = 4;
   const int band = t / (BAND * tj), first = band * BAND, h = min(BAND, ti - first), r = t - first * tj;
   i = first + r % h;
@@ -311,7 +354,7 @@ __device__ __forceinline__ void tile_of(int b, int ti, int tj, int& i, int& j) {
 }
 
 template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8>
-__device__ __forceinline__ void product_body(const Product& p, int block, int split, char* lds) {
+__device__ __forceinline__ void product_body(const Product& p, int block, char* lds) {
   constexpr int BI = K::BI, BJ = K::BJ, WI = K::WI, WJ = K::WJ, KW = K::KW;
   constexpr int BC = 128 / (int)sizeof(T);
   constexpr bool SHARED = KW == 1;
@@ -326,8 +369,8 @@ __device__ __forceinline__ void product_body(const Product& p, int block, int sp
   const int wi = SHARED ? wave / WJ : 0, wj = SHARED ? wave % WJ : 0;
   const int kw = SHARED ? 0 : __builtin_amdgcn_readfirstlane(wave);
   char* mine = lds + kw * 2 * STAGE;
-  int ti, tj;
-  tile_of(block, (p.I + BI - 1) / BI, (p.J + BJ - 1) / BJ, ti, tj);
+  int split, ti, tj;
+  place_of(block, (p.I + BI - 1) / BI, (p.J + BJ - 1) / BJ, p.splits, split, ti, tj);
   const int i0 = ti * BI, j0 = tj * BJ;
   const int64_t c0 = (int64_t)split * p.c_per;
   const int clen = (int)min((int64_t)p.c_per, p.C - c0);
@@ -336,8 +379,8 @@ __device__ __forceinline__ void product_body(const Product& p, int block, int sp
 
   Filler<T, FA, BI, BC, THREADS, KW, LA, Q8> fa;
   Filler<T, FB, BJ, BC, THREADS, KW, LB, false> fb;
-  fa.init(p.A, p.lda, i0, p.I, c0, clen, p.exps, p.lde, kw, tid);
-  fb.init(p.B, p.ldb, j0, p.J, c0, clen, nullptr, 0, kw, tid);
+  fa.init(p.A, p.lda, i0, p.I, c0, clen, p.C, p.exps, p.lde, kw, tid);
+  fb.init(p.B, p.ldb, j0, p.J, c0, clen, p.C, nullptr, 0, kw, tid);
 
   f32x4 acc[FI][FJ];
 #pragma unroll
@@ -485,7 +528,7 @@ __device__ __forceinline__ void product_body(const Product& p, int block, int sp
 template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8>
 __global__ __launch_bounds__(K::THREADS) void product_kernel(Product p) {
   extern __shared__ char lds[];
-  product_body<T, K, FA, FB, LA, LB, Q8>(p, blockIdx.x, blockIdx.y, lds);
+  product_body<T, K, FA, FB, LA, LB, Q8>(p, blockIdx.x, lds);
 }
 
 // The backward pass's two products and the join of its column sums as one launch: workgroups [0, nx) multiply the
@@ -495,10 +538,9 @@ __global__ __launch_bounds__(K::THREADS) void pair_kernel(Pair p) {
   extern __shared__ char lds[];
   const int b = blockIdx.x;
   if (b < p.nx) {
-    product_body<T, K, false, false, LX, LX, false>(p.x, b % p.tx, b / p.tx, lds);
+    product_body<T, K, false, false, LX, LX, false>(p.x, b, lds);
   } else if (b < p.nx + p.nk) {
-    const int d = b - p.nx;
-    product_body<T, K, true, true, Q8 ? kReg : LK, LK, Q8>(p.k, d % p.tk, d / p.tk, lds);
+    product_body<T, K, true, true, Q8 ? kReg : LK, LK, Q8>(p.k, b - p.nx, lds);
   } else {
     join_columns16(p.cols, b - p.nx - p.nk, threadIdx.x, reinterpret_cast<float*>(lds));
   }
@@ -524,7 +566,7 @@ hipError_t launch(const Product& p, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   auto k = product_kernel<T, K, FA, FB, LA, LB, Q8>;
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
-  hipLaunchKernelGGL(k, dim3((unsigned)tiles_of(p, K::BI, K::BJ), (unsigned)p.splits), dim3(K::THREADS), K::LDS, s, p);
+  hipLaunchKernelGGL(k, dim3((unsigned)(tiles_of(p, K::BI, K::BJ) * p.splits)), dim3(K::THREADS), K::LDS, s, p);
   return hipGetLastError();
 }
 
@@ -533,21 +575,19 @@ hipError_t launch_pair(Pair p, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   auto k = pair_kernel<T, K, LX, LK, Q8>;
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
-  p.tx = (int)tiles_of(p.x, K::BI, K::BJ);
-  p.tk = (int)tiles_of(p.k, K::BI, K::BJ);
-  p.nx = p.tx * p.x.splits;
-  p.nk = p.tk * p.k.splits;
+  p.nx = (int)(tiles_of(p.x, K::BI, K::BJ) * p.x.splits);
+  p.nk = (int)(tiles_of(p.k, K::BI, K::BJ) * p.k.splits);
   hipLaunchKernelGGL(k, dim3((unsigned)(p.nx + p.nk + (p.cols.N + 15) / 16)), dim3(K::THREADS), K::LDS, s, p);
   return hipGetLastError();
 }
 
 template <typename T, typename K>
 hipError_t product_kind(const Product& p, int layout, int loader, int q8, hipStream_t s) {
-  if constexpr (K::BI == 256) {      // the plan takes the largest tile only for operands that DMA can stage
+  if constexpr (K::BI == 256) {      // the plan takes the largest tile only where DMA stages both operands
     if (loader != kDma) return hipErrorInvalidValue;
     if (layout == kForward) return launch<T, K, false, true, kDma, kDma, false>(p, s);
     if (layout == kInputGrad) return launch<T, K, false, false, kDma, kDma, false>(p, s);
-    return q8 ? launch<T, K, true, true, kReg, kDma, true>(p, s) : launch<T, K, true, true, kDma, kDma, false>(p, s);
+    return q8 ? hipErrorInvalidValue : launch<T, K, true, true, kDma, kDma, false>(p, s);
   } else {
     if (layout == kForward)
       return loader == kDma ? launch<T, K, false, true, kDma, kDma, false>(p, s)

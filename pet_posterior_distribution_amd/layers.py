@@ -126,6 +126,16 @@ def _run(entry, workspace, args, dev, what):
         _check(rc, what)
 
 
+def _run_plain(entry, args, dev, what):
+    """The same for entries without a workspace; the stream is their last argument."""
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _run_plain(entry, args, dev, what)
+    rc = entry(*args, _stream(dev))
+    if rc:
+        _check(rc, what)
+
+
 def _stream(dev):
     return torch.cuda.current_stream(dev).cuda_stream
 
@@ -257,9 +267,8 @@ class ActivationCheckpoint:
         e2, lde = _rows(self.exponents, 'exponents')
         dev, k = self.codes.device, self.codes.shape[-1]
         x = torch.empty(self.codes.shape, dtype=self.dtype, device=dev)
-        with torch.cuda.device(dev):
-            _check(_lib.lib().petdense_restore(_ptr(c2), ldc, _ptr(e2), lde, x.numel() // k, k, _TYPES[self.dtype],
-                                               _ptr(x), k, _stream(dev)), 'restore')
+        _run_plain(_lib.lib().petdense_restore, (_ptr(c2), ldc, _ptr(e2), lde, x.numel() // k, k, _TYPES[self.dtype],
+                                                 _ptr(x), k), dev, 'restore')
         return x
 
 
@@ -274,7 +283,6 @@ def checkpoint_activations(x):
     nb = -(-k // BLOCK)
     codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     exps = torch.empty((*x.shape[:-1], nb), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        _check(_lib.lib().petdense_checkpoint(_ptr(x2), ldx, x.numel() // k, k, dt, _ptr(codes), k, _ptr(exps), nb,
-                                              _stream(x.device)), 'checkpoint_activations')
+    _run_plain(_lib.lib().petdense_checkpoint, (_ptr(x2), ldx, x.numel() // k, k, dt, _ptr(codes), k, _ptr(exps), nb),
+               x.device, 'checkpoint_activations')
     return ActivationCheckpoint(codes, exps, x.dtype)
