@@ -20,7 +20,7 @@
  * Optimizer: Keras Adam, each variable's gradient clipped to norm <= clipnorm
  * first, learning rate lr0 * decay_rate^(iterations / decay_steps).
  *
- * Numerics: fp32 everywhere (the reference trains fp32).  Convolutions run as
+ * Numerics: fp32 everywhere by default (the reference trains fp32; pettrain_set_precision below).  Convolutions run as
  * im2col + rocBLAS fp32 GEMMs (forward Y = A W, weight grad A^T dY, data grad
  * dY W^T then col2im); residual 1x1 convs are folded into the centre tap
  * (their gradient is the centre tap's).  Everything else is hand-written HIP.
@@ -65,6 +65,23 @@ int pettrain_default_config(pettrain_config* opt);
 int pettrain_create(const petdiff_config* net, const float* weights, size_t n_weights, const float* tab, int T,
                     const pettrain_config* opt, int device, pettrain_handle* out);
 void pettrain_destroy(pettrain_handle h);
+
+#define PETTRAIN_F32 0
+#define PETTRAIN_BF16 1
+#define PETTRAIN_KEEP 0
+#define PETTRAIN_KEEP_E4M3 1
+
+/* Precision of the products of the convolutions and of the condition encoder (99 % of the step's operations):
+ *   PETTRAIN_F32   rocBLAS fp32 (the default);
+ *   PETTRAIN_BF16  the dense layer's operators (petdense.h): bf16 operands, fp32 sums, bias and ReLU in the epilogue;
+ *                  activations between layers, weights, gradients and Adam stay fp32.
+ * keep: what a bf16 step holds of every product's input between its forward and backward passes: PETTRAIN_KEEP the
+ * bf16 values, PETTRAIN_KEEP_E4M3 8-bit checkpoints (8.25 bits a value; the convolutions' kernel gradients are those
+ * of the restored inputs, everything else is unchanged).  Frees the step's buffers when it changes anything; the
+ * caller's stream must be idle then.  PETDIFF_ERR_INVALID: unknown values, or e4m3 without bf16. */
+int pettrain_set_precision(pettrain_handle h, int precision, int keep);
+/* Device bytes the step holds for a batch of B samples at most so far: activations, gradients, workspaces. */
+size_t pettrain_step_bytes(pettrain_handle h);
 
 /* Forward + loss + backward of one batch.
  *   x0_dev [B][n_roi][n_par] (the training "images"), cond_dev [B][49][54];

@@ -98,6 +98,8 @@ SYMBOLS += [
     ('pettrain_create', C.c_int, [C.POINTER(PetdiffConfig), C.c_void_p, C.c_size_t, C.c_void_p, C.c_int,
                                   C.POINTER(PettrainConfig), C.c_int, C.POINTER(C.c_void_p)]),
     ('pettrain_destroy', None, [C.c_void_p]),
+    ('pettrain_set_precision', C.c_int, [C.c_void_p, C.c_int, C.c_int]),
+    ('pettrain_step_bytes', C.c_size_t, [C.c_void_p]),
     ('pettrain_compute_gradients', C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,
                                              C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p]),
     ('pettrain_compute_loss', C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,

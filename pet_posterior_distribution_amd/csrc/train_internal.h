@@ -40,6 +40,18 @@ hipError_t pool_mask_bwd(const float* out, const float* dpool, const float* dski
                          int C, hipStream_t s);
 hipError_t fold_weff(const float* W, const float* bw, const float* R, const float* br, float* Weff, int taps,
                      int padl, int C, int N, hipStream_t s);
+// bf16 step (operands of the dense layer's products): rows of the im2col matrix hold taps * cfull values and zeros up
+// to ld (no column of ones: the bias is added in the product's epilogue)
+hipError_t im2col16(const ConvIn& ci, int B, const float* lab, const float* tim, const float* x1, const float* x2,
+                    __bf16* A, int ld, hipStream_t s);
+hipError_t col2im16(const ConvIn& ci, int B, const __bf16* dA, int ld, float* dlab, float* dtim, float* dx1,
+                    float* dx2, hipStream_t s);
+hipError_t pool_mask_bwd16(const float* out, const float* dpool, const float* dskip, __bf16* dpre, int B, int L, int C,
+                           hipStream_t s);
+// [rows][N] bf16 of the folded kernel (R, br may be null: no residual), zeros past taps * C; bias [N] = bw + br
+hipError_t fold_weff16(const float* W, const float* bw, const float* R, const float* br, __bf16* Weff, float* bias,
+                       int rows, int taps, int padl, int C, int N, hipStream_t s);
+hipError_t to_bf16(const float* src, int M, int N, __bf16* dst, int ldd, hipStream_t s);   // dst[M][ldd], zeros past N
 hipError_t time_embed(const int* t, int B, int dim, float* emb, int ld, hipStream_t s);
 hipError_t qsample(const float* x0, const int* t_in, const float* noise_in, uint64_t seed, uint64_t goff,
                    int64_t iter, int B, int T, const float* tab, int* t_out, float* noise_out, float* xt,

@@ -156,8 +156,9 @@ __global__ void maxpool_fwd_kernel(const float* out, float* pool, int B, int L, 
 }
 
 // MaxPool gradient goes to the first maximum of each pair (TF MaxPoolGrad).
-__global__ void pool_mask_bwd_kernel(const float* out, const float* dpool, const float* dskip, float* dpre,
-                                     int B, int L, int C) {
+template <typename T>
+__global__ void pool_mask_bwd_kernel(const float* out, const float* dpool, const float* dskip, T* dpre, int B, int L,
+                                     int C) {
   const size_t n = (size_t)B * L * C;
   for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
     const int c = (int)(i % C);
@@ -171,7 +172,7 @@ __global__ void pool_mask_bwd_kernel(const float* out, const float* dpool, const
       const bool first = out[e0] >= out[e0 + C];
       if ((l & 1) == (first ? 0 : 1)) g += dpool[(b * (L / 2) + (l >> 1)) * C + c];
     }
-    dpre[i] = o > 0.f ? g : 0.f;
+    dpre[i] = (T)(o > 0.f ? g : 0.f);
   }
 }
 
@@ -188,6 +189,82 @@ __global__ void fold_weff_kernel(const float* W, const float* bw, const float* R
       const int j = (int)(i / CN);
       Weff[i] = W[i] + (j == padl ? R[i - (size_t)padl * CN] : 0.f);
     }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// bf16 step: the same gathers and masks, rounded to the products' operands
+// ---------------------------------------------------------------------------
+__global__ void im2col16_kernel(ConvIn ci, const float* lab, const float* tim, const float* x1, const float* x2,
+                                __bf16* A, int ld) {
+  const int Cf = ci.cfull(), Lout = ci.lout();
+  const int l = blockIdx.x % Lout, b = blockIdx.x / Lout;
+  __bf16* row = A + (size_t)blockIdx.x * ld;
+  for (int j = 0; j < ci.taps; ++j) {
+    const int p = l + j - ci.padl;
+    const bool in = p >= 0 && p < Lout;
+    const int sp = ci.ups ? p >> 1 : p;
+    for (int c = threadIdx.x; c < Cf; c += blockDim.x)
+      row[j * Cf + c] = (__bf16)(in ? conv_src(ci, b, sp, c, lab, tim, x1, x2) : 0.f);
+  }
+  for (int k = ci.taps * Cf + threadIdx.x; k < ld; k += blockDim.x) row[k] = (__bf16)0.f;
+}
+
+__global__ void col2im16_kernel(ConvIn ci, const __bf16* dA, int ld, float* dlab, float* dtim, float* dx1,
+                                float* dx2) {
+  const int Cf = ci.cfull(), Lout = ci.lout();
+  const int r = blockIdx.x;
+  const int sp = r % ci.Lsrc, b = r / ci.Lsrc;
+  const int np = ci.ups ? 2 : 1;
+  for (int c = threadIdx.x; c < Cf; c += blockDim.x) {
+    float acc = 0.f;
+    for (int q = 0; q < np; ++q) {
+      const int p = ci.ups ? 2 * sp + q : sp;
+      for (int j = 0; j < ci.taps; ++j) {
+        const int l = p - j + ci.padl;
+        if (l >= 0 && l < Lout) acc += (float)dA[((size_t)b * Lout + l) * ld + j * Cf + c];
+      }
+    }
+    int cc = c;
+    if (ci.has_cond) {
+      if (cc < 49) {
+        if (dlab) dlab[(size_t)r * 49 + cc] = acc;
+        continue;
+      }
+      if (cc == 49) {
+        if (dtim) dtim[r] = acc;
+        continue;
+      }
+      cc -= 50;
+    }
+    if (cc < ci.c1) {
+      if (dx1) dx1[(size_t)r * ci.c1 + cc] = acc;
+    } else if (dx2) {
+      dx2[(size_t)r * ci.c2 + (cc - ci.c1)] = acc;
+    }
+  }
+}
+
+__global__ void fold_weff16_kernel(const float* W, const float* bw, const float* R, const float* br, __bf16* Weff,
+                                   float* bias, int rows, int taps, int padl, int C, int N) {
+  const size_t CN = (size_t)C * N, kn = (size_t)taps * CN, n = (size_t)rows * N;
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
+    float v = 0.f;
+    if (i < kn) {
+      v = W[i];
+      if (R && i / CN == (size_t)padl) v += R[i - (size_t)padl * CN];
+    }
+    Weff[i] = (__bf16)v;
+    if (i < (size_t)N) bias[i] = bw[i] + (br ? br[i] : 0.f);
+  }
+}
+
+__global__ void to_bf16_kernel(const float* src, int M, int N, __bf16* dst, int ldd) {
+  const size_t n = (size_t)M * ldd;
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
+    const size_t m = i / ldd;
+    const int c = (int)(i - m * ldd);
+    dst[i] = (__bf16)(c < N ? src[m * N + c] : 0.f);
   }
 }
 
@@ -534,8 +611,39 @@ hipError_t maxpool_fwd(const float* out, float* pool, int B, int L, int C, hipSt
 
 hipError_t pool_mask_bwd(const float* out, const float* dpool, const float* dskip, float* dpre, int B, int L,
                          int C, hipStream_t s) {
-  hipLaunchKernelGGL(pool_mask_bwd_kernel, dim3(blocks_for((size_t)B * L * C)), dim3(kT), 0, s, out, dpool, dskip,
-                     dpre, B, L, C);
+  hipLaunchKernelGGL(pool_mask_bwd_kernel<float>, dim3(blocks_for((size_t)B * L * C)), dim3(kT), 0, s, out, dpool,
+                     dskip, dpre, B, L, C);
+  return hipGetLastError();
+}
+
+hipError_t pool_mask_bwd16(const float* out, const float* dpool, const float* dskip, __bf16* dpre, int B, int L, int C,
+                           hipStream_t s) {
+  hipLaunchKernelGGL(pool_mask_bwd_kernel<__bf16>, dim3(blocks_for((size_t)B * L * C)), dim3(kT), 0, s, out, dpool,
+                     dskip, dpre, B, L, C);
+  return hipGetLastError();
+}
+
+hipError_t im2col16(const ConvIn& ci, int B, const float* lab, const float* tim, const float* x1, const float* x2,
+                    __bf16* A, int ld, hipStream_t s) {
+  hipLaunchKernelGGL(im2col16_kernel, dim3(B * ci.lout()), dim3(kT), 0, s, ci, lab, tim, x1, x2, A, ld);
+  return hipGetLastError();
+}
+
+hipError_t col2im16(const ConvIn& ci, int B, const __bf16* dA, int ld, float* dlab, float* dtim, float* dx1,
+                    float* dx2, hipStream_t s) {
+  hipLaunchKernelGGL(col2im16_kernel, dim3(B * ci.Lsrc), dim3(kT), 0, s, ci, dA, ld, dlab, dtim, dx1, dx2);
+  return hipGetLastError();
+}
+
+hipError_t fold_weff16(const float* W, const float* bw, const float* R, const float* br, __bf16* Weff, float* bias,
+                       int rows, int taps, int padl, int C, int N, hipStream_t s) {
+  hipLaunchKernelGGL(fold_weff16_kernel, dim3(blocks_for((size_t)rows * N)), dim3(kT), 0, s, W, bw, R, br, Weff, bias,
+                     rows, taps, padl, C, N);
+  return hipGetLastError();
+}
+
+hipError_t to_bf16(const float* src, int M, int N, __bf16* dst, int ldd, hipStream_t s) {
+  hipLaunchKernelGGL(to_bf16_kernel, dim3(blocks_for((size_t)M * ldd)), dim3(kT), 0, s, src, M, N, dst, ldd);
   return hipGetLastError();
 }
 

@@ -207,10 +207,16 @@ class ImprovedDDPM:
         return h
 
     # ------------------------------------------------------------------ training (8(f) row 4)
-    def compile(self, optimizer=None, loss='MeanSquaredError', **kwargs):
-        """keras Model.compile as used by the reference (main_script.py:233-234)."""
-        from .training import Adam, _Mean
+    def compile(self, optimizer=None, loss='MeanSquaredError', precision='float32', activation_checkpoint=None,
+                **kwargs):
+        """keras Model.compile as used by the reference (main_script.py:233-234).
+
+        ``precision='bfloat16'`` trains with bf16 products (fp32 weights, gradients and optimizer);
+        ``activation_checkpoint='e4m3'`` then keeps the products' inputs in 8 bits for the backward pass."""
+        from .training import Adam, _Mean, check_precision
+        check_precision(precision, activation_checkpoint)
         self._sync_trained_weights()
+        self.precision, self.activation_checkpoint = precision, activation_checkpoint
         name = loss if isinstance(loss, str) else getattr(loss, '__name__', type(loss).__name__)
         if str(name).replace('_', '').lower() not in ('meansquarederror', 'mse'):
             raise NotImplementedError('only the MeanSquaredError loss of the reference is supported')
@@ -232,7 +238,7 @@ class ImprovedDDPM:
             raise RuntimeError('call compile(optimizer=...) before training')
         if self._trainer is None:
             self._sync_trained_weights()
-            self._trainer = Trainer(self, self.optimizer)
+            self._trainer = Trainer(self, self.optimizer, self.precision, self.activation_checkpoint)
         return self._trainer
 
     def _sync_trained_weights(self):

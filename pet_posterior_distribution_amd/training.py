@@ -15,7 +15,10 @@ diff_model.fit(x, y, batch_size, epochs, ...)     ``ImprovedDDPM.fit`` (main_scr
 
 The step runs in libpetdiff.so (include/pettrain.h): fp32 U-Net forward and
 backward (rocBLAS GEMMs + HIP kernels), loss = MSE + lambda_vlb * VLB, per-variable
-clip and Adam.  There is no CPU path.
+clip and Adam.  ``compile(..., precision='bfloat16')`` takes the convolutions and the
+condition encoder through the dense layer's operators (include/petdense.h, layers.py) in
+bf16, and ``activation_checkpoint='e4m3'`` keeps their inputs in 8 bits for the backward
+pass; weights, gradients and Adam stay fp32.  There is no CPU path.
 """
 from __future__ import annotations
 
@@ -127,10 +130,27 @@ def check(rc, what):
     raise _lib.PetdiffError(f'{what}: {msg}')
 
 
-class Trainer:
-    """Owns one pettrain handle (fp32 weights, gradients, Adam moments on the GPU)."""
+PRECISIONS = {'float32': 0, 'bfloat16': 1}               # PETTRAIN_F32, PETTRAIN_BF16
+CHECKPOINTS = {None: 0, 'e4m3': 1}                         # PETTRAIN_KEEP, PETTRAIN_KEEP_E4M3
 
-    def __init__(self, model, optimizer):
+
+def check_precision(precision, activation_checkpoint):
+    if precision not in PRECISIONS:
+        raise ValueError(f'precision must be one of {sorted(PRECISIONS)}, got {precision!r}')
+    if activation_checkpoint not in CHECKPOINTS:
+        raise ValueError(f"activation_checkpoint must be None or 'e4m3', got {activation_checkpoint!r}")
+    if activation_checkpoint is not None and precision != 'bfloat16':
+        raise ValueError("activation_checkpoint needs precision='bfloat16'")
+
+
+class Trainer:
+    """Owns one pettrain handle (fp32 weights, gradients, Adam moments on the GPU).
+
+    ``precision``: 'float32', or 'bfloat16' for the products of the convolutions and the condition encoder;
+    ``activation_checkpoint='e4m3'`` keeps their inputs in 8 bits between the passes (pettrain_set_precision)."""
+
+    def __init__(self, model, optimizer, precision='float32', activation_checkpoint=None):
+        check_precision(precision, activation_checkpoint)
         self.model = model
         self.device = model.device
         net = model.network
@@ -147,6 +167,8 @@ class Trainer:
                                          self.device.index, C.byref(h)), 'pettrain_create')
         self.handle = h
         self.n_weights = blob.size
+        check(_lib.lib().pettrain_set_precision(h, PRECISIONS[precision], CHECKPOINTS[activation_checkpoint]),
+              'pettrain_set_precision')
 
     def close(self):
         if self.handle is not None:
@@ -158,6 +180,11 @@ class Trainer:
             self.close()
         except Exception:
             pass
+
+    @property
+    def step_bytes(self):
+        """Device bytes held for a step at the largest batch so far (activations, gradients of them, workspaces)."""
+        return int(_lib.lib().pettrain_step_bytes(self.handle))
 
     @property
     def iterations(self):

@@ -139,3 +139,14 @@ def test_row_views():
     v, ld = rows(torch.zeros(10)[::2], 'x')
     assert v.is_contiguous() and ld == 5
     assert rows(torch.zeros(0, 5), 'x')[1] == 5
+
+
+def test_training_precisions_are_checked():
+    from pet_posterior_distribution_amd.training import check_precision
+    check_precision('float32', None)
+    check_precision('bfloat16', None)
+    check_precision('bfloat16', 'e4m3')
+    for bad in (('float16', None), ('bf16', None), ('bfloat16', 'int8'), ('float32', 'e4m3')):
+        with pytest.raises(ValueError):
+            check_precision(*bad)
+    assert L.pettrain_set_precision(None, 0, 0) == INVALID and L.pettrain_step_bytes(None) == 0
