@@ -46,19 +46,23 @@ struct Plan {
 
 // What a kind of tile costs, in microseconds, as measured on products of 64 .. 12288 rows.  A step (128 bytes of
 // contraction) takes `wait` when its workgroup has a compute unit to itself, and `share` per workgroup when several
-// fill it; `ends` is a workgroup's first load and its epilogue.  [operands by DMA, operands through registers]
+// fill it; `ends` is a workgroup's first load and its epilogue.  [operands by DMA, through registers, dP formed there]
 struct Cost {
   int tile, b, slots, k;   // b: rows and columns of the tile; slots: workgroups of a compute unit; k: steps at a time
-  double wait[2], share[2], ends;
+  double wait[3], share[3], ends;
 };
-constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.45, 1.45}, {1.45, 1.45}, 8.0},
-                             {kMid, 128, 2, 1, {0.65, 1.0}, {0.46, 0.8}, 3.5},
-                             {kSmall, 64, 4, 1, {0.28, 0.5}, {0.19, 0.3}, 2.0},
-                             {kSlice, 32, 1, 8, {0.7, 0.9}, {0.7, 0.9}, 2.5}};
-constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 6.9}, {6.9, 6.9}, 10.0},
-                             {kMid, 128, 2, 1, {2.3, 2.5}, {2.1, 2.3}, 4.0},
-                             {kSmall, 64, 4, 1, {0.65, 0.8}, {0.53, 0.65}, 2.0},
-                             {kSlice, 32, 1, 8, {1.2, 1.4}, {1.2, 1.4}, 2.5}};
+constexpr int kFormed = 2;
+constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.45, 0, 0}, {1.45, 0, 0}, 8.0},
+                             {kMid, 128, 2, 1, {0.65, 1.25, 0}, {0.46, 1.25, 0}, 3.5},
+                             {kSmall, 64, 4, 1, {0.28, 0.55, 1.1}, {0.19, 0.34, 0.7}, 2.0},
+                             {kSlice, 32, 1, 8, {1.0, 1.6, 2.6}, {1.0, 1.6, 2.6}, 2.0},
+                             {kSlice64, 64, 1, 4, {0.75, 2.4, 0}, {0.75, 2.4, 0}, 3.5}};
+constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 0, 0}, {6.9, 0, 0}, 10.0},
+                             {kMid, 128, 2, 1, {2.3, 2.7, 0}, {2.1, 2.5, 0}, 4.0},
+                             {kSmall, 64, 4, 1, {0.75, 0.95, 1.6}, {0.53, 0.65, 1.2}, 2.0},
+                             {kSlice, 32, 1, 8, {1.3, 2.2, 3.5}, {1.3, 2.2, 3.5}, 2.0},
+                             {kSlice64, 64, 1, 4, {2.75, 4.5, 0}, {2.75, 4.5, 0}, 3.5}};
+constexpr double kNever = 1e30;      // no plan
 constexpr double kLaunch = 2.5;      // a launch behind another
 constexpr int kUnits = 256;
 
@@ -103,7 +107,7 @@ Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader, bool q8 = false
     if (c.tile == kLarge && (loader != kDma || q8)) continue;
     const int64_t tiles = ceil_div(I, c.b) * ceil_div(J, c.b);
     for_splits(steps, 64, [&](int64_t s, int64_t per) {
-      const double t = product_us(c, tiles * s, per, loader) + join_us(I, J, s);
+      const double t = product_us(c, tiles * s, per, q8 ? kReg : loader) + join_us(I, J, s);
       if (best.c_per && t >= best.us) return;
       best.us = t;
       set_plan(best, c, s, per, bc, I, J);
@@ -112,27 +116,29 @@ Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader, bool q8 = false
   return best;
 }
 
-// The backward pass's two products as one launch (x: I = m, J = k, C = n; k: I = k, J = n, C = m), both with the same
-// kind of tile; only the kernel gradient's contraction is split.
-double plan_pair(int64_t m, int64_t k, int64_t n, int type, int lx, int lk, Plan& px, Plan& pk) {
+// The backward pass as one launch, or kNever where it has too many tiles for that (x: I = m, J = k, C = n; k: I = k, J = n, C = m), both products with the same kind of
+// tile; only the kernel gradient's contraction is split.  nx, nk: which products are wanted.
+double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, int lx, int lk, bool slice64,
+                 Plan& px, Plan& pk) {
   const int bc = type == kF32 ? 32 : 64;
   const int64_t sx = ceil_div(n, bc), sk = ceil_div(m, bc);
-  double best = -1;
+  double best = kNever;
   for (const Cost& c : type == kF32 ? kCosts32 : kCosts16) {
-    if (c.tile != kSmall && c.tile != kSlice) continue;
-    const int64_t tx = ceil_div(m, c.b) * ceil_div(k, c.b), tk = ceil_div(k, c.b) * ceil_div(n, c.b);
+    if (c.tile == kLarge || c.tile == kMid || (c.tile == kSlice64 && !slice64)) continue;
+    const int64_t tx = nx ? ceil_div(m, c.b) * ceil_div(k, c.b) : 0, tk = nk ? ceil_div(k, c.b) * ceil_div(n, c.b) : 0;
     if (tx > 16384 || tk > 16384) continue;
-    for_splits(sk, 64, [&](int64_t s, int64_t per) {
-      const double wx = (double)ceil_div(sx, c.k), wk = (double)ceil_div(per, c.k);
+    for_splits(nk ? sk : 1, 64, [&](int64_t s, int64_t per) {
+      const double wx = nx ? (double)ceil_div(sx, c.k) : 0, wk = nk ? (double)ceil_div(nk ? per : 0, c.k) : 0;
       const double groups = (double)(tx + tk * s);
       const double share = ((double)tx * (wx * c.share[lx] + c.ends / c.slots) +
                             (double)tk * s * (wk * c.share[lk] + c.ends / c.slots)) / kUnits;
       const double longest = std::max(wx * c.wait[lx], wk * c.wait[lk]) + c.ends;
       const double t = kLaunch + std::max(longest, share * (groups > kUnits * c.slots ? 1.1 : 1.0)) + join_us(k, n, s);
-      if (best >= 0 && t >= best) return;
+      if (t >= best) return;
       best = t;
       set_plan(px, c, 1, sx, bc, m, k);
       set_plan(pk, c, s, per, bc, k, n);
+      if (!nk) pk.splits = 1, pk.part_bytes = 0;
     });
   }
   return best;
@@ -143,6 +149,8 @@ bool dma_ok(const void* p, int64_t ld, int64_t contiguous, int size) {
          ld * size < (int64_t)0x7fffffff / 256;          // a tile's offsets fit 31 bits
 }
 
+bool planned(const Plan& p, int64_t C) { return p.c_per > 0 && (int64_t)p.splits * p.c_per >= C && (p.splits - 1) * (int64_t)p.c_per < C; }
+
 Product placed(Product p, const Plan& pl, void* part) {
   p.splits = pl.splits;
   p.c_per = pl.c_per;
@@ -152,6 +160,7 @@ Product placed(Product p, const Plan& pl, void* part) {
 
 int run_product(const Product& of, int layout, int loader, int type, int q8, const Plan& pl, void* part,
                 hipStream_t s) {
+  if (!planned(pl, of.C)) return fail(PETDIFF_ERR_HIP, "internal: a product without a plan");
   const Product p = placed(of, pl, part);
   HIPC(type == kF32    ? product_f32(p, layout, loader, pl.tile, q8, s)
        : type == kBF16 ? product_bf16(p, layout, loader, pl.tile, q8, s)
@@ -186,18 +195,64 @@ int check_forward(const petdense_forward_args* a) {
   return PETDIFF_OK;
 }
 
+// A copy of an operand that DMA can stage: its place in the workspace, or none.
+struct Copy {
+  bool on = false;
+  size_t at = 0;
+  int64_t ld = 0;
+};
+
+int64_t padded(int64_t n, int size) { return ceil_div(n, 16 / size) * (16 / size); }
+// (one launch copies at most 2^31 pieces of 16 bytes)
+bool copies_fit(double values, int size) { return values * size / 16 < 2e9; }
+// read and written once, by a launch of its own
+double copy_us(int64_t rows, int64_t n, int size) { return (double)rows * n * size * 2 / 3.5e6; }
+constexpr double kCopyLaunch = kLaunch + 1.5;
+
+Copy copy_of(bool on, int64_t rows, int64_t n, int size, size_t& o) {
+  Copy c;
+  if (!on) return c;
+  c.on = true;
+  c.at = o;
+  c.ld = padded(n, size);
+  o += up((size_t)rows * c.ld * size);
+  return c;
+}
+
+PadJob job_of(const Copy& c, const void* src, int64_t ld, int64_t rows, int64_t n, char* w) {
+  return c.on ? PadJob{src, w + c.at, ld, c.ld, (int)rows, (int)n} : PadJob{};
+}
+
 struct ForwardPlan {
   Plan p;
   int loader;
   bool rows;
+  Copy x, kernel;
+  size_t o_part, bytes;
 };
 
 ForwardPlan plan_forward(const petdense_forward_args* a) {
   ForwardPlan f{};
-  const int sz = size_of(a->dtype);
-  f.loader = dma_ok(a->x, a->ldx, a->k, sz) && dma_ok(a->kernel, a->ldk, a->n, sz) ? kDma : kReg;
   f.rows = a->m <= kMaxRows;
-  if (!f.rows && a->m > 0) f.p = plan(a->m, a->n, a->k, a->dtype, f.loader);
+  if (f.rows || a->m == 0) return f;
+  const int sz = size_of(a->dtype);
+  const bool x_ok = dma_ok(a->x, a->ldx, a->k, sz), w_ok = dma_ok(a->kernel, a->ldk, a->n, sz);
+  f.loader = x_ok && w_ok ? kDma : kReg;
+  f.p = plan(a->m, a->n, a->k, a->dtype, f.loader);
+  size_t o = 0;
+  if (f.loader == kReg) {
+    const Plan q = plan(a->m, a->n, a->k, a->dtype, kDma);
+    const double t = q.us + kCopyLaunch + (x_ok ? 0 : copy_us(a->m, a->k, sz)) + (w_ok ? 0 : copy_us(a->k, a->n, sz));
+    // (x's rows are filled up with zeros; rows past the kernel's last are not read, which stages zeros too)
+    if (t < f.p.us && copies_fit((double)a->k * (a->m + a->n), sz)) {
+      f.p = q;
+      f.loader = kDma;
+      f.x = copy_of(!x_ok, a->m, a->k, sz, o);
+      f.kernel = copy_of(!w_ok, a->k, a->n, sz, o);
+    }
+  }
+  f.o_part = o;
+  f.bytes = o + f.p.part_bytes;
   return f;
 }
 
@@ -229,64 +284,101 @@ int check_backward(const petdense_backward_args* a) {
 }
 
 struct BackwardPlan {
-  const void* dp;          // what the products read: dy, dresidual or the workspace
-  int64_t lddp;
-  bool make_dp;            // dp is made by act_grad
+  bool make_dp;            // dp is made by act_grad: in dresidual or in the workspace
   bool sums;               // column sums wanted
+  bool fused;              // one launch for everything: dp is never in memory
+  bool pair;               // one launch for both products and the bias gradient's join
   int chunks;
   Plan px, pk;
-  bool pair;               // one launch for both products and the bias gradient's join
   int load_x, load_k;
+  Copy dp, x, kernel;      // copies for DMA (dp: of dy or dresidual)
+  int64_t ld_dp;           // make_dp without dresidual: row stride of dp
   size_t o_dp, o_sums, o_part, bytes;
+  double us;
 };
 
-BackwardPlan plan_backward(const petdense_backward_args* a, void* work) {
-  BackwardPlan b{};
-  const int sz = size_of(a->dtype);
-  char* w = static_cast<char*>(work);
-  size_t o = 0;
-  b.make_dp = a->activation != PETDENSE_NONE || a->dresidual;
-  b.sums = a->dbias != nullptr;
-  b.dp = a->dy;
-  b.lddp = a->lddy;
-  if (b.make_dp) {
-    if (a->dresidual) {
-      b.dp = a->dresidual;
-      b.lddp = a->lddr;
-    } else {
-      b.lddp = ceil_div(a->n, 64) * 64;
-      b.o_dp = o;
-      b.dp = w + o;
-      o += up((size_t)a->m * b.lddp * sz);
-    }
-  }
-  // row chunks of the activation's gradient: about 1024 workgroups, each of two rounds of its rows at least
-  const int lanes = act_grad_lanes((int)a->n);
-  const int64_t most = std::max<int64_t>(1, 1024 / ceil_div(a->n, lanes * 8));
-  b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, ceil_div(a->m, 2 * 256 / lanes)));
-  if (b.sums) {
-    b.o_sums = o;
-    o += up((size_t)b.chunks * a->n * 4);
-  }
-  const void* base = work ? b.dp : (b.make_dp && !a->dresidual ? nullptr : b.dp);
-  if (a->dx) {
-    b.load_x = dma_ok(base, b.lddp, a->n, sz) && dma_ok(a->kernel, a->ldk, a->n, sz) ? kDma : kReg;
-    b.px = plan(a->m, a->k, a->n, a->dtype, b.load_x);
-  }
-  if (a->dkernel) {
-    // 8-bit inputs go through registers whatever their alignment: `loader` is dp's
-    b.load_k = dma_ok(base, b.lddp, a->n, sz) && (a->x_exponents || dma_ok(a->x, a->ldx, a->k, sz)) ? kDma : kReg;
-    b.pk = plan(a->k, a->n, a->m, a->dtype, b.load_k, a->x_exponents != nullptr);
-  }
+// The products from operands that are in memory (lx, lk: their loaders): one launch or two.
+double plan_products(const petdense_backward_args* a, int lx, int lk, BackwardPlan& b) {
+  const bool q8 = a->x_exponents;
+  b.load_x = lx;
+  b.load_k = lk;
+  b.px = b.pk = Plan{};
+  b.pair = false;
+  if (a->dx) b.px = plan(a->m, a->k, a->n, a->dtype, lx);
+  if (a->dkernel) b.pk = plan(a->k, a->n, a->m, a->dtype, lk, q8);
+  double us = b.px.us + b.pk.us + (b.sums ? kLaunch : 0.0);
   if (a->dx && a->dkernel) {
     Plan px, pk;
-    const double t = plan_pair(a->m, a->k, a->n, a->dtype, b.load_x, b.load_k, px, pk);
-    if (t >= 0 && t < b.px.us + b.pk.us + (b.sums ? kLaunch : 0.0)) {
+    const double t = plan_pair(true, true, a->m, a->k, a->n, a->dtype, lx, q8 ? kReg : lk, true, px, pk);
+    if (t < us) {
+      us = t;
       b.pair = true;
       b.px = px;
       b.pk = pk;
     }
   }
+  return us;
+}
+
+BackwardPlan plan_backward(const petdense_backward_args* a) {
+  BackwardPlan b{};
+  const int sz = size_of(a->dtype);
+  const bool q8 = a->x_exponents;
+  b.make_dp = a->activation != PETDENSE_NONE || a->dresidual;
+  b.sums = a->dbias != nullptr;
+  const bool own_dp = b.make_dp && !a->dresidual;
+  // row chunks of the activation's gradient: about 1024 workgroups, each of two rounds of its rows at least
+  const int lanes = act_grad_lanes((int)a->n);
+  const int64_t most = std::max<int64_t>(1, 1024 / ceil_div(a->n, lanes * 8));
+  b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, ceil_div(a->m, 2 * 256 / lanes)));
+  const double act_us =
+      b.make_dp || b.sums ? kLaunch + 2.0 + (double)a->m * a->n * sz * (b.make_dp ? 3 : 1) / 4e6 : 0.0;
+
+  // dp in the workspace has rows of whole pieces, with zeros: DMA takes it as it is
+  const bool dp_ok = own_dp || (a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz) : dma_ok(a->dy, a->lddy, a->n, sz));
+  const bool w_ok = !a->dx || dma_ok(a->kernel, a->ldk, a->n, sz);
+  const bool x_ok = !a->dkernel || q8 || dma_ok(a->x, a->ldx, a->k, sz);
+  // 8-bit inputs go through registers whatever their alignment: their loader is dp's
+  b.us = act_us + plan_products(a, dp_ok && w_ok ? kDma : kReg, dp_ok && x_ok ? kDma : kReg, b);
+  if (!(dp_ok && w_ok && x_ok) && (a->dx || a->dkernel) &&
+      copies_fit((double)a->m * a->n + (double)a->k * a->n + (double)a->m * a->k, sz)) {
+    BackwardPlan c = b;
+    c.us = act_us + plan_products(a, kDma, kDma, c) + kCopyLaunch + (dp_ok ? 0 : copy_us(a->m, a->n, sz)) +
+           (w_ok ? 0 : copy_us(a->k, a->n, sz)) + (x_ok ? 0 : copy_us(a->m, a->k, sz));
+    if (c.us < b.us) {
+      b = c;
+      b.dp.on = !dp_ok;
+      b.kernel.on = !w_ok;
+      b.x.on = !x_ok;
+    }
+  }
+  if ((a->dx || a->dkernel) && (b.make_dp || b.sums) && !a->dresidual) {
+    Plan px, pk;
+    double t = plan_pair(a->dx, a->dkernel, a->m, a->k, a->n, a->dtype, kFormed, kFormed, false, px, pk);
+    // a sum's workgroup walks all rows: 256 at a time, 4 of them in flight
+    if (b.sums) t = std::max(t, kLaunch + 2.5 + 0.7 * (double)a->m / 256);
+    if (t < b.us) {
+      b.us = t;
+      b.fused = true;
+      b.pair = false;
+      b.px = px;
+      b.pk = pk;
+      b.dp.on = b.x.on = b.kernel.on = false;
+    }
+  }
+  size_t o = 0;
+  if (own_dp && !b.fused) {
+    b.ld_dp = ceil_div(a->n, 64) * 64;
+    b.o_dp = o;
+    o += up((size_t)a->m * b.ld_dp * sz);
+  }
+  if (b.sums && !b.fused) {
+    b.o_sums = o;
+    o += up((size_t)b.chunks * a->n * 4);
+  }
+  b.dp = copy_of(b.dp.on, a->m, a->n, sz, o);
+  b.kernel = copy_of(b.kernel.on, a->k, a->n, sz, o);
+  b.x = copy_of(b.x.on, a->m, a->k, sz, o);
   b.o_part = o;
   b.bytes = o + std::max(b.px.part_bytes, b.pk.part_bytes);
   return b;
@@ -300,14 +392,14 @@ const char* petdense_last_error(void) { return g_err.c_str(); }
 
 size_t petdense_forward_workspace(const petdense_forward_args* a) {
   if (check_forward(a) != PETDIFF_OK || a->m == 0) return 0;
-  return plan_forward(a).p.part_bytes;
+  return plan_forward(a).bytes;
 }
 
 int petdense_forward(const petdense_forward_args* a, void* work, size_t work_bytes, void* stream) {
   if (int r = check_forward(a)) return r;
   if (a->m == 0) return PETDIFF_OK;
   const ForwardPlan f = plan_forward(a);
-  NEED(work_ok(work, work_bytes, f.p.part_bytes), "the workspace is missing, too small or not 256-byte aligned");
+  NEED(work_ok(work, work_bytes, f.bytes), "the workspace is missing, too small or not 256-byte aligned");
   Product p{};
   p.A = a->x;
   p.lda = a->ldx;
@@ -321,12 +413,19 @@ int petdense_forward(const petdense_forward_args* a, void* work, size_t work_byt
     HIPC(rows(p, a->dtype, (hipStream_t)stream));
     return PETDIFF_OK;
   }
-  return run_product(p, kForward, f.loader, a->dtype, 0, f.p, work, (hipStream_t)stream);
+  char* w = static_cast<char*>(work);
+  if (f.x.on || f.kernel.on) {
+    HIPC(pad(PadJobs{{job_of(f.x, a->x, a->ldx, a->m, a->k, w), job_of(f.kernel, a->kernel, a->ldk, a->k, a->n, w), {}}},
+             a->dtype, (hipStream_t)stream));
+    if (f.x.on) p.A = w + f.x.at, p.lda = f.x.ld;
+    if (f.kernel.on) p.B = w + f.kernel.at, p.ldb = f.kernel.ld;
+  }
+  return run_product(p, kForward, f.loader, a->dtype, 0, f.p, w + f.o_part, (hipStream_t)stream);
 }
 
 size_t petdense_backward_workspace(const petdense_backward_args* a) {
   if (check_backward(a) != PETDIFF_OK || a->m == 0) return 0;
-  return plan_backward(a, nullptr).bytes;
+  return plan_backward(a).bytes;
 }
 
 int petdense_backward(const petdense_backward_args* a, void* work, size_t work_bytes, void* stream) {
@@ -338,34 +437,48 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     if (a->dbias) HIPC(fill_zero(a->dbias, 1, a->n, a->n, gsz, s));
     return PETDIFF_OK;
   }
-  const BackwardPlan b = plan_backward(a, work);
+  const BackwardPlan b = plan_backward(a);
   NEED(work_ok(work, work_bytes, b.bytes), "the workspace is missing, too small or not 256-byte aligned");
   char* w = static_cast<char*>(work);
   float* sums = b.sums ? reinterpret_cast<float*>(w + b.o_sums) : nullptr;
-  if (b.make_dp || b.sums)
-    HIPC(act_grad(a->dy, a->lddy, a->activation == PETDENSE_NONE ? nullptr : a->saved, a->lds,
-                  b.make_dp ? const_cast<void*>(b.dp) : nullptr, b.lddp, sums, b.chunks, (int)a->m, (int)a->n, a->dtype,
-                  a->activation, s));
+  const void* dp = a->dy;
+  int64_t lddp = a->lddy, n_dp = a->n;      // n_dp: dp's columns with the zeros behind them
+  if (!b.fused && (b.make_dp || b.sums)) {
+    void* made = nullptr;
+    if (b.make_dp) {
+      made = a->dresidual ? a->dresidual : w + b.o_dp;
+      lddp = a->dresidual ? a->lddr : b.ld_dp;
+      dp = made;
+    }
+    HIPC(act_grad(a->dy, a->lddy, a->activation == PETDENSE_NONE ? nullptr : a->saved, a->lds, made, lddp,
+                  made && a->dresidual, sums, b.chunks, (int)a->m, (int)a->n, a->dtype, a->activation, s));
+  }
+  if (b.dp.on || b.kernel.on || b.x.on)
+    HIPC(pad(PadJobs{{job_of(b.dp, dp, lddp, a->m, a->n, w), job_of(b.kernel, a->kernel, a->ldk, a->k, a->n, w),
+                      job_of(b.x, a->x, a->ldx, a->m, a->k, w)}},
+             a->dtype, s));
+  if (b.dp.on) dp = w + b.dp.at, lddp = b.dp.ld;
+  if (b.load_x == kDma) n_dp = padded(a->n, size_of(a->dtype));
   const ColumnJoin cols{sums, a->dbias, b.chunks, b.sums ? (int)a->n : 0, a->grad_f32 ? kF32 : a->dtype};
   Product x{}, k{};
   if (a->dx) {
-    x.A = b.dp;
-    x.lda = b.lddp;
-    x.B = a->kernel;
-    x.ldb = a->ldk;
+    x.A = dp;
+    x.lda = lddp;
+    x.B = b.kernel.on ? w + b.kernel.at : a->kernel;
+    x.ldb = b.kernel.on ? b.kernel.ld : a->ldk;
     x.I = (int)a->m;
     x.J = (int)a->k;
-    x.C = (int)a->n;
+    x.C = (int)n_dp;
     x.e.out = a->dx;
     x.e.ldo = a->lddx;
   }
   if (a->dkernel) {
-    k.A = a->x;
-    k.lda = a->ldx;
+    k.A = b.x.on ? w + b.x.at : a->x;
+    k.lda = b.x.on ? b.x.ld : a->ldx;
     k.exps = a->x_exponents;
     k.lde = a->lde;
-    k.B = b.dp;
-    k.ldb = b.lddp;
+    k.B = dp;
+    k.ldb = lddp;
     k.I = (int)a->k;
     k.J = (int)a->n;
     k.C = (int)a->m;
@@ -374,6 +487,28 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     k.e.out_f32 = a->grad_f32;
   }
   const int q8 = a->x_exponents != nullptr;
+  if (b.fused || b.pair)
+    if ((a->dx && !planned(b.px, a->n)) || (a->dkernel && !planned(b.pk, a->m)))
+      return fail(PETDIFF_ERR_HIP, "internal: a product without a plan");
+  if (b.fused) {
+    const void* saved = a->activation == PETDENSE_NONE ? nullptr : a->saved;
+    Pair p{};
+    p.x = placed(x, b.px, nullptr);
+    p.k = placed(k, b.pk, w + b.o_part);
+    p.x.C = (int)a->n;
+    p.x.A = p.k.B = a->dy;
+    p.x.lda = p.k.ldb = a->lddy;
+    p.x.saved = p.k.saved = saved;
+    p.x.lds = p.k.lds = a->lds;
+    p.x.saved_act = p.k.saved_act = a->activation;
+    p.sums = ColumnSum{a->dy, saved, a->dbias, a->lddy, a->lds, (int)a->m, b.sums ? (int)a->n : 0, a->activation,
+                       cols.out_type};
+    HIPC(a->dtype == kF32    ? fused_f32(p, b.px.tile, q8, s)
+         : a->dtype == kBF16 ? fused_bf16(p, b.px.tile, q8, s)
+                             : fused_f16(p, b.px.tile, q8, s));
+    if (a->dkernel && b.pk.splits > 1) HIPC(join(p.k, a->dtype, s));
+    return PETDIFF_OK;
+  }
   if (b.pair) {
     Pair p{};
     p.x = placed(x, b.px, nullptr);

@@ -117,6 +117,74 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, int64_t i, int64_t 
   else store_row<T, 8>(static_cast<T*>(e.out) + i * e.ldo + j, n, v);
 }
 
+// g[q] = g[q] act'(v[q]) for W values, one uniform branch
+template <bool EXACT, int W>
+__device__ __forceinline__ void activate_grads(float* g, const float* v, int act) {
+  if (act == kRelu) {
+#pragma unroll
+    for (int q = 0; q < W; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], kRelu);
+  } else if (act == kGelu) {
+#pragma unroll
+    for (int q = 0; q < W; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], kGelu);
+  } else if (act == kSilu) {
+#pragma unroll
+    for (int q = 0; q < W; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], kSilu);
+  }
+}
+
+// Sums 8 columns of dy act'(saved) over all rows: a thread takes every THREADS-th row; the rows meet by shuffles, the
+// waves in LDS, in a fixed order.
+template <typename T, int THREADS>
+__device__ __forceinline__ void sum_columns8(const ColumnSum& p, int block, int t, float* red) {
+  constexpr int W = 8, AHEAD = 4;
+  const int j = block * W, n = p.N - j;
+  const T* dy = static_cast<const T*>(p.dy) + j;
+  const T* sv = static_cast<const T*>(p.saved) + j;
+  float sum[W];
+#pragma unroll
+  for (int q = 0; q < W; ++q) sum[q] = 0.f;
+  int64_t m = t;
+  if (n >= W) {
+    for (; m + (AHEAD - 1) * THREADS < p.M; m += AHEAD * THREADS) {
+      float g[AHEAD][W], v[AHEAD][W];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        load_row<T, W>(dy + (m + u * THREADS) * p.ldy, W, g[u]);
+        if (p.act != kNone) load_row<T, W>(sv + (m + u * THREADS) * p.lds, W, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        activate_grads<sizeof(T) == 4, W>(g[u], v[u], p.act);
+#pragma unroll
+        for (int q = 0; q < W; ++q) sum[q] += g[u][q];
+      }
+    }
+  }
+  for (; m < p.M; m += THREADS) {
+    float g[W], v[W];
+    load_row<T, W>(dy + m * p.ldy, n, g);
+    if (p.act != kNone) load_row<T, W>(sv + m * p.lds, n, v);
+    activate_grads<sizeof(T) == 4, W>(g, v, p.act);
+#pragma unroll
+    for (int q = 0; q < W; ++q) sum[q] += g[q];
+  }
+#pragma unroll
+  for (int q = 0; q < W; ++q) {
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) sum[q] += __shfl_xor(sum[q], o);
+    if ((t & 63) == 0) red[(t >> 6) * W + q] = sum[q];
+  }
+  __syncthreads();
+  if (t < W && t < n) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) s += red[w * W + t];
+    if (p.out_type == kF32) static_cast<float*>(p.out)[j + t] = s;
+    else if (p.out_type == kBF16) static_cast<__bf16*>(p.out)[j + t] = (__bf16)s;
+    else static_cast<_Float16*>(p.out)[j + t] = (_Float16)s;
+  }
+}
+
 // Sums 16 columns of a column join: thread t < 256 takes column t % 16 of the chunks t / 16, t / 16 + 16, ..; the 16
 // groups meet in LDS, in order.  Every thread of the workgroup comes here.
 __device__ __forceinline__ void join_columns16(const ColumnJoin& p, int block, int t, float* red) {

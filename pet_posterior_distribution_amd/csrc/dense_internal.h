@@ -28,6 +28,11 @@ struct Product {
   int64_t lda, ldb;
   const uint8_t* exps;   // A held in 8 bits: exponent bytes [C][I / 32] (row stride lde)
   int64_t lde;
+  // the operand dP = dy act'(saved), formed while it is staged: `saved` beside A (input gradient) or B (kernel
+  // gradient), row stride lds
+  const void* saved;
+  int64_t lds;
+  int saved_act;
   int I, J, C;
   int splits, c_per;     // contraction split into `splits` parts of c_per (a multiple of the k-step)
   float* part;           // [splits][I][J] fp32 when splits > 1 (the epilogue is then the joining kernel's)
@@ -36,7 +41,7 @@ struct Product {
 
 enum Layout { kForward = 0, kInputGrad = 1, kKernelGrad = 2 };   // (A, B): (c-, j-), (c-, c-), (i-, j-contiguous)
 enum Loader { kDma = 0, kReg = 1 };
-enum Tile { kLarge = 0, kMid = 1, kSmall = 2, kSlice = 3 };
+enum Tile { kLarge = 0, kMid = 1, kSmall = 2, kSlice = 3, kSlice64 = 4 };
 
 // out[n] = sum over chunks of part[chunk][n], in order
 struct ColumnJoin {
@@ -46,10 +51,21 @@ struct ColumnJoin {
   int out_type;
 };
 
-// The backward pass's products and its bias gradient as one launch (kSmall, kSlice).
+// out[n] = sum over rows of dy act'(saved), straight from the inputs
+struct ColumnSum {
+  const void* dy;
+  const void* saved;
+  void* out;
+  int64_t ldy, lds;
+  int M, N, act;         // N = 0: no sums wanted
+  int out_type;
+};
+
+// The backward pass's products and its bias gradient as one launch (kSmall, kSlice, kSlice64).
 struct Pair {
   Product x, k;
-  ColumnJoin cols;
+  ColumnJoin cols;       // pair: the sums' parts are there (act_grad)
+  ColumnSum sums;        // fused: they are made here
   int nx, nk;            // workgroups of each (the launcher's)
 };
 
@@ -61,6 +77,10 @@ hipError_t product_f16(const Product& p, int layout, int loader, int tile, int q
 hipError_t pair_f32(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s);
 hipError_t pair_bf16(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s);
 hipError_t pair_f16(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s);
+// The whole backward pass as one launch: dP is formed while the products stage it (all operands through registers).
+hipError_t fused_f32(const Pair& p, int tile, int q8, hipStream_t s);
+hipError_t fused_bf16(const Pair& p, int tile, int q8, hipStream_t s);
+hipError_t fused_f16(const Pair& p, int tile, int q8, hipStream_t s);
 
 // Joins split products: the sum of p.part over the splits, in order, through the epilogue.
 hipError_t join(const Product& p, int type, hipStream_t s);
@@ -76,9 +96,22 @@ inline int act_grad_lanes(int N) {
   return l;
 }
 
-// dp = dy act'(saved) (dp may be null), part[chunk][n] = column sums of dp over the chunk's rows (may be null)
-hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, float* part,
-                    int chunks, int M, int N, int type, int act, hipStream_t s);
+// Copies whose rows start and end on 16 bytes, zeros behind their values: DMA stages them whatever the source's
+// alignment.  Up to three matrices a launch.
+struct PadJob {
+  const void* src;
+  void* dst;
+  int64_t ld, ldd;       // ldd: values of a row with its zeros, a multiple of 16 bytes
+  int rows, n;           // rows = 0: no job
+};
+struct PadJobs {
+  PadJob job[3];
+};
+hipError_t pad(const PadJobs& p, int type, hipStream_t s);
+
+// dp = dy act'(saved) (dp may be null, its rows hold zeros up to a multiple of 8 columns, unless `bare`), part[chunk][n] = column sums of dp over the chunk's rows (may be null)
+hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, int bare,
+                    float* part, int chunks, int M, int N, int type, int act, hipStream_t s);
 hipError_t join_columns(const ColumnJoin& c, hipStream_t s);
 
 // rows x n values of `size` bytes (row stride ld) become zero; a kernel, so that a graph can hold it

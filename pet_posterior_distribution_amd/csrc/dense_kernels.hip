@@ -130,8 +130,8 @@ hipError_t rows_t(const Product& p, hipStream_t s) {
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* dy, int64_t ldy, const T* saved, int64_t lds, T* dp,
-                                                       int64_t ldd, float* part, int rows_per, int M, int N, int act,
-                                                       int lpr) {
+                                                       int64_t ldd, int bare, float* part, int rows_per, int M, int N,
+                                                       int act, int lpr) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int W = 8;
   __shared__ float red[4][64 * W];
@@ -146,19 +146,11 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* dy, int64_t ldy,
     float g[W];
 #pragma unroll
     for (int q = 0; q < W; ++q) g[q] = g0[q];
-    if (act == kRelu) {
-#pragma unroll
-      for (int q = 0; q < W; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], kRelu);
-    } else if (act == kGelu) {
-#pragma unroll
-      for (int q = 0; q < W; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], kGelu);
-    } else if (act == kSilu) {
-#pragma unroll
-      for (int q = 0; q < W; ++q) g[q] = activate_grad<EXACT>(g[q], v[q], kSilu);
-    }
+    activate_grads<EXACT, W>(g, v, act);
 #pragma unroll
     for (int q = 0; q < W; ++q) sum[q] += g[q];
-    if (dp) store_row<T, W>(dp + m * ldd + j, n, g);
+    // (columns past the last are zero: the next product may read them)
+    if (dp) store_row<T, W>(dp + m * ldd + j, bare ? n : W, g);
   };
   if (n > 0) {
     int64_t m = m0 + threadIdx.x / lpr;
@@ -198,11 +190,11 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* dy, int64_t ldy,
 }
 
 template <typename T>
-hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, float* part,
-                      int chunks, int M, int N, int act, hipStream_t s) {
+hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, int bare,
+                      float* part, int chunks, int M, int N, int act, hipStream_t s) {
   const int rows_per = (M + chunks - 1) / chunks, lpr = act_grad_lanes(N);
   hipLaunchKernelGGL((act_grad_kernel<T>), dim3(blocks_for(N, lpr * 8), chunks), dim3(256), 0, s,
-                     static_cast<const T*>(dy), ldy, static_cast<const T*>(saved), lds, static_cast<T*>(dp), ldd, part,
+                     static_cast<const T*>(dy), ldy, static_cast<const T*>(saved), lds, static_cast<T*>(dp), ldd, bare, part,
                      rows_per, M, N, act, lpr);
   return hipGetLastError();
 }
@@ -210,6 +202,37 @@ hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t ld
 __global__ __launch_bounds__(256) void join_columns_kernel(ColumnJoin p) {
   __shared__ float red[256];
   join_columns16(p, blockIdx.x, threadIdx.x, red);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Padded copies.  A thread moves 16 bytes; a row's last piece is filled up with zeros.  Memory bound.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void pad_kernel(PadJobs p) {
+  constexpr int W = 16 / (int)sizeof(T);
+  int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    const PadJob& job = p.job[q];
+    const int pieces = (int)(job.ldd / W);
+    const int64_t all = (int64_t)job.rows * pieces;
+    if (t < all) {
+      const int64_t r = t / pieces;
+      const int c = (int)(t - r * pieces) * W, n = job.n - c;
+      const T* src = static_cast<const T*>(job.src) + r * job.ld + c;
+      T v[W];
+      if (n >= W) {
+        __builtin_memcpy(v, src, 16);
+      } else {
+#pragma unroll
+        for (int x = 0; x < W; ++x) v[x] = x < n ? src[x] : (T)0.f;
+      }
+      __builtin_memcpy(__builtin_assume_aligned(static_cast<T*>(job.dst) + r * job.ldd + c, 16), v, 16);
+      return;
+    }
+    t -= all;
+    if (t < 0) return;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -342,10 +365,21 @@ hipError_t join(const Product& p, int type, hipStream_t s) {
 
 hipError_t rows(const Product& p, int type, hipStream_t s) { PETDENSE_BY_TYPE(type, return rows_t<T>(p, s)) }
 
-hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, float* part,
-                    int chunks, int M, int N, int type, int act, hipStream_t s) {
-  PETDENSE_BY_TYPE(type, return act_grad_t<T>(dy, ldy, saved, lds, dp, ldd, part, chunks, M, N, act, s))
+hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, int bare,
+                    float* part, int chunks, int M, int N, int type, int act, hipStream_t s) {
+  PETDENSE_BY_TYPE(type, return act_grad_t<T>(dy, ldy, saved, lds, dp, ldd, bare, part, chunks, M, N, act, s))
 }
+
+template <typename T>
+hipError_t pad_t(const PadJobs& p, hipStream_t s) {
+  int64_t pieces = 0;
+  for (const PadJob& j : p.job) pieces += (int64_t)j.rows * (j.ldd * (int64_t)sizeof(T) / 16);
+  if (pieces >= (int64_t)1 << 32) return hipErrorInvalidValue;      // the plan copies nothing of that size
+  hipLaunchKernelGGL((pad_kernel<T>), dim3(blocks_for(pieces, 256)), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+hipError_t pad(const PadJobs& p, int type, hipStream_t s) { PETDENSE_BY_TYPE(type, return pad_t<T>(p, s)) }
 
 hipError_t join_columns(const ColumnJoin& c, hipStream_t s) {
   hipLaunchKernelGGL(join_columns_kernel, dim3(blocks_for(c.N, 16)), dim3(256), 0, s, c);

@@ -1,0 +1,12 @@
+// Instances of the dense layer's backward pass as one launch for bf16 operands.
+#include "dense_product.h"
+
+namespace petdense_k {
+
+hipError_t pair_bf16(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s) {
+  return pair<__bf16>(p, lx, lk, tile, q8, s);
+}
+
+hipError_t fused_bf16(const Pair& p, int tile, int q8, hipStream_t s) { return fused<__bf16>(p, tile, q8, s); }
+
+}  // namespace petdense_k

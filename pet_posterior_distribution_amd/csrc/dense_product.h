@@ -128,8 +128,9 @@ __device__ __forceinline__ typename Frag<T>::type fragment(const char* st, int r
 //   the operand gets an offset past the buffer's end, and the hardware writes zeros for it.
 // LOADER kReg: any alignment: through registers, loaded a step ahead and stored after the step's first group.
 // Q8: the operand is e4m3 codes with exponent bytes, free-contiguous: through registers, restored to T on the way.
+// ACT: the operand is dP = dy act'(saved), made from two sources on the way (kReg), rounded to T as a dP in memory is.
 // KW > 1: the filler's wave takes every KW-th step, from step `kw`.
-template <typename T, bool FREE, int R, int BC, int THREADS, int KW, int LOADER, bool Q8>
+template <typename T, bool FREE, int R, int BC, int THREADS, int KW, int LOADER, bool Q8, bool ACT>
 struct Filler {
   using S = Stage<T, FREE, R, BC>;
   static constexpr int N = (S::PIECES + THREADS - 1) / THREADS;      // pieces of a thread
@@ -144,6 +145,11 @@ struct Filler {
   int64_t lde;
   int voff[LOADER == kDma ? N : 1];
   u32x4 reg[LOADER == kDma ? 1 : N];
+  const char* base2;     // ACT: the same of `saved`
+  int64_t ld2;
+  int act;
+  u32x4 reg2[ACT ? N : 1];
+  static_assert(!ACT || (LOADER == kReg && !Q8), "dP is staged through registers");
 
   __device__ void init(const void* p, int64_t ld_values, int f0, int f_limit, int64_t c0, int clen_, int c_all,
                        const uint8_t* ex, int64_t lde_, int kw_, int tid) {
@@ -166,10 +172,19 @@ struct Filler {
     }
   }
 
+  __device__ void init_saved(const void* p, int64_t ld_values, int act_, int f0, int64_t c0) {
+    act = act_;
+    ld2 = act ? ld_values * (int64_t)sizeof(T) : ld;
+    // without an activation nothing of `saved` counts: dy stands in for it
+    base2 = !act ? base : static_cast<const char*>(p) + (FREE ? c0 * ld2 + (int64_t)f0 * (int64_t)sizeof(T)
+                                                              : f0 * ld2 + c0 * (int64_t)sizeof(T));
+  }
+
   // what every piece of the t-th step needs
   struct Step {
     i32x4 rs;            // kDma: the buffer that begins at the step
     const char* p;
+    const char* p2;
     int t, left;         // contraction values of the step that exist (<= 0: a step past the end loads nothing)
     bool whole;          // kReg: no piece has to be cut
   };
@@ -178,9 +193,11 @@ struct Filler {
     u.t = KW > 1 ? t * KW + kw : t;
     u.left = clen - u.t * BC;
     u.p = base + (FREE ? (int64_t)u.t * BC * ld : (int64_t)u.t * BC * (int64_t)sizeof(T));
+    if constexpr (ACT) u.p2 = base2 + (FREE ? (int64_t)u.t * BC * ld2 : (int64_t)u.t * BC * (int64_t)sizeof(T));
     // free-contiguous: 16 bytes from a piece's first value may run into the next row, which then has to exist
     // (offsets within a step fit 31 bits)
-    u.whole = !brief && (FREE ? u.left > BC && ld >= 16 : u.left >= BC) && ld < 0x7fffffff / 256;
+    u.whole = !brief && (FREE ? u.left > BC && ld >= 16 : u.left >= BC) && ld < 0x7fffffff / 256 &&
+              (!ACT || ((!FREE || ld2 >= 16) && ld2 < 0x7fffffff / 256));
     if constexpr (LOADER == kDma) {
       const unsigned long long a = reinterpret_cast<unsigned long long>(u.p);
       u.rs[0] = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffull));
@@ -215,7 +232,8 @@ struct Filler {
         for (int q = 0; q < N; ++q) {
           const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
           const int rr = FREE ? r : min(r, limit - 1), cc = FREE && c * S::EPC >= limit ? 0 : c;
-          load_piece(q, u.p + (unsigned)(rr * (int)ld + cc * PB));
+          load_piece(reg[q], u.p + (unsigned)(rr * (int)ld + cc * PB));
+          if constexpr (ACT) load_piece(reg2[q], u.p2 + (unsigned)(rr * (int)ld2 + cc * PB));
           if constexpr (Q8)
             reg[q][2] = (exps + (int64_t)u.t * BC * lde)[(unsigned)(r * (int)lde + (cc * S::EPC) / 32)];
         }
@@ -233,59 +251,69 @@ struct Filler {
         const bool in = FREE ? r < u.left : r < limit;
         const int n = !in || after <= 0 ? 0 : after < S::EPC ? (int)after : S::EPC;
         const char* p = base + row * ld;
+        const char* p2 = ACT ? base2 + row * ld2 : nullptr;
         if (brief) {
 #pragma unroll 1
           for (int x = S::EPC - 1; x >= 0; --x) {
             // the values come in from the last to the first, each moving those behind it up
-            const char* s = p + min(first + x, (int64_t)(FREE ? limit : clen) - 1) * SZ;
+            const int64_t at = min(first + x, (int64_t)(FREE ? limit : clen) - 1) * SZ;
             unsigned one = 0;
-            __builtin_memcpy(&one, s, SZ);
-            push_value(q, x < n ? one : 0u);
+            __builtin_memcpy(&one, p + at, SZ);
+            push_value(reg[q], x < n ? one : 0u);
+            if constexpr (ACT) {
+              __builtin_memcpy(&one, p2 + at, SZ);
+              push_value(reg2[q], x < n ? one : 0u);
+            }
           }
         } else {
           const int64_t at = after >= S::EPC ? first : (int64_t)(FREE ? limit : clen) - S::EPC;
-          load_piece(q, p + at * SZ);
-          shift_piece(q, (after >= S::EPC && in ? 0 : S::EPC - n) * SZ * 8);
+          const int bits = (after >= S::EPC && in ? 0 : S::EPC - n) * SZ * 8;
+          load_piece(reg[q], p + at * SZ);
+          shift_piece(reg[q], bits);
+          if constexpr (ACT) {
+            load_piece(reg2[q], p2 + at * SZ);
+            shift_piece(reg2[q], bits);
+          }
         }
         if constexpr (Q8) reg[q][2] = exps[row * lde + min(first, (int64_t)limit - 1) / 32];
       }
     }
   }
 
-  __device__ __forceinline__ void load_piece(int q, const char* s) {
+  __device__ __forceinline__ void load_piece(u32x4& r, const char* s) {
     if constexpr (Q8) {
       unsigned w[2] = {0, 0};
       __builtin_memcpy(w, s, S::EPC);
-      reg[q][0] = w[0];
-      reg[q][1] = w[1];
+      r[0] = w[0];
+      r[1] = w[1];
     } else {
-      __builtin_memcpy(&reg[q], s, 16);
+      __builtin_memcpy(&r, s, 16);
     }
   }
   // moves the piece's values up by one and puts `v` in front
-  __device__ __forceinline__ void push_value(int q, unsigned v) {
+  __device__ __forceinline__ void push_value(u32x4& r, unsigned v) {
     constexpr int BITS = Q8 ? 8 : 8 * (int)sizeof(T);
 #pragma unroll
     for (int w = Q8 ? 1 : 3; w >= 0; --w) {
-      const unsigned below = w ? reg[q][w - 1] : 0;
-      if constexpr (BITS == 32) reg[q][w] = w ? below : v;
-      else reg[q][w] = reg[q][w] << BITS | (w ? below >> (32 - BITS) : v);
+      const unsigned below = w ? r[w - 1] : 0;
+      if constexpr (BITS == 32) r[w] = w ? below : v;
+      else r[w] = r[w] << BITS | (w ? below >> (32 - BITS) : v);
     }
   }
   // moves the piece's values down by `bits`, zeros behind them
-  __device__ __forceinline__ void shift_piece(int q, int bits) {
-    const uint64_t lo = reg[q][0] | (uint64_t)reg[q][1] << 32;
+  __device__ __forceinline__ void shift_piece(u32x4& r, int bits) {
+    const uint64_t lo = r[0] | (uint64_t)r[1] << 32;
     if constexpr (Q8) {
       constexpr int ALL = S::EPC * 8;
       const uint64_t v = bits >= ALL ? 0 : lo >> bits;
-      reg[q][0] = (unsigned)v;
-      reg[q][1] = (unsigned)(v >> 32);
+      r[0] = (unsigned)v;
+      r[1] = (unsigned)(v >> 32);
     } else {
-      const uint64_t hi = reg[q][2] | (uint64_t)reg[q][3] << 32;
+      const uint64_t hi = r[2] | (uint64_t)r[3] << 32;
       const int b = bits & 63;
       const uint64_t lo1 = (lo >> b) | (b ? hi << (64 - b) : 0), hi1 = hi >> b;
       const uint64_t l = bits >= 128 ? 0 : bits >= 64 ? hi1 : lo1, h = bits >= 64 ? 0 : hi1;
-      reg[q] = u32x4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
+      r = u32x4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
     }
   }
 
@@ -308,6 +336,17 @@ struct Filler {
           restore4<T>(w[0], sc, v);
           if constexpr (S::EPC == 8) restore4<T>(w[1], sc, v + 4);
           __builtin_memcpy(&w, v, 16);
+        } else if constexpr (ACT) {
+          T d[S::EPC], v[S::EPC];
+          __builtin_memcpy(d, &w, 16);
+          __builtin_memcpy(v, &reg2[q], 16);
+          float gf[S::EPC], vf[S::EPC];
+#pragma unroll
+          for (int x = 0; x < S::EPC; ++x) gf[x] = (float)d[x], vf[x] = (float)v[x];
+          activate_grads<sizeof(T) == 4, S::EPC>(gf, vf, act);
+#pragma unroll
+          for (int x = 0; x < S::EPC; ++x) d[x] = (T)gf[x];
+          __builtin_memcpy(&w, d, 16);
         }
         *reinterpret_cast<u32x4*>(st + (q * THREADS + tid) * 16) = w;
       }
@@ -337,6 +376,7 @@ typedef Kind<256, 256, 2, 4, 1> Large;
 typedef Kind<128, 128, 2, 2, 1> Mid;
 typedef Kind<64, 64, 2, 2, 1> Small;
 typedef Kind<32, 32, 1, 1, 8> Slice;
+typedef Kind<64, 64, 1, 1, 4> Slice64;
 
 // Workgroup -> part of the contraction and tile.  Neighbouring workgroup numbers go to different XCDs, each with its
 // own L2: every XCD gets a contiguous run of (part, tile), so that a part's rows are fetched by one XCD, and the tiles
@@ -353,7 +393,8 @@ __device__ __forceinline__ void place_of(int b, int ti, int tj, int splits, int&
   j = r / h;
 }
 
-template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8>
+// ACT_A, ACT_B: that operand is dP, made from dy and p.saved
+template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8, bool ACT_A = false, bool ACT_B = false>
 __device__ __forceinline__ void product_body(const Product& p, int block, char* lds) {
   constexpr int BI = K::BI, BJ = K::BJ, WI = K::WI, WJ = K::WJ, KW = K::KW;
   constexpr int BC = 128 / (int)sizeof(T);
@@ -377,10 +418,12 @@ __device__ __forceinline__ void product_body(const Product& p, int block, char* 
   // steps of this wave; one at least, which finds nothing past the end
   const int steps = SHARED ? (clen + BC - 1) / BC : max(1, ((clen + BC - 1) / BC - kw + KW - 1) / KW);
 
-  Filler<T, FA, BI, BC, THREADS, KW, LA, Q8> fa;
-  Filler<T, FB, BJ, BC, THREADS, KW, LB, false> fb;
+  Filler<T, FA, BI, BC, THREADS, KW, LA, Q8, ACT_A> fa;
+  Filler<T, FB, BJ, BC, THREADS, KW, LB, false, ACT_B> fb;
   fa.init(p.A, p.lda, i0, p.I, c0, clen, p.C, p.exps, p.lde, kw, tid);
   fb.init(p.B, p.ldb, j0, p.J, c0, clen, p.C, nullptr, 0, kw, tid);
+  if constexpr (ACT_A) fa.init_saved(p.saved, p.lds, p.saved_act, i0, c0);
+  if constexpr (ACT_B) fb.init_saved(p.saved, p.lds, p.saved_act, j0, c0);
 
   f32x4 acc[FI][FJ];
 #pragma unroll
@@ -546,6 +589,16 @@ __global__ __launch_bounds__(K::THREADS) void pair_kernel(Pair p) {
   }
 }
 
+// The same from dy and saved: dP is formed while it is staged, the other workgroups sum 8 columns each.
+template <typename T, typename K, bool Q8>
+__global__ __launch_bounds__(K::THREADS) void fused_kernel(Pair p) {
+  extern __shared__ char lds[];
+  const int b = blockIdx.x;
+  if (b < p.nx) product_body<T, K, false, false, kReg, kReg, false, true, false>(p.x, b, lds);
+  else if (b < p.nx + p.nk) product_body<T, K, true, true, kReg, kReg, Q8, false, true>(p.k, b - p.nx, lds);
+  else sum_columns8<T, K::THREADS>(p.sums, b - p.nx - p.nk, threadIdx.x, reinterpret_cast<float*>(lds));
+}
+
 // Marks a kernel's use of more LDS than the default, once per device.
 inline hipError_t allow_lds(const void* k, int bytes, std::atomic<uint64_t>& done) {
   int dev = 0;
@@ -581,6 +634,17 @@ hipError_t launch_pair(Pair p, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <typename T, typename K, bool Q8>
+hipError_t launch_fused(Pair p, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  auto k = fused_kernel<T, K, Q8>;
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
+  p.nx = p.x.e.out ? (int)(tiles_of(p.x, K::BI, K::BJ) * p.x.splits) : 0;
+  p.nk = p.k.e.out ? (int)(tiles_of(p.k, K::BI, K::BJ) * p.k.splits) : 0;
+  hipLaunchKernelGGL(k, dim3((unsigned)(p.nx + p.nk + (p.sums.N + 7) / 8)), dim3(K::THREADS), K::LDS, s, p);
+  return hipGetLastError();
+}
+
 template <typename T, typename K>
 hipError_t product_kind(const Product& p, int layout, int loader, int q8, hipStream_t s) {
   if constexpr (K::BI == 256) {      // the plan takes the largest tile only where DMA stages both operands
@@ -608,7 +672,8 @@ hipError_t product(const Product& p, int layout, int loader, int tile, int q8, h
   if (tile == kLarge) return product_kind<T, Large>(p, layout, loader, q8, s);
   if (tile == kMid) return product_kind<T, Mid>(p, layout, loader, q8, s);
   if (tile == kSmall) return product_kind<T, Small>(p, layout, loader, q8, s);
-  return product_kind<T, Slice>(p, layout, loader, q8, s);
+  if (tile == kSlice) return product_kind<T, Slice>(p, layout, loader, q8, s);
+  return product_kind<T, Slice64>(p, layout, loader, q8, s);
 }
 
 template <typename T, typename K>
@@ -625,7 +690,15 @@ hipError_t pair_kind(const Pair& p, int lx, int lk, int q8, hipStream_t s) {
 
 template <typename T>
 hipError_t pair(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s) {
-  return tile == kSmall ? pair_kind<T, Small>(p, lx, lk, q8, s) : pair_kind<T, Slice>(p, lx, lk, q8, s);
+  return tile == kSmall    ? pair_kind<T, Small>(p, lx, lk, q8, s)
+         : tile == kSlice ? pair_kind<T, Slice>(p, lx, lk, q8, s)
+                          : pair_kind<T, Slice64>(p, lx, lk, q8, s);
+}
+
+template <typename T>
+hipError_t fused(const Pair& p, int tile, int q8, hipStream_t s) {
+  if (tile == kSmall) return q8 ? launch_fused<T, Small, true>(p, s) : launch_fused<T, Small, false>(p, s);
+  return q8 ? launch_fused<T, Slice, true>(p, s) : launch_fused<T, Slice, false>(p, s);
 }
 
 }  // namespace petdense_k

@@ -7,8 +7,4 @@ hipError_t product_f16(const Product& p, int layout, int loader, int tile, int q
   return product<_Float16>(p, layout, loader, tile, q8, s);
 }
 
-hipError_t pair_f16(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s) {
-  return pair<_Float16>(p, lx, lk, tile, q8, s);
-}
-
 }  // namespace petdense_k

@@ -7,8 +7,4 @@ hipError_t product_f32(const Product& p, int layout, int loader, int tile, int q
   return product<float>(p, layout, loader, tile, q8, s);
 }
 
-hipError_t pair_f32(const Pair& p, int lx, int lk, int tile, int q8, hipStream_t s) {
-  return pair<float>(p, lx, lk, tile, q8, s);
-}
-
 }  // namespace petdense_k

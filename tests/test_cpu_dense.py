@@ -68,12 +68,19 @@ def test_missing_small_and_unaligned_workspaces_are_refused():
     for work, size in ((None, need), (0x10000, need - 1), (0x10010, need)):
         assert L.petdense_forward(C.byref(a), work, size, None) == INVALID
         assert 'workspace' in L.petdense_last_error().decode()
-    b = backward_args()
+    b = backward_args(m=40000)                         # dP and the parts of its sums
     need = L.petdense_backward_workspace(C.byref(b))
     assert need > 0
     for work, size in ((None, need), (0x10000, need - 1), (0x10010, need)):
         assert L.petdense_backward(C.byref(b), work, size, None) == INVALID
         assert 'workspace' in L.petdense_last_error().decode()
+
+
+def test_every_backward_pass_gets_a_plan():
+    """With more tiles than one launch takes, dP goes through the workspace (a launch without a plan reads outside)."""
+    for m, k, n in ((12288, 6144, 512), (8192, 8256, 24), (70000, 4096, 16), (16, 70000, 4096)):
+        a = backward_args(m=m, k=k, n=n, lddy=n, ldx=k, ldk=n, lds=n, lddx=k, lddk=n)
+        assert L.petdense_backward_workspace(C.byref(a)) >= m * n * 2
 
 
 def test_null_arguments():

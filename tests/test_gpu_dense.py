@@ -26,6 +26,8 @@ SHAPES = [(1, 1, 1), (1, 54, 256), (2, 300, 33), (7, 129, 64), (8, 64, 6), (9, 6
           (300, 72, 6)]
 # outputs of many tiles
 WIDE = [(2048, 128, 2048), (2040, 72, 4104)]
+# more tiles than one launch of the whole backward pass takes
+MANY = [(8192, 8256, 24)]
 
 
 def rand(shape, dtype, seed, scale=1.0):
@@ -160,6 +162,13 @@ def test_backward(m, k, n, t):
     for act in ACTS:
         saved = None if act is None else (p.clamp(min=0) if act == 'relu' else p)
         check_backward(dy, x, w, act, saved, residual=act in ('relu', 'gelu'))
+
+
+@pytest.mark.parametrize('act', [None, 'relu'])
+@pytest.mark.parametrize('m,k,n', MANY)
+def test_backward_of_many_tiles(m, k, n, act):
+    x, w, _, p, dy = inputs(m, k, n, BF16)
+    check_backward(dy, x, w, act, None if act is None else p, residual=False)
 
 
 @pytest.mark.parametrize('act', [None, 'relu', 'gelu'])
