@@ -40,6 +40,8 @@ int size_of(int dtype) { return dtype == PETDENSE_F32 ? 4 : 2; }
 
 struct Plan {
   int tile = kSmall, splits = 1, c_per = 0;
+  int b = 0, whole = 0;    // streamed products: rows of the tile, tiles that are not split
+  bool stream = false;
   size_t part_bytes = 0;
   double us = 0;           // estimate
 };
@@ -52,43 +54,54 @@ struct Cost {
   double wait[3], share[3], ends;
 };
 constexpr int kFormed = 2;
-constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.45, 0, 0}, {1.45, 0, 0}, 8.0},
+constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.47, 0, 0}, {1.47, 0, 0}, 5.5},
                              {kMid, 128, 2, 1, {0.65, 1.25, 0}, {0.46, 1.25, 0}, 3.5},
                              {kSmall, 64, 4, 1, {0.28, 0.55, 1.1}, {0.19, 0.34, 0.7}, 2.0},
                              {kSlice, 32, 1, 8, {1.0, 1.6, 2.6}, {1.0, 1.6, 2.6}, 2.0},
                              {kSlice64, 64, 1, 4, {0.75, 2.4, 0}, {0.75, 2.4, 0}, 3.5}};
-constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 0, 0}, {6.9, 0, 0}, 10.0},
+constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 0, 0}, {6.9, 0, 0}, 8.0},
                              {kMid, 128, 2, 1, {2.3, 2.7, 0}, {2.1, 2.5, 0}, 4.0},
                              {kSmall, 64, 4, 1, {0.75, 0.95, 1.6}, {0.53, 0.65, 1.2}, 2.0},
                              {kSlice, 32, 1, 8, {1.3, 2.2, 3.5}, {1.3, 2.2, 3.5}, 2.0},
                              {kSlice64, 64, 1, 4, {2.75, 4.5, 0}, {2.75, 4.5, 0}, 3.5}};
 constexpr double kNever = 1e30;      // no plan
-constexpr double kLaunch = 2.5;      // a launch behind another
+constexpr double kLaunch = 3.5;      // a launch behind another, here and on the host
 constexpr int kUnits = 256;
 
 double step_us(const Cost& c, double per_unit, int loader) {
   return std::max(c.wait[loader], c.share[loader] * per_unit);
 }
 
-double product_us(const Cost& c, int64_t groups, int64_t steps, int loader) {
+// `groups` workgroups of `steps` each, one after another where they are too many
+double groups_us(const Cost& c, int64_t groups, int64_t steps, int loader) {
   const double per = (double)ceil_div(steps, c.k);
   const int64_t whole = groups / (kUnits * c.slots), rest = groups % (kUnits * c.slots);
-  double t = kLaunch + whole * (per * step_us(c, c.slots, loader) + c.ends);
+  double t = whole * (per * step_us(c, c.slots, loader) + c.ends);
   if (rest) t += per * step_us(c, (double)ceil_div(rest, kUnits), loader) + c.ends;
   return t;
 }
 
-double join_us(int64_t I, int64_t J, int64_t splits) {
-  return splits > 1 ? kLaunch + 1.0 + (double)I * J * (splits + 1) * 4 / 3.5e6 : 0.0;
+double join_us(double values, int64_t splits) {
+  return splits > 1 ? kLaunch + 1.0 + values * (splits + 1) * 4 / 3.5e6 : 0.0;
 }
 
-// Splits of `steps` into equal parts (the last may be shorter), few to many.
+// Splits of `steps` into s <= most equal parts (the last may be shorter), few to many.
 template <typename F>
 void for_splits(int64_t steps, int64_t most, F f) {
-  for (int64_t s = 1; s <= most && s <= steps; s = s < 4 ? s + 1 : s * 5 / 4) {
-    const int64_t per = ceil_div(steps, s);
-    if (ceil_div(steps, per) == s) f(s, per);
+  constexpr int kParts[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64};
+  int64_t last = 0;
+  for (const int want : kParts) {
+    if (want > most || want > steps) break;
+    const int64_t per = ceil_div(steps, want), s = ceil_div(steps, per);
+    if (s == last) continue;
+    last = s;
+    f(s, per);
   }
+}
+
+// More parts than make twice the workgroups that the card holds gain nothing.
+int64_t most_splits(const Cost& c, int64_t tiles) {
+  return std::max<int64_t>(1, std::min<int64_t>(64, 2 * kUnits * c.slots / std::max<int64_t>(1, tiles)));
 }
 
 void set_plan(Plan& p, const Cost& c, int64_t splits, int64_t per, int bc, int64_t I, int64_t J) {
@@ -106,12 +119,32 @@ Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader, bool q8 = false
   for (const Cost& c : type == kF32 ? kCosts32 : kCosts16) {
     if (c.tile == kLarge && (loader != kDma || q8)) continue;
     const int64_t tiles = ceil_div(I, c.b) * ceil_div(J, c.b);
-    for_splits(steps, 64, [&](int64_t s, int64_t per) {
-      const double t = product_us(c, tiles * s, per, q8 ? kReg : loader) + join_us(I, J, s);
-      if (best.c_per && t >= best.us) return;
-      best.us = t;
-      set_plan(best, c, s, per, bc, I, J);
-    });
+    if (c.k > 1 && tiles > 4 * kUnits) continue;        // sliced tiles are for few outputs
+    const int l = q8 ? kReg : loader;
+    const bool stream = c.tile == kLarge;
+    // streamed: as many tiles whole as fill the card evenly, the others split; or all split
+    const int64_t even = stream ? tiles / (kUnits * c.slots) * (kUnits * c.slots) : 0;
+    for (int64_t whole : {(int64_t)0, even}) {
+      const int64_t rest = tiles - whole;
+      if (whole && !rest) continue;                    // nothing is left to split: the unsplit plan
+      const double before = kLaunch + (whole ? groups_us(c, whole, steps, l) : 0);
+      if (best.c_per && before >= best.us) continue;
+      for_splits(steps, whole ? 64 : most_splits(c, tiles), [&](int64_t s, int64_t per) {
+        if (whole && s == 1) return;
+        // split tiles' sums in fp32
+        const double values = stream ? (double)rest * c.b * c.b : (double)I * J;
+        if (s > 1 && values * s * 4 > 8e9) return;
+        const double t = before + groups_us(c, rest * s, per, l) + join_us(values, s);
+        if (best.c_per && t >= best.us) return;
+        best.us = t;
+        set_plan(best, c, s, per, bc, I, J);
+        best.stream = stream;
+        best.b = c.b;
+        best.whole = stream ? (int)(s > 1 ? whole : tiles) : 0;
+        if (stream && s > 1) best.part_bytes = up((size_t)rest * c.b * c.b * s * 4);
+      });
+      if (!even) break;
+    }
   }
   return best;
 }
@@ -127,13 +160,14 @@ double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, in
     if (c.tile == kLarge || c.tile == kMid || (c.tile == kSlice64 && !slice64)) continue;
     const int64_t tx = nx ? ceil_div(m, c.b) * ceil_div(k, c.b) : 0, tk = nk ? ceil_div(k, c.b) * ceil_div(n, c.b) : 0;
     if (tx > 16384 || tk > 16384) continue;
-    for_splits(nk ? sk : 1, 64, [&](int64_t s, int64_t per) {
+    if (c.k > 1 && tx + tk > 8 * kUnits) continue;
+    for_splits(nk ? sk : 1, most_splits(c, tx + tk), [&](int64_t s, int64_t per) {
       const double wx = nx ? (double)ceil_div(sx, c.k) : 0, wk = nk ? (double)ceil_div(nk ? per : 0, c.k) : 0;
       const double groups = (double)(tx + tk * s);
       const double share = ((double)tx * (wx * c.share[lx] + c.ends / c.slots) +
                             (double)tk * s * (wk * c.share[lk] + c.ends / c.slots)) / kUnits;
       const double longest = std::max(wx * c.wait[lx], wk * c.wait[lk]) + c.ends;
-      const double t = kLaunch + std::max(longest, share * (groups > kUnits * c.slots ? 1.1 : 1.0)) + join_us(k, n, s);
+      const double t = kLaunch + std::max(longest, share * (groups > kUnits * c.slots ? 1.1 : 1.0)) + join_us((double)k * n, s);
       if (t >= best) return;
       best = t;
       set_plan(px, c, 1, sx, bc, m, k);
@@ -149,12 +183,15 @@ bool dma_ok(const void* p, int64_t ld, int64_t contiguous, int size) {
          ld * size < (int64_t)0x7fffffff / 256;          // a tile's offsets fit 31 bits
 }
 
-bool planned(const Plan& p, int64_t C) { return p.c_per > 0 && (int64_t)p.splits * p.c_per >= C && (p.splits - 1) * (int64_t)p.c_per < C; }
+bool planned(const Plan& p, int64_t C) {
+  return p.c_per > 0 && (int64_t)p.splits * p.c_per >= C && (p.splits - 1) * (int64_t)p.c_per < C;
+}
 
 Product placed(Product p, const Plan& pl, void* part) {
   p.splits = pl.splits;
   p.c_per = pl.c_per;
   p.part = static_cast<float*>(part);
+  p.whole = pl.whole;
   return p;
 }
 
@@ -165,7 +202,7 @@ int run_product(const Product& of, int layout, int loader, int type, int q8, con
   HIPC(type == kF32    ? product_f32(p, layout, loader, pl.tile, q8, s)
        : type == kBF16 ? product_bf16(p, layout, loader, pl.tile, q8, s)
                        : product_f16(p, layout, loader, pl.tile, q8, s));
-  if (pl.splits > 1) HIPC(join(p, type, s));
+  if (pl.splits > 1) HIPC(pl.stream ? join_tiles(p, type, pl.b, s) : join(p, type, s));
   return PETDIFF_OK;
 }
 

@@ -34,6 +34,27 @@ __global__ __launch_bounds__(256) void join_kernel(Product p, int64_t octets, in
   epilogue8<T>(p.e, i, j, n, v);
 }
 
+template <typename T>
+__global__ __launch_bounds__(256) void join_tiles_kernel(Product p, int b, int ti, int tj) {
+  // blockIdx.y: the split tile; a thread takes eight columns of one of its rows
+  const int per = b / 8, t = blockIdx.x * 256 + threadIdx.x, r = t / per, c = (t % per) * 8;
+  int a, d;
+  tile_at(p.whole + blockIdx.y, ti, tj, a, d);
+  const int64_t i = (int64_t)a * b + r;
+  const int j = d * b + c, n = p.J - j;
+  if (r >= b || i >= p.I || n <= 0) return;
+  const float* src = p.part + (int64_t)blockIdx.y * p.splits * b * b + r * b + c;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    float w[8];
+    load_row<float, 8>(src + (int64_t)s * b * b, 8, w);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] += w[q];
+  }
+  epilogue8<T>(p.e, i, j, n, v);
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // Few rows (decoding, a single sample): every value of B is read once by one workgroup, which owns COLS columns and
 // the whole contraction, so that one launch ends the call.  4 lanes share a row's 8-column pieces; the other lanes
@@ -360,6 +381,13 @@ hipError_t join(const Product& p, int type, hipStream_t s) {
   const int64_t octets = (int64_t)p.I * orow;
   PETDENSE_BY_TYPE(type, hipLaunchKernelGGL((join_kernel<T>), dim3(blocks_for(octets, 256)), dim3(256), 0, s, p,
                                             octets, orow);
+                   return hipGetLastError())
+}
+
+hipError_t join_tiles(const Product& p, int type, int b, hipStream_t s) {
+  const int ti = (p.I + b - 1) / b, tj = (p.J + b - 1) / b;
+  PETDENSE_BY_TYPE(type, hipLaunchKernelGGL((join_tiles_kernel<T>), dim3(blocks_for(b * (b / 8), 256), ti * tj - p.whole),
+                                            dim3(256), 0, s, p, b, ti, tj);
                    return hipGetLastError())
 }
 

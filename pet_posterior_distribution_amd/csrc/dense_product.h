@@ -23,6 +23,7 @@
 #pragma once
 #include "dense_epilogue.h"
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -40,9 +41,9 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 // One wave's buffer load of 64 x 16 bytes straight into LDS at `lds` (wave-uniform) + 16 lane.  In assembly, because
 // the compiler would put a wait for it before every LDS read that follows; the kernel waits for it itself, before the
 // barrier that publishes a stage.  (No output register: nothing the compiler could reuse early.)
-__device__ __forceinline__ void load_to_lds(i32x4 rsrc, unsigned lds, int voffset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset),
-               "s"(rsrc)
+__device__ __forceinline__ void load_to_lds(i32x4 rsrc, unsigned lds, int voffset, int soffset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voffset),
+               "s"(rsrc), "s"(soffset)
                : "memory", "m0");
 }
 
@@ -55,7 +56,7 @@ struct Stage {
   static constexpr int CPR = (FREE ? R : BC) / EPC;
   static constexpr int PIECES = ROWS * CPR;
   static constexpr int BYTES = PIECES * 16;
-  __device__ static int key(int r) {
+  __host__ __device__ static constexpr int key(int r) {
     if constexpr (!FREE) return r & 7;                               // CPR = 8
     else if constexpr (sizeof(T) == 4) return ((r >> 2) & (CPR >= 16 ? 3 : CPR / 4 - 1)) << 2;
     else if constexpr (CPR >= 16) return ((r & 3) | ((r >> 1) & 4)) << 1;
@@ -143,7 +144,17 @@ struct Filler {
   int clen, kw;
   const uint8_t* exps;   // Q8: exponent byte of the tile's first block at the part's first row
   int64_t lde;
-  int voff[LOADER == kDma ? N : 1];
+  // pieces of a thread: rows r0, r0 + RPQ, ..; `same`: all at one place of their rows
+  static constexpr int RPQ = THREADS / S::CPR;
+  static constexpr bool same() {
+    for (int q = 1; q < N; ++q)
+      for (int r = 0; r < RPQ; ++r)
+        if (S::key(r + q * RPQ) != S::key(r)) return false;
+    return true;
+  }
+  static constexpr bool SAME = same();
+  static_assert(THREADS % S::CPR == 0, "");
+  int v0;                // kDma: bytes from a step's first to the thread's first row, and with SAME to its piece
   u32x4 reg[LOADER == kDma ? 1 : N];
   const char* base2;     // ACT: the same of `saved`
   int64_t ld2;
@@ -163,12 +174,8 @@ struct Filler {
     exps = Q8 ? ex + c0 * lde_ + f0 / 32 : nullptr;
     lde = lde_;
     if constexpr (LOADER == kDma) {
-#pragma unroll
-      for (int q = 0; q < N; ++q) {
-        const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
-        const bool in = FREE ? c * S::EPC < limit : r < limit;
-        voff[q] = in ? (int)(r * ld) + c * 16 : (int)0x80000000;
-      }
+      const int r = tid / S::CPR;
+      v0 = r * (int)ld + (SAME ? ((tid % S::CPR) ^ S::key(r)) * 16 : 0);
     }
   }
 
@@ -211,10 +218,11 @@ struct Filler {
   // begins the load of the thread's piece q of a step into LDS at `st`
   __device__ __forceinline__ void begin(char* st, const Step& u, int q, int tid) {
     if constexpr (LOADER == kDma) {
-      const int k = q * THREADS + tid, r = k / S::CPR, c = (k % S::CPR) ^ S::key(r);
+      const int r = tid / S::CPR + q * RPQ, c = (tid % S::CPR) ^ S::key(r);
       const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-      const int o = (FREE ? r >= u.left : c * S::EPC >= u.left) ? (int)0x80000000 : voff[q];
-      load_to_lds(u.rs, (unsigned)(uintptr_t)(PETDENSE_LDS char*)st + (q * THREADS + wave * 64) * 16, o);
+      const bool in = FREE ? r < u.left && c * S::EPC < limit : r < limit && c * S::EPC < u.left;
+      load_to_lds(u.rs, (unsigned)(uintptr_t)(PETDENSE_LDS char*)st + (q * THREADS + wave * 64) * 16,
+                  in ? v0 + (SAME ? 0 : c * 16) : (int)0x80000000, q * RPQ * (int)ld);
     }
   }
 
@@ -236,6 +244,14 @@ struct Filler {
           if constexpr (ACT) load_piece(reg2[q], u.p2 + (unsigned)(rr * (int)ld2 + cc * PB));
           if constexpr (Q8)
             reg[q][2] = (exps + (int64_t)u.t * BC * lde)[(unsigned)(r * (int)lde + (cc * S::EPC) / 32)];
+        }
+        return;
+      }
+      if (u.left <= 0) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+          reg[q] = u32x4{0, 0, Q8 ? 127u : 0u, 0};
+          if constexpr (ACT) reg2[q] = u32x4{0, 0, 0, 0};
         }
         return;
       }
@@ -370,6 +386,11 @@ struct Kind {
   static constexpr int BI = BI_, BJ = BJ_, WI = WI_, WJ = WJ_, KW = KW_;
   static constexpr int THREADS = WI * WJ * KW * 64;
   static constexpr int LDS = 2 * KW * (BI + BJ) * 128;
+  static constexpr int TURN = 16 * (BJ / WJ) * 4;                        // a wave's 16 rows of outputs in fp32
+  // the largest tile's workgroups stay and walk (its first loads and its stores are a large part of a tile's time;
+  // smaller tiles run several workgroups on a compute unit, which hide them from each other)
+  static constexpr bool STREAM = BI == 256;
+  static constexpr int LAUNCH_LDS = LDS + (STREAM ? WI * WJ * TURN : 0);
   static_assert(KW == 1 || WI * WJ == 1, "");
 };
 typedef Kind<256, 256, 2, 4, 1> Large;
@@ -378,19 +399,22 @@ typedef Kind<64, 64, 2, 2, 1> Small;
 typedef Kind<32, 32, 1, 1, 8> Slice;
 typedef Kind<64, 64, 1, 1, 4> Slice64;
 
-// Workgroup -> part of the contraction and tile.  Neighbouring workgroup numbers go to different XCDs, each with its
-// own L2: every XCD gets a contiguous run of (part, tile), so that a part's rows are fetched by one XCD, and the tiles
-// of a part run in bands of 4 tile rows, so that the workgroups an XCD runs together share rows of A and columns of B.
+// Neighbouring workgroup numbers go to different XCDs, each with its own L2: XCD x takes a contiguous run of the n
+// pieces of work, [first, first + len).
+__device__ __forceinline__ void run_of(int n, int x, int& first, int& len) {
+  const int per = n / 8, rest = n % 8;
+  first = x * per + min(x, rest);
+  len = per + (x < rest ? 1 : 0);
+}
+
+// Workgroup -> part of the contraction and tile: a part's rows are fetched by one XCD.
 __device__ __forceinline__ void place_of(int b, int ti, int tj, int splits, int& split, int& i, int& j) {
-  const int tiles = ti * tj, n = tiles * splits;
-  const int per = n / 8, rest = n % 8, x = b % 8;
-  const int u = x * per + min(x, rest) + b / 8;
+  const int tiles = ti * tj;
+  int first, len;
+  run_of(tiles * splits, b % 8, first, len);
+  const int u = first + b / 8;
   split = u / tiles;
-  const int t = u - split * tiles;
-  constexpr int BAND = 4;
-  const int band = t / (BAND * tj), first = band * BAND, h = min(BAND, ti - first), r = t - first * tj;
-  i = first + r % h;
-  j = r / h;
+  tile_at(u - split * tiles, ti, tj, i, j);
 }
 
 // ACT_A, ACT_B: that operand is dP, made from dy and p.saved
@@ -568,10 +592,197 @@ __device__ __forceinline__ void product_body(const Product& p, int block, char* 
   }
 }
 
+// A product whose workgroups stay: each walks several tiles, and the loads run ahead across tiles, so that the next
+// tile's first two steps land while this one's outputs are stored.  The first p.whole tiles of the walk are multiplied
+// whole; the others, too few to fill the card once more, are split along the contraction (p.splits parts each).
+template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8>
+__device__ __forceinline__ void stream_body(const Product& p, char* lds) {
+  constexpr int BI = K::BI, BJ = K::BJ, WI = K::WI, WJ = K::WJ, BC = 128 / (int)sizeof(T), THREADS = K::THREADS;
+  static_assert(K::KW == 1, "");
+  using SA = Stage<T, FA, BI, BC>;
+  using SB = Stage<T, FB, BJ, BC>;
+  constexpr int STAGE = SA::BYTES + SB::BYTES;
+  constexpr int FI = BI / WI / 16, FJ = BJ / WJ / 16, KS = 2;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wi = wave / WJ, wj = wave % WJ;
+  const int ti = (p.I + BI - 1) / BI, tj = (p.J + BJ - 1) / BJ, rest = ti * tj - p.whole;
+
+  // this workgroup's work: every `stride`-th of its XCD's runs over the whole tiles and over the (part, tile) pairs
+  const int x8 = blockIdx.x % 8, r8 = blockIdx.x / 8, stride = ((int)gridDim.x - x8 + 7) / 8;
+  int first1, len1, first2, len2;
+  run_of(p.whole, x8, first1, len1);
+  run_of(rest * p.splits, x8, first2, len2);
+  const int n1 = len1 > r8 ? (len1 - r8 + stride - 1) / stride : 0;
+  const int count = n1 + (len2 > r8 ? (len2 - r8 + stride - 1) / stride : 0);
+  if (count == 0) return;
+  struct Item {
+    int i0, j0, c0, clen, steps, slot;       // slot: place of its sums in p.part, or -1: a whole contraction
+  };
+  auto item = [&](int n) {
+    Item m;
+    int tile;
+    if (n < n1) {
+      tile = first1 + r8 + n * stride;
+      m.slot = -1;
+      m.c0 = 0;
+      m.clen = p.C;
+    } else {
+      const int u = first2 + r8 + (n - n1) * stride, split = u / rest, q = u - split * rest;
+      tile = p.whole + q;
+      m.slot = p.splits > 1 ? q * p.splits + split : -1;
+      m.c0 = split * p.c_per;
+      m.clen = min(p.c_per, p.C - m.c0);
+    }
+    int a, b;
+    tile_at(tile, ti, tj, a, b);
+    m.i0 = a * BI;
+    m.j0 = b * BJ;
+    m.steps = (m.clen + BC - 1) / BC;
+    return m;
+  };
+
+  Filler<T, FA, BI, BC, THREADS, 1, LA, Q8, false> fa;
+  Filler<T, FB, BJ, BC, THREADS, 1, LB, false, false> fb;
+  int at_item = 0, at_step = 0, at_steps;    // what is loaded next
+  auto take = [&](int n) {
+    const Item m = item(n);
+    fa.init(p.A, p.lda, m.i0, p.I, m.c0, m.clen, p.C, p.exps, p.lde, 0, tid);
+    fb.init(p.B, p.ldb, m.j0, p.J, m.c0, m.clen, p.C, nullptr, 0, 0, tid);
+    at_steps = m.steps;
+  };
+  auto ahead = [&]() {
+    if (++at_step < at_steps) return;
+    at_step = 0;
+    if (++at_item < count) {
+      take(at_item);
+    } else {
+      fa.clen = fb.clen = 0;                 // nothing more: the steps that follow load nothing
+      at_steps = 0x7fffffff;
+    }
+  };
+
+  f32x4 acc[FI][FJ];
+  typename Frag<T>::type a[KS][FI], b[KS][FJ];
+  const int ra = wi * (BI / WI), rb = wj * (BJ / WJ);
+  auto read = [&](const char* st, int ks, int f) {
+    if (f < FJ) b[ks][f] = fragment<T, FB, BJ, BC>(st + SA::BYTES, rb + f * 16, ks, lane);
+    else a[ks][f - FJ] = fragment<T, FA, BI, BC>(st, ra + (f - FJ) * 16, ks, lane);
+  };
+  // as in product_body: group ks multiplied row by row while group kn of `rd` is read and a step's pieces are begun
+  constexpr int READS = FI + FJ, ROWS = FI > 1 ? FI - 1 : 1;
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
+  constexpr int NA = decltype(fa)::N, NB = decltype(fb)::N;
+  auto group = [&](int ks, int kn, const char* rd, auto loads, char* ld, const auto& ua, const auto& ub) {
+#pragma unroll
+    for (int x = 0; x < FI; ++x) {
+      if constexpr (decltype(loads)::value) {
+        if (x == 0) {
+          fa.begin_reg(ua, tid);
+          fb.begin_reg(ub, tid);
+        }
+#pragma unroll
+        for (int q = 0; q < NA; ++q)
+          if (q * FI / NA == x) fa.begin(ld, ua, q, tid);
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+          if (q * FI / NB == x) fb.begin(ld + SA::BYTES, ub, q, tid);
+      }
+#pragma unroll
+      for (int f = 0; f < READS; ++f)
+        if (f * ROWS / READS == x) read(rd, kn, f);
+      multiply_row<T, FJ>(b[ks], a[ks][x], acc[x]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  take(0);
+  fa.begin_all(lds, 0, tid);
+  fb.begin_all(lds + SA::BYTES, 0, tid);
+  ahead();
+  fa.end(lds, tid);
+  fb.end(lds + SA::BYTES, tid);
+  fa.begin_all(lds + STAGE, at_step, tid);
+  fb.begin_all(lds + STAGE + SA::BYTES, at_step, tid);
+  ahead();
+  step_barrier<(LA == kDma ? NA : 0) + (LB == kDma ? NB : 0), true>();
+#pragma unroll
+  for (int f = 0; f < READS; ++f) read(lds, 0, f);
+  char* cur = lds;
+  char* nxt = lds + STAGE;
+  for (int n = 0; n < count; ++n) {
+    const Item m = item(n);
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+      for (int y = 0; y < FJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < m.steps; ++t) {
+      const auto ua = fa.at(at_step);
+      const auto ub = fb.at(at_step);
+      group(0, 1, cur, no, nullptr, ua, ub);
+      fa.end(nxt, tid);
+      fb.end(nxt + SA::BYTES, tid);
+      // a tile's first step: the loads landed before the last tile's stores began, and those need not be waited for
+      if (t == 0 && n > 0) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      else step_barrier<0, true>();
+      group(1, 0, nxt, yes, cur, ua, ub);
+      ahead();
+      char* s = cur;
+      cur = nxt;
+      nxt = s;
+    }
+
+    // Epilogue.  A wave turns its accumulators, 16 rows at a time, through LDS of its own (16-byte piece c of row r at
+    // place c ^ r), so that a lane gets eight neighbouring outputs of a row and a row's lanes touch whole cache lines.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    constexpr int TJ = BJ / WJ, PIECES = TJ / 4, MASK = PIECES < 16 ? PIECES - 1 : 15;
+    const bool part = m.slot >= 0;
+    Epilogue e = p.e;
+    int rows = p.I, cols = p.J, i1 = m.i0 + ra, j1 = m.j0 + rb;
+    if (part) {
+      e = Epilogue{};
+      e.out = p.part + (int64_t)m.slot * (BI * BJ);
+      e.ldo = BJ;
+      e.out_f32 = 1;
+      rows = BI;
+      cols = BJ;
+      i1 = ra;
+      j1 = rb;
+    }
+    char* own = lds + K::LDS + wave * K::TURN;
+    const int g = lane >> 4, il = lane & 15;
+#pragma unroll 1
+    for (int x = 0; x < FI; ++x) {
+#pragma unroll
+      for (int u = 0; u < FI; ++u)
+        if (u == x) {
+#pragma unroll
+          for (int y = 0; y < FJ; ++y)
+            *reinterpret_cast<f32x4*>(own + (il * PIECES + ((y * 4 + g) ^ (il & MASK))) * 16) = acc[u][y];
+        }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // other lanes of the wave read what this one wrote
+#pragma unroll 1
+      for (int k = lane; k < 16 * (TJ / 8); k += 64) {
+        const int r = k / (TJ / 8), c = (k % (TJ / 8)) * 2, key = r & MASK;
+        const int i = i1 + x * 16 + r, j = j1 + c * 4;
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(own + (r * PIECES + (c ^ key)) * 16);
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(own + (r * PIECES + ((c + 1) ^ key)) * 16);
+        if (i < rows && j < cols) {
+          float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          epilogue8<T>(e, i, j, cols - j, v);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  }
+  // the loads of nothing behind the last step end before the workgroup's LDS is given away
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
 template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8>
 __global__ __launch_bounds__(K::THREADS) void product_kernel(Product p) {
   extern __shared__ char lds[];
-  product_body<T, K, FA, FB, LA, LB, Q8>(p, blockIdx.x, lds);
+  if constexpr (K::STREAM) stream_body<T, K, FA, FB, LA, LB, Q8>(p, lds);
+  else product_body<T, K, FA, FB, LA, LB, Q8>(p, blockIdx.x, lds);
 }
 
 // The backward pass's two products and the join of its column sums as one launch: workgroups [0, nx) multiply the
@@ -618,8 +829,13 @@ template <typename T, typename K, bool FA, bool FB, int LA, int LB, bool Q8>
 hipError_t launch(const Product& p, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   auto k = product_kernel<T, K, FA, FB, LA, LB, Q8>;
-  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
-  hipLaunchKernelGGL(k, dim3((unsigned)(tiles_of(p, K::BI, K::BJ) * p.splits)), dim3(K::THREADS), K::LDS, s, p);
+  constexpr int LDS = K::LAUNCH_LDS;
+  if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), LDS, done)) return e;
+  const int64_t tiles = tiles_of(p, K::BI, K::BJ);
+  // workgroups that stay: as many as the card holds at once (256 compute units, 160 KB of LDS each)
+  const int64_t groups = K::STREAM ? std::min<int64_t>(p.whole + (tiles - p.whole) * p.splits, 256 * (163840 / LDS))
+                                    : tiles * p.splits;
+  hipLaunchKernelGGL(k, dim3((unsigned)groups), dim3(K::THREADS), LDS, s, p);
   return hipGetLastError();
 }
 
