@@ -56,16 +56,17 @@ struct Cost {
 constexpr int kFormed = 2;
 constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.47, 0, 0}, {1.47, 0, 0}, 5.5},
                              {kMid, 128, 2, 1, {0.65, 1.25, 0}, {0.46, 1.25, 0}, 3.5},
-                             {kSmall, 64, 4, 1, {0.28, 0.55, 1.1}, {0.19, 0.34, 0.7}, 2.0},
+                             {kSmall, 64, 4, 1, {0.28, 0.55, 1.6}, {0.19, 0.34, 1.3}, 2.0},
                              {kSlice, 32, 1, 8, {1.0, 1.6, 2.6}, {1.0, 1.6, 2.6}, 2.0},
                              {kSlice64, 64, 1, 4, {0.75, 2.4, 0}, {0.75, 2.4, 0}, 3.5}};
 constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 0, 0}, {6.9, 0, 0}, 8.0},
                              {kMid, 128, 2, 1, {2.3, 2.7, 0}, {2.1, 2.5, 0}, 4.0},
-                             {kSmall, 64, 4, 1, {0.75, 0.95, 1.6}, {0.53, 0.65, 1.2}, 2.0},
+                             {kSmall, 64, 4, 1, {0.75, 0.95, 2.4}, {0.53, 0.65, 2.0}, 2.0},
                              {kSlice, 32, 1, 8, {1.3, 2.2, 3.5}, {1.3, 2.2, 3.5}, 2.0},
                              {kSlice64, 64, 1, 4, {2.75, 4.5, 0}, {2.75, 4.5, 0}, 3.5}};
 constexpr double kNever = 1e30;      // no plan
 constexpr double kLaunch = 3.5;      // a launch behind another, here and on the host
+constexpr double kWorkspace = 2.0;   // a small call that needs a workspace: the host's time for it
 constexpr int kUnits = 256;
 
 double step_us(const Cost& c, double per_unit, int loader) {
@@ -112,29 +113,28 @@ void set_plan(Plan& p, const Cost& c, int64_t splits, int64_t per, int bc, int64
 }
 
 // Tile and split of a product by their estimated time.
-Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader, bool q8 = false) {
+Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
   const int bc = type == kF32 ? 32 : 64;
   const int64_t steps = ceil_div(C, bc);
   Plan best;
   for (const Cost& c : type == kF32 ? kCosts32 : kCosts16) {
-    if (c.tile == kLarge && (loader != kDma || q8)) continue;
+    if (c.tile == kLarge && loader != kDma) continue;
     const int64_t tiles = ceil_div(I, c.b) * ceil_div(J, c.b);
     if (c.k > 1 && tiles > 4 * kUnits) continue;        // sliced tiles are for few outputs
-    const int l = q8 ? kReg : loader;
     const bool stream = c.tile == kLarge;
     // streamed: as many tiles whole as fill the card evenly, the others split; or all split
     const int64_t even = stream ? tiles / (kUnits * c.slots) * (kUnits * c.slots) : 0;
     for (int64_t whole : {(int64_t)0, even}) {
       const int64_t rest = tiles - whole;
       if (whole && !rest) continue;                    // nothing is left to split: the unsplit plan
-      const double before = kLaunch + (whole ? groups_us(c, whole, steps, l) : 0);
+      const double before = kLaunch + (whole ? groups_us(c, whole, steps, loader) : 0);
       if (best.c_per && before >= best.us) continue;
       for_splits(steps, whole ? 64 : most_splits(c, tiles), [&](int64_t s, int64_t per) {
         if (whole && s == 1) return;
         // split tiles' sums in fp32
         const double values = stream ? (double)rest * c.b * c.b : (double)I * J;
         if (s > 1 && values * s * 4 > 8e9) return;
-        const double t = before + groups_us(c, rest * s, per, l) + join_us(values, s);
+        const double t = before + groups_us(c, rest * s, per, loader) + join_us(values, s);
         if (best.c_per && t >= best.us) return;
         best.us = t;
         set_plan(best, c, s, per, bc, I, J);
@@ -161,13 +161,14 @@ double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, in
     const int64_t tx = nx ? ceil_div(m, c.b) * ceil_div(k, c.b) : 0, tk = nk ? ceil_div(k, c.b) * ceil_div(n, c.b) : 0;
     if (tx > 16384 || tk > 16384) continue;
     if (c.k > 1 && tx + tk > 8 * kUnits) continue;
-    for_splits(nk ? sk : 1, most_splits(c, tx + tk), [&](int64_t s, int64_t per) {
+    for_splits(nk ? sk : 1, most_splits(c, tk), [&](int64_t s, int64_t per) {
       const double wx = nx ? (double)ceil_div(sx, c.k) : 0, wk = nk ? (double)ceil_div(nk ? per : 0, c.k) : 0;
       const double groups = (double)(tx + tk * s);
       const double share = ((double)tx * (wx * c.share[lx] + c.ends / c.slots) +
                             (double)tk * s * (wk * c.share[lk] + c.ends / c.slots)) / kUnits;
       const double longest = std::max(wx * c.wait[lx], wk * c.wait[lk]) + c.ends;
-      const double t = kLaunch + std::max(longest, share * (groups > kUnits * c.slots ? 1.1 : 1.0)) + join_us((double)k * n, s);
+      const double t = kLaunch + std::max(longest, share * (groups > kUnits * c.slots ? 1.1 : 1.0)) +
+                       (s > 1 ? join_us((double)k * n, s) + kWorkspace : 0.0);
       if (t >= best) return;
       best = t;
       set_plan(px, c, 1, sx, bc, m, k);
@@ -271,7 +272,17 @@ struct ForwardPlan {
 ForwardPlan plan_forward(const petdense_forward_args* a) {
   ForwardPlan f{};
   f.rows = a->m <= kMaxRows;
-  if (f.rows || a->m == 0) return f;
+  if (a->m == 0) return f;
+  if (f.rows) {
+    // narrow layers leave compute units without columns: the contraction is split, where that is worth the join
+    const int64_t groups = ceil_div(a->n, kRowCols);
+    const int64_t want = std::min<int64_t>(kUnits / groups, a->k / 1024);
+    f.p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, 16));
+    f.p.c_per = (int)ceil_div(a->k, f.p.splits);
+    f.p.splits = (int)ceil_div(a->k, f.p.c_per);
+    f.bytes = f.p.splits > 1 ? up((size_t)f.p.splits * a->m * a->n * 4) : 0;
+    return f;
+  }
   const int sz = size_of(a->dtype);
   const bool x_ok = dma_ok(a->x, a->ldx, a->k, sz), w_ok = dma_ok(a->kernel, a->ldk, a->n, sz);
   f.loader = x_ok && w_ok ? kDma : kReg;
@@ -342,11 +353,11 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, BackwardPl
   b.px = b.pk = Plan{};
   b.pair = false;
   if (a->dx) b.px = plan(a->m, a->k, a->n, a->dtype, lx);
-  if (a->dkernel) b.pk = plan(a->k, a->n, a->m, a->dtype, lk, q8);
+  if (a->dkernel) b.pk = plan(a->k, a->n, a->m, a->dtype, lk);
   double us = b.px.us + b.pk.us + (b.sums ? kLaunch : 0.0);
   if (a->dx && a->dkernel) {
     Plan px, pk;
-    const double t = plan_pair(true, true, a->m, a->k, a->n, a->dtype, lx, q8 ? kReg : lk, true, px, pk);
+    const double t = plan_pair(true, true, a->m, a->k, a->n, a->dtype, lx, lk, true, px, pk);
     if (t < us) {
       us = t;
       b.pair = true;
@@ -354,6 +365,9 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, BackwardPl
       b.pk = pk;
     }
   }
+  // 8-bit inputs come through registers.  Nothing but their product's own plan goes by them: the input's gradient is
+  // the same, bit by bit, with either.
+  if (q8 && !b.pair) b.pk = plan(a->k, a->n, a->m, a->dtype, kReg);
   return us;
 }
 
@@ -374,8 +388,8 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
   // dp in the workspace has rows of whole pieces, with zeros: DMA takes it as it is
   const bool dp_ok = own_dp || (a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz) : dma_ok(a->dy, a->lddy, a->n, sz));
   const bool w_ok = !a->dx || dma_ok(a->kernel, a->ldk, a->n, sz);
-  const bool x_ok = !a->dkernel || q8 || dma_ok(a->x, a->ldx, a->k, sz);
-  // 8-bit inputs go through registers whatever their alignment: their loader is dp's
+  const bool x_ok = !a->dkernel || (q8 ? a->k * sz % 16 == 0 : dma_ok(a->x, a->ldx, a->k, sz));
+  // (8-bit inputs go through registers whatever their alignment: their loader is dp's)
   b.us = act_us + plan_products(a, dp_ok && w_ok ? kDma : kReg, dp_ok && x_ok ? kDma : kReg, b);
   if (!(dp_ok && w_ok && x_ok) && (a->dx || a->dkernel) &&
       copies_fit((double)a->m * a->n + (double)a->k * a->n + (double)a->m * a->k, sz)) {
@@ -386,7 +400,7 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
       b = c;
       b.dp.on = !dp_ok;
       b.kernel.on = !w_ok;
-      b.x.on = !x_ok;
+      b.x.on = !x_ok && !q8;
     }
   }
   if ((a->dx || a->dkernel) && (b.make_dp || b.sums) && !a->dresidual) {
@@ -447,7 +461,9 @@ int petdense_forward(const petdense_forward_args* a, void* work, size_t work_byt
   p.C = (int)a->k;
   p.e = Epilogue{a->bias, a->residual, a->y, a->pre, a->ldr, a->ldy, a->ldp, a->activation, a->bias_f32, a->out_f32};
   if (f.rows) {
+    p = placed(p, f.p, work);
     HIPC(rows(p, a->dtype, (hipStream_t)stream));
+    if (p.splits > 1) HIPC(join(p, a->dtype, (hipStream_t)stream));
     return PETDIFF_OK;
   }
   char* w = static_cast<char*>(work);

@@ -4,6 +4,18 @@
 
 namespace petdense_k {
 
+// hipLaunchKernel itself: the launch syntax pushes and pops a configuration first, which a small call would notice
+template <typename A>
+struct Same {
+  typedef A type;
+};
+template <typename... A>
+inline hipError_t launch_kernel(void (*k)(A...), dim3 grid, dim3 block, size_t lds, hipStream_t s,
+                                typename Same<A>::type... a) {
+  void* args[] = {static_cast<void*>(&a)...};
+  return hipLaunchKernel(reinterpret_cast<const void*>(k), grid, block, args, lds, s);
+}
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Phi(x) = (1 + erf(x / sqrt 2)) / 2.

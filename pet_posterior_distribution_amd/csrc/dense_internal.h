@@ -99,7 +99,7 @@ __host__ __device__ inline void tile_at(int t, int ti, int tj, int& i, int& j) {
 }
 
 // Few rows: one pass over B ([C][J], j-contiguous), I <= kMaxRows.
-constexpr int kMaxRows = 8;
+constexpr int kMaxRows = 8, kRowThreads = 1024, kRowCols = 32;
 hipError_t rows(const Product& p, int type, hipStream_t s);
 
 // lanes that share a row of N columns in act_grad: a power of two

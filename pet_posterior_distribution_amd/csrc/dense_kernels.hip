@@ -56,12 +56,10 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(Product p, int b, int t
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Few rows (decoding, a single sample): every value of B is read once by one workgroup, which owns COLS columns and
-// the whole contraction, so that one launch ends the call.  4 lanes share a row's 8-column pieces; the other lanes
+// Few rows (decoding, a single sample): every value of B is read once by one workgroup, which owns 32 columns and, where
+// those are enough workgroups, the whole contraction, so that one launch ends the call.  4 lanes share a row's 8-column pieces; the other lanes
 // and waves take other rows; their sums meet by shuffles and then in LDS, in a fixed order.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kRowThreads = 1024, kRowCols = 32;
-
 template <typename T, int ROWS>
 __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
   constexpr int W = 8, LANES = kRowCols / W, GROUPS = kRowThreads / LANES;   // 4 lanes a row, 256 rows at a time
@@ -86,9 +84,10 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) x[r] = A[(r < p.I ? r : 0) * p.lda + c];      // rows past the last are not stored
   };
-  int c = grp;
+  const int end = min(p.C, ((int)blockIdx.y + 1) * p.c_per);      // this part of the contraction
+  int c = blockIdx.y * p.c_per + grp;
   if (n >= W) {
-    for (; c + (AHEAD - 1) * GROUPS < p.C; c += AHEAD * GROUPS) {
+    for (; c + (AHEAD - 1) * GROUPS < end; c += AHEAD * GROUPS) {
       T w[AHEAD][W], x[AHEAD][ROWS];
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) __builtin_memcpy(w[u], B + (int64_t)(c + u * GROUPS) * p.ldb, sizeof(w[u]));
@@ -97,14 +96,14 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) add(w[u], x[u]);
     }
-    for (; c < p.C; c += GROUPS) {
+    for (; c < end; c += GROUPS) {
       T w[W], x[ROWS];
       __builtin_memcpy(w, B + (int64_t)c * p.ldb, sizeof(w));
       xs(c, x);
       add(w, x);
     }
   } else if (n > 0) {
-    for (; c < p.C; c += GROUPS) {
+    for (; c < end; c += GROUPS) {
       T w[W], x[ROWS];
 #pragma unroll
       for (int q = 0; q < W; ++q) w[q] = q < n ? B[(int64_t)c * p.ldb + q] : (T)0.f;
@@ -129,19 +128,19 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
       for (int w = 0; w < kRowThreads / 64; ++w)
 #pragma unroll
         for (int q = 0; q < W; ++q) v[q] += red[w][r][c + q];
-      epilogue8<T>(p.e, r, j0 + c, p.J - j0 - c, v);
+      if (p.splits > 1) store_row<float, W>(p.part + ((int64_t)blockIdx.y * p.I + r) * p.J + j0 + c, p.J - j0 - c, v);
+      else epilogue8<T>(p.e, r, j0 + c, p.J - j0 - c, v);
     }
   }
 }
 
 template <typename T>
 hipError_t rows_t(const Product& p, hipStream_t s) {
-  const dim3 grid(blocks_for(p.J, kRowCols)), block(kRowThreads);
-  if (p.I == 1) hipLaunchKernelGGL((rows_kernel<T, 1>), grid, block, 0, s, p);
-  else if (p.I == 2) hipLaunchKernelGGL((rows_kernel<T, 2>), grid, block, 0, s, p);
-  else if (p.I <= 4) hipLaunchKernelGGL((rows_kernel<T, 4>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((rows_kernel<T, 8>), grid, block, 0, s, p);
-  return hipGetLastError();
+  const dim3 grid(blocks_for(p.J, kRowCols), p.splits), block(kRowThreads);
+  if (p.I == 1) return launch_kernel(rows_kernel<T, 1>, grid, block, 0, s, p);
+  else if (p.I == 2) return launch_kernel(rows_kernel<T, 2>, grid, block, 0, s, p);
+  else if (p.I <= 4) return launch_kernel(rows_kernel<T, 4>, grid, block, 0, s, p);
+  else return launch_kernel(rows_kernel<T, 8>, grid, block, 0, s, p);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -214,10 +213,9 @@ template <typename T>
 hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, int bare,
                       float* part, int chunks, int M, int N, int act, hipStream_t s) {
   const int rows_per = (M + chunks - 1) / chunks, lpr = act_grad_lanes(N);
-  hipLaunchKernelGGL((act_grad_kernel<T>), dim3(blocks_for(N, lpr * 8), chunks), dim3(256), 0, s,
+  return launch_kernel(act_grad_kernel<T>, dim3(blocks_for(N, lpr * 8), chunks), dim3(256), 0, s,
                      static_cast<const T*>(dy), ldy, static_cast<const T*>(saved), lds, static_cast<T*>(dp), ldd, bare, part,
                      rows_per, M, N, act, lpr);
-  return hipGetLastError();
 }
 
 __global__ __launch_bounds__(256) void join_columns_kernel(ColumnJoin p) {
@@ -345,10 +343,9 @@ hipError_t quantize_t(const void* x, int64_t ldx, int64_t M, int K, uint8_t* cod
   const int64_t slab = std::max<int64_t>(1, kSlab / orow);
   for (int64_t m = 0; m < M; m += slab) {
     const int64_t octets = std::min(slab, M - m) * orow;
-    hipLaunchKernelGGL((quantize_kernel<T>), dim3(blocks_for(octets, 256)), dim3(256), 0, s,
-                       static_cast<const T*>(x) + m * ldx, ldx, octets, orow, K, codes + m * ldc, ldc, exps + m * lde,
-                       lde);
-    if (hipError_t e = hipGetLastError()) return e;
+    if (hipError_t e = launch_kernel(quantize_kernel<T>, dim3(blocks_for(octets, 256)), dim3(256), 0, s,
+                       static_cast<const T*>(x) + m * ldx, ldx, octets, orow, K, codes + m * ldc, ldc, exps + m * lde, lde))
+      return e;
   }
   return hipSuccess;
 }
@@ -360,9 +357,9 @@ hipError_t restore_t(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int
   const int64_t slab = std::max<int64_t>(1, kSlab / orow);
   for (int64_t m = 0; m < M; m += slab) {
     const int64_t octets = std::min(slab, M - m) * orow;
-    hipLaunchKernelGGL((restore_kernel<T>), dim3(blocks_for(octets, 256)), dim3(256), 0, s, codes + m * ldc, ldc,
-                       exps + m * lde, lde, octets, orow, K, static_cast<T*>(x) + m * ldx, ldx);
-    if (hipError_t e = hipGetLastError()) return e;
+    if (hipError_t e = launch_kernel(restore_kernel<T>, dim3(blocks_for(octets, 256)), dim3(256), 0, s, codes + m * ldc, ldc,
+                       exps + m * lde, lde, octets, orow, K, static_cast<T*>(x) + m * ldx, ldx))
+      return e;
   }
   return hipSuccess;
 }
@@ -379,16 +376,14 @@ hipError_t restore_t(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int
 hipError_t join(const Product& p, int type, hipStream_t s) {
   const int orow = (p.J + 7) / 8;
   const int64_t octets = (int64_t)p.I * orow;
-  PETDENSE_BY_TYPE(type, hipLaunchKernelGGL((join_kernel<T>), dim3(blocks_for(octets, 256)), dim3(256), 0, s, p,
-                                            octets, orow);
-                   return hipGetLastError())
+  PETDENSE_BY_TYPE(type, return launch_kernel(join_kernel<T>, dim3(blocks_for(octets, 256)), dim3(256), 0, s, p,
+                                            octets, orow);)
 }
 
 hipError_t join_tiles(const Product& p, int type, int b, hipStream_t s) {
   const int ti = (p.I + b - 1) / b, tj = (p.J + b - 1) / b;
-  PETDENSE_BY_TYPE(type, hipLaunchKernelGGL((join_tiles_kernel<T>), dim3(blocks_for(b * (b / 8), 256), ti * tj - p.whole),
-                                            dim3(256), 0, s, p, b, ti, tj);
-                   return hipGetLastError())
+  PETDENSE_BY_TYPE(type, return launch_kernel(join_tiles_kernel<T>, dim3(blocks_for(b * (b / 8), 256), ti * tj - p.whole),
+                                            dim3(256), 0, s, p, b, ti, tj);)
 }
 
 hipError_t rows(const Product& p, int type, hipStream_t s) { PETDENSE_BY_TYPE(type, return rows_t<T>(p, s)) }
@@ -403,15 +398,13 @@ hipError_t pad_t(const PadJobs& p, hipStream_t s) {
   int64_t pieces = 0;
   for (const PadJob& j : p.job) pieces += (int64_t)j.rows * (j.ldd * (int64_t)sizeof(T) / 16);
   if (pieces >= (int64_t)1 << 32) return hipErrorInvalidValue;      // the plan copies nothing of that size
-  hipLaunchKernelGGL((pad_kernel<T>), dim3(blocks_for(pieces, 256)), dim3(256), 0, s, p);
-  return hipGetLastError();
+  return launch_kernel(pad_kernel<T>, dim3(blocks_for(pieces, 256)), dim3(256), 0, s, p);
 }
 
 hipError_t pad(const PadJobs& p, int type, hipStream_t s) { PETDENSE_BY_TYPE(type, return pad_t<T>(p, s)) }
 
 hipError_t join_columns(const ColumnJoin& c, hipStream_t s) {
-  hipLaunchKernelGGL(join_columns_kernel, dim3(blocks_for(c.N, 16)), dim3(256), 0, s, c);
-  return hipGetLastError();
+  return launch_kernel(join_columns_kernel, dim3(blocks_for(c.N, 16)), dim3(256), 0, s, c);
 }
 
 __global__ __launch_bounds__(256) void fill_zero_kernel(char* p, int64_t total, int n, int64_t ld, int size) {
@@ -425,9 +418,8 @@ __global__ __launch_bounds__(256) void fill_zero_kernel(char* p, int64_t total, 
 
 hipError_t fill_zero(void* p, int64_t rows, int n, int64_t ld, int size, hipStream_t s) {
   const int64_t total = rows * n;
-  hipLaunchKernelGGL(fill_zero_kernel, dim3((unsigned)std::min<int64_t>(4096, (total + 255) / 256)), dim3(256), 0, s,
+  return launch_kernel(fill_zero_kernel, dim3((unsigned)std::min<int64_t>(4096, (total + 255) / 256)), dim3(256), 0, s,
                      static_cast<char*>(p), total, n, ld, size);
-  return hipGetLastError();
 }
 
 hipError_t quantize(const void* x, int64_t ldx, int64_t M, int K, int type, uint8_t* codes, int64_t ldc, uint8_t* exps,

@@ -835,8 +835,7 @@ hipError_t launch(const Product& p, hipStream_t s) {
   // workgroups that stay: as many as the card holds at once (256 compute units, 160 KB of LDS each)
   const int64_t groups = K::STREAM ? std::min<int64_t>(p.whole + (tiles - p.whole) * p.splits, 256 * (163840 / LDS))
                                     : tiles * p.splits;
-  hipLaunchKernelGGL(k, dim3((unsigned)groups), dim3(K::THREADS), LDS, s, p);
-  return hipGetLastError();
+  return launch_kernel(k, dim3((unsigned)groups), dim3(K::THREADS), LDS, s, p);
 }
 
 template <typename T, typename K, int LX, int LK, bool Q8>
@@ -846,8 +845,7 @@ hipError_t launch_pair(Pair p, hipStream_t s) {
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
   p.nx = (int)(tiles_of(p.x, K::BI, K::BJ) * p.x.splits);
   p.nk = (int)(tiles_of(p.k, K::BI, K::BJ) * p.k.splits);
-  hipLaunchKernelGGL(k, dim3((unsigned)(p.nx + p.nk + (p.cols.N + 15) / 16)), dim3(K::THREADS), K::LDS, s, p);
-  return hipGetLastError();
+  return launch_kernel(k, dim3((unsigned)(p.nx + p.nk + (p.cols.N + 15) / 16)), dim3(K::THREADS), K::LDS, s, p);
 }
 
 template <typename T, typename K, bool Q8>
@@ -857,8 +855,7 @@ hipError_t launch_fused(Pair p, hipStream_t s) {
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
   p.nx = p.x.e.out ? (int)(tiles_of(p.x, K::BI, K::BJ) * p.x.splits) : 0;
   p.nk = p.k.e.out ? (int)(tiles_of(p.k, K::BI, K::BJ) * p.k.splits) : 0;
-  hipLaunchKernelGGL(k, dim3((unsigned)(p.nx + p.nk + (p.sums.N + 7) / 8)), dim3(K::THREADS), K::LDS, s, p);
-  return hipGetLastError();
+  return launch_kernel(k, dim3((unsigned)(p.nx + p.nk + (p.sums.N + 7) / 8)), dim3(K::THREADS), K::LDS, s, p);
 }
 
 template <typename T, typename K>

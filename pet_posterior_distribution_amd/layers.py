@@ -52,56 +52,62 @@ def _check(rc, what):
 
 
 def _activation(activation):
-    name = activation.lower() if isinstance(activation, str) else activation
-    if name not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation) if activation is None or isinstance(activation, str) else None
+    if act is None and isinstance(activation, str):
+        act = ACTIVATIONS.get(activation.lower())
+    if act is None:
         raise ValueError(f'activation must be one of {sorted(k for k in ACTIVATIONS if k)} or None, got {activation!r}')
-    return ACTIVATIONS[name]
+    return act
 
 
-def _dtype(t, what):
-    if t.dtype not in _TYPES:
-        raise ValueError(f'{what} must be bfloat16, float16 or float32, got {t.dtype}')
-    return _TYPES[t.dtype]
-
-
-def _on(t, device, what):
+def _lead(t, what):
+    """(type code, device) of the call's leading operand."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f'{what} must be a CUDA tensor')
-    if device is not None and t.device != device:
-        raise ValueError(f'{what} is on {t.device}, x is on {device}')
-    return t
+    dt = _TYPES.get(t.dtype)
+    if dt is None:
+        raise ValueError(f'{what} must be bfloat16, float16 or float32, got {t.dtype}')
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f'{what} must have a last dimension of at least 1, got shape {tuple(t.shape)}')
+    return dt, t.device
 
 
-def _rows(t, what):
-    """(..., n) as rows that are contiguous and do not overlap (copied if they have to be), and their stride."""
+def _operand(t, shape, dtype, dev, what):
+    """t as rows (see _rows) after the checks that it is what the call's other operands ask for."""
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype or t.device != dev:
+        _refuse(t, shape, dtype, dev, what)
     if t.is_contiguous():
-        return t, t.shape[-1]
+        return t, shape[-1]
+    return _rows(t)
+
+
+def _refuse(t, shape, dtype, dev, what):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f'{what} must be a CUDA tensor')
+    if t.device != dev:
+        raise ValueError(f'{what} is on {t.device}, not on {dev}')
+    if t.shape != shape:
+        raise ValueError(f'{what} must have shape {tuple(shape)}, got {tuple(t.shape)}')
+    raise ValueError(f'{what} must be {dtype}, got {t.dtype}')
+
+
+def _rows(t):
+    """(..., n) as rows that are contiguous and do not overlap (copied if they have to be), and their stride."""
     n = t.shape[-1]
+    if t.is_contiguous():
+        return t, n
     v = t if t.dim() <= 2 else t.reshape(-1, n)      # a view where the leading dimensions can be merged
     if v.dim() == 2 and (n == 1 or v.stride(1) == 1) and v.stride(0) >= n:
         return v, v.stride(0)
     return v.contiguous(), n
 
 
-def _same_rows(t, shape, dtype, device, what):
-    _on(t, device, what)
-    if t.shape != shape:
-        raise ValueError(f'{what} must have shape {tuple(shape)}, got {tuple(t.shape)}')
-    if t.dtype != dtype:
-        raise ValueError(f'{what} must be {dtype}, got {t.dtype}')
-    return _rows(t, what)
-
-
-def _kernel(kernel, k, dtype, device):
-    _on(kernel, device, 'kernel')
-    shape = kernel.shape
-    if len(shape) != 2 or shape[0] != k:
-        raise ValueError(f'kernel must be (k, n) with k = {k}, got {tuple(shape)}')
-    if kernel.dtype != dtype:
-        raise ValueError(f'kernel must be {dtype}, got {kernel.dtype}')
-    if shape[1] < 1:
-        raise ValueError('kernel must not be empty')
-    return _rows(kernel, 'kernel')
+def _units(kernel, k):
+    """n of a kernel (k, n)."""
+    if not isinstance(kernel, torch.Tensor) or kernel.dim() != 2 or kernel.shape[0] != k or kernel.shape[1] < 1:
+        got = tuple(kernel.shape) if isinstance(kernel, torch.Tensor) else type(kernel).__name__
+        raise ValueError(f'kernel must be (k, n) with k = {k} and n >= 1, got {got}')
+    return kernel.shape[1]
 
 
 def _ptr(t):
@@ -150,34 +156,32 @@ def dense(x, kernel, bias=None, activation=None, residual=None, return_preactiva
     x (..., k), kernel (k, n), bias (n,) of x's type or float32, residual (..., n); activation None, 'relu', 'gelu'
     (erf) or 'silu'.  ``out_dtype``: x's type (default) or float32.  With ``return_preactivation`` also returns the
     value before the activation, in the output's type (what ``dense_backward`` wants saved for GELU and SiLU)."""
-    _on(x, None, 'x')
-    dt = _dtype(x, 'x')
-    dev = x.device
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError('x must be (..., k) with k >= 1')
+    dt, dev = _lead(x, 'x')
+    t = x.dtype
     shape = x.shape
     k = shape[-1]
-    w, ldk = _kernel(kernel, k, x.dtype, dev)
-    n = kernel.shape[1]
-    m = x.numel() // k
+    n = _units(kernel, k)
     out = (*shape[:-1], n)
     act = _activation(activation)
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in (x.dtype, torch.float32):
-        raise ValueError(f'out_dtype must be {x.dtype} or float32, got {out_dtype}')
+    if out_dtype is None:
+        out_dtype = t
+    elif out_dtype not in (t, torch.float32):
+        raise ValueError(f'out_dtype must be {t} or float32, got {out_dtype}')
+    bias_f32 = False
     if bias is not None:
-        _on(bias, dev, 'bias')
-        if tuple(bias.shape) != (n,) or bias.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f'bias must be ({n},) of {x.dtype} or float32, got {tuple(bias.shape)} of {bias.dtype}')
-        bias = bias.contiguous()
-    x2, ldx = _rows(x, 'x')
-    r2, ldr = (None, 0) if residual is None else _same_rows(residual, out, x.dtype, dev, 'residual')
+        bias_f32 = isinstance(bias, torch.Tensor) and bias.dtype == torch.float32
+        bias, _ = _operand(bias, (n,), torch.float32 if bias_f32 else t, dev, 'bias')
+    x, ldx = _rows(x)
+    kernel, ldk = _operand(kernel, (k, n), t, dev, 'kernel')
+    ldr = 0
+    if residual is not None:
+        residual, ldr = _operand(residual, out, t, dev, 'residual')
     y = torch.empty(out, dtype=out_dtype, device=dev)
     pre = torch.empty(out, dtype=out_dtype, device=dev) if return_preactivation else None
     L = _lib.lib()
     _run(L.petdense_forward, L.petdense_forward_workspace, _FORWARD.pack(
-        _ptr(x2), _ptr(w), _ptr(bias), _ptr(r2), _ptr(y), _ptr(pre), ldx, ldk, ldr, n, n, m, k, n, dt, act,
-        bias is not None and bias.dtype == torch.float32, out_dtype == torch.float32), dev, 'dense')
+        x.data_ptr(), kernel.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(pre), ldx, ldk, ldr, n, n,
+        y.numel() // n, k, n, dt, act, bias_f32, out_dtype == torch.float32), dev, 'dense')
     return (y, pre) if return_preactivation else y
 
 
@@ -189,50 +193,48 @@ def dense_backward(dy, x, kernel, activation=None, saved=None, need_x=True, need
     'silu', the pre-activation or the output for 'relu', of dy's type.  ``grad_dtype``: type of the kernel's and the
     bias's gradients, dy's (default) or float32; dx and the residual's gradient have dy's type.  Returns
     ``DenseGradients``."""
-    _on(dy, None, 'dy')
-    dt = _dtype(dy, 'dy')
-    dev = dy.device
-    if dy.dim() < 1 or dy.shape[-1] < 1:
-        raise ValueError('dy must be (..., n) with n >= 1')
+    dt, dev = _lead(dy, 'dy')
+    t = dy.dtype
     shape = dy.shape
     lead, n = shape[:-1], shape[-1]
     act = _activation(activation)
-    grad_dtype = dy.dtype if grad_dtype is None else grad_dtype
-    if grad_dtype not in (dy.dtype, torch.float32):
-        raise ValueError(f'grad_dtype must be {dy.dtype} or float32, got {grad_dtype}')
+    if grad_dtype is None:
+        grad_dtype = t
+    elif grad_dtype not in (t, torch.float32):
+        raise ValueError(f'grad_dtype must be {t} or float32, got {grad_dtype}')
     exps, lde = None, 0
     if isinstance(x, ActivationCheckpoint):
-        if x.dtype != dy.dtype:
-            raise ValueError(f'the checkpoint is of {x.dtype} activations, dy is {dy.dtype}')
-        k = x.shape[-1]
-        if x.shape[:-1] != lead:
-            raise ValueError(f'the checkpoint must have shape {(*lead, k)}, got {tuple(x.shape)}')
-        _on(x.codes, dev, 'the checkpoint')
-        x2, ldx = _rows(x.codes, 'codes')
-        exps, lde = _rows(x.exponents, 'exponents')
+        if x.dtype != t:
+            raise ValueError(f'the checkpoint is of {x.dtype} activations, dy is {t}')
+        k = x.codes.shape[-1]
+        exps, lde = _operand(x.exponents, (*lead, -(-k // BLOCK)), torch.uint8, dev, "the checkpoint's exponents")
+        x, ldx = _operand(x.codes, (*lead, k), x.codes.dtype, dev, 'the checkpoint')
     else:
         k = x.shape[-1] if isinstance(x, torch.Tensor) and x.dim() else 0
-        x2, ldx = _same_rows(x, (*lead, k), dy.dtype, dev, 'x')
+        x, ldx = _operand(x, (*lead, k), t, dev, 'x')
         if k < 1:
             raise ValueError('x must be (..., k) with k >= 1')
-    w, ldk = _kernel(kernel, k, dy.dtype, dev)
-    if kernel.shape[1] != n:
+    if _units(kernel, k) != n:
         raise ValueError(f'kernel must be ({k}, {n}), got {tuple(kernel.shape)}')
-    s2, lds = None, 0
+    kernel, ldk = _operand(kernel, (k, n), t, dev, 'kernel')
+    lds = 0
     if act:
         if saved is None:
             raise ValueError(f'activation {activation!r} needs saved=')
-        s2, lds = _same_rows(saved, shape, dy.dtype, dev, 'saved')
-    d2, ldd = _rows(dy, 'dy')
-
-    gx = torch.empty((*lead, k), dtype=dy.dtype, device=dev) if need_x else None
+        saved, lds = _operand(saved, shape, t, dev, 'saved')
+    else:
+        saved = None
+    m = dy.numel() // n
+    dy, ldd = _rows(dy)
+    gx = torch.empty((*lead, k), dtype=t, device=dev) if need_x else None
     gk = torch.empty((k, n), dtype=grad_dtype, device=dev) if need_kernel else None
     gb = torch.empty((n,), dtype=grad_dtype, device=dev) if need_bias else None
-    gr = torch.empty(shape, dtype=dy.dtype, device=dev) if need_residual else None
+    gr = torch.empty(shape, dtype=t, device=dev) if need_residual else None
     L = _lib.lib()
     _run(L.petdense_backward, L.petdense_backward_workspace, _BACKWARD.pack(
-        _ptr(d2), _ptr(x2), _ptr(exps), _ptr(w), _ptr(s2), _ptr(gx), _ptr(gk), _ptr(gb), _ptr(gr), ldd, ldx, lde, ldk,
-        lds, k, n, n, dy.numel() // n, k, n, dt, act, grad_dtype == torch.float32), dev, 'dense_backward')
+        dy.data_ptr(), x.data_ptr(), _ptr(exps), kernel.data_ptr(), _ptr(saved), _ptr(gx), _ptr(gk), _ptr(gb),
+        _ptr(gr), ldd, ldx, lde, ldk, lds, k, n, n, m, k, n, dt, act, grad_dtype == torch.float32), dev,
+        'dense_backward')
     return DenseGradients(gx, gk, gb, gr)
 
 
@@ -242,13 +244,11 @@ class ActivationCheckpoint:
     a value is off by at most 2^-4 of itself, or 2^-10 of its block's 2^E, a part in 2^17.8 of the block's largest."""
 
     def __init__(self, codes, exponents, dtype):
-        _on(codes, None, 'codes')
+        if not isinstance(codes, torch.Tensor) or not codes.is_cuda:
+            raise ValueError('codes must be a CUDA tensor')
         if codes.dtype not in (torch.float8_e4m3fn, torch.uint8) or codes.dim() < 1 or codes.shape[-1] < 1:
             raise ValueError('codes must be (..., k) of float8_e4m3fn, k >= 1')
-        want = (*codes.shape[:-1], -(-codes.shape[-1] // BLOCK))
-        _on(exponents, codes.device, 'exponents')
-        if tuple(exponents.shape) != want or exponents.dtype != torch.uint8:
-            raise ValueError(f'exponents must be {want} of uint8, got {tuple(exponents.shape)} of {exponents.dtype}')
+        _operand(exponents, (*codes.shape[:-1], -(-codes.shape[-1] // BLOCK)), torch.uint8, codes.device, 'exponents')
         if dtype not in _TYPES:
             raise ValueError(f'dtype must be bfloat16, float16 or float32, got {dtype}')
         self.codes, self.exponents, self.dtype = codes, exponents, dtype
@@ -267,26 +267,26 @@ class ActivationCheckpoint:
 
     def restore(self):
         """The activations that the codes stand for (..., k), in ``dtype``."""
-        c2, ldc = _rows(self.codes, 'codes')
-        e2, lde = _rows(self.exponents, 'exponents')
-        dev, k = self.codes.device, self.codes.shape[-1]
+        codes, ldc = _rows(self.codes)
+        exps, lde = _rows(self.exponents)
+        dev, k = codes.device, codes.shape[-1]
         x = torch.empty(self.codes.shape, dtype=self.dtype, device=dev)
-        _run_plain(_lib.lib().petdense_restore, (_ptr(c2), ldc, _ptr(e2), lde, x.numel() // k, k, _TYPES[self.dtype],
-                                                 _ptr(x), k), dev, 'restore')
+        _run_plain(_lib.lib().petdense_restore, (codes.data_ptr(), ldc, exps.data_ptr(), lde, x.numel() // k, k,
+                                                 _TYPES[self.dtype], x.data_ptr(), k), dev, 'restore')
         return x
 
 
 def checkpoint_activations(x):
     """``ActivationCheckpoint`` of x (..., k): what a layer's backward pass needs of its input, in 8 bits."""
-    _on(x, None, 'x')
-    dt = _dtype(x, 'x')
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError('x must be (..., k) with k >= 1')
-    x2, ldx = _rows(x, 'x')
-    k = x.shape[-1]
+    dt, dev = _lead(x, 'x')
+    shape = x.shape
+    k = shape[-1]
     nb = -(-k // BLOCK)
-    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    exps = torch.empty((*x.shape[:-1], nb), dtype=torch.uint8, device=x.device)
-    _run_plain(_lib.lib().petdense_checkpoint, (_ptr(x2), ldx, x.numel() // k, k, dt, _ptr(codes), k, _ptr(exps), nb),
-               x.device, 'checkpoint_activations')
-    return ActivationCheckpoint(codes, exps, x.dtype)
+    c = ActivationCheckpoint.__new__(ActivationCheckpoint)
+    c.codes = codes = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev)
+    c.exponents = exps = torch.empty((*shape[:-1], nb), dtype=torch.uint8, device=dev)
+    c.dtype = x.dtype
+    x, ldx = _rows(x)
+    _run_plain(_lib.lib().petdense_checkpoint, (x.data_ptr(), ldx, codes.numel() // k, k, dt, codes.data_ptr(), k,
+                                                exps.data_ptr(), nb), dev, 'checkpoint_activations')
+    return c

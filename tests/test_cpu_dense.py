@@ -130,7 +130,7 @@ def test_packed_arguments_are_the_structs():
 
 def test_row_views():
     def rows(t, what):
-        return layers._rows(t, what)
+        return layers._rows(t)
 
     x = torch.zeros(6, 10)
     assert rows(x, 'x')[1] == 10 and rows(x[:, :4], 'x')[1] == 10 and rows(x[::2, :4], 'x')[1] == 20
