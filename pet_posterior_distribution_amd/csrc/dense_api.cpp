@@ -54,16 +54,16 @@ struct Cost {
   double wait[3], share[3], ends;
 };
 constexpr int kFormed = 2;
-constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.47, 0, 0}, {1.47, 0, 0}, 5.5},
+constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.47, 0, 0}, {1.47, 0, 0}, 7.5},
                              {kMid, 128, 2, 1, {0.65, 1.25, 0}, {0.46, 1.25, 0}, 3.5},
-                             {kSmall, 64, 4, 1, {0.28, 0.55, 1.6}, {0.19, 0.34, 1.3}, 2.0},
-                             {kSlice, 32, 1, 8, {1.0, 1.6, 2.6}, {1.0, 1.6, 2.6}, 2.0},
-                             {kSlice64, 64, 1, 4, {0.75, 2.4, 0}, {0.75, 2.4, 0}, 3.5}};
+                             {kSmall, 64, 4, 1, {0.28, 0.55, 2.0}, {0.19, 0.34, 1.5}, 2.0},
+                             {kSlice, 32, 1, 8, {0.5, 1.0, 3.4}, {1.2, 1.5, 3.4}, 2.0},
+                             {kSlice64, 64, 1, 4, {0.7, 2.4, 0}, {0.75, 2.4, 0}, 3.5}};
 constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 0, 0}, {6.9, 0, 0}, 8.0},
                              {kMid, 128, 2, 1, {2.3, 2.7, 0}, {2.1, 2.5, 0}, 4.0},
                              {kSmall, 64, 4, 1, {0.75, 0.95, 2.4}, {0.53, 0.65, 2.0}, 2.0},
-                             {kSlice, 32, 1, 8, {1.3, 2.2, 3.5}, {1.3, 2.2, 3.5}, 2.0},
-                             {kSlice64, 64, 1, 4, {2.75, 4.5, 0}, {2.75, 4.5, 0}, 3.5}};
+                             {kSlice, 32, 1, 8, {1.1, 1.3, 3.5}, {1.3, 1.5, 3.5}, 2.0},
+                             {kSlice64, 64, 1, 4, {2.6, 4.5, 0}, {2.75, 4.5, 0}, 3.5}};
 constexpr double kNever = 1e30;      // no plan
 constexpr double kLaunch = 3.5;      // a launch behind another, here and on the host
 constexpr double kWorkspace = 2.0;   // a small call that needs a workspace: the host's time for it
@@ -73,12 +73,18 @@ double step_us(const Cost& c, double per_unit, int loader) {
   return std::max(c.wait[loader], c.share[loader] * per_unit);
 }
 
+// a workgroup's first load and its epilogue; through registers also its last step, whose pieces are cut to size
+double ends_us(const Cost& c, int loader) { return c.ends + (loader == kReg ? 1.2 : 0.0); }
+
 // `groups` workgroups of `steps` each, one after another where they are too many
 double groups_us(const Cost& c, int64_t groups, int64_t steps, int loader) {
-  const double per = (double)ceil_div(steps, c.k);
+  const double per = (double)ceil_div(steps, c.k), ends = ends_us(c, loader);
   const int64_t whole = groups / (kUnits * c.slots), rest = groups % (kUnits * c.slots);
-  double t = whole * (per * step_us(c, c.slots, loader) + c.ends);
-  if (rest) t += per * step_us(c, (double)ceil_div(rest, kUnits), loader) + c.ends;
+  double t = whole * (per * step_us(c, c.slots, loader) + ends);
+  if (rest) {
+    const double unit = rest < kUnits ? (double)rest / kUnits : (double)ceil_div(rest, kUnits);
+    t += per * step_us(c, unit, loader) + ends;
+  }
   return t;
 }
 
@@ -112,10 +118,16 @@ void set_plan(Plan& p, const Cost& c, int64_t splits, int64_t per, int bc, int64
   p.part_bytes = splits > 1 ? up((size_t)splits * I * J * 4) : 0;
 }
 
+// operands read and outputs written once
+double memory_us(double I, double J, double C, int type) {
+  return (C * (I + J) + I * J) * (type == kF32 ? 4 : 2) / 4.5e6;
+}
+
 // Tile and split of a product by their estimated time.
 Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
   const int bc = type == kF32 ? 32 : 64;
   const int64_t steps = ceil_div(C, bc);
+  const double memory = memory_us(I, J, C, type);
   Plan best;
   for (const Cost& c : type == kF32 ? kCosts32 : kCosts16) {
     if (c.tile == kLarge && loader != kDma) continue;
@@ -134,7 +146,7 @@ Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
         // split tiles' sums in fp32
         const double values = stream ? (double)rest * c.b * c.b : (double)I * J;
         if (s > 1 && values * s * 4 > 8e9) return;
-        const double t = before + groups_us(c, rest * s, per, loader) + join_us(values, s);
+        const double t = std::max(before + groups_us(c, rest * s, per, loader), kLaunch + 2.0 + memory) + join_us(values, s);
         if (best.c_per && t >= best.us) return;
         best.us = t;
         set_plan(best, c, s, per, bc, I, J);
@@ -155,6 +167,7 @@ double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, in
                  Plan& px, Plan& pk) {
   const int bc = type == kF32 ? 32 : 64;
   const int64_t sx = ceil_div(n, bc), sk = ceil_div(m, bc);
+  const double memory = (nx ? memory_us(m, k, n, type) : 0) + (nk ? memory_us(k, n, m, type) : 0);
   double best = kNever;
   for (const Cost& c : type == kF32 ? kCosts32 : kCosts16) {
     if (c.tile == kLarge || c.tile == kMid || (c.tile == kSlice64 && !slice64)) continue;
@@ -164,10 +177,11 @@ double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, in
     for_splits(nk ? sk : 1, most_splits(c, tk), [&](int64_t s, int64_t per) {
       const double wx = nx ? (double)ceil_div(sx, c.k) : 0, wk = nk ? (double)ceil_div(nk ? per : 0, c.k) : 0;
       const double groups = (double)(tx + tk * s);
-      const double share = ((double)tx * (wx * c.share[lx] + c.ends / c.slots) +
-                            (double)tk * s * (wk * c.share[lk] + c.ends / c.slots)) / kUnits;
-      const double longest = std::max(wx * c.wait[lx], wk * c.wait[lk]) + c.ends;
-      const double t = kLaunch + std::max(longest, share * (groups > kUnits * c.slots ? 1.1 : 1.0)) +
+      const double ex = ends_us(c, lx), ek = ends_us(c, lk);
+      const double share = ((double)tx * (wx * c.share[lx] + ex / c.slots) +
+                            (double)tk * s * (wk * c.share[lk] + ek / c.slots)) / kUnits;
+      const double longest = std::max(wx * c.wait[lx] + ex, wk * c.wait[lk] + ek);
+      const double t = kLaunch + std::max({longest, share * (groups > kUnits * c.slots ? 1.25 : 1.0), 2.0 + memory}) +
                        (s > 1 ? join_us((double)k * n, s) + kWorkspace : 0.0);
       if (t >= best) return;
       best = t;
@@ -177,6 +191,13 @@ double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, in
     });
   }
   return best;
+}
+
+// A whole product with a tile that is given.
+double unsplit_us(int tile, int64_t I, int64_t J, int64_t C, int type, int loader) {
+  const Cost& c = (type == kF32 ? kCosts32 : kCosts16)[tile];
+  return kLaunch + std::max(groups_us(c, ceil_div(I, c.b) * ceil_div(J, c.b), ceil_div(C, type == kF32 ? 32 : 64), loader),
+                            2.0 + memory_us(I, J, C, type));
 }
 
 bool dma_ok(const void* p, int64_t ld, int64_t contiguous, int size) {
@@ -340,6 +361,7 @@ struct BackwardPlan {
   Plan px, pk;
   int load_x, load_k;
   Copy dp, x, kernel;      // copies for DMA (dp: of dy or dresidual)
+  bool restore;            // 8-bit inputs: x is their restored copy
   int64_t ld_dp;           // make_dp without dresidual: row stride of dp
   size_t o_dp, o_sums, o_part, bytes;
   double us;
@@ -365,9 +387,27 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, BackwardPl
       b.pk = pk;
     }
   }
-  // 8-bit inputs come through registers.  Nothing but their product's own plan goes by them: the input's gradient is
-  // the same, bit by bit, with either.
-  if (q8 && !b.pair) b.pk = plan(a->k, a->n, a->m, a->dtype, kReg);
+  // 8-bit inputs come through registers, or are restored into the workspace once where that costs less.  Their product
+  // has a plan of its own; the input gradient keeps the tile and split that it has without them, and so its bits
+  // (the price that is returned is the one without them: what it decides stays the same too).
+  b.restore = false;
+  if (q8 && a->dkernel) {
+    const int sz = size_of(a->dtype);
+    const double once = kCopyLaunch + (double)a->m * a->k * (1 + sz) / 3.5e6;
+    const bool may = lk == kDma && copies_fit((double)a->m * a->k, sz);
+    const Plan apart = plan(a->k, a->n, a->m, a->dtype, kReg), restored = plan(a->k, a->n, a->m, a->dtype, kDma);
+    const bool cheaper = may && restored.us + once < apart.us;
+    const double own = cheaper ? restored.us + once : apart.us;
+    if (b.pair) {
+      // the pair with the steps of a register load for the kernel's gradient, against launches of their own
+      const double slower = us + 1.25 * (apart.us - restored.us);
+      const double alone = unsplit_us(b.px.tile, a->m, a->k, a->n, a->dtype, lx) + own + (b.sums ? kLaunch : 0.0);
+      if (slower < alone) return us;
+      b.pair = false;
+    }
+    b.pk = cheaper ? restored : apart;
+    b.restore = cheaper;
+  }
   return us;
 }
 
@@ -378,10 +418,10 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
   b.make_dp = a->activation != PETDENSE_NONE || a->dresidual;
   b.sums = a->dbias != nullptr;
   const bool own_dp = b.make_dp && !a->dresidual;
-  // row chunks of the activation's gradient: about 1024 workgroups, each of two rounds of its rows at least
+  // row chunks of the activation's gradient: about 1024 workgroups, each of one round of its rows at least
   const int lanes = act_grad_lanes((int)a->n);
   const int64_t most = std::max<int64_t>(1, 1024 / ceil_div(a->n, lanes * 8));
-  b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, ceil_div(a->m, 2 * 256 / lanes)));
+  b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, ceil_div(a->m, 256 / lanes)));
   const double act_us =
       b.make_dp || b.sums ? kLaunch + 2.0 + (double)a->m * a->n * sz * (b.make_dp ? 3 : 1) / 4e6 : 0.0;
 
@@ -403,7 +443,8 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
       b.x.on = !x_ok && !q8;
     }
   }
-  if ((a->dx || a->dkernel) && (b.make_dp || b.sums) && !a->dresidual) {
+  // (dP is formed again for every tile that reads it: for small ones)
+  if ((a->dx || a->dkernel) && (b.make_dp || b.sums) && !a->dresidual && a->m * a->n <= 1 << 18) {
     Plan px, pk;
     double t = plan_pair(a->dx, a->dkernel, a->m, a->k, a->n, a->dtype, kFormed, kFormed, false, px, pk);
     // a sum's workgroup walks all rows: 256 at a time, 4 of them in flight
@@ -429,7 +470,8 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
   }
   b.dp = copy_of(b.dp.on, a->m, a->n, sz, o);
   b.kernel = copy_of(b.kernel.on, a->k, a->n, sz, o);
-  b.x = copy_of(b.x.on, a->m, a->k, sz, o);
+  if (b.fused) b.restore = false;
+  b.x = copy_of(b.x.on || b.restore, a->m, a->k, sz, o);
   b.o_part = o;
   b.bytes = o + std::max(b.px.part_bytes, b.pk.part_bytes);
   return b;
@@ -506,9 +548,12 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     HIPC(act_grad(a->dy, a->lddy, a->activation == PETDENSE_NONE ? nullptr : a->saved, a->lds, made, lddp,
                   made && a->dresidual, sums, b.chunks, (int)a->m, (int)a->n, a->dtype, a->activation, s));
   }
-  if (b.dp.on || b.kernel.on || b.x.on)
+  if (b.restore)
+    HIPC(restore(static_cast<const uint8_t*>(a->x), a->ldx, a->x_exponents, a->lde, a->m, (int)a->k, a->dtype,
+                 w + b.x.at, b.x.ld, s));
+  if (b.dp.on || b.kernel.on || (b.x.on && !b.restore))
     HIPC(pad(PadJobs{{job_of(b.dp, dp, lddp, a->m, a->n, w), job_of(b.kernel, a->kernel, a->ldk, a->k, a->n, w),
-                      job_of(b.x, a->x, a->ldx, a->m, a->k, w)}},
+                      b.restore ? PadJob{} : job_of(b.x, a->x, a->ldx, a->m, a->k, w)}},
              a->dtype, s));
   if (b.dp.on) dp = w + b.dp.at, lddp = b.dp.ld;
   if (b.load_x == kDma) n_dp = padded(a->n, size_of(a->dtype));
@@ -528,7 +573,7 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
   if (a->dkernel) {
     k.A = b.x.on ? w + b.x.at : a->x;
     k.lda = b.x.on ? b.x.ld : a->ldx;
-    k.exps = a->x_exponents;
+    k.exps = b.restore ? nullptr : a->x_exponents;
     k.lde = a->lde;
     k.B = dp;
     k.ldb = lddp;
@@ -539,7 +584,7 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     k.e.ldo = a->lddk;
     k.e.out_f32 = a->grad_f32;
   }
-  const int q8 = a->x_exponents != nullptr;
+  const int q8 = a->x_exponents != nullptr && !b.restore;
   if (b.fused || b.pair)
     if ((a->dx && !planned(b.px, a->n)) || (a->dkernel && !planned(b.pk, a->m)))
       return fail(PETDIFF_ERR_HIP, "internal: a product without a plan");

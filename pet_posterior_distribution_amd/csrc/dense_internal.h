@@ -68,7 +68,7 @@ struct Pair {
   Product x, k;
   ColumnJoin cols;       // pair: the sums' parts are there (act_grad)
   ColumnSum sums;        // fused: they are made here
-  int nx, nk;            // workgroups of each (the launcher's)
+  int nx, nk, x0, k0;    // workgroups of each, and the first of them (the launcher's)
 };
 
 // One launch of the tiled product: `q8`: A is e4m3 codes with exponent bytes (kKernelGrad only).
@@ -98,11 +98,12 @@ __host__ __device__ inline void tile_at(int t, int ti, int tj, int& i, int& j) {
   j = r / h;
 }
 
-// Few rows: one pass over B ([C][J], j-contiguous), I <= kMaxRows.
-constexpr int kMaxRows = 8, kRowThreads = 1024, kRowCols = 32;
+// One or two rows: one pass over B ([C][J], j-contiguous), I <= kMaxRows.
+constexpr int kMaxRows = 2, kRowThreads = 1024, kRowCols = 32;
 hipError_t rows(const Product& p, int type, hipStream_t s);
 
-// lanes that share a row of N columns in act_grad: a power of two
+// rows of a lane in flight in act_grad, and the lanes that share a row of N columns: a power of two
+constexpr int kActGradAhead = 2;
 inline int act_grad_lanes(int N) {
   int l = 1;
   while (l < 64 && l * 8 < N) l *= 2;
@@ -122,7 +123,8 @@ struct PadJobs {
 };
 hipError_t pad(const PadJobs& p, int type, hipStream_t s);
 
-// dp = dy act'(saved) (dp may be null, its rows hold zeros up to a multiple of 8 columns, unless `bare`), part[chunk][n] = column sums of dp over the chunk's rows (may be null)
+// dp = dy act'(saved) (dp may be null, its rows hold zeros up to a multiple of 8 columns, unless `bare`),
+// part[chunk][n] = column sums of dp over the chunk's rows (may be null)
 hipError_t act_grad(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, int bare,
                     float* part, int chunks, int M, int N, int type, int act, hipStream_t s);
 hipError_t join_columns(const ColumnJoin& c, hipStream_t s);

@@ -3,6 +3,7 @@
 #include "dense_epilogue.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace petdense_k {
 
@@ -13,23 +14,45 @@ constexpr int64_t kSlab = (int64_t)1 << 29;     // threads of one launch (a grid
 inline unsigned blocks_for(int64_t n, int per) { return (unsigned)((n + per - 1) / per); }
 
 // ---------------------------------------------------------------------------------------------------------------
-// join: out = epilogue(sum over splits, in order).  Bound by reading the parts; a thread takes eight columns.
+// join: out = epilogue(sum over splits).  Bound by reading the parts.  A thread takes eight columns and every G-th
+// split; the G sums meet in LDS, in order.  G = 8 where outputs are few and splits many: one thread after another
+// would wait for memory split by split (63 x 31 outputs of 64 splits: 15.6 us with G = 1).
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T>
+template <typename T, int G>
 __global__ __launch_bounds__(256) void join_kernel(Product p, int64_t octets, int orow) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= octets) return;
-  const int64_t i = t / orow;
-  const int j = (int)(t - i * orow) * 8, n = p.J - j;
+  constexpr int PER = 256 / G;
+  __shared__ f32x4 red[G > 1 ? G : 1][PER][2];
+  const int q8 = threadIdx.x % PER, g = threadIdx.x / PER;
+  const int64_t t = (int64_t)blockIdx.x * PER + q8;
+  const bool live = t < octets;
+  const int64_t i = live ? t / orow : 0;
+  const int j = live ? (int)(t - i * orow) * 8 : 0, n = p.J - j;
   const float* src = p.part + i * p.J + j;
   const int64_t plane = (int64_t)p.I * p.J;
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    float w[8];
-    load_row<float, 8>(src + s * plane, n, w);
+  if (live) {
+#pragma unroll 8
+    for (int s = g; s < p.splits; s += G) {
+      float w[8];
+      load_row<float, 8>(src + s * plane, n, w);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] += w[q];
+      for (int q = 0; q < 8; ++q) v[q] += w[q];
+    }
+  }
+  if constexpr (G > 1) {
+    red[g][q8][0] = f32x4{v[0], v[1], v[2], v[3]};
+    red[g][q8][1] = f32x4{v[4], v[5], v[6], v[7]};
+    __syncthreads();
+    if (g != 0 || !live) return;
+    f32x4 lo = red[0][q8][0], hi = red[0][q8][1];
+#pragma unroll
+    for (int k = 1; k < G; ++k) {
+      lo += red[k][q8][0];
+      hi += red[k][q8][1];
+    }
+    for (int q = 0; q < 4; ++q) v[q] = lo[q], v[4 + q] = hi[q];
+  } else if (!live) {
+    return;
   }
   epilogue8<T>(p.e, i, j, n, v);
 }
@@ -56,15 +79,39 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(Product p, int b, int t
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Few rows (decoding, a single sample): every value of B is read once by one workgroup, which owns 32 columns and, where
-// those are enough workgroups, the whole contraction, so that one launch ends the call.  4 lanes share a row's 8-column pieces; the other lanes
-// and waves take other rows; their sums meet by shuffles and then in LDS, in a fixed order.
+// One or two rows (decoding, a single sample): every value of B is read once by one workgroup, which owns 32 columns
+// and, where those are enough workgroups, the whole contraction, so that one launch ends the call.  Bound by latency:
+// 4 lanes share a row's 8-column pieces, 256 rows of B are in flight four deep, and the sums meet by two rotations of
+// 16 lanes and once in LDS, in a fixed order.
 // ---------------------------------------------------------------------------------------------------------------
+// v summed over the four lanes l, l + 4, l + 8, l + 12 of a row of 16, in each of them (two rotations of the row: no
+// LDS, which ROWS x 8 shuffles of 16 waves would keep busy for microseconds)
+__device__ __forceinline__ float sum_row4(float v) {
+  const int a = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + 8, 0xf, 0xf, false);     // row_ror:8
+  v += __int_as_float(a);
+  const int b = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + 4, 0xf, 0xf, false);     // row_ror:4
+  return v + __int_as_float(b);
+}
+
+// W neighbouring values of a row, all there or 0 < n < W of them.  The cut piece reads its last value again rather than
+// branch, so that its loads go out together.
+template <typename T, int W, bool WHOLE>
+__device__ __forceinline__ void load_piece(const T* __restrict__ src, int n, T* w) {
+  if constexpr (WHOLE) {
+    __builtin_memcpy(w, src, W * sizeof(T));
+  } else {
+#pragma unroll
+    for (int q = 0; q < W; ++q) w[q] = src[q < n ? q : n - 1];
+  }
+}
+
 template <typename T, int ROWS>
 __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
   constexpr int W = 8, LANES = kRowCols / W, GROUPS = kRowThreads / LANES;   // 4 lanes a row, 256 rows at a time
-  constexpr int AHEAD = ROWS <= 4 ? 4 : 2;                                  // rows of a lane in flight
-  __shared__ float red[kRowThreads / 64][ROWS][kRowCols];
+  constexpr int AHEAD = 4;                                                  // rows of a lane in flight
+  constexpr int PARTS = kRowThreads / 16;                                   // sums of 16 lanes that meet in LDS
+  __shared__ float red[PARTS][ROWS][kRowCols];
+  __shared__ float sum[ROWS][kRowCols];
   const int tid = threadIdx.x, l = tid % LANES, grp = tid / LANES;
   const int j0 = blockIdx.x * kRowCols, j = j0 + l * W, n = p.J - j;
   const T* A = static_cast<const T*>(p.A);
@@ -74,63 +121,59 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int q = 0; q < W; ++q) acc[r][q] = 0.f;
-  auto add = [&](const T* w, const T* x) {
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-      for (int q = 0; q < W; ++q) acc[r][q] = fmaf((float)x[r], (float)w[q], acc[r][q]);
-  };
-  auto xs = [&](int c, T* x) {
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) x[r] = A[(r < p.I ? r : 0) * p.lda + c];      // rows past the last are not stored
-  };
   const int end = min(p.C, ((int)blockIdx.y + 1) * p.c_per);      // this part of the contraction
-  int c = blockIdx.y * p.c_per + grp;
-  if (n >= W) {
+  auto walk = [&](auto whole) {
+    auto add = [&](const T* w, const T* x) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int q = 0; q < W; ++q) acc[r][q] = fmaf((float)x[r], (float)w[q], acc[r][q]);
+    };
+    auto fetch = [&](int c, T* w, T* x) {
+      load_piece<T, W, decltype(whole)::value>(B + (int64_t)c * p.ldb, n, w);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) x[r] = A[r * p.lda + c];
+    };
+    int c = blockIdx.y * p.c_per + grp;
     for (; c + (AHEAD - 1) * GROUPS < end; c += AHEAD * GROUPS) {
       T w[AHEAD][W], x[AHEAD][ROWS];
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) __builtin_memcpy(w[u], B + (int64_t)(c + u * GROUPS) * p.ldb, sizeof(w[u]));
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) xs(c + u * GROUPS, x[u]);
+      for (int u = 0; u < AHEAD; ++u) fetch(c + u * GROUPS, w[u], x[u]);
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) add(w[u], x[u]);
     }
     for (; c < end; c += GROUPS) {
       T w[W], x[ROWS];
-      __builtin_memcpy(w, B + (int64_t)c * p.ldb, sizeof(w));
-      xs(c, x);
+      fetch(c, w, x);
       add(w, x);
     }
-  } else if (n > 0) {
-    for (; c < end; c += GROUPS) {
-      T w[W], x[ROWS];
-#pragma unroll
-      for (int q = 0; q < W; ++q) w[q] = q < n ? B[(int64_t)c * p.ldb + q] : (T)0.f;
-      xs(c, x);
-      add(w, x);
-    }
-  }
+  };
+  if (n >= W) walk(std::true_type{});
+  else if (n > 0) walk(std::false_type{});        // past n: sums that nothing stores
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int q = 0; q < W; ++q) {
-#pragma unroll
-      for (int o = LANES; o < 64; o *= 2) acc[r][q] += __shfl_xor(acc[r][q], o);
-      if ((tid & 63) < LANES) red[tid >> 6][r][l * W + q] = acc[r][q];
+      const float v = sum_row4(acc[r][q]);
+      if ((tid & 15) < LANES) red[tid >> 4][r][l * W + q] = v;
     }
   __syncthreads();
-  // thread t: row t / 4, columns 8 (t % 4) ..
-  if (tid < ROWS * LANES) {
-    const int r = tid / LANES, c = (tid % LANES) * W;
-    if (r < p.I && j0 + c < p.J) {
-      float v[W] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int w = 0; w < kRowThreads / 64; ++w)
+  if (tid < ROWS * kRowCols) {
+    const int r = tid / kRowCols, q = tid % kRowCols;
+    float v = 0.f;
 #pragma unroll
-        for (int q = 0; q < W; ++q) v[q] += red[w][r][c + q];
-      if (p.splits > 1) store_row<float, W>(p.part + ((int64_t)blockIdx.y * p.I + r) * p.J + j0 + c, p.J - j0 - c, v);
-      else epilogue8<T>(p.e, r, j0 + c, p.J - j0 - c, v);
-    }
+    for (int k = 0; k < PARTS; ++k) v += red[k][r][q];
+    sum[r][q] = v;
+  }
+  __syncthreads();
+  // thread t: row t / 4, columns 8 (t % 4) ..
+  if (tid < ROWS * LANES && j < p.J) {
+    const int r = tid / LANES;
+    float v[W];
+#pragma unroll
+    for (int q = 0; q < W; ++q) v[q] = sum[r][l * W + q];
+    if (p.splits > 1) store_row<float, W>(p.part + ((int64_t)blockIdx.y * p.I + r) * p.J + j, n, v);
+    else epilogue8<T>(p.e, r, j, n, v);
   }
 }
 
@@ -138,22 +181,20 @@ template <typename T>
 hipError_t rows_t(const Product& p, hipStream_t s) {
   const dim3 grid(blocks_for(p.J, kRowCols), p.splits), block(kRowThreads);
   if (p.I == 1) return launch_kernel(rows_kernel<T, 1>, grid, block, 0, s, p);
-  else if (p.I == 2) return launch_kernel(rows_kernel<T, 2>, grid, block, 0, s, p);
-  else if (p.I <= 4) return launch_kernel(rows_kernel<T, 4>, grid, block, 0, s, p);
-  else return launch_kernel(rows_kernel<T, 8>, grid, block, 0, s, p);
+  return launch_kernel(rows_kernel<T, 2>, grid, block, 0, s, p);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // dp = dy act'(saved), and column sums of the unrounded dp over a chunk of rows.  One pass, memory bound: a lane takes
-// 8 columns, LPR lanes a row (a power of two, so that narrow layers fill the wave with rows); the wave's rows meet by
-// shuffles, the block's waves in LDS, in a fixed order.
+// 8 columns, lpr lanes a row (a power of two, so that narrow layers fill the wave with rows) and four rows at a time,
+// whose loads go out together; the wave's rows meet by shuffles, the block's waves in LDS, in a fixed order.
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* dy, int64_t ldy, const T* saved, int64_t lds, T* dp,
                                                        int64_t ldd, int bare, float* part, int rows_per, int M, int N,
-                                                       int act, int lpr) {
+                                                       int lpr) {
   constexpr bool EXACT = sizeof(T) == 4;
-  constexpr int W = 8;
+  constexpr int W = 8, AHEAD = kActGradAhead;
   __shared__ float red[4][64 * W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane & (lpr - 1), rows = 256 / lpr;             // rows the block takes at a time
@@ -162,38 +203,36 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* dy, int64_t ldy,
   float sum[W];
 #pragma unroll
   for (int q = 0; q < W; ++q) sum[q] = 0.f;
-  auto row = [&](const float* g0, const float* v, int64_t m) {
-    float g[W];
+  auto walk = [&](auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    for (int64_t m = m0 + threadIdx.x / lpr; m < m1; m += AHEAD * rows) {
+      T dyv[AHEAD][W], sv[AHEAD][W];
 #pragma unroll
-    for (int q = 0; q < W; ++q) g[q] = g0[q];
-    activate_grads<EXACT, W>(g, v, act);
+      for (int u = 0; u < AHEAD; ++u) {
+        const int64_t r = min(m + u * rows, m1 - 1);            // past the chunk: its last row again, and not used
+        load_piece<T, W, WHOLE>(dy + r * ldy + j, n, dyv[u]);
+        if constexpr (ACT != kNone) load_piece<T, W, WHOLE>(saved + r * lds + j, n, sv[u]);
+      }
 #pragma unroll
-    for (int q = 0; q < W; ++q) sum[q] += g[q];
-    // (columns past the last are zero: the next product may read them)
-    if (dp) store_row<T, W>(dp + m * ldd + j, bare ? n : W, g);
-  };
-  if (n > 0) {
-    int64_t m = m0 + threadIdx.x / lpr;
-    if (n >= W) {
-      // two rows in flight
-      for (; m + rows < m1; m += 2 * rows) {
-        float g[2][W], v[2][W];
+      for (int u = 0; u < AHEAD; ++u) {
+        if (m + u * rows >= m1) break;
+        float g[W], v[W];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          load_row<T, W>(dy + (m + u * rows) * ldy + j, W, g[u]);
-          if (act != kNone) load_row<T, W>(saved + (m + u * rows) * lds + j, W, v[u]);
+        for (int q = 0; q < W; ++q) {
+          const bool there = WHOLE || q < n;
+          g[q] = there ? (float)dyv[u][q] : 0.f;
+          v[q] = there && ACT != kNone ? (float)sv[u][q] : 0.f;
         }
+        activate_grads<EXACT, W>(g, v, ACT);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) row(g[u], v[u], m + u * rows);
+        for (int q = 0; q < W; ++q) sum[q] += g[q];
+        // (columns past the last are zero: the next product may read them)
+        if (dp) store_row<T, W>(dp + (m + u * rows) * ldd + j, bare ? n : W, g);
       }
     }
-    for (; m < m1; m += rows) {
-      float g[W], v[W];
-      load_row<T, W>(dy + m * ldy + j, n, g);
-      if (act != kNone) load_row<T, W>(saved + m * lds + j, n, v);
-      row(g, v, m);
-    }
-  }
+  };
+  if (n >= W) walk(std::true_type{});
+  else if (n > 0) walk(std::false_type{});
   if (!part) return;
 #pragma unroll
   for (int q = 0; q < W; ++q)
@@ -209,13 +248,23 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* dy, int64_t ldy,
   }
 }
 
+template <typename T, int ACT>
+hipError_t act_grad_a(const T* dy, int64_t ldy, const T* saved, int64_t lds, T* dp, int64_t ldd, int bare, float* part,
+                      int chunks, int M, int N, hipStream_t s) {
+  const int rows_per = (M + chunks - 1) / chunks, lpr = act_grad_lanes(N);
+  return launch_kernel(act_grad_kernel<T, ACT>, dim3(blocks_for(N, lpr * 8), chunks), dim3(256), 0, s, dy, ldy, saved, lds,
+                       dp, ldd, bare, part, rows_per, M, N, lpr);
+}
+
 template <typename T>
 hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t lds, void* dp, int64_t ldd, int bare,
                       float* part, int chunks, int M, int N, int act, hipStream_t s) {
-  const int rows_per = (M + chunks - 1) / chunks, lpr = act_grad_lanes(N);
-  return launch_kernel(act_grad_kernel<T>, dim3(blocks_for(N, lpr * 8), chunks), dim3(256), 0, s,
-                     static_cast<const T*>(dy), ldy, static_cast<const T*>(saved), lds, static_cast<T*>(dp), ldd, bare, part,
-                     rows_per, M, N, act, lpr);
+  auto* f = act == kRelu   ? act_grad_a<T, kRelu>
+            : act == kGelu ? act_grad_a<T, kGelu>
+            : act == kSilu ? act_grad_a<T, kSilu>
+                           : act_grad_a<T, kNone>;
+  return f(static_cast<const T*>(dy), ldy, static_cast<const T*>(saved), lds, static_cast<T*>(dp), ldd, bare, part, chunks,
+           M, N, s);
 }
 
 __global__ __launch_bounds__(256) void join_columns_kernel(ColumnJoin p) {
@@ -344,7 +393,8 @@ hipError_t quantize_t(const void* x, int64_t ldx, int64_t M, int K, uint8_t* cod
   for (int64_t m = 0; m < M; m += slab) {
     const int64_t octets = std::min(slab, M - m) * orow;
     if (hipError_t e = launch_kernel(quantize_kernel<T>, dim3(blocks_for(octets, 256)), dim3(256), 0, s,
-                       static_cast<const T*>(x) + m * ldx, ldx, octets, orow, K, codes + m * ldc, ldc, exps + m * lde, lde))
+                                     static_cast<const T*>(x) + m * ldx, ldx, octets, orow, K, codes + m * ldc, ldc,
+                                     exps + m * lde, lde))
       return e;
   }
   return hipSuccess;
@@ -357,8 +407,9 @@ hipError_t restore_t(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int
   const int64_t slab = std::max<int64_t>(1, kSlab / orow);
   for (int64_t m = 0; m < M; m += slab) {
     const int64_t octets = std::min(slab, M - m) * orow;
-    if (hipError_t e = launch_kernel(restore_kernel<T>, dim3(blocks_for(octets, 256)), dim3(256), 0, s, codes + m * ldc, ldc,
-                       exps + m * lde, lde, octets, orow, K, static_cast<T*>(x) + m * ldx, ldx))
+    if (hipError_t e = launch_kernel(restore_kernel<T>, dim3(blocks_for(octets, 256)), dim3(256), 0, s,
+                                     codes + m * ldc, ldc, exps + m * lde, lde, octets, orow, K,
+                                     static_cast<T*>(x) + m * ldx, ldx))
       return e;
   }
   return hipSuccess;
@@ -376,14 +427,17 @@ hipError_t restore_t(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int
 hipError_t join(const Product& p, int type, hipStream_t s) {
   const int orow = (p.J + 7) / 8;
   const int64_t octets = (int64_t)p.I * orow;
-  PETDENSE_BY_TYPE(type, return launch_kernel(join_kernel<T>, dim3(blocks_for(octets, 256)), dim3(256), 0, s, p,
-                                            octets, orow);)
+  if (p.splits > 2 && octets < 65536)
+    PETDENSE_BY_TYPE(type, return launch_kernel(join_kernel<T, 8>, dim3(blocks_for(octets, 32)), dim3(256), 0, s, p,
+                                                octets, orow))
+  PETDENSE_BY_TYPE(type, return launch_kernel(join_kernel<T, 1>, dim3(blocks_for(octets, 256)), dim3(256), 0, s, p,
+                                              octets, orow))
 }
 
 hipError_t join_tiles(const Product& p, int type, int b, hipStream_t s) {
   const int ti = (p.I + b - 1) / b, tj = (p.J + b - 1) / b;
-  PETDENSE_BY_TYPE(type, return launch_kernel(join_tiles_kernel<T>, dim3(blocks_for(b * (b / 8), 256), ti * tj - p.whole),
-                                            dim3(256), 0, s, p, b, ti, tj);)
+  const dim3 grid(blocks_for(b * (b / 8), 256), ti * tj - p.whole);
+  PETDENSE_BY_TYPE(type, return launch_kernel(join_tiles_kernel<T>, grid, dim3(256), 0, s, p, b, ti, tj))
 }
 
 hipError_t rows(const Product& p, int type, hipStream_t s) { PETDENSE_BY_TYPE(type, return rows_t<T>(p, s)) }
@@ -419,7 +473,7 @@ __global__ __launch_bounds__(256) void fill_zero_kernel(char* p, int64_t total, 
 hipError_t fill_zero(void* p, int64_t rows, int n, int64_t ld, int size, hipStream_t s) {
   const int64_t total = rows * n;
   return launch_kernel(fill_zero_kernel, dim3((unsigned)std::min<int64_t>(4096, (total + 255) / 256)), dim3(256), 0, s,
-                     static_cast<char*>(p), total, n, ld, size);
+                       static_cast<char*>(p), total, n, ld, size);
 }
 
 hipError_t quantize(const void* x, int64_t ldx, int64_t M, int K, int type, uint8_t* codes, int64_t ldc, uint8_t* exps,

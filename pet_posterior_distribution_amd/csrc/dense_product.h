@@ -785,16 +785,16 @@ __global__ __launch_bounds__(K::THREADS) void product_kernel(Product p) {
   else product_body<T, K, FA, FB, LA, LB, Q8>(p, blockIdx.x, lds);
 }
 
-// The backward pass's two products and the join of its column sums as one launch: workgroups [0, nx) multiply the
-// input gradient, the next nk the kernel gradient, the others join 16 columns each.
+// The backward pass's two products and the join of its column sums as one launch: the product whose workgroups take
+// longer starts first (what starts last should end soon), the last workgroups join 16 columns each.
 template <typename T, typename K, int LX, int LK, bool Q8>
 __global__ __launch_bounds__(K::THREADS) void pair_kernel(Pair p) {
   extern __shared__ char lds[];
-  const int b = blockIdx.x;
-  if (b < p.nx) {
-    product_body<T, K, false, false, LX, LX, false>(p.x, b, lds);
-  } else if (b < p.nx + p.nk) {
-    product_body<T, K, true, true, Q8 ? kReg : LK, LK, Q8>(p.k, b - p.nx, lds);
+  const int b = blockIdx.x, bx = b - p.x0, bk = b - p.k0;
+  if (bk >= 0 && bk < p.nk) {
+    product_body<T, K, true, true, Q8 ? kReg : LK, LK, Q8>(p.k, bk, lds);
+  } else if (bx >= 0 && bx < p.nx) {
+    product_body<T, K, false, false, LX, LX, false>(p.x, bx, lds);
   } else {
     join_columns16(p.cols, b - p.nx - p.nk, threadIdx.x, reinterpret_cast<float*>(lds));
   }
@@ -804,9 +804,9 @@ __global__ __launch_bounds__(K::THREADS) void pair_kernel(Pair p) {
 template <typename T, typename K, bool Q8>
 __global__ __launch_bounds__(K::THREADS) void fused_kernel(Pair p) {
   extern __shared__ char lds[];
-  const int b = blockIdx.x;
-  if (b < p.nx) product_body<T, K, false, false, kReg, kReg, false, true, false>(p.x, b, lds);
-  else if (b < p.nx + p.nk) product_body<T, K, true, true, kReg, kReg, Q8, false, true>(p.k, b - p.nx, lds);
+  const int b = blockIdx.x, bx = b - p.x0, bk = b - p.k0;
+  if (bk >= 0 && bk < p.nk) product_body<T, K, true, true, kReg, kReg, Q8, false, true>(p.k, bk, lds);
+  else if (bx >= 0 && bx < p.nx) product_body<T, K, false, false, kReg, kReg, false, true, false>(p.x, bx, lds);
   else sum_columns8<T, K::THREADS>(p.sums, b - p.nx - p.nk, threadIdx.x, reinterpret_cast<float*>(lds));
 }
 
@@ -838,13 +838,21 @@ hipError_t launch(const Product& p, hipStream_t s) {
   return launch_kernel(k, dim3((unsigned)groups), dim3(K::THREADS), LDS, s, p);
 }
 
+// (a pair's kernel may have one product only: the other's workgroups are none)
+inline void place_pair(Pair& p, int64_t nx, int64_t nk) {
+  const bool x_first = p.x.c_per > p.k.c_per;
+  p.nx = (int)nx;
+  p.nk = (int)nk;
+  p.x0 = x_first ? 0 : p.nk;
+  p.k0 = x_first ? p.nx : 0;
+}
+
 template <typename T, typename K, int LX, int LK, bool Q8>
 hipError_t launch_pair(Pair p, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   auto k = pair_kernel<T, K, LX, LK, Q8>;
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
-  p.nx = (int)(tiles_of(p.x, K::BI, K::BJ) * p.x.splits);
-  p.nk = (int)(tiles_of(p.k, K::BI, K::BJ) * p.k.splits);
+  place_pair(p, tiles_of(p.x, K::BI, K::BJ) * p.x.splits, tiles_of(p.k, K::BI, K::BJ) * p.k.splits);
   return launch_kernel(k, dim3((unsigned)(p.nx + p.nk + (p.cols.N + 15) / 16)), dim3(K::THREADS), K::LDS, s, p);
 }
 
@@ -853,8 +861,8 @@ hipError_t launch_fused(Pair p, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   auto k = fused_kernel<T, K, Q8>;
   if (hipError_t e = allow_lds(reinterpret_cast<const void*>(k), K::LDS, done)) return e;
-  p.nx = p.x.e.out ? (int)(tiles_of(p.x, K::BI, K::BJ) * p.x.splits) : 0;
-  p.nk = p.k.e.out ? (int)(tiles_of(p.k, K::BI, K::BJ) * p.k.splits) : 0;
+  place_pair(p, p.x.e.out ? tiles_of(p.x, K::BI, K::BJ) * p.x.splits : 0,
+             p.k.e.out ? tiles_of(p.k, K::BI, K::BJ) * p.k.splits : 0);
   return launch_kernel(k, dim3((unsigned)(p.nx + p.nk + (p.sums.N + 7) / 8)), dim3(K::THREADS), K::LDS, s, p);
 }
 

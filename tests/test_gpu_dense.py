@@ -425,7 +425,8 @@ def test_checkpoint_views():
 
 
 @pytest.mark.parametrize('t', TYPES, ids=str)
-@pytest.mark.parametrize('m,k,n', SHAPES + [(2048, 2048, 256)])
+# (the last: large enough for its inputs to be restored once)
+@pytest.mark.parametrize('m,k,n', SHAPES + [(2048, 2048, 256), (8200, 2056, 2048)])
 def test_backward_from_checkpoint(m, k, n, t):
     """dX and db are those of the layer; dW is the product with the restored activations, which it reads as they lie
     (fp16 restores values below 2^-14 to a multiple of 2^-24: half of it times |dP|)."""
@@ -439,6 +440,32 @@ def test_backward_from_checkpoint(m, k, n, t):
                            grad_dtype=F32 if act == 'relu' else None)
         whole = dense_backward(dy, x, w, activation=act, saved=saved, grad_dtype=F32 if act == 'relu' else None)
         assert torch.equal(g.x, whole.x) and torch.equal(g.bias, whole.bias)
+
+
+def test_offsets_past_32_bits():
+    """2.8e9 activations: row offsets pass 2^32 bytes in every operand that has m rows.  Rows and columns are checked
+    against 64 bits at both ends and past the border."""
+    from pet_posterior_distribution_amd import checkpoint_activations, dense, dense_backward
+    m, k, n, t = 70000, 40000, 8, BF16
+    x = torch.empty(m, k, dtype=t, device='cuda').normal_(generator=torch.Generator(device='cuda').manual_seed(3))
+    w, dy = rand((k, n), t, 1, k ** -0.5), rand((m, n), t, 2)
+    rows = torch.tensor([0, 1, 26843, 26844, 53688, 53690, m - 2, m - 1], device='cuda')
+    cols = torch.tensor([0, 7, 31, 20000, k - 1], device='cuda')
+    x6, w6, d6 = x[rows].double(), w.double(), dy.double()
+    y = dense(x, w)
+    close(y[rows], x6 @ w6, (k + 4) * E23 * (x6.abs() @ w6.abs()), 'output')
+    g = dense_backward(dy, x, w, need_bias=False)
+    close(g.x[rows], d6[rows] @ w6.T, (n + 4) * E23 * (d6[rows].abs() @ w6.abs().T), 'dx')
+    xc = x[:, cols].double()
+    close(g.kernel[cols], xc.T @ d6, (m + 4) * E23 * (xc.abs().T @ d6.abs()), 'dkernel')
+    del g, y
+    c = checkpoint_activations(x)
+    back = c.restore()
+    ref, e = quantize64(x[rows])
+    assert torch.equal(c.exponents[rows], e) and torch.equal(back[rows].double(), ref)
+    g = dense_backward(dy, c, w, need_x=False, need_bias=False)
+    xc = back[:, cols].double()
+    close(g.kernel[cols], xc.T @ d6, (m + 4) * E23 * (xc.abs().T @ d6.abs()), 'dkernel from 8 bits')
 
 
 # ------------------------------------------------------------------------------------------- streams and graphs
