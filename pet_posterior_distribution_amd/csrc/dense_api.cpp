@@ -48,22 +48,23 @@ struct Plan {
 
 // What a kind of tile costs, in microseconds, as measured on products of 64 .. 12288 rows.  A step (128 bytes of
 // contraction) takes `wait` when its workgroup has a compute unit to itself, and `share` per workgroup when several
-// fill it; `ends` is a workgroup's first load and its epilogue.  [operands by DMA, through registers, dP formed there]
+// fill it; `ends` is a workgroup's first load and its epilogue.  [operands by DMA, through registers, dP formed there,
+// one operand restored there from 8 bits]
 struct Cost {
   int tile, b, slots, k;   // b: rows and columns of the tile; slots: workgroups of a compute unit; k: steps at a time
-  double wait[3], share[3], ends;
+  double wait[4], share[4], ends;
 };
-constexpr int kFormed = 2;
-constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.47, 0, 0}, {1.47, 0, 0}, 7.5},
-                             {kMid, 128, 2, 1, {0.65, 1.25, 0}, {0.46, 1.25, 0}, 3.5},
-                             {kSmall, 64, 4, 1, {0.28, 0.55, 2.0}, {0.19, 0.34, 1.5}, 2.0},
-                             {kSlice, 32, 1, 8, {0.5, 1.0, 3.4}, {1.2, 1.5, 3.4}, 2.0},
-                             {kSlice64, 64, 1, 4, {0.7, 2.4, 0}, {0.75, 2.4, 0}, 3.5}};
-constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 0, 0}, {6.9, 0, 0}, 8.0},
-                             {kMid, 128, 2, 1, {2.3, 2.7, 0}, {2.1, 2.5, 0}, 4.0},
-                             {kSmall, 64, 4, 1, {0.75, 0.95, 2.4}, {0.53, 0.65, 2.0}, 2.0},
-                             {kSlice, 32, 1, 8, {1.1, 1.3, 3.5}, {1.3, 1.5, 3.5}, 2.0},
-                             {kSlice64, 64, 1, 4, {2.6, 4.5, 0}, {2.75, 4.5, 0}, 3.5}};
+constexpr int kFormed = 2, kCodes = 3;
+constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.47, 0, 0, 0}, {1.47, 0, 0, 0}, 7.5},
+                             {kMid, 128, 2, 1, {0.65, 1.25, 0, 0.95}, {0.46, 1.25, 0, 0.62}, 3.5},
+                             {kSmall, 64, 4, 1, {0.28, 0.55, 2.0, 0.65}, {0.19, 0.34, 1.5, 0.3}, 2.0},
+                             {kSlice, 32, 1, 8, {0.5, 1.0, 3.4, 0.65}, {1.2, 1.5, 3.4, 1.4}, 2.0},
+                             {kSlice64, 64, 1, 4, {0.78, 2.4, 0, 1.15}, {0.8, 2.4, 0, 1.15}, 3.5}};
+constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 0, 0, 0}, {6.9, 0, 0, 0}, 8.0},
+                             {kMid, 128, 2, 1, {2.3, 2.7, 0, 2.5}, {2.1, 2.5, 0, 2.3}, 4.0},
+                             {kSmall, 64, 4, 1, {0.75, 0.95, 2.4, 0.87}, {0.53, 0.65, 2.0, 0.6}, 2.0},
+                             {kSlice, 32, 1, 8, {1.1, 1.3, 3.5, 1.3}, {1.3, 1.5, 3.5, 1.5}, 2.0},
+                             {kSlice64, 64, 1, 4, {2.6, 4.5, 0, 3.0}, {2.75, 4.5, 0, 3.1}, 3.5}};
 constexpr double kNever = 1e30;      // no plan
 constexpr double kLaunch = 3.5;      // a launch behind another, here and on the host
 constexpr double kWorkspace = 2.0;   // a small call that needs a workspace: the host's time for it
@@ -146,7 +147,8 @@ Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
         // split tiles' sums in fp32
         const double values = stream ? (double)rest * c.b * c.b : (double)I * J;
         if (s > 1 && values * s * 4 > 8e9) return;
-        const double t = std::max(before + groups_us(c, rest * s, per, loader), kLaunch + 2.0 + memory) + join_us(values, s);
+        const double t =
+            std::max(before + groups_us(c, rest * s, per, loader), kLaunch + 2.0 + memory) + join_us(values, s);
         if (best.c_per && t >= best.us) return;
         best.us = t;
         set_plan(best, c, s, per, bc, I, J);
@@ -161,8 +163,9 @@ Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
   return best;
 }
 
-// The backward pass as one launch, or kNever where it has too many tiles for that (x: I = m, J = k, C = n; k: I = k, J = n, C = m), both products with the same kind of
-// tile; only the kernel gradient's contraction is split.  nx, nk: which products are wanted.
+// The backward pass as one launch, or kNever where it has too many tiles for that: x (I = m, J = k, C = n) and k
+// (I = k, J = n, C = m) with the same kind of tile; only the kernel gradient's contraction is split.  nx, nk: which
+// products are wanted.
 double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, int lx, int lk, bool slice64,
                  Plan& px, Plan& pk) {
   const int bc = type == kF32 ? 32 : 64;
@@ -196,8 +199,8 @@ double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, in
 // A whole product with a tile that is given.
 double unsplit_us(int tile, int64_t I, int64_t J, int64_t C, int type, int loader) {
   const Cost& c = (type == kF32 ? kCosts32 : kCosts16)[tile];
-  return kLaunch + std::max(groups_us(c, ceil_div(I, c.b) * ceil_div(J, c.b), ceil_div(C, type == kF32 ? 32 : 64), loader),
-                            2.0 + memory_us(I, J, C, type));
+  const int64_t tiles = ceil_div(I, c.b) * ceil_div(J, c.b), steps = ceil_div(C, type == kF32 ? 32 : 64);
+  return kLaunch + std::max(groups_us(c, tiles, steps, loader), 2.0 + memory_us(I, J, C, type));
 }
 
 bool dma_ok(const void* p, int64_t ld, int64_t contiguous, int size) {
@@ -217,14 +220,15 @@ Product placed(Product p, const Plan& pl, void* part) {
   return p;
 }
 
+// `cols`: column sums that its join may carry (it has one where the plan splits)
 int run_product(const Product& of, int layout, int loader, int type, int q8, const Plan& pl, void* part,
-                hipStream_t s) {
+                const ColumnJoin& cols, hipStream_t s) {
   if (!planned(pl, of.C)) return fail(PETDIFF_ERR_HIP, "internal: a product without a plan");
   const Product p = placed(of, pl, part);
   HIPC(type == kF32    ? product_f32(p, layout, loader, pl.tile, q8, s)
        : type == kBF16 ? product_bf16(p, layout, loader, pl.tile, q8, s)
                        : product_f16(p, layout, loader, pl.tile, q8, s));
-  if (pl.splits > 1) HIPC(pl.stream ? join_tiles(p, type, pl.b, s) : join(p, type, s));
+  if (pl.splits > 1) HIPC(pl.stream ? join_tiles(p, cols, type, pl.b, s) : join(p, cols, type, s));
   return PETDIFF_OK;
 }
 
@@ -337,7 +341,8 @@ int check_backward(const petdense_backward_args* a) {
     NEED(a->dy && a->lddy >= a->n, "dy must be given, with a row stride of at least n");
     NEED(a->activation == PETDENSE_NONE || (a->saved && a->lds >= a->n),
          "an activation's backward pass needs what the forward pass saved, with a row stride of at least n");
-    NEED(!a->dx || (a->kernel && a->ldk >= a->n && a->lddx >= a->k), "dx needs the kernel, and row strides of the rows");
+    NEED(!a->dx || (a->kernel && a->ldk >= a->n && a->lddx >= a->k),
+         "dx needs the kernel, and row strides of the rows");
     NEED(!a->dkernel || (a->x && a->ldx >= a->k), "dkernel needs x, with a row stride of at least k");
     NEED(!a->dkernel || !a->x_exponents || a->lde >= ceil_div(a->k, PETDENSE_BLOCK),
          "the exponents' row stride is shorter than a row's blocks");
@@ -376,7 +381,8 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, BackwardPl
   b.pair = false;
   if (a->dx) b.px = plan(a->m, a->k, a->n, a->dtype, lx);
   if (a->dkernel) b.pk = plan(a->k, a->n, a->m, a->dtype, lk);
-  double us = b.px.us + b.pk.us + (b.sums ? kLaunch : 0.0);
+  const bool joins = b.sums && !(a->dkernel && b.pk.splits > 1);      // a launch for the column sums
+  double us = b.px.us + b.pk.us + (joins ? kLaunch : 0.0);
   if (a->dx && a->dkernel) {
     Plan px, pk;
     const double t = plan_pair(true, true, a->m, a->k, a->n, a->dtype, lx, lk, true, px, pk);
@@ -395,13 +401,14 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, BackwardPl
     const int sz = size_of(a->dtype);
     const double once = kCopyLaunch + (double)a->m * a->k * (1 + sz) / 3.5e6;
     const bool may = lk == kDma && copies_fit((double)a->m * a->k, sz);
-    const Plan apart = plan(a->k, a->n, a->m, a->dtype, kReg), restored = plan(a->k, a->n, a->m, a->dtype, kDma);
+    const Plan apart = plan(a->k, a->n, a->m, a->dtype, lk == kDma ? kCodes : kReg);
+    const Plan restored = plan(a->k, a->n, a->m, a->dtype, kDma);
     const bool cheaper = may && restored.us + once < apart.us;
     const double own = cheaper ? restored.us + once : apart.us;
     if (b.pair) {
       // the pair with the steps of a register load for the kernel's gradient, against launches of their own
-      const double slower = us + 1.25 * (apart.us - restored.us);
-      const double alone = unsplit_us(b.px.tile, a->m, a->k, a->n, a->dtype, lx) + own + (b.sums ? kLaunch : 0.0);
+      const double slower = us + (lk == kDma ? 1.25 * (apart.us - restored.us) : 0.0);
+      const double alone = unsplit_us(b.px.tile, a->m, a->k, a->n, a->dtype, lx) + own + (joins ? kLaunch : 0.0);
       if (slower < alone) return us;
       b.pair = false;
     }
@@ -426,7 +433,8 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
       b.make_dp || b.sums ? kLaunch + 2.0 + (double)a->m * a->n * sz * (b.make_dp ? 3 : 1) / 4e6 : 0.0;
 
   // dp in the workspace has rows of whole pieces, with zeros: DMA takes it as it is
-  const bool dp_ok = own_dp || (a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz) : dma_ok(a->dy, a->lddy, a->n, sz));
+  const bool dp_ok =
+      own_dp || (a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz) : dma_ok(a->dy, a->lddy, a->n, sz));
   const bool w_ok = !a->dx || dma_ok(a->kernel, a->ldk, a->n, sz);
   const bool x_ok = !a->dkernel || (q8 ? a->k * sz % 16 == 0 : dma_ok(a->x, a->ldx, a->k, sz));
   // (8-bit inputs go through registers whatever their alignment: their loader is dp's)
@@ -505,17 +513,18 @@ int petdense_forward(const petdense_forward_args* a, void* work, size_t work_byt
   if (f.rows) {
     p = placed(p, f.p, work);
     HIPC(rows(p, a->dtype, (hipStream_t)stream));
-    if (p.splits > 1) HIPC(join(p, a->dtype, (hipStream_t)stream));
+    if (p.splits > 1) HIPC(join(p, ColumnJoin{}, a->dtype, (hipStream_t)stream));
     return PETDIFF_OK;
   }
   char* w = static_cast<char*>(work);
   if (f.x.on || f.kernel.on) {
-    HIPC(pad(PadJobs{{job_of(f.x, a->x, a->ldx, a->m, a->k, w), job_of(f.kernel, a->kernel, a->ldk, a->k, a->n, w), {}}},
+    HIPC(pad(PadJobs{{job_of(f.x, a->x, a->ldx, a->m, a->k, w),
+                      job_of(f.kernel, a->kernel, a->ldk, a->k, a->n, w), {}}},
              a->dtype, (hipStream_t)stream));
     if (f.x.on) p.A = w + f.x.at, p.lda = f.x.ld;
     if (f.kernel.on) p.B = w + f.kernel.at, p.ldb = f.kernel.ld;
   }
-  return run_product(p, kForward, f.loader, a->dtype, 0, f.p, w + f.o_part, (hipStream_t)stream);
+  return run_product(p, kForward, f.loader, a->dtype, 0, f.p, w + f.o_part, ColumnJoin{}, (hipStream_t)stream);
 }
 
 size_t petdense_backward_workspace(const petdense_backward_args* a) {
@@ -604,7 +613,7 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     HIPC(a->dtype == kF32    ? fused_f32(p, b.px.tile, q8, s)
          : a->dtype == kBF16 ? fused_bf16(p, b.px.tile, q8, s)
                              : fused_f16(p, b.px.tile, q8, s));
-    if (a->dkernel && b.pk.splits > 1) HIPC(join(p.k, a->dtype, s));
+    if (a->dkernel && b.pk.splits > 1) HIPC(join(p.k, ColumnJoin{}, a->dtype, s));
     return PETDIFF_OK;
   }
   if (b.pair) {
@@ -615,14 +624,15 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     HIPC(a->dtype == kF32    ? pair_f32(p, b.load_x, b.load_k, b.px.tile, q8, s)
          : a->dtype == kBF16 ? pair_bf16(p, b.load_x, b.load_k, b.px.tile, q8, s)
                              : pair_f16(p, b.load_x, b.load_k, b.px.tile, q8, s));
-    if (b.pk.splits > 1) HIPC(join(p.k, a->dtype, s));
+    if (b.pk.splits > 1) HIPC(join(p.k, ColumnJoin{}, a->dtype, s));
     return PETDIFF_OK;
   }
-  if (b.sums) HIPC(join_columns(cols, s));
+  const bool carried = a->dkernel && b.pk.splits > 1;
+  if (b.sums && !carried) HIPC(join_columns(cols, s));
   if (a->dx)
-    if (int r = run_product(x, kInputGrad, b.load_x, a->dtype, 0, b.px, w + b.o_part, s)) return r;
+    if (int r = run_product(x, kInputGrad, b.load_x, a->dtype, 0, b.px, w + b.o_part, ColumnJoin{}, s)) return r;
   if (a->dkernel)
-    if (int r = run_product(k, kKernelGrad, b.load_k, a->dtype, q8, b.pk, w + b.o_part, s)) return r;
+    if (int r = run_product(k, kKernelGrad, b.load_k, a->dtype, q8, b.pk, w + b.o_part, cols, s)) return r;
   return PETDIFF_OK;
 }
 

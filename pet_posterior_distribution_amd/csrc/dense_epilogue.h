@@ -19,22 +19,23 @@ inline hipError_t launch_kernel(void (*k)(A...), dim3 grid, dim3 block, size_t l
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Phi(x) = (1 + erf(x / sqrt 2)) / 2.
-// 16-bit outputs: Abramowitz & Stegun 7.1.26, |error of erf| <= 1.5e-7, i.e. 2^-22.7 beside the 2^-9 and 2^-12
-// of a rounded output; about a third of erff's instructions, and the epilogue pays them once per output.
+// 16-bit outputs: 1 / (1 + 2^(-x P(x^2))), P of degree 6: the least largest error of x Phi(x) over |x| <= 6 (a linear
+// program over log2(Phi / (1 - Phi)) / x), 7e-8 there and less beyond, 1.1e-7 of Phi; beside the 2^-9 and 2^-12 of a
+// rounded output.  A third of erff's instructions, and the epilogue pays them once per output.  P >= 2.3 everywhere, so
+// that both tails end in 0 and 1.
 template <bool EXACT>
 __device__ __forceinline__ float normal_cdf(float x) {
-  const float z = x * 0.70710678118654752f;
   if constexpr (EXACT) {
-    return 0.5f * (1.0f + erff(z));
+    return 0.5f * (1.0f + erff(x * 0.70710678118654752f));
   } else {
-    const float a = fabsf(z);
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.0f));
-    float p = fmaf(1.061405429f, t, -1.453152027f);
-    p = fmaf(p, t, 1.421413741f);
-    p = fmaf(p, t, -0.284496736f);
-    p = fmaf(p, t, 0.254829592f);
-    const float q = 0.5f * p * t * __expf(-a * a);          // 1 - Phi(|x|)
-    return x < 0.f ? q : 1.0f - q;
+    const float u = x * x;
+    float p = fmaf(5.20990380e-09f, u, -3.85044763e-07f);
+    p = fmaf(p, u, 1.14524259e-05f);
+    p = fmaf(p, u, -1.59389380e-04f);
+    p = fmaf(p, u, -9.55930483e-05f);
+    p = fmaf(p, u, 1.04838581e-01f);
+    p = fmaf(p, u, 2.30220720f);
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * p));
   }
 }
 
@@ -95,16 +96,23 @@ __device__ __forceinline__ void store_row(T* dst, int n, const float* v) {
   }
 }
 
-// Eight outputs (i, j .. j + 7) of which `n` exist.
+// The bias of columns j .. j + 7, of which `n` exist.
 template <typename T>
-__device__ __forceinline__ void epilogue8(const Epilogue& e, int64_t i, int64_t j, int n, float* v) {
+__device__ __forceinline__ void bias8(const Epilogue& e, int64_t j, int n, float* w) {
+  if (e.bias_f32) load_row<float, 8>(static_cast<const float*>(e.bias) + j, n, w);
+  else load_row<T, 8>(static_cast<const T*>(e.bias) + j, n, w);
+}
+
+// Eight outputs (i, j .. j + 7) of which `n` exist; `bias`: theirs, read already, or null.
+template <typename T>
+__device__ __forceinline__ void epilogue8(const Epilogue& e, int64_t i, int64_t j, int n, float* v,
+                                          const float* bias = nullptr) {
   constexpr bool EXACT = sizeof(T) == 4;
   float w[8];
   if (e.bias) {
-    if (e.bias_f32) load_row<float, 8>(static_cast<const float*>(e.bias) + j, n, w);
-    else load_row<T, 8>(static_cast<const T*>(e.bias) + j, n, w);
+    if (!bias) bias8<T>(e, j, n, w);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] += w[q];
+    for (int q = 0; q < 8; ++q) v[q] += bias ? bias[q] : w[q];
   }
   if (e.res) {
     load_row<T, 8>(static_cast<const T*>(e.res) + i * e.ldr + j, n, w);
@@ -197,14 +205,21 @@ __device__ __forceinline__ void sum_columns8(const ColumnSum& p, int block, int 
   }
 }
 
-// Sums 16 columns of a column join: thread t < 256 takes column t % 16 of the chunks t / 16, t / 16 + 16, ..; the 16
-// groups meet in LDS, in order.  Every thread of the workgroup comes here.
+// Sums 16 columns of a column join: thread t < 256 takes column t % 16 of the chunks t / 16, t / 16 + 16, .., sixteen
+// loads at a time (past the last: its value again, not added); the 16 groups meet in LDS, in order.  Every thread of
+// the workgroup comes here.
 __device__ __forceinline__ void join_columns16(const ColumnJoin& p, int block, int t, float* red) {
+  constexpr int AHEAD = 16;
   const int c = t & 15, g = t >> 4, j = block * 16 + c;
   float v = 0.f;
   if (t < 256 && j < p.N) {
-#pragma unroll 8
-    for (int k = g; k < p.chunks; k += 16) v += p.part[(int64_t)k * p.N + j];
+    for (int k = g; k < p.chunks; k += 16 * AHEAD) {
+      float w[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) w[u] = p.part[(int64_t)min(k + 16 * u, p.chunks - 1) * p.N + j];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) v += k + 16 * u < p.chunks ? w[u] : 0.f;
+    }
   }
   if (t < 256) red[t] = v;
   __syncthreads();

@@ -35,7 +35,7 @@ struct Product {
   int saved_act;
   int I, J, C;
   int splits, c_per;     // contraction split into `splits` parts of c_per (a multiple of the k-step)
-  float* part;           // their sums in fp32 when splits > 1 (the epilogue is then the joining kernel's): [splits][I][J],
+  float* part;           // their sums in fp32 when splits > 1 (the join has the epilogue then): [splits][I][J],
                          // or of a streamed product [tile - whole][splits][tile rows][tile columns]
   int whole;             // streamed products: the first tiles of the walk, a whole contraction each
   Epilogue e;
@@ -84,10 +84,10 @@ hipError_t fused_f32(const Pair& p, int tile, int q8, hipStream_t s);
 hipError_t fused_bf16(const Pair& p, int tile, int q8, hipStream_t s);
 hipError_t fused_f16(const Pair& p, int tile, int q8, hipStream_t s);
 
-// Joins split products: the sum of p.part over the splits, in order, through the epilogue.
-hipError_t join(const Product& p, int type, hipStream_t s);
+// Joins split products: the sum of p.part over the splits, in order, through the epilogue; and column sums (N > 0).
+hipError_t join(const Product& p, const ColumnJoin& cols, int type, hipStream_t s);
 // The same for the split tiles of a streamed product with b x b tiles.
-hipError_t join_tiles(const Product& p, int type, int b, hipStream_t s);
+hipError_t join_tiles(const Product& p, const ColumnJoin& cols, int type, int b, hipStream_t s);
 
 // Tile number t of the walk over ti x tj tiles: bands of 4 tile rows, column by column, so that workgroups that run
 // together share rows of A and columns of B.

@@ -16,14 +16,16 @@ inline unsigned blocks_for(int64_t n, int per) { return (unsigned)((n + per - 1)
 // ---------------------------------------------------------------------------------------------------------------
 // join: out = epilogue(sum over splits).  Bound by reading the parts.  A thread takes eight columns and every G-th
 // split; the G sums meet in LDS, in order.  G = 8 where outputs are few and splits many: one thread after another
-// would wait for memory split by split (63 x 31 outputs of 64 splits: 15.6 us with G = 1).
+// would wait for memory split by split (63 x 31 outputs of 64 splits: 15.6 us with G = 1).  The first workgroups
+// join a bias gradient's column sums, which saves it a launch (they take longest: last, they would end last).
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int G>
-__global__ __launch_bounds__(256) void join_kernel(Product p, int64_t octets, int orow) {
+__global__ __launch_bounds__(256) void join_kernel(Product p, ColumnJoin cols, int64_t octets, int orow, int first) {
   constexpr int PER = 256 / G;
   __shared__ f32x4 red[G > 1 ? G : 1][PER][2];
+  if ((int)blockIdx.x < first) return join_columns16(cols, blockIdx.x, threadIdx.x, reinterpret_cast<float*>(red));
   const int q8 = threadIdx.x % PER, g = threadIdx.x / PER;
-  const int64_t t = (int64_t)blockIdx.x * PER + q8;
+  const int64_t t = (int64_t)(blockIdx.x - first) * PER + q8;
   const bool live = t < octets;
   const int64_t i = live ? t / orow : 0;
   const int j = live ? (int)(t - i * orow) * 8 : 0, n = p.J - j;
@@ -58,15 +60,21 @@ __global__ __launch_bounds__(256) void join_kernel(Product p, int64_t octets, in
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void join_tiles_kernel(Product p, int b, int ti, int tj) {
-  // blockIdx.y: the split tile; a thread takes eight columns of one of its rows
-  const int per = b / 8, t = blockIdx.x * 256 + threadIdx.x, r = t / per, c = (t % per) * 8;
+__global__ __launch_bounds__(256) void join_tiles_kernel(Product p, ColumnJoin cols, int b, int ti, int tj, int first) {
+  __shared__ float red[256];
+  if ((int)blockIdx.y < first) {
+    const int k = blockIdx.y * gridDim.x + blockIdx.x;
+    if (k * 16 < cols.N) join_columns16(cols, k, threadIdx.x, red);
+    return;
+  }
+  // split tile y; a thread takes eight columns of one of its rows
+  const int per = b / 8, t = blockIdx.x * 256 + threadIdx.x, r = t / per, c = (t % per) * 8, y = blockIdx.y - first;
   int a, d;
-  tile_at(p.whole + blockIdx.y, ti, tj, a, d);
+  tile_at(p.whole + y, ti, tj, a, d);
   const int64_t i = (int64_t)a * b + r;
   const int j = d * b + c, n = p.J - j;
   if (r >= b || i >= p.I || n <= 0) return;
-  const float* src = p.part + (int64_t)blockIdx.y * p.splits * b * b + r * b + c;
+  const float* src = p.part + (int64_t)y * p.splits * b * b + r * b + c;
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
@@ -252,8 +260,8 @@ template <typename T, int ACT>
 hipError_t act_grad_a(const T* dy, int64_t ldy, const T* saved, int64_t lds, T* dp, int64_t ldd, int bare, float* part,
                       int chunks, int M, int N, hipStream_t s) {
   const int rows_per = (M + chunks - 1) / chunks, lpr = act_grad_lanes(N);
-  return launch_kernel(act_grad_kernel<T, ACT>, dim3(blocks_for(N, lpr * 8), chunks), dim3(256), 0, s, dy, ldy, saved, lds,
-                       dp, ldd, bare, part, rows_per, M, N, lpr);
+  return launch_kernel(act_grad_kernel<T, ACT>, dim3(blocks_for(N, lpr * 8), chunks), dim3(256), 0, s, dy, ldy, saved,
+                       lds, dp, ldd, bare, part, rows_per, M, N, lpr);
 }
 
 template <typename T>
@@ -263,8 +271,8 @@ hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t ld
             : act == kGelu ? act_grad_a<T, kGelu>
             : act == kSilu ? act_grad_a<T, kSilu>
                            : act_grad_a<T, kNone>;
-  return f(static_cast<const T*>(dy), ldy, static_cast<const T*>(saved), lds, static_cast<T*>(dp), ldd, bare, part, chunks,
-           M, N, s);
+  return f(static_cast<const T*>(dy), ldy, static_cast<const T*>(saved), lds, static_cast<T*>(dp), ldd, bare, part,
+           chunks, M, N, s);
 }
 
 __global__ __launch_bounds__(256) void join_columns_kernel(ColumnJoin p) {
@@ -386,8 +394,8 @@ __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* codes, int6
 }
 
 template <typename T>
-hipError_t quantize_t(const void* x, int64_t ldx, int64_t M, int K, uint8_t* codes, int64_t ldc, uint8_t* exps, int64_t lde,
-                      hipStream_t s) {
+hipError_t quantize_t(const void* x, int64_t ldx, int64_t M, int K, uint8_t* codes, int64_t ldc, uint8_t* exps,
+                      int64_t lde, hipStream_t s) {
   const int orow = (K + 31) / 32 * 4;
   const int64_t slab = std::max<int64_t>(1, kSlab / orow);
   for (int64_t m = 0; m < M; m += slab) {
@@ -424,20 +432,26 @@ hipError_t restore_t(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int
     default: { using T = _Float16; call; }   \
   }
 
-hipError_t join(const Product& p, int type, hipStream_t s) {
+template <typename T, int G>
+hipError_t join_t(const Product& p, const ColumnJoin& cols, hipStream_t s) {
   const int orow = (p.J + 7) / 8;
   const int64_t octets = (int64_t)p.I * orow;
-  if (p.splits > 2 && octets < 65536)
-    PETDENSE_BY_TYPE(type, return launch_kernel(join_kernel<T, 8>, dim3(blocks_for(octets, 32)), dim3(256), 0, s, p,
-                                                octets, orow))
-  PETDENSE_BY_TYPE(type, return launch_kernel(join_kernel<T, 1>, dim3(blocks_for(octets, 256)), dim3(256), 0, s, p,
-                                              octets, orow))
+  const unsigned first = blocks_for(cols.N, 16);
+  return launch_kernel(join_kernel<T, G>, dim3(first + blocks_for(octets, 256 / G)), dim3(256), 0, s, p, cols, octets,
+                       orow, (int)first);
 }
 
-hipError_t join_tiles(const Product& p, int type, int b, hipStream_t s) {
-  const int ti = (p.I + b - 1) / b, tj = (p.J + b - 1) / b;
-  const dim3 grid(blocks_for(b * (b / 8), 256), ti * tj - p.whole);
-  PETDENSE_BY_TYPE(type, return launch_kernel(join_tiles_kernel<T>, grid, dim3(256), 0, s, p, b, ti, tj))
+hipError_t join(const Product& p, const ColumnJoin& cols, int type, hipStream_t s) {
+  if (p.splits > 2 && (int64_t)p.I * ((p.J + 7) / 8) < 65536)
+    PETDENSE_BY_TYPE(type, return (join_t<T, 8>(p, cols, s)))
+  PETDENSE_BY_TYPE(type, return (join_t<T, 1>(p, cols, s)))
+}
+
+hipError_t join_tiles(const Product& p, const ColumnJoin& cols, int type, int b, hipStream_t s) {
+  const int ti = (p.I + b - 1) / b, tj = (p.J + b - 1) / b, tiles = ti * tj - p.whole;
+  const unsigned row = blocks_for(b * (b / 8), 256), first = blocks_for(cols.N, 16 * row);
+  PETDENSE_BY_TYPE(type, return launch_kernel(join_tiles_kernel<T>, dim3(row, first + tiles), dim3(256), 0, s, p, cols,
+                                              b, ti, tj, (int)first))
 }
 
 hipError_t rows(const Product& p, int type, hipStream_t s) { PETDENSE_BY_TYPE(type, return rows_t<T>(p, s)) }
@@ -481,8 +495,8 @@ hipError_t quantize(const void* x, int64_t ldx, int64_t M, int K, int type, uint
   PETDENSE_BY_TYPE(type, return quantize_t<T>(x, ldx, M, K, codes, ldc, exps, lde, s))
 }
 
-hipError_t restore(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int64_t lde, int64_t M, int K, int type, void* x,
-                   int64_t ldx, hipStream_t s) {
+hipError_t restore(const uint8_t* codes, int64_t ldc, const uint8_t* exps, int64_t lde, int64_t M, int K, int type,
+                   void* x, int64_t ldx, hipStream_t s) {
   PETDENSE_BY_TYPE(type, return restore_t<T>(codes, ldc, exps, lde, M, K, x, ldx, s))
 }
 

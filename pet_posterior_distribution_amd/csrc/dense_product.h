@@ -386,10 +386,10 @@ struct Kind {
   static constexpr int BI = BI_, BJ = BJ_, WI = WI_, WJ = WJ_, KW = KW_;
   static constexpr int THREADS = WI * WJ * KW * 64;
   static constexpr int LDS = 2 * KW * (BI + BJ) * 128;
-  static constexpr int TURN = 16 * (BJ / WJ) * 4;                        // a wave's 16 rows of outputs in fp32
   // the largest tile's workgroups stay and walk (its first loads and its stores are a large part of a tile's time;
   // smaller tiles run several workgroups on a compute unit, which hide them from each other)
   static constexpr bool STREAM = BI == 256;
+  static constexpr int TURN = 16 * (BJ / WJ) * 4;                         // a wave's 16 rows of outputs in fp32
   static constexpr int LAUNCH_LDS = LDS + (STREAM ? WI * WJ * TURN : 0);
   static_assert(KW == 1 || WI * WJ == 1, "");
 };
@@ -415,6 +415,44 @@ __device__ __forceinline__ void place_of(int b, int ti, int tj, int splits, int&
   const int u = first + b / 8;
   split = u / tiles;
   tile_at(u - split * tiles, ti, tj, i, j);
+}
+
+// A wave's outputs, from row i and column j on.  Its accumulators hold four neighbouring columns of a row in a lane;
+// 16 rows at a time turn through LDS of the wave's own (16-byte piece c of row r at place c ^ r), so that a lane gets
+// eight neighbouring outputs of a row and neighbouring lanes fill whole cache lines.  (Two swaps between rows of 16
+// lanes give a lane its eight outputs without LDS, but neighbouring lanes then belong to different rows: 50176 x 256 x
+// 128 took 21.5 us, not 13.2.)  A lane keeps its columns, so the bias is read once: 8192 x 4096 x 8192 with GELU and
+// the pre-activation 465 us, 479 with a read for every 8 rows.
+template <typename T, int FI, int FJ>
+__device__ __forceinline__ void store_tile(const Epilogue& e, const f32x4 (&acc)[FI][FJ], int i, int j, int rows,
+                                           int cols, int lane, char* own) {
+  constexpr int PIECES = FJ * 4, MASK = PIECES < 16 ? PIECES - 1 : 15, OCTETS = FJ * 2, AT = 64 / OCTETS;
+  static_assert(FJ == 2 || FJ == 4, "");
+  constexpr int PASSES = AT < 16 ? 16 / AT : 1;                          // of AT rows
+  const int g = lane >> 4, il = lane & 15, r = lane / OCTETS, c = lane % OCTETS * 2;
+  const int n = cols - j - c * 4;
+  float bias[8];
+  if (e.bias && n > 0) bias8<T>(e, j + c * 4, n, bias);
+#pragma unroll 1
+  for (int x = 0; x < FI; ++x) {
+#pragma unroll
+    for (int u = 0; u < FI; ++u)
+      if (u == x) {
+#pragma unroll
+        for (int y = 0; y < FJ; ++y)
+          *reinterpret_cast<f32x4*>(own + (il * PIECES + ((y * 4 + g) ^ (il & MASK))) * 16) = acc[u][y];
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // other lanes of the wave read what this one wrote
+#pragma unroll
+    for (int h = 0; h < PASSES; ++h) {
+      const int lr = r + h * AT, row = i + x * 16 + lr;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(own + (lr * PIECES + (c ^ (lr & MASK))) * 16);
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(own + (lr * PIECES + ((c + 1) ^ (lr & MASK))) * 16);
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if (row < rows && n > 0) epilogue8<T>(e, row, j + c * 4, n, v, bias);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
 }
 
 // ACT_A, ACT_B: that operand is dP, made from dy and p.saved
@@ -526,10 +564,7 @@ __device__ __forceinline__ void product_body(const Product& p, int block, char* 
   // loads into LDS past the last step (of zeros) end before the workgroup's LDS is given away
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-  // Epilogue.  A wave turns its accumulators, ROWS_AT x 16 rows at a time, through its own part of LDS (16-byte piece
-  // c of row r at place c ^ r), so that a lane gets eight neighbouring outputs of a row and a row's lanes touch whole
-  // cache lines.
-  __syncthreads();
+  // Epilogue
   Epilogue e = p.e;
   if (p.splits > 1) {
     e = Epilogue{};
@@ -537,8 +572,9 @@ __device__ __forceinline__ void product_body(const Product& p, int block, char* 
     e.ldo = p.J;
     e.out_f32 = 1;
   }
-  const int g = lane >> 4, il = lane & 15;
   if constexpr (!SHARED) {
+    __syncthreads();
+    const int g = lane >> 4, il = lane & 15;
     // every wave's sums of the whole tile, then one octet of outputs a thread: the waves' parts added in order
     constexpr int PIECES = BJ / 4, MASK = PIECES < 16 ? PIECES - 1 : 15, PLANE = BI * BJ * 4;
 #pragma unroll
@@ -561,34 +597,9 @@ __device__ __forceinline__ void product_body(const Product& p, int block, char* 
         epilogue8<T>(e, i, j, p.J - j, v);
       }
     }
-    return;
   } else {
-  constexpr int TJ = BJ / WJ, PIECES = TJ / 4, MASK = PIECES < 16 ? PIECES - 1 : 15;
-  constexpr int ROWS_FIT = STAGE * 2 / (WI * WJ) / (16 * TJ * 4);
-  constexpr int ROWS_AT = ROWS_FIT < FI ? ROWS_FIT : FI;
-  static_assert(ROWS_FIT >= 1 && FI % ROWS_AT == 0, "the tile's rows pass through LDS in equal parts");
-  char* own = lds + wave * (ROWS_AT * 16 * TJ * 4);
-#pragma unroll
-  for (int x0 = 0; x0 < FI; x0 += ROWS_AT) {
-#pragma unroll
-    for (int x = 0; x < ROWS_AT; ++x)
-#pragma unroll
-      for (int y = 0; y < FJ; ++y)
-        *reinterpret_cast<f32x4*>(own + ((x * 16 + il) * PIECES + ((y * 4 + g) ^ (il & MASK))) * 16) = acc[x0 + x][y];
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // other lanes of the wave read what this one wrote
-#pragma unroll 1
-    for (int k = lane; k < ROWS_AT * 16 * (TJ / 8); k += 64) {
-      const int r = k / (TJ / 8), c = (k % (TJ / 8)) * 2, key = r & MASK;
-      const int i = i0 + ra + x0 * 16 + r, j = j0 + rb + c * 4;
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(own + (r * PIECES + (c ^ key)) * 16);
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(own + (r * PIECES + ((c + 1) ^ key)) * 16);
-      if (i < p.I && j < p.J) {
-        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        epilogue8<T>(e, i, j, p.J - j, v);
-      }
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  }
+    __syncthreads();                                      // the stages are free for the outputs
+    store_tile<T>(e, acc, i0 + ra, j0 + rb, p.I, p.J, lane, lds + wave * K::TURN);
   }
 }
 
@@ -709,6 +720,7 @@ __device__ __forceinline__ void stream_body(const Product& p, char* lds) {
   for (int f = 0; f < READS; ++f) read(lds, 0, f);
   char* cur = lds;
   char* nxt = lds + STAGE;
+  bool inside = false;                       // the last tile's outputs of this wave all exist
   for (int n = 0; n < count; ++n) {
     const Item m = item(n);
 #pragma unroll
@@ -721,8 +733,9 @@ __device__ __forceinline__ void stream_body(const Product& p, char* lds) {
       group(0, 1, cur, no, nullptr, ua, ub);
       fa.end(nxt, tid);
       fb.end(nxt + SA::BYTES, tid);
-      // a tile's first step: the loads landed before the last tile's stores began, and those need not be waited for
-      if (t == 0 && n > 0) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      // a tile's first step: the loads it waits for are older than the last tile's stores, of which there were FI FJ/2
+      // at least where the wave's outputs all exist: as many newer accesses may still be on their way
+      if (t == 0 && inside) step_barrier<FI * FJ / 2, true>();
       else step_barrier<0, true>();
       group(1, 0, nxt, yes, cur, ua, ub);
       ahead();
@@ -731,14 +744,9 @@ __device__ __forceinline__ void stream_body(const Product& p, char* lds) {
       nxt = s;
     }
 
-    // Epilogue.  A wave turns its accumulators, 16 rows at a time, through LDS of its own (16-byte piece c of row r at
-    // place c ^ r), so that a lane gets eight neighbouring outputs of a row and a row's lanes touch whole cache lines.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    constexpr int TJ = BJ / WJ, PIECES = TJ / 4, MASK = PIECES < 16 ? PIECES - 1 : 15;
-    const bool part = m.slot >= 0;
     Epilogue e = p.e;
     int rows = p.I, cols = p.J, i1 = m.i0 + ra, j1 = m.j0 + rb;
-    if (part) {
+    if (m.slot >= 0) {
       e = Epilogue{};
       e.out = p.part + (int64_t)m.slot * (BI * BJ);
       e.ldo = BJ;
@@ -748,31 +756,8 @@ __device__ __forceinline__ void stream_body(const Product& p, char* lds) {
       i1 = ra;
       j1 = rb;
     }
-    char* own = lds + K::LDS + wave * K::TURN;
-    const int g = lane >> 4, il = lane & 15;
-#pragma unroll 1
-    for (int x = 0; x < FI; ++x) {
-#pragma unroll
-      for (int u = 0; u < FI; ++u)
-        if (u == x) {
-#pragma unroll
-          for (int y = 0; y < FJ; ++y)
-            *reinterpret_cast<f32x4*>(own + (il * PIECES + ((y * 4 + g) ^ (il & MASK))) * 16) = acc[u][y];
-        }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // other lanes of the wave read what this one wrote
-#pragma unroll 1
-      for (int k = lane; k < 16 * (TJ / 8); k += 64) {
-        const int r = k / (TJ / 8), c = (k % (TJ / 8)) * 2, key = r & MASK;
-        const int i = i1 + x * 16 + r, j = j1 + c * 4;
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(own + (r * PIECES + (c ^ key)) * 16);
-        const f32x4 hi = *reinterpret_cast<const f32x4*>(own + (r * PIECES + ((c + 1) ^ key)) * 16);
-        if (i < rows && j < cols) {
-          float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          epilogue8<T>(e, i, j, cols - j, v);
-        }
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+    store_tile<T>(e, acc, i1, j1, rows, cols, lane, lds + K::LDS + wave * K::TURN);
+    inside = i1 + FI * 16 <= rows && j1 + FJ * 16 <= cols;
   }
   // the loads of nothing behind the last step end before the workgroup's LDS is given away
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
