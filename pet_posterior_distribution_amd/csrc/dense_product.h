@@ -431,8 +431,11 @@ __device__ __forceinline__ void store_tile(const Epilogue& e, const f32x4 (&acc)
   constexpr int PASSES = AT < 16 ? 16 / AT : 1;                          // of AT rows
   const int g = lane >> 4, il = lane & 15, r = lane / OCTETS, c = lane % OCTETS * 2;
   const int n = cols - j - c * 4;
+  // (fp32: erff and expf twice over and a bias in registers would spill the accumulators of the largest tile)
+  constexpr bool LEAN = sizeof(T) == 4;
+  constexpr int AT_ONCE = LEAN ? 1 : PASSES;
   float bias[8];
-  if (e.bias && n > 0) bias8<T>(e, j + c * 4, n, bias);
+  if (!LEAN && e.bias && n > 0) bias8<T>(e, j + c * 4, n, bias);
 #pragma unroll 1
   for (int x = 0; x < FI; ++x) {
 #pragma unroll
@@ -443,13 +446,13 @@ __device__ __forceinline__ void store_tile(const Epilogue& e, const f32x4 (&acc)
           *reinterpret_cast<f32x4*>(own + (il * PIECES + ((y * 4 + g) ^ (il & MASK))) * 16) = acc[u][y];
       }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // other lanes of the wave read what this one wrote
-#pragma unroll
+#pragma unroll AT_ONCE
     for (int h = 0; h < PASSES; ++h) {
       const int lr = r + h * AT, row = i + x * 16 + lr;
       const f32x4 lo = *reinterpret_cast<const f32x4*>(own + (lr * PIECES + (c ^ (lr & MASK))) * 16);
       const f32x4 hi = *reinterpret_cast<const f32x4*>(own + (lr * PIECES + ((c + 1) ^ (lr & MASK))) * 16);
       float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      if (row < rows && n > 0) epilogue8<T>(e, row, j + c * 4, n, v, bias);
+      if (row < rows && n > 0) epilogue8<T>(e, row, j + c * 4, n, v, LEAN ? nullptr : bias);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
