@@ -19,7 +19,8 @@
  * All pointers are device memory of the current device and belong to the caller; work runs on `stream`, in order,
  * with no synchronisation and no allocation, so every call can be captured into a graph.  Workspaces: at least
  * petdense_*_workspace bytes, 256-byte aligned, not shared by calls that may run at once (two streams, two captured
- * graphs that may replay together).  Row strides (ld*) are in values, at least the row's length; rows do not overlap.
+ * graphs that may replay together).  Their sizes go by every argument, which outputs are asked for and the pointers'
+ * alignment included: ask with the arguments of the call.  Row strides (ld*) are in values, at least the row's length; rows do not overlap.
  * Outputs do not alias inputs, with one exception: y may be the residual itself.  Sums are in a fixed order: results
  * are the same from run to run.
  *
@@ -56,7 +57,7 @@ typedef struct petdense_forward_args {
   void* y;                 /* [m][n] */
   void* pre;               /* [m][n] or NULL: P, in y's type (what GELU and SiLU need saved for the backward pass) */
   int64_t ldx, ldk, ldr, ldy, ldp;
-  int64_t m, k, n;         /* m >= 0; k, n >= 1; all < 2^31 - 256 */
+  int64_t m, k, n;         /* m >= 0; k, n >= 1; all < 2^31 - 65536 */
   int dtype, activation;
   int bias_f32;            /* bias is fp32 */
   int out_f32;             /* y and pre are fp32 */

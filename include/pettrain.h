@@ -76,8 +76,8 @@ void pettrain_destroy(pettrain_handle h);
  *   PETTRAIN_BF16  the dense layer's operators (petdense.h): bf16 operands, fp32 sums, bias and ReLU in the epilogue;
  *                  activations between layers, weights, gradients and Adam stay fp32.
  * keep: what a bf16 step holds of every product's input between its forward and backward passes: PETTRAIN_KEEP the
- * bf16 values, PETTRAIN_KEEP_E4M3 8-bit checkpoints (8.25 bits a value; the convolutions' kernel gradients are those
- * of the restored inputs, everything else is unchanged).  Frees the step's buffers when it changes anything; the
+ * bf16 values, PETTRAIN_KEEP_E4M3 8-bit checkpoints (8.25 bits a value; the products' kernel gradients are those of
+ * the restored inputs, everything else is unchanged).  Frees the step's buffers when it changes anything; the
  * caller's stream must be idle then.  PETDIFF_ERR_INVALID: unknown values, or e4m3 without bf16. */
 int pettrain_set_precision(pettrain_handle h, int precision, int keep);
 /* Device bytes the step holds for a batch of B samples at most so far: activations, gradients, workspaces. */

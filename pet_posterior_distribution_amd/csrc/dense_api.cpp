@@ -31,7 +31,7 @@ int fail(int code, const char* what) noexcept {
     if (!(cond)) return fail(PETDIFF_ERR_INVALID, what); \
   } while (0)
 
-constexpr int64_t kMaxDim = 0x7fffffff - 256;
+constexpr int64_t kMaxDim = 0x7fffffff - 0xffff;      // offsets a few steps and chunks past an end fit 31 bits
 constexpr size_t kAlign = 256;
 
 size_t up(size_t b) { return (b + kAlign - 1) / kAlign * kAlign; }
@@ -296,7 +296,7 @@ struct ForwardPlan {
 
 ForwardPlan plan_forward(const petdense_forward_args* a) {
   ForwardPlan f{};
-  f.rows = a->m <= kMaxRows;
+  f.rows = a->m <= kMaxRows && a->n <= 1 << 26;          // (a grid has fewer than 2^32 threads)
   if (a->m == 0) return f;
   if (f.rows) {
     // narrow layers leave compute units without columns: the contraction is split, where that is worth the join

@@ -20,9 +20,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Phi(x) = (1 + erf(x / sqrt 2)) / 2.
 // 16-bit outputs: 1 / (1 + 2^(-x P(x^2))), P of degree 6: the least largest error of x Phi(x) over |x| <= 6 (a linear
-// program over log2(Phi / (1 - Phi)) / x), 7e-8 there and less beyond, 1.1e-7 of Phi; beside the 2^-9 and 2^-12 of a
-// rounded output.  A third of erff's instructions, and the epilogue pays them once per output.  P >= 2.3 everywhere, so
-// that both tails end in 0 and 1.
+// program over log2(Phi / (1 - Phi)) / x), 7e-8 there and less beyond, 1.8e-7 of Phi with its fp32 steps; beside the
+// 2^-9 and 2^-12 of a rounded output.  A third of erff's instructions, and the epilogue pays them once per output.
+// P >= 2.3 everywhere, so that both tails end in 0 and 1.
 template <bool EXACT>
 __device__ __forceinline__ float normal_cdf(float x) {
   if constexpr (EXACT) {

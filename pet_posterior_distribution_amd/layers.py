@@ -9,7 +9,8 @@ once.  In a 16-bit layer's backward pass the pre-activation's gradient is rounde
 products (exact for ReLU and linear layers); the bias gradient sums it unrounded.
 
 Tensors may have any leading dimensions and row stride; a tensor whose rows are not contiguous is copied first.
-No call synchronises, so each can be captured into a graph.
+No call synchronises, so each can be captured into a graph.  Autograd does not record them: the gradients are
+``dense_backward``'s.
 
 ================================================  =============================================
 reference (file:line)                             here

@@ -9,6 +9,9 @@ terms of an output (from the 64-bit reference):
 * a 16-bit layer's dP is rounded once more before the products: u |dP| through |W| and |X|.
 """
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -144,6 +147,29 @@ def test_forward(m, k, n, t):
     for j, act in enumerate(ACTS):
         # every activation meets every mix of bias and residual over the shapes
         check_forward(x, w, b if (i + j) % 3 else None, act, r if (i + j) % 2 else None, pre=(i + j) % 4 < 2)
+
+
+@pytest.mark.parametrize('t', TYPES, ids=str)
+@pytest.mark.parametrize('m,k,n', [(1, 8000, 16), (2, 5000, 100), (2, 4100, 64), (1, 1024, 4096), (1, 2819, 10),
+                                   (2, 1023, 31)])
+def test_one_and_two_rows(m, k, n, t):
+    """One workgroup's whole contraction, and contractions that several share."""
+    x, w, b, r, dy = inputs(m, k, n, t)
+    for j, act in enumerate(ACTS):
+        check_forward(x, w, b if j % 2 else None, act, r if j < 2 else None, pre=j in (1, 2))
+        check_backward(dy, x, w, act, None if act is None else r)
+
+
+@pytest.mark.parametrize('t', TYPES, ids=str)
+def test_tiles_that_one_workgroup_walks(t):
+    """297 tiles of 256 x 256, of which the last row and column are cut, on 256 compute units."""
+    x, w, b, r, _ = inputs(8200, 2048, 2056, t)
+    check_forward(x, w, b, 'gelu', r, pre=True)
+    check_forward(x, w, None, 'relu', None, pre=False)
+    y = check_forward(x, w, b, None, None, pre=False)
+    from pet_posterior_distribution_amd import dense
+    for rep in range(3):
+        assert torch.equal(dense(x, w, b), y)
 
 
 @pytest.mark.parametrize('t', [BF16, F16], ids=str)
@@ -468,6 +494,21 @@ def test_offsets_past_32_bits():
     close(g.kernel[cols], xc.T @ d6, (m + 4) * E23 * (xc.abs().T @ d6.abs()), 'dkernel from 8 bits')
 
 
+def test_one_row_of_more_columns_than_a_launch_has_threads():
+    """2^27 columns: more than one launch of a kernel of 1024 threads for 32 columns could take.  Signs and whole
+    numbers, so that every sum is exact in fp32 whatever its order."""
+    from pet_posterior_distribution_amd import dense, dense_backward
+    n = (1 << 27) + 8
+    gen = torch.Generator(device='cuda').manual_seed(5)
+    w = torch.randint(0, 2, (1, n), device='cuda', generator=gen, dtype=torch.int8).mul_(2).sub_(1).to(BF16)
+    dy = torch.randint(-1, 2, (1, n), device='cuda', generator=gen, dtype=torch.int8).to(BF16)
+    x = torch.full((1, 1), 3.0, dtype=BF16, device='cuda')
+    assert torch.equal(dense(x, w), 3 * w)
+    g = dense_backward(dy, x, w)
+    assert torch.equal(g.kernel, 3 * dy) and torch.equal(g.bias, dy[0])
+    assert torch.equal(g.x, (dy * w).sum(dtype=torch.float64).to(BF16).reshape(1, 1))
+
+
 # ------------------------------------------------------------------------------------------- streams and graphs
 def chain(x, ws, bs, dy):
     """Two layers forward, the first one's input kept in 8 bits, and their backward passes."""
@@ -549,3 +590,37 @@ def test_two_captured_graphs_replay_like_eager_runs():
     torch.cuda.synchronize()
     for a, b in zip(outs[0], chain(*fresh)):
         assert torch.equal(a, b)
+
+
+FIRST_CALLS = """
+import sys
+import torch
+from pet_posterior_distribution_amd import checkpoint_activations, dense, dense_backward
+t = torch.bfloat16
+x, w = torch.randn(300, 256, device='cuda').to(t), (torch.randn(256, 512, device='cuda') / 16).to(t)
+big, wide = torch.randn(2048, 512, device='cuda').to(t), (torch.randn(512, 4096, device='cuda') / 16).to(t)
+dy, dz = torch.randn(300, 512, device='cuda').to(t), torch.randn(2048, 4096, device='cuda').to(t)
+torch.cuda.synchronize()
+def run():
+    c = checkpoint_activations(x)
+    y, p = dense(x, w, activation='gelu', return_preactivation=True)
+    return [y, *dense_backward(dy, c, w, activation='gelu', saved=p)[:3], dense(big, wide),
+            *dense_backward(dz, big, wide)[:3], dense(x[:1], w), c.restore()]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = run()
+for rep in range(3):
+    for v in out:
+        v.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, run())), rep
+print('same')
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    """Loading the code and allowing the larger tiles their LDS happen inside the capture."""
+    r = subprocess.run([sys.executable, '-c', FIRST_CALLS], capture_output=True, text=True, timeout=100,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and 'same' in r.stdout, r.stderr[-2000:]
