@@ -101,12 +101,21 @@ __device__ __forceinline__ float sum_row4(float v) {
   return v + __int_as_float(b);
 }
 
+// W neighbouring values as one access of any alignment
+template <typename T, int W>
+struct Octet {
+  typedef T type __attribute__((ext_vector_type(W)));
+  typedef type any __attribute__((aligned(sizeof(T)), may_alias));
+};
+
 // W neighbouring values of a row, all there or 0 < n < W of them.  The cut piece reads its last value again rather than
 // branch, so that its loads go out together.
 template <typename T, int W, bool WHOLE>
 __device__ __forceinline__ void load_piece(const T* __restrict__ src, int n, T* w) {
   if constexpr (WHOLE) {
-    __builtin_memcpy(w, src, W * sizeof(T));
+    const typename Octet<T, W>::type v = *reinterpret_cast<const typename Octet<T, W>::any*>(src);
+#pragma unroll
+    for (int q = 0; q < W; ++q) w[q] = v[q];
   } else {
 #pragma unroll
     for (int q = 0; q < W; ++q) w[q] = src[q < n ? q : n - 1];
