@@ -20,9 +20,9 @@
  * with no synchronisation and no allocation, so every call can be captured into a graph.  Workspaces: at least
  * petdense_*_workspace bytes, 256-byte aligned, not shared by calls that may run at once (two streams, two captured
  * graphs that may replay together).  Their sizes go by every argument, which outputs are asked for and the pointers'
- * alignment included: ask with the arguments of the call.  Row strides (ld*) are in values, at least the row's length; rows do not overlap.
- * Outputs do not alias inputs, with one exception: y may be the residual itself.  Sums are in a fixed order: results
- * are the same from run to run.
+ * alignment included: ask with the arguments of the call.  Row strides (ld*) are in values, at least the row's
+ * length; rows do not overlap.  Outputs do not alias inputs, with one exception: y may be the residual itself.  Sums
+ * are in a fixed order: results are the same from run to run.
  *
  * Every function returns a PETDIFF_* code (petdiff.h); petdense_last_error() names the last failure of the thread.
  */

@@ -102,8 +102,7 @@ __host__ __device__ inline void tile_at(int t, int ti, int tj, int& i, int& j) {
 constexpr int kMaxRows = 2, kRowThreads = 1024, kRowCols = 32;
 hipError_t rows(const Product& p, int type, hipStream_t s);
 
-// rows of a lane in flight in act_grad, and the lanes that share a row of N columns: a power of two
-constexpr int kActGradAhead = 2;
+// lanes that share a row of N columns in act_grad: a power of two
 inline int act_grad_lanes(int N) {
   int l = 1;
   while (l < 64 && l * 8 < N) l *= 2;
