@@ -372,8 +372,9 @@ struct BackwardPlan {
   double us;
 };
 
-// The products from operands that are in memory (lx, lk: their loaders): one launch or two.
-double plan_products(const petdense_backward_args* a, int lx, int lk, BackwardPlan& b) {
+// The products from operands that are in memory (lx, lk: their loaders; dp_dma: dP's beside 8-bit inputs): one launch
+// or two.
+double plan_products(const petdense_backward_args* a, int lx, int lk, bool dp_dma, BackwardPlan& b) {
   const bool q8 = a->x_exponents;
   b.load_x = lx;
   b.load_k = lk;
@@ -401,7 +402,7 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, BackwardPl
     const int sz = size_of(a->dtype);
     const double once = kCopyLaunch + (double)a->m * a->k * (1 + sz) / 3.5e6;
     const bool may = lk == kDma && copies_fit((double)a->m * a->k, sz);
-    const Plan apart = plan(a->k, a->n, a->m, a->dtype, lk == kDma ? kCodes : kReg);
+    const Plan apart = plan(a->k, a->n, a->m, a->dtype, dp_dma ? kCodes : kReg);
     const Plan restored = plan(a->k, a->n, a->m, a->dtype, kDma);
     const bool cheaper = may && restored.us + once < apart.us;
     const double own = cheaper ? restored.us + once : apart.us;
@@ -438,11 +439,11 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
   const bool w_ok = !a->dx || dma_ok(a->kernel, a->ldk, a->n, sz);
   const bool x_ok = !a->dkernel || (q8 ? a->k * sz % 16 == 0 : dma_ok(a->x, a->ldx, a->k, sz));
   // (8-bit inputs go through registers whatever their alignment: their loader is dp's)
-  b.us = act_us + plan_products(a, dp_ok && w_ok ? kDma : kReg, dp_ok && x_ok ? kDma : kReg, b);
+  b.us = act_us + plan_products(a, dp_ok && w_ok ? kDma : kReg, dp_ok && x_ok ? kDma : kReg, dp_ok, b);
   if (!(dp_ok && w_ok && x_ok) && (a->dx || a->dkernel) &&
       copies_fit((double)a->m * a->n + (double)a->k * a->n + (double)a->m * a->k, sz)) {
     BackwardPlan c = b;
-    c.us = act_us + plan_products(a, kDma, kDma, c) + kCopyLaunch + (dp_ok ? 0 : copy_us(a->m, a->n, sz)) +
+    c.us = act_us + plan_products(a, kDma, kDma, true, c) + kCopyLaunch + (dp_ok ? 0 : copy_us(a->m, a->n, sz)) +
            (w_ok ? 0 : copy_us(a->k, a->n, sz)) + (x_ok ? 0 : copy_us(a->m, a->k, sz));
     if (c.us < b.us) {
       b = c;
@@ -451,6 +452,8 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
       b.x.on = !x_ok && !q8;
     }
   }
+  // 8-bit inputs are staged through registers whatever their alignment: beside them dP takes the loader that it can
+  if (q8 && a->dkernel && !b.restore && (dp_ok || b.dp.on)) b.load_k = kDma;
   // (dP is formed again for every tile that reads it: for small ones)
   if ((a->dx || a->dkernel) && (b.make_dp || b.sums) && !a->dresidual && a->m * a->n <= 1 << 18) {
     Plan px, pk;
