@@ -48,26 +48,37 @@ struct Plan {
 
 // What a kind of tile costs, in microseconds, as measured on products of 64 .. 12288 rows.  A step (128 bytes of
 // contraction) takes `wait` when its workgroup has a compute unit to itself, and `share` per workgroup when several
-// fill it; `ends` is a workgroup's first load and its epilogue.  [operands by DMA, through registers, dP formed there,
-// one operand restored there from 8 bits]
+// fill it; `ends` is a workgroup's first load and its epilogue.  [operands by DMA; through registers; dP formed there
+// of ReLU or linear layers; of GELU and SiLU; one operand restored there from 8 bits]
 struct Cost {
   int tile, b, slots, k;   // b: rows and columns of the tile; slots: workgroups of a compute unit; k: steps at a time
-  double wait[4], share[4], ends;
+  double wait[5], share[5], ends;
 };
-constexpr int kFormed = 2, kCodes = 3;
-constexpr Cost kCosts16[] = {{kLarge, 256, 1, 1, {1.47, 0, 0, 0}, {1.47, 0, 0, 0}, 7.5},
-                             {kMid, 128, 2, 1, {0.65, 1.25, 0, 0.95}, {0.46, 1.25, 0, 0.62}, 3.5},
-                             {kSmall, 64, 4, 1, {0.28, 0.55, 2.0, 0.65}, {0.19, 0.34, 1.5, 0.3}, 2.0},
-                             {kSlice, 32, 1, 8, {0.5, 1.0, 3.4, 0.65}, {1.2, 1.5, 3.4, 1.4}, 2.0},
-                             {kSlice64, 64, 1, 4, {0.78, 2.4, 0, 1.15}, {0.8, 2.4, 0, 1.15}, 3.5}};
-constexpr Cost kCosts32[] = {{kLarge, 256, 1, 1, {6.9, 0, 0, 0}, {6.9, 0, 0, 0}, 8.0},
-                             {kMid, 128, 2, 1, {2.3, 2.7, 0, 2.5}, {2.1, 2.5, 0, 2.3}, 4.0},
-                             {kSmall, 64, 4, 1, {0.75, 0.95, 2.4, 0.87}, {0.53, 0.65, 2.0, 0.6}, 2.0},
-                             {kSlice, 32, 1, 8, {1.1, 1.3, 3.5, 1.3}, {1.3, 1.5, 3.5, 1.5}, 2.0},
-                             {kSlice64, 64, 1, 4, {2.6, 4.5, 0, 3.0}, {2.75, 4.5, 0, 3.1}, 3.5}};
+constexpr int kFormed = 2, kFormedCurve = 3, kCodes = 4;
+constexpr Cost kCosts16[] = {
+    {kLarge, 256, 1, 1, {1.47, 0, 0, 0, 0}, {1.47, 0, 0, 0, 0}, 7.5},
+    {kMid, 128, 2, 1, {0.65, 1.25, 0, 0, 0.95}, {0.46, 1.25, 0, 0, 0.62}, 3.5},
+    {kSmall, 64, 4, 1, {0.28, 0.55, 2.0, 2.0, 0.65}, {0.19, 0.34, 1.5, 1.5, 0.3}, 2.0},
+    {kSlice, 32, 1, 8, {0.5, 1.0, 1.8, 3.8, 0.65}, {1.2, 1.5, 3.0, 3.2, 1.4}, 2.0},
+    {kSlice64, 64, 1, 4, {0.78, 2.4, 0, 0, 1.15}, {0.8, 2.4, 0, 0, 1.15}, 3.5}};
+constexpr Cost kCosts32[] = {
+    {kLarge, 256, 1, 1, {6.9, 0, 0, 0, 0}, {6.9, 0, 0, 0, 0}, 8.0},
+    {kMid, 128, 2, 1, {2.3, 2.7, 0, 0, 2.5}, {2.1, 2.5, 0, 0, 2.3}, 4.0},
+    {kSmall, 64, 4, 1, {0.75, 0.95, 2.4, 2.4, 0.87}, {0.53, 0.65, 2.0, 2.0, 0.6}, 2.0},
+    {kSlice, 32, 1, 8, {1.1, 1.3, 1.9, 4.5, 1.3}, {1.3, 1.5, 3.5, 5.0, 1.5}, 2.0},
+    {kSlice64, 64, 1, 4, {2.6, 4.5, 0, 0, 3.0}, {2.75, 4.5, 0, 0, 3.1}, 3.5}};
 constexpr double kNever = 1e30;      // no plan
 constexpr double kLaunch = 3.5;      // a launch behind another, here and on the host
 constexpr double kWorkspace = 2.0;   // a small call that needs a workspace: the host's time for it
+// The host's time for a call is longer than a small one's on the device: from Python 4 us forward, 8 us backward (its
+// outputs), and 3.2 us a launch.
+constexpr double kHostForward = 4.0, kHostBackward = 8.0, kHostLaunch = 3.2;
+
+// A call's price when calls follow each other: what is longer, the device's time or the host's (and a little for the
+// device's where it is the host's, which a captured graph saves).
+double call_us(double device, double host, int launches, bool work) {
+  return std::max(device, host + kHostLaunch * launches + (work ? kWorkspace : 0.0)) + 0.02 * device;
+}
 constexpr int kUnits = 256;
 
 double step_us(const Cost& c, double per_unit, int loader) {
@@ -124,8 +135,8 @@ double memory_us(double I, double J, double C, int type) {
   return (C * (I + J) + I * J) * (type == kF32 ? 4 : 2) / 4.5e6;
 }
 
-// Tile and split of a product by their estimated time.
-Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
+// Tile and split of a product by their estimated time; `call`: it is all of a call.
+Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader, bool call = false) {
   const int bc = type == kF32 ? 32 : 64;
   const int64_t steps = ceil_div(C, bc);
   const double memory = memory_us(I, J, C, type);
@@ -147,8 +158,9 @@ Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
         // split tiles' sums in fp32
         const double values = stream ? (double)rest * c.b * c.b : (double)I * J;
         if (s > 1 && values * s * 4 > 8e9) return;
-        const double t =
+        const double device =
             std::max(before + groups_us(c, rest * s, per, loader), kLaunch + 2.0 + memory) + join_us(values, s);
+        const double t = call ? call_us(device, kHostForward, s > 1 ? 2 : 1, s > 1) : device;
         if (best.c_per && t >= best.us) return;
         best.us = t;
         set_plan(best, c, s, per, bc, I, J);
@@ -165,13 +177,13 @@ Plan plan(int64_t I, int64_t J, int64_t C, int type, int loader) {
 
 // The backward pass as one launch, or kNever where it has too many tiles for that: x (I = m, J = k, C = n) and k
 // (I = k, J = n, C = m) with the same kind of tile; only the kernel gradient's contraction is split.  nx, nk: which
-// products are wanted.
+// products are wanted; `call`: it is all of a call (but for the join of a split).
 double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, int lx, int lk, bool slice64,
-                 Plan& px, Plan& pk) {
+                 bool call, Plan& px, Plan& pk) {
   const int bc = type == kF32 ? 32 : 64;
   const int64_t sx = ceil_div(n, bc), sk = ceil_div(m, bc);
   const double memory = (nx ? memory_us(m, k, n, type) : 0) + (nk ? memory_us(k, n, m, type) : 0);
-  double best = kNever;
+  double best = kNever, least = kNever;
   for (const Cost& c : type == kF32 ? kCosts32 : kCosts16) {
     if (c.tile == kLarge || c.tile == kMid || (c.tile == kSlice64 && !slice64)) continue;
     const int64_t tx = nx ? ceil_div(m, c.b) * ceil_div(k, c.b) : 0, tk = nk ? ceil_div(k, c.b) * ceil_div(n, c.b) : 0;
@@ -186,7 +198,9 @@ double plan_pair(bool nx, bool nk, int64_t m, int64_t k, int64_t n, int type, in
       const double longest = std::max(wx * c.wait[lx] + ex, wk * c.wait[lk] + ek);
       const double t = kLaunch + std::max({longest, share * (groups > kUnits * c.slots ? 1.25 : 1.0), 2.0 + memory}) +
                        (s > 1 ? join_us((double)k * n, s) + kWorkspace : 0.0);
-      if (t >= best) return;
+      const double price = call ? call_us(t, kHostBackward, s > 1 ? 2 : 1, s > 1) : t;
+      if (price >= least) return;
+      least = price;
       best = t;
       set_plan(px, c, 1, sx, bc, m, k);
       set_plan(pk, c, s, per, bc, k, n);
@@ -299,9 +313,12 @@ ForwardPlan plan_forward(const petdense_forward_args* a) {
   f.rows = a->m <= kMaxRows && a->n <= 1 << 26;          // (a grid has fewer than 2^32 threads)
   if (a->m == 0) return f;
   if (f.rows) {
-    // narrow layers leave compute units without columns: the contraction is split, where that is worth the join
+    // narrow layers leave compute units without columns: the contraction is split, where that is worth the join's
+    // launch, 4 us and more of the host's (1 x 4096 x 1024: a call takes 8.0 us, 11.6 us split; rows that do not lie on
+    // 16 bytes are slower: 1 x 3500 x 1356 takes 13.5 us on the device, 10.3 us split)
     const int64_t groups = ceil_div(a->n, kRowCols);
-    const int64_t want = std::min<int64_t>(kUnits / groups, a->k / 1024);
+    const int64_t alone = dma_ok(a->kernel, a->ldk, a->n, size_of(a->dtype)) ? 5120 : 3584;
+    const int64_t want = a->k >= alone ? std::min<int64_t>(kUnits / groups, a->k / 1024) : 1;
     f.p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, 16));
     f.p.c_per = (int)ceil_div(a->k, f.p.splits);
     f.p.splits = (int)ceil_div(a->k, f.p.c_per);
@@ -311,10 +328,10 @@ ForwardPlan plan_forward(const petdense_forward_args* a) {
   const int sz = size_of(a->dtype);
   const bool x_ok = dma_ok(a->x, a->ldx, a->k, sz), w_ok = dma_ok(a->kernel, a->ldk, a->n, sz);
   f.loader = x_ok && w_ok ? kDma : kReg;
-  f.p = plan(a->m, a->n, a->k, a->dtype, f.loader);
+  f.p = plan(a->m, a->n, a->k, a->dtype, f.loader, true);
   size_t o = 0;
   if (f.loader == kReg) {
-    const Plan q = plan(a->m, a->n, a->k, a->dtype, kDma);
+    const Plan q = plan(a->m, a->n, a->k, a->dtype, kDma, true);
     const double t = q.us + kCopyLaunch + (x_ok ? 0 : copy_us(a->m, a->k, sz)) + (w_ok ? 0 : copy_us(a->k, a->n, sz));
     // (x's rows are filled up with zeros; rows past the kernel's last are not read, which stages zeros too)
     if (t < f.p.us && copies_fit((double)a->k * (a->m + a->n), sz)) {
@@ -386,7 +403,7 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, bool dp_dm
   double us = b.px.us + b.pk.us + (joins ? kLaunch : 0.0);
   if (a->dx && a->dkernel) {
     Plan px, pk;
-    const double t = plan_pair(true, true, a->m, a->k, a->n, a->dtype, lx, lk, true, px, pk);
+    const double t = plan_pair(true, true, a->m, a->k, a->n, a->dtype, lx, lk, true, false, px, pk);
     if (t < us) {
       us = t;
       b.pair = true;
@@ -457,10 +474,15 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
   // (dP is formed again for every tile that reads it: for small ones)
   if ((a->dx || a->dkernel) && (b.make_dp || b.sums) && !a->dresidual && a->m * a->n <= 1 << 18) {
     Plan px, pk;
-    double t = plan_pair(a->dx, a->dkernel, a->m, a->k, a->n, a->dtype, kFormed, kFormed, false, px, pk);
+    const int form = a->activation == PETDENSE_GELU || a->activation == PETDENSE_SILU ? kFormedCurve : kFormed;
+    double t = plan_pair(a->dx, a->dkernel, a->m, a->k, a->n, a->dtype, form, form, false, true, px, pk);
     // a sum's workgroup walks all rows: 256 at a time, 4 of them in flight
     if (b.sums) t = std::max(t, kLaunch + 2.5 + 0.7 * (double)a->m / 256);
-    if (t < b.us) {
+    const bool joined = a->dkernel && b.pk.splits > 1;
+    const int launches = 1 + (b.pair ? 1 : (a->dx ? 1 : 0) + (a->dkernel ? 1 : 0) + (b.sums && !joined ? 1 : 0)) +
+                         (joined ? 1 : 0) + (b.dp.on || b.x.on || b.kernel.on ? 1 : 0);
+    const bool split = a->dkernel && pk.splits > 1;
+    if (call_us(t, kHostBackward, split ? 2 : 1, split) < call_us(b.us, kHostBackward, launches, true)) {
       b.us = t;
       b.fused = true;
       b.pair = false;

@@ -18,6 +18,14 @@ inline hipError_t launch_kernel(void (*k)(A...), dim3 grid, dim3 block, size_t l
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// Neighbouring workgroup numbers go to different XCDs, each with its own L2: XCD x takes a contiguous run of the n
+// pieces of work, [first, first + len).
+__device__ __forceinline__ void run_of(int n, int x, int& first, int& len) {
+  const int per = n / 8, rest = n % 8;
+  first = x * per + min(x, rest);
+  len = per + (x < rest ? 1 : 0);
+}
+
 // Phi(x) = (1 + erf(x / sqrt 2)) / 2.
 // 16-bit outputs: 1 / (1 + 2^(-x P(x^2))), P of degree 6: the least largest error of x Phi(x) over |x| <= 6 (a linear
 // program over log2(Phi / (1 - Phi)) / x), 7e-8 there and less beyond, 1.8e-7 of Phi with its fp32 steps; beside the

@@ -92,8 +92,10 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(Product p, ColumnJoin c
 // One or two rows (decoding, a single sample): every value of B is read once by one workgroup, which owns 32 columns
 // and, where those are enough workgroups, the whole contraction, so that one launch ends the call.  Bound by latency:
 // 4 lanes share a row's 8-column pieces, 256 rows of B are in flight four deep, and the sums meet by two rotations of
-// 16 lanes and once in LDS, in a fixed order.  1 x 1024 x 4096 bf16 in 4.4 us, 1.9 TB/s of weights; a launch alone
-// takes 3 us.  From three rows on the sliced tiles are quicker (3 x 3608 x 4882 fp16: 29 us here).
+// 16 lanes and once in LDS, in a fixed order.  Neighbouring columns go to one XCD, whose L2 has the other half of their
+// cache lines: 1 x 8192 x 8192 bf16 in 27.6 us, 4.9 TB/s of weights (42 us with them spread).  1 x 1024 x 4096 in
+// 4.4 us, where a launch alone takes 3 us.  From three rows on the sliced tiles are quicker (3 x 3608 x 4882 fp16: 29 us
+// here).
 // ---------------------------------------------------------------------------------------------------------------
 // v summed over the four lanes l, l + 4, l + 8, l + 12 of a row of 16, in each of them (two rotations of the row: no
 // LDS, which ROWS x 8 shuffles of 16 waves would keep busy for microseconds)
@@ -133,7 +135,11 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
   __shared__ float red[PARTS][ROWS][kRowCols];
   __shared__ float sum[ROWS][kRowCols];
   const int tid = threadIdx.x, l = tid % LANES, grp = tid / LANES;
-  const int j0 = blockIdx.x * kRowCols, j = j0 + l * W, n = p.J - j;
+  const int groups = (p.J + kRowCols - 1) / kRowCols;
+  int first, len;
+  run_of(groups * p.splits, blockIdx.x % 8, first, len);
+  const int piece = first + blockIdx.x / 8, split = piece / groups, j0 = (piece - split * groups) * kRowCols;
+  const int j = j0 + l * W, n = p.J - j;
   const T* A = static_cast<const T*>(p.A);
   const T* B = static_cast<const T*>(p.B) + j;
   float acc[ROWS][W];
@@ -141,7 +147,7 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int q = 0; q < W; ++q) acc[r][q] = 0.f;
-  const int end = min(p.C, ((int)blockIdx.y + 1) * p.c_per);      // this part of the contraction
+  const int end = min(p.C, (split + 1) * p.c_per);      // this part of the contraction
   auto walk = [&](auto whole) {
     auto add = [&](const T* w, const T* x) {
 #pragma unroll
@@ -154,7 +160,7 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) x[r] = A[r * p.lda + c];
     };
-    int c = blockIdx.y * p.c_per + grp;
+    int c = split * p.c_per + grp;
     for (; c + (AHEAD - 1) * GROUPS < end; c += AHEAD * GROUPS) {
       T w[AHEAD][W], x[AHEAD][ROWS];
 #pragma unroll
@@ -192,14 +198,14 @@ __global__ __launch_bounds__(kRowThreads) void rows_kernel(Product p) {
     float v[W];
 #pragma unroll
     for (int q = 0; q < W; ++q) v[q] = sum[r][l * W + q];
-    if (p.splits > 1) store_row<float, W>(p.part + ((int64_t)blockIdx.y * p.I + r) * p.J + j, n, v);
+    if (p.splits > 1) store_row<float, W>(p.part + ((int64_t)split * p.I + r) * p.J + j, n, v);
     else epilogue8<T>(p.e, r, j, n, v);
   }
 }
 
 template <typename T>
 hipError_t rows_t(const Product& p, hipStream_t s) {
-  const dim3 grid(blocks_for(p.J, kRowCols), p.splits), block(kRowThreads);
+  const dim3 grid(blocks_for(p.J, kRowCols) * p.splits), block(kRowThreads);
   if (p.I == 1) return launch_kernel(rows_kernel<T, 1>, grid, block, 0, s, p);
   return launch_kernel(rows_kernel<T, 2>, grid, block, 0, s, p);
 }

@@ -414,14 +414,6 @@ typedef Kind<64, 64, 2, 2, 1> Small;
 typedef Kind<32, 32, 1, 1, 8> Slice;
 typedef Kind<64, 64, 1, 1, 4> Slice64;
 
-// Neighbouring workgroup numbers go to different XCDs, each with its own L2: XCD x takes a contiguous run of the n
-// pieces of work, [first, first + len).
-__device__ __forceinline__ void run_of(int n, int x, int& first, int& len) {
-  const int per = n / 8, rest = n % 8;
-  first = x * per + min(x, rest);
-  len = per + (x < rest ? 1 : 0);
-}
-
 // Workgroup -> part of the contraction and tile: a part's rows are fetched by one XCD.
 __device__ __forceinline__ void place_of(int b, int ti, int tj, int splits, int& split, int& i, int& j) {
   const int tiles = ti * tj;
@@ -807,8 +799,9 @@ __global__ __launch_bounds__(K::THREADS) void pair_kernel(Pair p) {
 }
 
 // The same from dy and saved: dP is formed while it is staged, the other workgroups sum 8 columns each.  One launch
-// for a small backward pass (310 x 256 x 48 fp16 from 8 bits: 8.4 us); every tile that reads dP forms it again, so it
-// is taken for at most 2^18 values of dP.
+// for a small backward pass, for which the host takes longer than the device (1568 x 128 x 64 bf16: 10.3 us and 13 us a
+// call, 10.6 us and 17 us as two launches); every tile that reads dP forms it again, so it is taken for at most 2^18
+// values of dP.
 template <typename T, typename K, bool Q8>
 __global__ __launch_bounds__(K::THREADS) void fused_kernel(Pair p) {
   extern __shared__ char lds[];
