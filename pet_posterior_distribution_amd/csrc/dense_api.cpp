@@ -399,7 +399,8 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, bool dp_dm
   b.pair = false;
   if (a->dx) b.px = plan(a->m, a->k, a->n, a->dtype, lx);
   if (a->dkernel) b.pk = plan(a->k, a->n, a->m, a->dtype, lk);
-  const bool joins = b.sums && !(a->dkernel && b.pk.splits > 1);      // a launch for the column sums
+  // a launch for the column sums, where no product's join carries them
+  const bool joins = b.sums && !(a->dx && b.px.splits > 1) && !(a->dkernel && b.pk.splits > 1);
   double us = b.px.us + b.pk.us + (joins ? kLaunch : 0.0);
   if (a->dx && a->dkernel) {
     Plan px, pk;
@@ -478,9 +479,9 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
     double t = plan_pair(a->dx, a->dkernel, a->m, a->k, a->n, a->dtype, form, form, false, true, px, pk);
     // a sum's workgroup walks all rows: 256 at a time, 4 of them in flight
     if (b.sums) t = std::max(t, kLaunch + 2.5 + 0.7 * (double)a->m / 256);
-    const bool joined = a->dkernel && b.pk.splits > 1;
-    const int launches = 1 + (b.pair ? 1 : (a->dx ? 1 : 0) + (a->dkernel ? 1 : 0) + (b.sums && !joined ? 1 : 0)) +
-                         (joined ? 1 : 0) + (b.dp.on || b.x.on || b.kernel.on ? 1 : 0);
+    const int joins = (a->dx && b.px.splits > 1 ? 1 : 0) + (a->dkernel && b.pk.splits > 1 ? 1 : 0);
+    const int products = b.pair ? 1 : (a->dx ? 1 : 0) + (a->dkernel ? 1 : 0) + (b.sums && !joins ? 1 : 0);
+    const int launches = 1 + products + joins + (b.dp.on || b.x.on || b.kernel.on ? 1 : 0);
     const bool split = a->dkernel && pk.splits > 1;
     if (call_us(t, kHostBackward, split ? 2 : 1, split) < call_us(b.us, kHostBackward, launches, true)) {
       b.us = t;
@@ -652,12 +653,14 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     if (b.pk.splits > 1) HIPC(join(p.k, ColumnJoin{}, a->dtype, s));
     return PETDIFF_OK;
   }
-  const bool carried = a->dkernel && b.pk.splits > 1;
-  if (b.sums && !carried) HIPC(join_columns(cols, s));
+  const bool with_x = a->dx && b.px.splits > 1, with_k = !with_x && a->dkernel && b.pk.splits > 1;
+  if (b.sums && !with_x && !with_k) HIPC(join_columns(cols, s));
+  const ColumnJoin none{};
+  char* part = w + b.o_part;
   if (a->dx)
-    if (int r = run_product(x, kInputGrad, b.load_x, a->dtype, 0, b.px, w + b.o_part, ColumnJoin{}, s)) return r;
+    if (int r = run_product(x, kInputGrad, b.load_x, a->dtype, 0, b.px, part, with_x ? cols : none, s)) return r;
   if (a->dkernel)
-    if (int r = run_product(k, kKernelGrad, b.load_k, a->dtype, q8, b.pk, w + b.o_part, cols, s)) return r;
+    if (int r = run_product(k, kKernelGrad, b.load_k, a->dtype, q8, b.pk, part, with_k ? cols : none, s)) return r;
   return PETDIFF_OK;
 }
 

@@ -94,8 +94,8 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(Product p, ColumnJoin c
 // 4 lanes share a row's 8-column pieces, 256 rows of B are in flight four deep, and the sums meet by two rotations of
 // 16 lanes and once in LDS, in a fixed order.  Neighbouring columns go to one XCD, whose L2 has the other half of their
 // cache lines: 1 x 8192 x 8192 bf16 in 27.6 us, 4.9 TB/s of weights (42 us with them spread).  1 x 1024 x 4096 in
-// 4.4 us, where a launch alone takes 3 us.  From three rows on the sliced tiles are quicker (3 x 3608 x 4882 fp16: 29 us
-// here).
+// 4.4 us, where a launch alone takes 3 us.  From three rows on the sliced tiles are quicker (3 x 3608 x 4882 fp16 took
+// 29 us here).
 // ---------------------------------------------------------------------------------------------------------------
 // v summed over the four lanes l, l + 4, l + 8, l + 12 of a row of 16, in each of them (two rotations of the row: no
 // LDS, which ROWS x 8 shuffles of 16 waves would keep busy for microseconds)
