@@ -209,10 +209,7 @@ struct Filler {
     u.left = clen - u.t * BC;
     u.p = base + (FREE ? (int64_t)u.t * BC * ld : (int64_t)u.t * BC * (int64_t)sizeof(T));
     if constexpr (ACT) u.p2 = base2 + (FREE ? (int64_t)u.t * BC * ld2 : (int64_t)u.t * BC * (int64_t)sizeof(T));
-    // free-contiguous: 16 bytes from a piece's first value may run into the next row, which then has to exist
-    // (offsets within a step fit 31 bits)
-    u.whole = !brief && (FREE ? u.left > BC && ld >= 16 : u.left >= BC) && ld < 0x7fffffff / 256 &&
-              (!ACT || ((!FREE || ld2 >= 16) && ld2 < 0x7fffffff / 256));
+    u.whole = !brief && whole_step(FREE, u.left, BC, ld, ACT ? ld2 : ld, Q8 ? lde : 0);
     if constexpr (LOADER == kDma) {
       const unsigned long long a = reinterpret_cast<unsigned long long>(u.p);
       u.rs[0] = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffull));
@@ -251,7 +248,7 @@ struct Filler {
           load_piece(reg[q], u.p + (unsigned)(rr * (int)ld + cc * PB));
           if constexpr (ACT) load_piece(reg2[q], u.p2 + (unsigned)(rr * (int)ld2 + cc * PB));
           if constexpr (Q8)
-            reg[q][2] = (exps + (int64_t)u.t * BC * lde)[(unsigned)(r * (int)lde + (cc * S::EPC) / 32)];
+            reg[q][2] = (exps + (int64_t)u.t * BC * lde)[exponent_offset(r, lde, (cc * S::EPC) / 32)];
         }
         return;
       }

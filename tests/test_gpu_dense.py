@@ -494,6 +494,24 @@ def test_offsets_past_32_bits():
     close(g.kernel[cols], xc.T @ d6, (m + 4) * E23 * (xc.abs().T @ d6.abs()), 'dkernel from 8 bits')
 
 
+@pytest.mark.parametrize('t', TYPES, ids=str)
+@pytest.mark.parametrize('n', [24, 2100])
+def test_exponents_of_a_column_slice_of_a_wide_tensor(n, t):
+    """Row strides of 70,000,000 exponent bytes: rows 62 and 63 of a step lie past 2^32."""
+    from pet_posterior_distribution_amd import ActivationCheckpoint, checkpoint_activations, dense_backward
+    m, k = 130, 96
+    x, w, _, _, dy = inputs(m, k, n, t)
+    x = x * torch.exp2(torch.arange(m, device='cuda') % 9 - 4).to(t)[:, None]
+    c = checkpoint_activations(x)
+    wide = torch.empty(m, 70_000_000, dtype=torch.uint8, device='cuda')
+    wide[:, 5:8] = c.exponents
+    s = ActivationCheckpoint(c.codes, wide[:, 5:8], t)
+    assert torch.equal(s.restore(), c.restore())
+    g, ref = dense_backward(dy, s, w), dense_backward(dy, c, w)
+    for a, b in zip(g[:3], ref[:3]):
+        assert torch.equal(a, b)
+
+
 def test_one_row_of_more_columns_than_a_launch_has_threads():
     """2^27 columns: more than one launch of a kernel of 1024 threads for 32 columns could take.  Signs and whole
     numbers, so that every sum is exact in fp32 whatever its order."""
