@@ -217,9 +217,14 @@ double unsplit_us(int tile, int64_t I, int64_t J, int64_t C, int type, int loade
   return kLaunch + std::max(groups_us(c, tiles, steps, loader), 2.0 + memory_us(I, J, C, type));
 }
 
+int64_t padded(int64_t n, int size) { return ceil_div(n, 16 / size) * (16 / size); }
+
+// A tile's rows, `ld` values apart, lie within the offsets that DMA has.
+bool row_fits(int64_t ld, int size) { return ld < kMaxRowBytes / size; }
+
 bool dma_ok(const void* p, int64_t ld, int64_t contiguous, int size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0 && (contiguous * size) % 16 == 0 &&
-         ld * size < (int64_t)0x7fffffff / 256;          // a tile's offsets fit 31 bits
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row_fits(ld, size) && (ld * size) % 16 == 0 &&
+         (contiguous * size) % 16 == 0;
 }
 
 bool planned(const Plan& p, int64_t C) {
@@ -279,9 +284,14 @@ struct Copy {
   int64_t ld = 0;
 };
 
-int64_t padded(int64_t n, int size) { return ceil_div(n, 16 / size) * (16 / size); }
-// (one launch copies at most 2^31 pieces of 16 bytes)
-bool copies_fit(double values, int size) { return values * size / 16 < 2e9; }
+// Pieces of 16 bytes that the copy of an operand moves, or kNoCopy where its rows would be too long for DMA even so.
+// One launch copies at most kMaxPieces.
+constexpr int64_t kMaxPieces = (int64_t)1 << 31, kNoCopy = kMaxPieces;
+int64_t pieces_of(bool on, int64_t rows, int64_t n, int size) {
+  if (!on) return 0;
+  const int64_t ld = padded(n, size);
+  return row_fits(ld, size) ? std::min(kNoCopy, rows * (ld * size / 16)) : kNoCopy;
+}
 // read and written once, by a launch of its own
 double copy_us(int64_t rows, int64_t n, int size) { return (double)rows * n * size * 2 / 3.5e6; }
 constexpr double kCopyLaunch = kLaunch + 1.5;
@@ -334,7 +344,7 @@ ForwardPlan plan_forward(const petdense_forward_args* a) {
     const Plan q = plan(a->m, a->n, a->k, a->dtype, kDma, true);
     const double t = q.us + kCopyLaunch + (x_ok ? 0 : copy_us(a->m, a->k, sz)) + (w_ok ? 0 : copy_us(a->k, a->n, sz));
     // (x's rows are filled up with zeros; rows past the kernel's last are not read, which stages zeros too)
-    if (t < f.p.us && copies_fit((double)a->k * (a->m + a->n), sz)) {
+    if (t < f.p.us && pieces_of(!x_ok, a->m, a->k, sz) + pieces_of(!w_ok, a->k, a->n, sz) < kMaxPieces) {
       f.p = q;
       f.loader = kDma;
       f.x = copy_of(!x_ok, a->m, a->k, sz, o);
@@ -419,7 +429,7 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, bool dp_dm
   if (q8 && a->dkernel) {
     const int sz = size_of(a->dtype);
     const double once = kCopyLaunch + (double)a->m * a->k * (1 + sz) / 3.5e6;
-    const bool may = lk == kDma && copies_fit((double)a->m * a->k, sz);
+    const bool may = lk == kDma && pieces_of(true, a->m, a->k, sz) < kMaxPieces;
     const Plan apart = plan(a->k, a->n, a->m, a->dtype, dp_dma ? kCodes : kReg);
     const Plan restored = plan(a->k, a->n, a->m, a->dtype, kDma);
     const bool cheaper = may && restored.us + once < apart.us;
@@ -444,6 +454,7 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
   b.make_dp = a->activation != PETDENSE_NONE || a->dresidual;
   b.sums = a->dbias != nullptr;
   const bool own_dp = b.make_dp && !a->dresidual;
+  const int64_t ld_dp = ceil_div(a->n, 64) * 64;
   // row chunks of the activation's gradient: about 1024 workgroups, each of one round of its rows at least
   const int lanes = act_grad_lanes((int)a->n);
   const int64_t most = std::max<int64_t>(1, 1024 / ceil_div(a->n, lanes * 8));
@@ -453,13 +464,14 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
 
   // dp in the workspace has rows of whole pieces, with zeros: DMA takes it as it is
   const bool dp_ok =
-      own_dp || (a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz) : dma_ok(a->dy, a->lddy, a->n, sz));
+      own_dp ? row_fits(ld_dp, sz) : (a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz) : dma_ok(a->dy, a->lddy, a->n, sz));
   const bool w_ok = !a->dx || dma_ok(a->kernel, a->ldk, a->n, sz);
   const bool x_ok = !a->dkernel || (q8 ? a->k * sz % 16 == 0 : dma_ok(a->x, a->ldx, a->k, sz));
   // (8-bit inputs go through registers whatever their alignment: their loader is dp's)
   b.us = act_us + plan_products(a, dp_ok && w_ok ? kDma : kReg, dp_ok && x_ok ? kDma : kReg, dp_ok, b);
   if (!(dp_ok && w_ok && x_ok) && (a->dx || a->dkernel) &&
-      copies_fit((double)a->m * a->n + (double)a->k * a->n + (double)a->m * a->k, sz)) {
+      pieces_of(!dp_ok, a->m, a->n, sz) + pieces_of(!w_ok, a->k, a->n, sz) +
+              pieces_of(!x_ok && !q8, a->m, a->k, sz) < kMaxPieces) {
     BackwardPlan c = b;
     c.us = act_us + plan_products(a, kDma, kDma, true, c) + kCopyLaunch + (dp_ok ? 0 : copy_us(a->m, a->n, sz)) +
            (w_ok ? 0 : copy_us(a->k, a->n, sz)) + (x_ok ? 0 : copy_us(a->m, a->k, sz));
@@ -494,7 +506,7 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
   }
   size_t o = 0;
   if (own_dp && !b.fused) {
-    b.ld_dp = ceil_div(a->n, 64) * 64;
+    b.ld_dp = ld_dp;
     b.o_dp = o;
     o += up((size_t)a->m * b.ld_dp * sz);
   }

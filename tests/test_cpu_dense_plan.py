@@ -43,3 +43,81 @@ def test_exponent_bytes_of_a_whole_step_are_reached_at_any_row_stride(plan, bc):
         for r in range(bc):
             assert plan.plan_exponent_offset(r, lde, block) == r * lde + block, (lde, r)
     assert plan.plan_whole_step(1, bc + 1, bc, 4096, 4096, 128)          # dense exponents: the quick way
+
+
+# ------------------------------------------------------------------------------------------------ the plan's launches
+F32, BF16, F16 = 0, 1, 2
+SIZE = {F32: 4, BF16: 2, F16: 2}
+TILE = {0: 256, 1: 128, 2: 64, 3: 32, 4: 64}
+FORWARD, INPUT_GRAD, KERNEL_GRAD = 0, 1, 2
+DMA = 0
+
+
+def launches(plan, name, args):
+    """The launches of one call, as (kind, {field: number}); its workspace is an address that nothing reads."""
+    need = getattr(plan, f'petdense_{name}_workspace')(C.byref(args))
+    plan.plan_clear()
+    rc = getattr(plan, f'petdense_{name}')(C.byref(args), 0x10000 if need else None, need, None)
+    assert rc == 0, plan.petdense_last_error().decode()
+    out = []
+    for line in plan.plan_log().decode().splitlines():
+        kind, *fields = line.split()
+        out.append((kind, {k: int(v) for k, v in (f.split('=') for f in fields)}))
+    return out
+
+
+def forward(m, k, n, dtype, ldx=None, ldk=None, **kw):
+    a = _lib.PetdenseForwardArgs(0x1000, 0x2000, 0x3000, None, 0x4000, None, ldx or k, ldk or n, 0, n, 0, m, k, n, dtype,
+                                 0, 0, 0)
+    for key, v in kw.items():
+        setattr(a, key, v)
+    return a
+
+
+def backward(m, k, n, dtype, activation=0, codes=False, **kw):
+    a = _lib.PetdenseBackwardArgs(0x1000, 0x2000, 0x8000 if codes else None, 0x3000, 0x4000, 0x5000, 0x6000, 0x7000,
+                                  None, n, k, -(-k // 32) if codes else 0, n, n, k, n, 0, m, k, n, dtype, activation, 0)
+    for key, v in kw.items():
+        setattr(a, key, v)
+    return a
+
+
+def check_products(log):
+    """What DMA stages lies within the 31-bit offsets of a tile: its rows (contraction-contiguous), or the rows of one
+    step (free-contiguous)."""
+    seen = 0
+    for kind, p in log:
+        if kind not in ('product', 'pair') or p['loader'] != DMA:
+            continue
+        tile, size = TILE[p['tile']], SIZE[p['type']]
+        step = 128 // size
+        rows_a = step if p['layout'] == KERNEL_GRAD else tile
+        rows_b = tile if p['layout'] == INPUT_GRAD else step
+        if not p['q8']:                           # 8-bit inputs go through registers
+            assert rows_a * p['lda'] * size < 2 ** 31, (kind, p)
+            assert p['lda'] * size % 16 == 0, (kind, p)
+        assert rows_b * p['ldb'] * size < 2 ** 31, (kind, p)
+        assert p['ldb'] * size % 16 == 0, (kind, p)
+        seen += 1
+    return seen
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32])
+def test_what_dma_stages_lies_within_its_offsets(plan, dtype):
+    """Contractions and layers longer than a DMA row may be: no copy of the same length either."""
+    for k in (4_194_248, 4_300_000, 4_300_001, 5_000_000, 6_000_000, 2_097_144, 2_200_000, 2_200_001, 20_000_000):
+        for m, n in ((1024, 1024), (512, 512), (70, 300), (3, 40)):
+            check_products(launches(plan, 'forward', forward(m, k, n, dtype)))
+    for n in (4_300_000, 4_300_001, 2_200_000, 2_200_003, 20_000_000, 20_000_003):
+        for m, k in ((1024, 1024), (300, 64), (64, 72), (33, 9)):
+            check_products(launches(plan, 'forward', forward(m, k, n, dtype)))
+            for act in (0, 1, 2):
+                for codes in (False, True):
+                    check_products(launches(plan, 'backward', backward(m, k, n, dtype, act, codes)))
+                    check_products(launches(plan, 'backward', backward(m, n, k, dtype, act, codes)))
+                    check_products(launches(plan, 'backward', backward(m, k, n, dtype, act, codes, dresidual=0x9000,
+                                                                       lddr=n)))
+    # long strides of short rows are copied to short ones, and small rows are staged as they lie
+    log = launches(plan, 'forward', forward(4096, 4096, 4096, dtype, ldx=30_000_000))
+    assert check_products(log) == 1 and any(kind == 'pad' for kind, _ in log)
+    assert check_products(launches(plan, 'forward', forward(4096, 4096, 4096, dtype))) == 1

@@ -512,6 +512,35 @@ def test_exponents_of_a_column_slice_of_a_wide_tensor(n, t):
         assert torch.equal(a, b)
 
 
+def signs(shape, seed):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    return torch.randint(0, 2, shape, device='cuda', generator=g, dtype=torch.int8).mul_(2).sub_(1)
+
+
+@pytest.mark.parametrize('t,length', [(BF16, 4_300_000), (BF16, 4_300_003), (F16, 6_000_000), (F32, 2_200_000)],
+                         ids=str)
+def test_rows_longer_than_dma_offsets(t, length):
+    """Rows of more than 2^23 bytes, as the contraction and as the layer's width.  Signs, so that every sum is exact in
+    fp32 whatever its order."""
+    from pet_posterior_distribution_amd import checkpoint_activations, dense, dense_backward
+    m, n = 300, 264
+    x, w = signs((m, length), 1).to(t), signs((length, n), 2).to(t)
+    y = x.float() @ w.float()
+    assert torch.equal(dense(x, w, out_dtype=F32), y)
+    dy = signs((m, n), 3).to(t)
+    for saved_x in (x, checkpoint_activations(x)):
+        g = dense_backward(dy, saved_x, w, grad_dtype=F32)
+        assert torch.equal(g.kernel, x.float().T @ dy.float()) and torch.equal(g.bias, dy.float().sum(0))
+        assert torch.equal(g.x, (dy.float() @ w.float().T).to(t))
+    # the same matrices as a layer of `length` units: dP is long
+    wide, keep, dz = w.T.contiguous(), x, signs((m, length), 4).to(t)
+    small = signs((m, n), 5).to(t)
+    dp = torch.where(keep > 0, dz, torch.zeros_like(dz)).float()
+    g = dense_backward(dz, small, wide, activation='relu', saved=keep, grad_dtype=F32)
+    assert torch.equal(g.x, (dp @ w.float()).to(t))
+    assert torch.equal(g.kernel, small.float().T @ dp) and torch.equal(g.bias, dp.sum(0))
+
+
 def test_one_row_of_more_columns_than_a_launch_has_threads():
     """2^27 columns: more than one launch of a kernel of 1024 threads for 32 columns could take.  Signs and whole
     numbers, so that every sum is exact in fp32 whatever its order."""
