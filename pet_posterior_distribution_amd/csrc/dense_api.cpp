@@ -399,6 +399,10 @@ struct BackwardPlan {
   double us;
 };
 
+// Column sums that a product's join may carry: 2^20 workgroups at most, in any of its grids.  More get a launch of
+// their own, whose workgroups walk.
+bool carried(int64_t n) { return n <= (int64_t)1 << 24; }
+
 // The products from operands that are in memory (lx, lk: their loaders; dp_dma: dP's beside 8-bit inputs): one launch
 // or two.
 double plan_products(const petdense_backward_args* a, int lx, int lk, bool dp_dma, BackwardPlan& b) {
@@ -410,7 +414,8 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, bool dp_dm
   if (a->dx) b.px = plan(a->m, a->k, a->n, a->dtype, lx);
   if (a->dkernel) b.pk = plan(a->k, a->n, a->m, a->dtype, lk);
   // a launch for the column sums, where no product's join carries them
-  const bool joins = b.sums && !(a->dx && b.px.splits > 1) && !(a->dkernel && b.pk.splits > 1);
+  const bool joins =
+      b.sums && !(carried(a->n) && ((a->dx && b.px.splits > 1) || (a->dkernel && b.pk.splits > 1)));
   double us = b.px.us + b.pk.us + (joins ? kLaunch : 0.0);
   if (a->dx && a->dkernel) {
     Plan px, pk;
@@ -665,7 +670,8 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
     if (b.pk.splits > 1) HIPC(join(p.k, ColumnJoin{}, a->dtype, s));
     return PETDIFF_OK;
   }
-  const bool with_x = a->dx && b.px.splits > 1, with_k = !with_x && a->dkernel && b.pk.splits > 1;
+  const bool with_x = carried(a->n) && a->dx && b.px.splits > 1;
+  const bool with_k = carried(a->n) && !with_x && a->dkernel && b.pk.splits > 1;
   if (b.sums && !with_x && !with_k) HIPC(join_columns(cols, s));
   const ColumnJoin none{};
   char* part = w + b.o_part;

@@ -297,7 +297,10 @@ hipError_t act_grad_t(const void* dy, int64_t ldy, const void* saved, int64_t ld
 
 __global__ __launch_bounds__(256) void join_columns_kernel(ColumnJoin p) {
   __shared__ float red[256];
-  join_columns16(p, blockIdx.x, threadIdx.x, red);
+  for (int64_t b = blockIdx.x; b * 16 < p.N; b += gridDim.x) {
+    join_columns16(p, (int)b, threadIdx.x, red);
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -494,7 +497,8 @@ hipError_t pad_t(const PadJobs& p, hipStream_t s) {
 hipError_t pad(const PadJobs& p, int type, hipStream_t s) { PETDENSE_BY_TYPE(type, return pad_t<T>(p, s)) }
 
 hipError_t join_columns(const ColumnJoin& c, hipStream_t s) {
-  return launch_kernel(join_columns_kernel, dim3(blocks_for(c.N, 16)), dim3(256), 0, s, c);
+  const unsigned blocks = std::min(blocks_for(c.N, 16), 1u << 20);      // (2^28 columns would be 2^32 threads)
+  return launch_kernel(join_columns_kernel, dim3(blocks), dim3(256), 0, s, c);
 }
 
 __global__ __launch_bounds__(256) void fill_zero_kernel(char* p, int64_t total, int n, int64_t ld, int size) {

@@ -121,3 +121,22 @@ def test_what_dma_stages_lies_within_its_offsets(plan, dtype):
     log = launches(plan, 'forward', forward(4096, 4096, 4096, dtype, ldx=30_000_000))
     assert check_products(log) == 1 and any(kind == 'pad' for kind, _ in log)
     assert check_products(launches(plan, 'forward', forward(4096, 4096, 4096, dtype))) == 1
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
+def test_column_sums_beside_a_join_leave_its_grid_in_bounds(plan, dtype):
+    """A grid holds fewer than 2^32 threads, and 65,535 workgroups in y; a join of column sums by itself walks."""
+    joined = 0
+    for m, k, n in ((1, 1, 2 ** 28 + 8), (1, 1, 2 ** 27), (1376, 228, 34_629_222), (4, 3, 2 ** 26), (300, 256, 2 ** 25),
+                    (2048, 256, 2 ** 24 + 64), (40, 48, 5000), (4096, 4096, 512)):
+        for act in (0, 1):
+            for kind, p in launches(plan, 'backward', backward(m, k, n, dtype, act)):
+                if kind == 'join':
+                    outputs = p['I'] * -(-p['J'] // 8) * (8 if p['splits'] > 2 else 1)
+                    assert (-(-p['N'] // 16) + -(-outputs // 256)) * 256 < 2 ** 32, (m, k, n, p)
+                elif kind == 'join_tiles':
+                    row = p['b'] * p['b'] // 8 // 256
+                    tiles = -(-p['I'] // p['b']) * -(-p['J'] // p['b']) - p['whole']
+                    assert -(-p['N'] // (16 * row)) + tiles <= 65535, (m, k, n, p)
+                joined += p.get('N') == n and kind in ('join', 'join_tiles', 'join_columns')
+    assert joined

@@ -556,6 +556,19 @@ def test_one_row_of_more_columns_than_a_launch_has_threads():
     assert torch.equal(g.x, (dy * w).sum(dtype=torch.float64).to(BF16).reshape(1, 1))
 
 
+def test_column_sums_of_more_columns_than_a_launch_of_their_own_takes():
+    """2^28 columns and more: sixteen to a workgroup of 256 threads, they would be 2^32 threads.  Whole numbers, so that
+    every sum is exact."""
+    from pet_posterior_distribution_amd import dense_backward
+    for m in (1, 3):
+        n = (1 << 28) + 8
+        w, dy = signs((1, n), 6).to(BF16), signs((m, n), 7).to(BF16)
+        x = torch.full((m, 1), 3.0, dtype=BF16, device='cuda')
+        g = dense_backward(dy, x, w)
+        assert torch.equal(g.bias, dy.float().sum(0).to(BF16)) and torch.equal(g.kernel, (3 * dy.float().sum(0, True)).to(BF16))
+        assert torch.equal(g.x, (dy.float() * w.float()).sum(1, True, dtype=torch.float64).to(BF16))
+
+
 # ------------------------------------------------------------------------------------------- streams and graphs
 def chain(x, ws, bs, dy):
     """Two layers forward, the first one's input kept in 8 bits, and their backward passes."""
