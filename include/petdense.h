@@ -22,7 +22,8 @@
  * graphs that may replay together).  Their sizes go by every argument, which outputs are asked for and the pointers'
  * alignment included: ask with the arguments of the call.  Row strides (ld*) are in values, at least the row's
  * length; rows do not overlap.  Outputs do not alias inputs, with one exception: y may be the residual itself.  Sums
- * are in a fixed order: results are the same from run to run.
+ * are in a fixed order: results are the same from run to run.  A call's y, dx and dkernel, where asked for, have fewer
+ * than 2^23 tiles of 64 x 64 values each (2^35 values).
  *
  * Every function returns a PETDIFF_* code (petdiff.h); petdense_last_error() names the last failure of the thread.
  */

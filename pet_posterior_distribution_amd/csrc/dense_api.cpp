@@ -257,6 +257,9 @@ bool work_ok(const void* w, size_t have, size_t need) {
   return need == 0 || (w && have >= need && reinterpret_cast<uintptr_t>(w) % kAlign == 0);
 }
 
+// a product's outputs: fewer than 2^23 tiles of 64 x 64
+bool outputs_fit(int64_t i, int64_t j) { return ceil_div(i, 64) * ceil_div(j, 64) < (int64_t)1 << 23; }
+
 // ---------------------------------------------------------------- forward
 int check_forward(const petdense_forward_args* a) {
   NEED(a, "null arguments");
@@ -273,7 +276,7 @@ int check_forward(const petdense_forward_args* a) {
        "outputs must not alias inputs");
   NEED(a->y != a->residual || (a->ldy == a->ldr && (!a->out_f32 || a->dtype == PETDENSE_F32)),
        "y may be the residual only with its stride and type");
-  NEED(ceil_div(a->m, 64) * ceil_div(a->n, 64) < (int64_t)1 << 23, "too many outputs in one call");
+  NEED(outputs_fit(a->m, a->n), "too many outputs in one call");
   return PETDIFF_OK;
 }
 
@@ -378,8 +381,7 @@ int check_backward(const petdense_backward_args* a) {
     for (const void* o : outs)
       NEED(!o || (o != a->dy && o != a->x && o != a->kernel && o != a->saved), "outputs must not alias inputs");
   }
-  NEED(ceil_div(a->m, 64) * ceil_div(a->k, 64) < (int64_t)1 << 23 &&
-           ceil_div(a->k, 64) * ceil_div(a->n, 64) < (int64_t)1 << 23,
+  NEED((!a->dx || outputs_fit(a->m, a->k)) && (!a->dkernel || outputs_fit(a->k, a->n)),
        "too many outputs in one call");
   return PETDIFF_OK;
 }

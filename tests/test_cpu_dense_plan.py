@@ -140,3 +140,27 @@ def test_column_sums_beside_a_join_leave_its_grid_in_bounds(plan, dtype):
                     assert -(-p['N'] // (16 * row)) + tiles <= 65535, (m, k, n, p)
                 joined += p.get('N') == n and kind in ('join', 'join_tiles', 'join_columns')
     assert joined
+
+
+def test_outputs_that_are_not_asked_for_do_not_limit_a_call(plan):
+    """2^23 tiles of 64 x 64 is the limit of an output that is asked for."""
+    tall = dict(m=2 ** 29 + 100, k=64, n=8)                       # x's gradient would be too large
+    assert launches(plan, 'backward', backward(**tall, dtype=BF16, dx=None))
+    wide = dict(m=8, k=2 ** 20, n=2 ** 16)                        # the kernel's gradient would be
+    assert launches(plan, 'backward', backward(**wide, dtype=BF16, dkernel=None))
+    assert launches(plan, 'backward', backward(m=2, k=2 ** 20, n=2 ** 31 - 2 ** 17, dtype=BF16, dx=None, dkernel=None))
+    for size, gone in ((tall, 'dkernel'), (wide, 'dx')):
+        a = backward(**size, dtype=BF16, **{gone: None})
+        assert plan.petdense_backward_workspace(C.byref(a)) == 0
+        assert plan.petdense_backward(C.byref(a), None, 0, None) == _lib.PETDIFF_ERR_INVALID
+        assert b'too many' in plan.petdense_last_error()
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
+def test_copies_fit_one_launch(plan, dtype):
+    """A copy's rows are filled up to whole pieces of 16 bytes: narrow rows move more than their values."""
+    for m, k, n in ((2 ** 31 - 2 ** 17, 1, 1), (1_600_000_000, 1, 9), (1_000_000_000, 9, 17), (600_000_000, 3, 5)):
+        for args in (backward(m, k, n, dtype, dx=None), backward(m, k, n, dtype, dx=None, codes=True)):
+            pieces = sum(p['rows'] * (p['ldd'] * SIZE[dtype] // 16)
+                         for kind, p in launches(plan, 'backward', args) if kind == 'pad')
+            assert pieces + 256 < 2 ** 32, (m, k, n, pieces)

@@ -569,6 +569,22 @@ def test_column_sums_of_more_columns_than_a_launch_of_their_own_takes():
         assert torch.equal(g.x, (dy.float() * w.float()).sum(1, True, dtype=torch.float64).to(BF16))
 
 
+def test_a_kernel_gradient_over_more_rows_than_an_input_gradient_may_have():
+    """2^29 rows: x's gradient would be more outputs than a call has; it is not asked for.  Signs: sums are exact."""
+    from pet_posterior_distribution_amd import checkpoint_activations, dense_backward
+    m, k, n = (1 << 29) + 100, 8, 8
+    x, dy, w = signs((m, k), 8).to(BF16), signs((m, n), 9).to(BF16), rand((k, n), BF16, 1)
+    ref, at = torch.zeros(k, n, dtype=torch.float64, device='cuda'), 1 << 24
+    for i in range(0, m, at):
+        ref += x[i:i + at].float().T @ dy[i:i + at].float()
+    for saved_x in (x, checkpoint_activations(x)):
+        g = dense_backward(dy, saved_x, w, need_x=False, grad_dtype=F32)
+        assert g.x is None and torch.equal(g.kernel.double(), ref)
+        assert torch.equal(g.bias.double(), dy.sum(0, dtype=torch.float64))
+    with pytest.raises(ValueError, match='too many'):
+        dense_backward(dy, x, w)
+
+
 # ------------------------------------------------------------------------------------------- streams and graphs
 def chain(x, ws, bs, dy):
     """Two layers forward, the first one's input kept in 8 bits, and their backward passes."""
