@@ -21,9 +21,9 @@
  * petdense_*_workspace bytes, 256-byte aligned, not shared by calls that may run at once (two streams, two captured
  * graphs that may replay together).  Their sizes go by every argument, which outputs are asked for and the pointers'
  * alignment included: ask with the arguments of the call.  Row strides (ld*) are in values, at least the row's
- * length; rows do not overlap.  Outputs do not alias inputs, with one exception: y may be the residual itself.  Sums
- * are in a fixed order: results are the same from run to run.  A call's y, dx and dkernel, where asked for, have fewer
- * than 2^23 tiles of 64 x 64 values each (2^35 values).
+ * length; rows do not overlap.  Outputs do not alias inputs or each other, with one exception: y may be the residual
+ * itself.  Sums are in a fixed order: results are the same from run to run.  A call's y, dx and dkernel, where asked
+ * for, have fewer than 2^23 tiles of 64 x 64 values each (2^35 values).
  *
  * Every function returns a PETDIFF_* code (petdiff.h); petdense_last_error() names the last failure of the thread.
  */
@@ -86,7 +86,8 @@ int petdense_forward(const petdense_forward_args* a, void* work, size_t work_byt
 size_t petdense_backward_workspace(const petdense_backward_args* a);
 int petdense_backward(const petdense_backward_args* a, void* work, size_t work_bytes, void* stream);
 
-/* x [m][k] of dtype (row stride ldx) -> codes [m][k] bytes (row stride ldc), exponents [m][ceil(k / 32)] (lde) */
+/* m >= 0, k >= 1, both < 2^31 - 65536.
+ * x [m][k] of dtype (row stride ldx) -> codes [m][k] bytes (row stride ldc), exponents [m][ceil(k / 32)] (lde) */
 int petdense_checkpoint(const void* x, int64_t ldx, int64_t m, int64_t k, int dtype, uint8_t* codes, int64_t ldc,
                         uint8_t* exponents, int64_t lde, void* stream);
 /* the values that the codes stand for, in dtype: exact, but that fp16 rounds what is below 2^-14.  Exponent bytes

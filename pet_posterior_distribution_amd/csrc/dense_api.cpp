@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 using namespace petdense_k;
@@ -257,6 +258,18 @@ bool work_ok(const void* w, size_t have, size_t need) {
   return need == 0 || (w && have >= need && reinterpret_cast<uintptr_t>(w) % kAlign == 0);
 }
 
+// No output that is given is an input or another output.
+bool apart(std::initializer_list<const void*> outputs, std::initializer_list<const void*> inputs) {
+  for (const void* const* o = outputs.begin(); o != outputs.end(); ++o) {
+    if (!*o) continue;
+    for (const void* i : inputs)
+      if (*o == i) return false;
+    for (const void* const* other = outputs.begin(); other != o; ++other)
+      if (*o == *other) return false;
+  }
+  return true;
+}
+
 // a product's outputs: fewer than 2^23 tiles of 64 x 64
 bool outputs_fit(int64_t i, int64_t j) { return ceil_div(i, 64) * ceil_div(j, 64) < (int64_t)1 << 23; }
 
@@ -272,8 +285,8 @@ int check_forward(const petdense_forward_args* a) {
   NEED(a->ldx >= a->k && a->ldk >= a->n && a->ldy >= a->n, "a row stride is shorter than its row");
   NEED(!a->residual || a->ldr >= a->n, "the residual's row stride is shorter than its row");
   NEED(!a->pre || a->ldp >= a->n, "the pre-activation's row stride is shorter than its row");
-  NEED(a->y != a->x && a->y != a->kernel && (!a->pre || (a->pre != a->y && a->pre != a->x)),
-       "outputs must not alias inputs");
+  NEED(apart({a->y, a->pre}, {a->x, a->kernel, a->bias}) && (!a->pre || a->pre != a->residual),
+       "outputs must not alias inputs, nor each other");
   NEED(a->y != a->residual || (a->ldy == a->ldr && (!a->out_f32 || a->dtype == PETDENSE_F32)),
        "y may be the residual only with its stride and type");
   NEED(outputs_fit(a->m, a->n), "too many outputs in one call");
@@ -377,9 +390,8 @@ int check_backward(const petdense_backward_args* a) {
     NEED(!a->dkernel || !a->x_exponents || a->lde >= ceil_div(a->k, PETDENSE_BLOCK),
          "the exponents' row stride is shorter than a row's blocks");
     NEED(!a->dresidual || a->lddr >= a->n, "dresidual's row stride is shorter than its row");
-    const void* outs[] = {a->dx, a->dkernel, a->dbias, a->dresidual};
-    for (const void* o : outs)
-      NEED(!o || (o != a->dy && o != a->x && o != a->kernel && o != a->saved), "outputs must not alias inputs");
+    NEED(apart({a->dx, a->dkernel, a->dbias, a->dresidual}, {a->dy, a->x, a->x_exponents, a->kernel, a->saved}),
+         "outputs must not alias inputs, nor each other");
   }
   NEED((!a->dx || outputs_fit(a->m, a->k)) && (!a->dkernel || outputs_fit(a->k, a->n)),
        "too many outputs in one call");
@@ -687,10 +699,11 @@ int petdense_backward(const petdense_backward_args* a, void* work, size_t work_b
 int petdense_checkpoint(const void* x, int64_t ldx, int64_t m, int64_t k, int dtype, uint8_t* codes, int64_t ldc,
                         uint8_t* exponents, int64_t lde, void* stream) {
   NEED(type_ok(dtype), "dtype must be PETDENSE_F32, PETDENSE_BF16 or PETDENSE_F16");
-  NEED(m >= 0 && k >= 1 && m < kMaxDim && k < kMaxDim, "m must be >= 0, k >= 1, both < 2^31 - 256");
+  NEED(m >= 0 && k >= 1 && m < kMaxDim && k < kMaxDim, "m must be >= 0, k >= 1, both < 2^31 - 65536");
   if (m == 0) return PETDIFF_OK;
   NEED(x && codes && exponents, "x, codes and exponents must be given");
   NEED(ldx >= k && ldc >= k && lde >= ceil_div(k, PETDENSE_BLOCK), "a row stride is shorter than its row");
+  NEED(apart({codes, exponents}, {x}), "outputs must not alias inputs, nor each other");
   HIPC(quantize(x, ldx, m, (int)k, dtype, codes, ldc, exponents, lde, (hipStream_t)stream));
   return PETDIFF_OK;
 }
@@ -698,10 +711,11 @@ int petdense_checkpoint(const void* x, int64_t ldx, int64_t m, int64_t k, int dt
 int petdense_restore(const uint8_t* codes, int64_t ldc, const uint8_t* exponents, int64_t lde, int64_t m, int64_t k,
                      int dtype, void* x, int64_t ldx, void* stream) {
   NEED(type_ok(dtype), "dtype must be PETDENSE_F32, PETDENSE_BF16 or PETDENSE_F16");
-  NEED(m >= 0 && k >= 1 && m < kMaxDim && k < kMaxDim, "m must be >= 0, k >= 1, both < 2^31 - 256");
+  NEED(m >= 0 && k >= 1 && m < kMaxDim && k < kMaxDim, "m must be >= 0, k >= 1, both < 2^31 - 65536");
   if (m == 0) return PETDIFF_OK;
   NEED(x && codes && exponents, "x, codes and exponents must be given");
   NEED(ldx >= k && ldc >= k && lde >= ceil_div(k, PETDENSE_BLOCK), "a row stride is shorter than its row");
+  NEED(apart({x}, {codes, exponents}), "outputs must not alias inputs");
   HIPC(restore(codes, ldc, exponents, lde, m, (int)k, dtype, x, ldx, (hipStream_t)stream));
   return PETDIFF_OK;
 }

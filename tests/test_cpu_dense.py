@@ -157,3 +157,41 @@ def test_training_precisions_are_checked():
         with pytest.raises(ValueError):
             check_precision(*bad)
     assert L.pettrain_set_precision(None, 0, 0) == INVALID and L.pettrain_step_bytes(None) == 0
+
+
+@pytest.mark.parametrize('kw', [
+    dict(y=0x9000, bias=0x9000), dict(pre=0x2000, ldp=32), dict(pre=0x9000, ldp=32, bias=0x9000),
+    dict(pre=0x9000, ldp=32, residual=0x9000, ldr=32), dict(pre=0x1000, ldp=32),
+])
+def test_forward_outputs_are_no_inputs(kw):
+    a = forward_args(**kw)
+    assert L.petdense_forward(C.byref(a), None, 0, None) == INVALID
+    assert 'alias' in L.petdense_last_error().decode()
+
+
+@pytest.mark.parametrize('kw', [
+    dict(dx=0x8000, x_exponents=0x8000, lde=2), dict(dkernel=0x8000, x_exponents=0x8000, lde=2),
+    dict(dresidual=0x5000, lddr=32), dict(dresidual=0x6000, lddr=32), dict(dbias=0x5000), dict(dbias=0x6000),
+    dict(dkernel=0x5000), dict(dbias=0x4000), dict(dx=0x3000),
+])
+def test_backward_outputs_are_no_inputs_and_differ(kw):
+    a = backward_args(**kw)
+    assert L.petdense_backward(C.byref(a), None, 0, None) == INVALID
+    assert 'alias' in L.petdense_last_error().decode()
+
+
+@pytest.mark.parametrize('x,codes,exps', [(0x1000, 0x1000, 0x3000), (0x1000, 0x2000, 0x1000), (0x1000, 0x2000, 0x2000)])
+def test_checkpoints_are_in_memory_of_their_own(x, codes, exps):
+    assert L.petdense_checkpoint(x, 100, 10, 100, 1, codes, 100, exps, 4, None) == INVALID
+    assert 'alias' in L.petdense_last_error().decode()
+    if codes != exps:                       # two inputs may be one
+        assert L.petdense_restore(codes, 100, exps, 4, 10, 100, 1, x, 100, None) == INVALID
+        assert 'alias' in L.petdense_last_error().decode()
+
+
+def test_the_largest_checkpoint_is_named():
+    for m, k in ((BIG, 8), (8, BIG), (2 ** 31 - 65535, 8)):
+        assert L.petdense_checkpoint(0x1000, BIG, m, k, 1, 0x2000, BIG, 0x3000, BIG, None) == INVALID
+        assert '2^31 - 65536' in L.petdense_last_error().decode()
+        assert L.petdense_restore(0x2000, BIG, 0x3000, BIG, m, k, 1, 0x1000, BIG, None) == INVALID
+        assert '2^31 - 65536' in L.petdense_last_error().decode()
