@@ -44,16 +44,10 @@ struct Product {
 // Rows of a tile are reached by 32-bit offsets from its first: 256 rows at most, each shorter than this.
 constexpr int64_t kMaxRowBytes = 0x7fffffff / 256;
 
-// Whether a step's pieces of 16 bytes may be read whole, at 32-bit offsets from the step's first value.  `left`: values
-// of the contraction from the step on, of `bc` a step; ld, ld2: bytes from row to row of the operand and of what is
-// read beside it; lde: of its exponent bytes (0: none).  Free-contiguous: a piece may run into the next row, which then
-// has to exist.
-__host__ __device__ inline bool whole_step(bool free, int left, int bc, int64_t ld, int64_t ld2, int64_t lde) {
-  return (free ? left > bc && ld >= 16 && ld2 >= 16 : left >= bc) && ld < kMaxRowBytes && ld2 < kMaxRowBytes &&
-         lde < kMaxRowBytes;
-}
+// Whether exponent bytes, `lde` from row to row, are reached by 32-bit offsets from a step's first.
+__host__ __device__ inline bool exponents_fit(int64_t lde) { return lde < kMaxRowBytes; }
 
-// Offset of the exponent byte of block `block` in row r of a whole step.
+// Offset of the exponent byte of block `block` in a step's row r.
 __host__ __device__ inline unsigned exponent_offset(int r, int64_t lde, int block) {
   return (unsigned)(r * (int)lde + block);
 }

@@ -148,7 +148,7 @@ struct Filler {
   const char* base;      // the tile's first value at contraction value 0 of this part
   int64_t ld;            // bytes from row to row
   int limit;             // free values of the tile that exist
-  bool brief;            // kReg: the operand's rows are shorter than a piece
+  bool brief;            // kReg: value by value: rows shorter than a piece, or exponents too far apart for its offsets
   int clen, kw;
   const uint8_t* exps;   // Q8: exponent byte of the tile's first block at the part's first row
   int64_t lde;
@@ -173,7 +173,7 @@ struct Filler {
   __device__ void init(const void* p, int64_t ld_values, int f0, int f_limit, int64_t c0, int clen_, int c_all,
                        const uint8_t* ex, int64_t lde_, int kw_, int tid) {
     kw = kw_;
-    brief = (FREE ? f_limit : c_all) < S::EPC;
+    brief = (FREE ? f_limit : c_all) < S::EPC || (Q8 && !exponents_fit(lde_));
     constexpr int SZ = Q8 ? 1 : (int)sizeof(T);
     ld = ld_values * SZ;
     base = static_cast<const char*>(p) + (FREE ? c0 * ld + (int64_t)f0 * SZ : f0 * ld + c0 * SZ);
@@ -209,7 +209,10 @@ struct Filler {
     u.left = clen - u.t * BC;
     u.p = base + (FREE ? (int64_t)u.t * BC * ld : (int64_t)u.t * BC * (int64_t)sizeof(T));
     if constexpr (ACT) u.p2 = base2 + (FREE ? (int64_t)u.t * BC * ld2 : (int64_t)u.t * BC * (int64_t)sizeof(T));
-    u.whole = !brief && whole_step(FREE, u.left, BC, ld, ACT ? ld2 : ld, Q8 ? lde : 0);
+    // free-contiguous: 16 bytes from a piece's first value may run into the next row, which then has to exist
+    // (offsets within a step fit 31 bits)
+    u.whole = !brief && (FREE ? u.left > BC && ld >= 16 : u.left >= BC) && ld < kMaxRowBytes &&
+              (!ACT || ((!FREE || ld2 >= 16) && ld2 < kMaxRowBytes));
     if constexpr (LOADER == kDma) {
       const unsigned long long a = reinterpret_cast<unsigned long long>(u.p);
       u.rs[0] = __builtin_amdgcn_readfirstlane((int)(a & 0xffffffffull));
@@ -236,7 +239,7 @@ struct Filler {
   //    stored);
   //  - cut steps: a piece that ends past its row is read so that it ends with it, and shifted; what does not exist
   //    becomes zero;
-  //  - rows shorter than a piece: value by value.
+  //  - `brief`: value by value, by 64-bit offsets.
   __device__ __forceinline__ void begin_reg(const Step& u, int tid) {
     if constexpr (LOADER == kReg) {
       constexpr int SZ = Q8 ? 1 : (int)sizeof(T), PB = SZ * S::EPC;        // bytes of a value and a piece in memory

@@ -88,8 +88,6 @@ hipError_t restore(const uint8_t*, int64_t, const uint8_t*, int64_t, int64_t M, 
 extern "C" {
 const char* plan_log() { return g_log.c_str(); }
 void plan_clear() { g_log.clear(); }
-int plan_whole_step(int free, int left, int bc, int64_t ld, int64_t ld2, int64_t lde) {
-  return petdense_k::whole_step(free, left, bc, ld, ld2, lde);
-}
+int plan_exponents_fit(int64_t lde) { return petdense_k::exponents_fit(lde); }
 uint64_t plan_exponent_offset(int r, int64_t lde, int block) { return petdense_k::exponent_offset(r, lde, block); }
 }
