@@ -26,24 +26,33 @@ __device__ __forceinline__ void run_of(int n, int x, int& first, int& len) {
   len = per + (x < rest ? 1 : 0);
 }
 
-// Phi(x) = (1 + erf(x / sqrt 2)) / 2.
-// 16-bit outputs: 1 / (1 + 2^(-x P(x^2))), P of degree 6: the least largest error of x Phi(x) over |x| <= 6 (a linear
-// program over log2(Phi / (1 - Phi)) / x), 7e-8 there and less beyond, 1.8e-7 of Phi with its fp32 steps; beside the
-// 2^-9 and 2^-12 of a rounded output.  A third of erff's instructions, and the epilogue pays them once per output.
-// P >= 2.3 everywhere, so that both tails end in 0 and 1.
+// Phi(x) = erfc(-x / sqrt 2) / 2: right relative to itself in the lower tail too, where 1 + erf would cancel (5 % off at
+// x = -4.9).
+// 16-bit outputs: Phi(-a) = e^(-a^2/2) t P(t) with t = 1 / (1 + 0.35 a), a = |x|, and Phi(a) = 1 - Phi(-a).  P of degree
+// 6 has the least largest error beside min(1e-7, 1e-5 Phi) over a <= 14 (a linear program over Phi(-a) e^(a^2/2)): 4e-8
+// absolute and 4e-6 relative, 2.1e-7 and 2^-16 with its fp32 steps (the exponent's roundings are a^2 2^-24 of the
+// value), beside the 2^-9 and 2^-12 of an output that is rounded to 16 bits.  About half of erfcf's instructions, and
+// the epilogue pays them once per output.  The gradient needs the exponential as well (`e`).
+__device__ __forceinline__ float normal_cdf_fast(float x, float& e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, fabsf(x), 1.0f));
+  e = __builtin_amdgcn_exp2f(x * x * -0.72134752f);
+  float p = fmaf(0.0446154723f, t, -0.184429168f);
+  p = fmaf(p, t, 0.211082418f);
+  p = fmaf(p, t, 0.0089271389f);
+  p = fmaf(p, t, 0.143156413f);
+  p = fmaf(p, t, 0.136871306f);
+  p = fmaf(p, t, 0.139776456f);
+  const float q = p * t * e;
+  return x < 0.f ? q : 1.0f - q;
+}
+
 template <bool EXACT>
 __device__ __forceinline__ float normal_cdf(float x) {
   if constexpr (EXACT) {
-    return 0.5f * (1.0f + erff(x * 0.70710678118654752f));
+    return 0.5f * erfcf(x * -0.70710678118654752f);
   } else {
-    const float u = x * x;
-    float p = fmaf(5.20990380e-09f, u, -3.85044763e-07f);
-    p = fmaf(p, u, 1.14524259e-05f);
-    p = fmaf(p, u, -1.59389380e-04f);
-    p = fmaf(p, u, -9.55930483e-05f);
-    p = fmaf(p, u, 1.04838581e-01f);
-    p = fmaf(p, u, 2.30220720f);
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * p));
+    float e;
+    return normal_cdf_fast(x, e);
   }
 }
 
@@ -66,8 +75,14 @@ template <bool EXACT>
 __device__ __forceinline__ float activate_grad(float g, float v, int act) {
   if (act == kRelu) return v <= 0.f ? 0.f : g;
   if (act == kGelu) {
-    const float pdf = 0.39894228040143268f * (EXACT ? expf(-0.5f * v * v) : __expf(-0.5f * v * v));
-    return g * fmaf(v, pdf, normal_cdf<EXACT>(v));
+    float cdf, e;
+    if constexpr (EXACT) {
+      cdf = normal_cdf<true>(v);
+      e = expf(-0.5f * v * v);
+    } else {
+      cdf = normal_cdf_fast(v, e);
+    }
+    return g * fmaf(v, 0.39894228040143268f * e, cdf);
   }
   if (act == kSilu) {
     const float s = sigmoid<EXACT>(v);

@@ -368,6 +368,36 @@ def test_rows_between_and_behind_the_outputs_are_left_as_they_were():
             close(gb[:n], ref[2], tol[2], 'dbias')
 
 
+@pytest.mark.parametrize('t,out', [(BF16, BF16), (F16, F16), (BF16, F32), (F16, F32), (F32, F32)], ids=str)
+def test_the_lower_tail_of_gelu(t, out):
+    """x Phi(x) from -3 down to where the type ends, relative to itself.
+    fp32: the argument x / sqrt 2 is off by 2^-24 and 2^-25 of itself, which is x^2 times as much of Phi; the
+    complementary error function and the two products after it by less than 8 2^-23.
+    16-bit layers: Phi is off by 2^-16 of itself (the fit 4e-6, the exponent's two roundings x^2 2^-24, 1e-5 at -13)."""
+    from pet_posterior_distribution_amd import dense, dense_backward
+    v = torch.linspace(-13, -3, 8000, device='cuda').to(t)
+    one = torch.ones(1, 8, dtype=t, device='cuda')
+    v6 = v.double()
+    cdf = 0.5 * torch.special.erfc(-v6 * 0.5 ** 0.5)             # (torch's ndtr cancels below -7, in 64 bits too)
+    ref, pdf = v6 * cdf, torch.exp(-v6 * v6 / 2) / (2 * torch.pi) ** 0.5
+    off = (v6 * v6 + 8) * E23 if t == F32 else torch.full_like(v6, 2.0 ** -16)
+
+    def same(got, want, tol, what):
+        tol = tol + half_step(got.dtype) * (want.abs() + tol) + (2.0 ** -25 if got.dtype == F16 else 1e-37)
+        worst = ((got.double() - want).abs() / tol).max().item()
+        assert worst <= 1.0, f'{what}: {worst:.3g} of its tolerance'
+
+    y = dense(v[:, None], one, activation='gelu', out_dtype=out)                        # a tile's epilogue
+    for j in (0, 7):
+        same(y[:, j], ref, off * ref.abs(), 'tiles')
+    y = dense(one[:, :1].expand(2, 1), v[None], activation='gelu', out_dtype=out)        # few rows
+    same(y[1], ref, off * ref.abs(), 'rows')
+    if out == t:
+        g = dense_backward(torch.ones(8000, 1, dtype=t, device='cuda'), v[:, None], one[:, :1], activation='gelu',
+                           saved=v[:, None], need_residual=True)
+        same(g.residual[:, 0], cdf + v6 * pdf, 2 * off * (cdf + v6.abs() * pdf), 'gradient')
+
+
 # ---------------------------------------------------------------------------------------------------- checkpoints
 def power(e):
     """2^e in 64 bits, exactly (torch.exp2 and torch.ldexp of 64-bit GPU tensors may be off by a bit)."""
