@@ -733,11 +733,18 @@ int pettrain_set_precision(pettrain_handle h, int precision, int keep) {
     return fail(PETDIFF_ERR_INVALID, "8-bit checkpoints need PETTRAIN_BF16");
   if (precision == h->precision && keep == h->keep) return PETDIFF_OK;
   HIPC(hipSetDevice(h->device));
-  for (int d = 0; d < 4; ++d) h->A_dn[d].release();
-  for (int u = 0; u < 3; ++u) {
-    h->A_uc[u].release();
-    h->A_bk[u].release();
-  }
+  const auto release = [](Buf* b, size_t count) {
+    for (size_t i = 0; i < count; ++i) b[i].release();
+  };
+  // what one of the precisions alone holds
+  release(h->A_dn, 4);
+  release(h->A_uc, 3);
+  release(h->A_bk, 3);
+  release(h->w16, 10);
+  release(h->b16, 10);
+  release(h->we16, 4);
+  release(h->e16, 4);
+  release(h->de16, 4);
   for (Kept* k = h->in16; k != h->in16 + 10; ++k) {
     k->rows.release();
     k->exps.release();
@@ -746,7 +753,9 @@ int pettrain_set_precision(pettrain_handle h, int precision, int keep) {
     k->rows.release();
     k->exps.release();
   }
-  for (Buf* b : {&h->cond_aug, &h->e1, &h->e2, &h->e3, &h->de1, &h->de2, &h->de3, &h->dA, &h->dpre, &h->a16, &h->da16, &h->dp16, &h->gk16, &h->work16}) b->release();
+  for (Buf* b : {&h->cond_aug, &h->e1, &h->e2, &h->e3, &h->de1, &h->de2, &h->de3, &h->dA, &h->dpre, &h->a16, &h->da16,
+                 &h->dp16, &h->gk16, &h->work16})
+    b->release();
   h->B_cap = 0;                 // the next step allocates what its precision needs
   h->precision = precision;
   h->keep = keep;

@@ -77,6 +77,26 @@ def test_less_memory():
     assert held[2] < held[1] < held[0], held
 
 
+def test_a_change_of_precision_frees_what_the_other_one_held():
+    from pet_posterior_distribution_amd import _lib
+    L = _lib.lib()
+    data = batch(B=16, seed=6)
+    kinds = [('float32', None), ('bfloat16', None), ('bfloat16', 'e4m3')]
+    code = {kinds[0]: (0, 0), kinds[1]: (1, 0), kinds[2]: (1, 1)}
+    held = {}
+    for kind in kinds:
+        m, tr = trainer(*kind)
+        gradients(m, tr, data)
+        held[kind] = tr.step_bytes
+    for before in kinds:
+        for after in kinds:
+            m, tr = trainer(*before)
+            gradients(m, tr, data)
+            assert L.pettrain_set_precision(tr.handle, *code[after]) == 0
+            gradients(m, tr, data)
+            assert tr.step_bytes == held[after], (before, after)
+
+
 def test_runs_repeat_and_batches_may_change():
     """Growing and shrinking batches: the buffers and the workspace follow, and results do not depend on what ran
     before."""
