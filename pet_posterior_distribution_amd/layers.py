@@ -10,7 +10,8 @@ products (exact for ReLU and linear layers); the bias gradient sums it unrounded
 
 Tensors may have any leading dimensions and row stride; a tensor whose rows are not contiguous is copied first.
 No call synchronises, so each can be captured into a graph.  Autograd does not record them: the gradients are
-``dense_backward``'s.
+``dense_backward``'s.  Where an input of ``dense`` requires a gradient, a backward pass through its result raises
+RuntimeError; what ``dense_backward`` and checkpoints return has no history.
 
 ================================================  =============================================
 reference (file:line)                             here
@@ -115,6 +116,25 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
+class _Unrecorded(torch.autograd.Function):
+    """Outputs whose backward pass is refused.  The node hangs on a tensor of its own, not on the call's inputs, so it
+    keeps nothing of theirs alive."""
+
+    @staticmethod
+    def forward(ctx, root, *outputs):
+        ctx.mark_dirty(*outputs)
+        return outputs
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError('dense is not recorded by autograd: take its gradients from dense_backward '
+                           '(or call it under torch.no_grad())')
+
+
+def _unrecorded(*outputs):
+    return _Unrecorded.apply(torch.empty(0, requires_grad=True), *outputs)
+
+
 def _new(shape, dtype, dev):
     """torch.empty; with strides given torch takes 0.4 us less, of which a small call would notice every one."""
     if len(shape) == 2:
@@ -181,6 +201,9 @@ def dense(x, kernel, bias=None, activation=None, residual=None, return_preactiva
     if bias is not None:
         bias_f32 = isinstance(bias, torch.Tensor) and bias.dtype == torch.float32
         bias, _ = _operand(bias, (n,), torch.float32 if bias_f32 else t, dev, 'bias')
+    dropped = torch.is_grad_enabled() and (x.requires_grad or kernel.requires_grad or
+                                           bias is not None and bias.requires_grad or
+                                           isinstance(residual, torch.Tensor) and residual.requires_grad)
     x, ldx = _rows(x)
     kernel, ldk = _operand(kernel, (k, n), t, dev, 'kernel')
     ldr = 0
@@ -192,6 +215,8 @@ def dense(x, kernel, bias=None, activation=None, residual=None, return_preactiva
     _run(L.petdense_forward, L.petdense_forward_workspace, _FORWARD.pack(
         x.data_ptr(), kernel.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(pre), ldx, ldk, ldr, n, n,
         y.numel() // n, k, n, dt, act, bias_f32, out_dtype == torch.float32), dev, 'dense')
+    if dropped:
+        y, pre = _unrecorded(y, pre) if pre is not None else (_unrecorded(y)[0], None)
     return (y, pre) if return_preactivation else y
 
 

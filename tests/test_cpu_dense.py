@@ -195,3 +195,16 @@ def test_the_largest_checkpoint_is_named():
         assert '2^31 - 65536' in L.petdense_last_error().decode()
         assert L.petdense_restore(0x2000, BIG, 0x3000, BIG, m, k, 1, 0x1000, BIG, None) == INVALID
         assert '2^31 - 65536' in L.petdense_last_error().decode()
+
+
+def test_a_gradient_through_an_output_is_refused():
+    """Autograd does not record the layer: backward says so instead of leaving gradients out."""
+    leaf = torch.ones(3, requires_grad=True)
+    y, pre = layers._unrecorded(torch.zeros(3), torch.zeros(3))
+    for out in (y, pre):
+        with pytest.raises(RuntimeError, match='dense_backward'):
+            (out * leaf).sum().backward()
+    y = layers._unrecorded(torch.zeros(3))[0]
+    y.mul_(2)                                           # written to like any other result
+    dy, = torch.autograd.grad((y * leaf).sum(), y)      # what dense_backward takes
+    assert torch.equal(dy, torch.ones(3)) and y.detach().numpy().shape == (3,)

@@ -334,6 +334,27 @@ def test_only_what_is_asked_for():
         assert torch.equal(g[i], full[i])
 
 
+def test_gradients_are_refused_where_autograd_would_drop_them():
+    from pet_posterior_distribution_amd import dense, dense_backward
+    x, w, b, r, dy = inputs(130, 72, 40, BF16)
+    plain = dense(x, w, b, activation='gelu', residual=r, return_preactivation=True)
+    for i, t in enumerate((x, w, b, r)):
+        t.requires_grad_()
+        y, pre = dense(x, w, b, activation='gelu', residual=r, return_preactivation=True)
+        assert torch.equal(y, plain[0]) and torch.equal(pre, plain[1])
+        with pytest.raises(RuntimeError, match='dense_backward'):
+            y.float().sum().backward()
+        assert t.grad is None
+        # the gradient with respect to the output is what dense_backward takes; its own results have no history
+        g, = torch.autograd.grad((y.float() * dy.float()).sum(), y)
+        got = dense_backward(g, x, w, activation='gelu', saved=pre, need_residual=True)
+        assert not any(v.requires_grad for v in got)
+        with torch.no_grad():
+            assert not dense(x, w, b, residual=r).requires_grad
+        t.requires_grad_(False)
+    assert not dense(x, w, b, residual=r).requires_grad
+
+
 def test_rows_between_and_behind_the_outputs_are_left_as_they_were():
     """C entry with output strides wider than the rows, and spare rows behind them."""
     from pet_posterior_distribution_amd import _lib
