@@ -185,7 +185,8 @@ def dense(x, kernel, bias=None, activation=None, residual=None, return_preactiva
 
     x (..., k), kernel (k, n), bias (n,) of x's type or float32, residual (..., n); activation None, 'relu', 'gelu'
     (erf) or 'silu'.  ``out_dtype``: x's type (default) or float32.  With ``return_preactivation`` also returns the
-    value before the activation, in the output's type (what ``dense_backward`` wants saved for GELU and SiLU)."""
+    value before the activation, in the output's type: what ``dense_backward`` wants saved for GELU and SiLU.  (It
+    wants it in the layer's type: cast the float32 outputs of a 16-bit layer, and their gradient, to x's.)"""
     dt, dev = _lead(x, 'x')
     t = x.dtype
     shape = x.shape
@@ -226,8 +227,9 @@ def dense_backward(dy, x, kernel, activation=None, saved=None, need_x=True, need
 
     x: the layer's input (..., k), or its ``ActivationCheckpoint``.  saved (..., n): the pre-activation for 'gelu' and
     'silu', the pre-activation or the output for 'relu', of dy's type.  ``grad_dtype``: type of the kernel's and the
-    bias's gradients, dy's (default) or float32; dx and the residual's gradient have dy's type.  Returns
-    ``DenseGradients``."""
+    bias's gradients, dy's (default) or float32; dx and the residual's gradient have dy's type.  It is the type that
+    their sums are rounded to: a 16-bit layer's products take a pre-activation's gradient of 16 bits either way.
+    Returns ``DenseGradients``."""
     dt, dev = _lead(dy, 'dy')
     t = dy.dtype
     shape = dy.shape

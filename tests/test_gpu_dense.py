@@ -181,6 +181,19 @@ def test_forward_fp32_outputs_and_bias(t):
     check_forward(x[:3], w, b.float() * 1.001, 'gelu', r[:3], True, out_dtype=F32)
 
 
+@pytest.mark.parametrize('t', [BF16, F16], ids=str)
+def test_the_backward_pass_of_fp32_outputs_is_the_layers(t):
+    """A 16-bit layer's backward pass takes dy and saved in its own type, whatever its outputs had."""
+    from pet_posterior_distribution_amd import dense, dense_backward
+    x, w, b, _, _ = inputs(150, 96, 72, t)
+    dy = rand((150, 72), F32, 9)
+    _, pre = dense(x, w, b, activation='gelu', return_preactivation=True, out_dtype=F32)
+    for bad in (dict(dy=dy, saved=pre), dict(dy=dy.to(t), saved=pre)):
+        with pytest.raises(ValueError, match='must be'):
+            dense_backward(bad['dy'], x, w, activation='gelu', saved=bad['saved'])
+    check_backward(dy.to(t), x, w, 'gelu', pre.to(t), grad_dtype=F32)
+
+
 @pytest.mark.parametrize('t', TYPES, ids=str)
 @pytest.mark.parametrize('m,k,n', SHAPES + WIDE)
 def test_backward(m, k, n, t):
