@@ -14,7 +14,9 @@
  * Types: x, kernel, residual, dy and saved are of one type, PETDENSE_F32 / BF16 / F16.  Sums run in fp32 (fp32
  * products on the fp32 matrix instructions) and every output is rounded once.  In the backward pass of a 16-bit
  * layer dP is rounded to the layer's type before the two products, which take 16-bit operands; db sums the
- * unrounded dP.  ReLU and linear layers' dP are exact.
+ * unrounded dP.  ReLU and linear layers' dP are exact; the others' products carry its rounding, into an fp32 dkernel
+ * too.  GELU and SiLU are evaluated to 2^-16 of themselves in 16-bit layers, to (x^2 + 8) 2^-23 in fp32 ones, lower
+ * tails included.  ReLU's gradient where saved is NaN is dy.
  *
  * All pointers are device memory of the current device and belong to the caller; work runs on `stream`, in order,
  * with no synchronisation and no allocation, so every call can be captured into a graph.  Workspaces: at least

@@ -77,9 +77,11 @@ void pettrain_destroy(pettrain_handle h);
  *                  activations between layers, weights, gradients and Adam stay fp32.
  * keep: what a bf16 step holds of every product's input between its forward and backward passes: PETTRAIN_KEEP the
  * bf16 values, PETTRAIN_KEEP_E4M3 8-bit checkpoints (8.25 bits a value; the products' kernel gradients are those of
- * the restored inputs, everything else is unchanged).  When it changes anything it frees the buffers that only the
- * old precision needs; the caller's stream must be idle then.  PETDIFF_ERR_INVALID: unknown values, or e4m3 without
- * bf16. */
+ * the restored inputs, everything else is unchanged).  The gradient of a convolution's pre-activation is rounded to
+ * bf16, and its bias gradient sums the rounded values.  The condition encoder's bf16 activations (49 KB a sample)
+ * stay beside their checkpoints: they are the backward pass's ReLU masks.
+ * When it changes anything it frees the buffers that only the old precision needs; the caller's stream must be idle
+ * then.  PETDIFF_ERR_INVALID: unknown values, or e4m3 without bf16. */
 int pettrain_set_precision(pettrain_handle h, int precision, int keep);
 /* Device bytes the step holds for a batch of B samples at most so far: activations, gradients, workspaces. */
 size_t pettrain_step_bytes(pettrain_handle h);

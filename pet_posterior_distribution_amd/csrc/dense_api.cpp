@@ -72,7 +72,8 @@ constexpr double kNever = 1e30;      // no plan
 constexpr double kLaunch = 3.5;      // a launch behind another, here and on the host
 constexpr double kWorkspace = 2.0;   // a small call that needs a workspace: the host's time for it
 // The host's time for a call is longer than a small one's on the device: from Python 4 us forward, 8 us backward (its
-// outputs), and 3.2 us a launch.
+// outputs), and 3.2 us a launch.  C callers and captured graphs spend less there and get the same plan: it goes by the
+// arguments alone, so that a call has the same bits wherever it comes from.
 constexpr double kHostForward = 4.0, kHostBackward = 8.0, kHostLaunch = 3.2;
 
 // A call's price when calls follow each other: what is longer, the device's time or the host's (and a little for the
@@ -482,8 +483,9 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
       b.make_dp || b.sums ? kLaunch + 2.0 + (double)a->m * a->n * sz * (b.make_dp ? 3 : 1) / 4e6 : 0.0;
 
   // dp in the workspace has rows of whole pieces, with zeros: DMA takes it as it is
-  const bool dp_ok =
-      own_dp ? row_fits(ld_dp, sz) : (a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz) : dma_ok(a->dy, a->lddy, a->n, sz));
+  const bool dp_ok = own_dp         ? row_fits(ld_dp, sz)
+                     : a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz)
+                                    : dma_ok(a->dy, a->lddy, a->n, sz);
   const bool w_ok = !a->dx || dma_ok(a->kernel, a->ldk, a->n, sz);
   const bool x_ok = !a->dkernel || (q8 ? a->k * sz % 16 == 0 : dma_ok(a->x, a->ldx, a->k, sz));
   // (8-bit inputs go through registers whatever their alignment: their loader is dp's)

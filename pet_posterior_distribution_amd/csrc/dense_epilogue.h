@@ -26,13 +26,14 @@ __device__ __forceinline__ void run_of(int n, int x, int& first, int& len) {
   len = per + (x < rest ? 1 : 0);
 }
 
-// Phi(x) = erfc(-x / sqrt 2) / 2: right relative to itself in the lower tail too, where 1 + erf would cancel (5 % off at
-// x = -4.9).
-// 16-bit outputs: Phi(-a) = e^(-a^2/2) t P(t) with t = 1 / (1 + 0.35 a), a = |x|, and Phi(a) = 1 - Phi(-a).  P of degree
-// 6 has the least largest error beside min(1e-7, 1e-5 Phi) over a <= 14 (a linear program over Phi(-a) e^(a^2/2)): 4e-8
-// absolute and 4e-6 relative, 2.1e-7 and 2^-16 with its fp32 steps (the exponent's roundings are a^2 2^-24 of the
-// value), beside the 2^-9 and 2^-12 of an output that is rounded to 16 bits.  About half of erfcf's instructions, and
-// the epilogue pays them once per output.  The gradient needs the exponential as well (`e`).
+// Phi(x) = erfc(-x / sqrt 2) / 2: right relative to itself in the lower tail too, where 1 + erf would cancel (5 % off
+// at x = -4.9).
+// 16-bit outputs: Phi(-a) = e^(-a^2/2) t P(t) with t = 1 / (1 + 0.35 a), a = |x|, and Phi(a) = 1 - Phi(-a).  P of
+// degree 6 has the least largest error beside min(1e-7, 1e-5 Phi) over a <= 14 (a linear program over
+// Phi(-a) e^(a^2/2)): 4e-8 absolute and 4e-6 relative, 2.1e-7 and 2^-16 with its fp32 steps (the exponent's roundings
+// are a^2 2^-24 of the value), beside the 2^-9 and 2^-12 of an output that is rounded to 16 bits.  A third of the
+// instructions that erfcf takes (17 of 51), and the epilogue pays them once per output.  The gradient needs the
+// exponential as well (`e`).
 __device__ __forceinline__ float normal_cdf_fast(float x, float& e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, fabsf(x), 1.0f));
   e = __builtin_amdgcn_exp2f(x * x * -0.72134752f);

@@ -23,10 +23,11 @@
 //
 // What bounds it, and what it measured (the library's product of the same operands in brackets, no epilogue):
 //  - large products by the matrix units at the clock that power leaves: 8192 x 4096 x 8192 bf16 in 424 us, 1.30 PFLOP/s
-//    (423 us), its input gradient 405 us, its kernel gradient 412 us; matrix instructions in 66 % of the busy cycles,
-//    no LDS bank conflict; fp32 83 % (its matrix instructions take as many cycles for a sixteenth of the work);
+//    (412 .. 423 us), its input gradient 405 us, its kernel gradient 412 us; matrix instructions in 66 % of the busy
+//    cycles, no LDS bank conflict; fp32 83 % (its matrix instructions take as many cycles for a sixteenth of the work),
+//    76 % with 64 x 64 tiles (6144 x 1836 x 512, 103 us);
 //  - short contractions by the tile's first loads and its stores: input gradient of 12288 x 6144 x 512 in 103 us
-//    (119 us), where its operations alone take 59 us and its stores 30 us;
+//    (115 .. 122 us), where its operations alone take 59 us and its stores 30 us;
 //  - few outputs by latency: 9 x 600 x 5000 in 4.2 us, 40 x 4100 x 64 in 4.9 us and 4.0 us for the join.
 #pragma once
 #include "dense_epilogue.h"
@@ -428,8 +429,8 @@ __device__ __forceinline__ void place_of(int b, int ti, int tj, int splits, int&
 // 16 rows at a time turn through LDS of the wave's own (16-byte piece c of row r at place c ^ r), so that a lane gets
 // eight neighbouring outputs of a row and neighbouring lanes fill whole cache lines.  (Two swaps between rows of 16
 // lanes give a lane its eight outputs without LDS, but neighbouring lanes then belong to different rows: 50176 x 256 x
-// 128 took 21.5 us, not 13.2.)  A lane keeps its columns, so the bias is read once: 8192 x 4096 x 8192 with GELU and
-// the pre-activation 465 us, 479 with a read for every 8 rows.
+// 128 took 21.5 us, not 13.2.)  A lane keeps its columns, so the bias is read once: a read for every 8 rows took
+// 14 us more of 8192 x 4096 x 8192 with GELU and the pre-activation (460 us).
 template <typename T, int FI, int FJ>
 __device__ __forceinline__ void store_tile(const Epilogue& e, const f32x4 (&acc)[FI][FJ], int i, int j, int rows,
                                            int cols, int lane, char* own) {

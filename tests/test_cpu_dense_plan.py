@@ -67,8 +67,8 @@ def launches(plan, name, args):
 
 
 def forward(m, k, n, dtype, ldx=None, ldk=None, **kw):
-    a = _lib.PetdenseForwardArgs(0x1000, 0x2000, 0x3000, None, 0x4000, None, ldx or k, ldk or n, 0, n, 0, m, k, n, dtype,
-                                 0, 0, 0)
+    a = _lib.PetdenseForwardArgs(0x1000, 0x2000, 0x3000, None, 0x4000, None, ldx or k, ldk or n, 0, n, 0, m, k, n,
+                                 dtype, 0, 0, 0)
     for key, v in kw.items():
         setattr(a, key, v)
     return a
