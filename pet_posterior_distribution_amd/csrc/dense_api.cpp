@@ -221,11 +221,16 @@ double unsplit_us(int tile, int64_t I, int64_t J, int64_t C, int type, int loade
 
 int64_t padded(int64_t n, int size) { return ceil_div(n, 16 / size) * (16 / size); }
 
-// A tile's rows, `ld` values apart, lie within the offsets that DMA has.
-bool row_fits(int64_t ld, int size) { return ld < kMaxRowBytes / size; }
+// How an operand lies: DMA stages a whole tile's rows of it, or (free-contiguous) the rows of one step.
+enum Lie { kAlongC, kAlongFree };
+
+// These rows, `ld` values apart, lie within the 31-bit offsets that DMA has.
+bool row_fits(int64_t ld, int size, Lie lie) {
+  return ld < (lie == kAlongC ? kMaxRowBytes : 0x7fffffff / (128 / size)) / size;
+}
 
 bool dma_ok(const void* p, int64_t ld, int64_t contiguous, int size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row_fits(ld, size) && (ld * size) % 16 == 0 &&
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row_fits(ld, size, kAlongC) && (ld * size) % 16 == 0 &&
          (contiguous * size) % 16 == 0;
 }
 
@@ -301,14 +306,11 @@ struct Copy {
   int64_t ld = 0;
 };
 
-// Pieces of 16 bytes that the copy of an operand moves, or kNoCopy where its rows would be too long for DMA even so.
-// One launch copies at most kMaxPieces.
-constexpr int64_t kMaxPieces = (int64_t)1 << 31, kNoCopy = kMaxPieces;
-int64_t pieces_of(bool on, int64_t rows, int64_t n, int size) {
-  if (!on) return 0;
-  const int64_t ld = padded(n, size);
-  return row_fits(ld, size) ? std::min(kNoCopy, rows * (ld * size / 16)) : kNoCopy;
-}
+// Pieces of 16 bytes that the copy of an operand moves.  One launch copies fewer than kMaxPieces.
+constexpr int64_t kMaxPieces = (int64_t)1 << 31;
+int64_t pieces_of(bool on, int64_t rows, int64_t n, int size) { return on ? rows * (padded(n, size) * size / 16) : 0; }
+// whether DMA can stage that copy
+bool copy_fits(int64_t n, int size, Lie lie) { return row_fits(padded(n, size), size, lie); }
 // read and written once, by a launch of its own
 double copy_us(int64_t rows, int64_t n, int size) { return (double)rows * n * size * 2 / 3.5e6; }
 constexpr double kCopyLaunch = kLaunch + 1.5;
@@ -361,7 +363,8 @@ ForwardPlan plan_forward(const petdense_forward_args* a) {
     const Plan q = plan(a->m, a->n, a->k, a->dtype, kDma, true);
     const double t = q.us + kCopyLaunch + (x_ok ? 0 : copy_us(a->m, a->k, sz)) + (w_ok ? 0 : copy_us(a->k, a->n, sz));
     // (x's rows are filled up with zeros; rows past the kernel's last are not read, which stages zeros too)
-    if (t < f.p.us && pieces_of(!x_ok, a->m, a->k, sz) + pieces_of(!w_ok, a->k, a->n, sz) < kMaxPieces) {
+    if (t < f.p.us && (x_ok || copy_fits(a->k, sz, kAlongC)) && (w_ok || copy_fits(a->n, sz, kAlongFree)) &&
+        pieces_of(!x_ok, a->m, a->k, sz) + pieces_of(!w_ok, a->k, a->n, sz) < kMaxPieces) {
       f.p = q;
       f.loader = kDma;
       f.x = copy_of(!x_ok, a->m, a->k, sz, o);
@@ -449,7 +452,7 @@ double plan_products(const petdense_backward_args* a, int lx, int lk, bool dp_dm
   if (q8 && a->dkernel) {
     const int sz = size_of(a->dtype);
     const double once = kCopyLaunch + (double)a->m * a->k * (1 + sz) / 3.5e6;
-    const bool may = lk == kDma && pieces_of(true, a->m, a->k, sz) < kMaxPieces;
+    const bool may = lk == kDma && copy_fits(a->k, sz, kAlongFree) && pieces_of(true, a->m, a->k, sz) < kMaxPieces;
     const Plan apart = plan(a->k, a->n, a->m, a->dtype, dp_dma ? kCodes : kReg);
     const Plan restored = plan(a->k, a->n, a->m, a->dtype, kDma);
     const bool cheaper = may && restored.us + once < apart.us;
@@ -482,29 +485,38 @@ BackwardPlan plan_backward(const petdense_backward_args* a) {
   const double act_us =
       b.make_dp || b.sums ? kLaunch + 2.0 + (double)a->m * a->n * sz * (b.make_dp ? 3 : 1) / 4e6 : 0.0;
 
-  // dp in the workspace has rows of whole pieces, with zeros: DMA takes it as it is
-  const bool dp_ok = own_dp         ? row_fits(ld_dp, sz)
-                     : a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz)
-                                    : dma_ok(a->dy, a->lddy, a->n, sz);
+  // dp in the workspace has rows of whole pieces, with zeros: DMA takes it as it is.  dX's product reads dp and the
+  // kernel along their contraction, dW's reads dp and x along their free values.
+  const bool dp_ok =
+      own_dp || (a->dresidual ? dma_ok(a->dresidual, a->lddr, a->n, sz) : dma_ok(a->dy, a->lddy, a->n, sz));
+  const bool dp_x = !own_dp || row_fits(ld_dp, sz, kAlongC), dp_k = !own_dp || row_fits(ld_dp, sz, kAlongFree);
   const bool w_ok = !a->dx || dma_ok(a->kernel, a->ldk, a->n, sz);
   const bool x_ok = !a->dkernel || (q8 ? a->k * sz % 16 == 0 : dma_ok(a->x, a->ldx, a->k, sz));
   // (8-bit inputs go through registers whatever their alignment: their loader is dp's)
-  b.us = act_us + plan_products(a, dp_ok && w_ok ? kDma : kReg, dp_ok && x_ok ? kDma : kReg, dp_ok, b);
-  if (!(dp_ok && w_ok && x_ok) && (a->dx || a->dkernel) &&
-      pieces_of(!dp_ok, a->m, a->n, sz) + pieces_of(!w_ok, a->k, a->n, sz) +
-              pieces_of(!x_ok && !q8, a->m, a->k, sz) < kMaxPieces) {
+  b.us = act_us + plan_products(a, dp_ok && dp_x && w_ok ? kDma : kReg, dp_ok && dp_k && x_ok ? kDma : kReg,
+                                dp_ok && dp_k, b);
+  // with copies of what DMA does not take as it is, where their rows are short enough for it
+  const bool copy_x = dp_x && (dp_ok || copy_fits(a->n, sz, kAlongC)) && (w_ok || copy_fits(a->n, sz, kAlongC));
+  const bool copy_dp_k = dp_k && (dp_ok || copy_fits(a->n, sz, kAlongFree));
+  const bool copy_k = copy_dp_k && (x_ok || q8 || copy_fits(a->k, sz, kAlongFree));
+  const bool dp_on = !dp_ok && ((a->dx && copy_x) || (a->dkernel && copy_dp_k));
+  const bool w_on = !w_ok && copy_x, x_on = !x_ok && !q8 && copy_k;
+  if ((dp_on || w_on || x_on || (!x_ok && q8 && copy_k)) && (a->dx || a->dkernel) &&
+      pieces_of(dp_on, a->m, a->n, sz) + pieces_of(w_on, a->k, a->n, sz) + pieces_of(x_on, a->m, a->k, sz) <
+          kMaxPieces) {
     BackwardPlan c = b;
-    c.us = act_us + plan_products(a, kDma, kDma, true, c) + kCopyLaunch + (dp_ok ? 0 : copy_us(a->m, a->n, sz)) +
-           (w_ok ? 0 : copy_us(a->k, a->n, sz)) + (x_ok ? 0 : copy_us(a->m, a->k, sz));
+    c.us = act_us + plan_products(a, copy_x ? kDma : kReg, copy_k ? kDma : kReg, copy_dp_k, c) + kCopyLaunch +
+           (dp_on ? copy_us(a->m, a->n, sz) : 0) + (w_on ? copy_us(a->k, a->n, sz) : 0) +
+           (!x_ok && copy_k ? copy_us(a->m, a->k, sz) : 0);
     if (c.us < b.us) {
       b = c;
-      b.dp.on = !dp_ok;
-      b.kernel.on = !w_ok;
-      b.x.on = !x_ok && !q8;
+      b.dp.on = dp_on;
+      b.kernel.on = w_on;
+      b.x.on = x_on;
     }
   }
   // 8-bit inputs are staged through registers whatever their alignment: beside them dP takes the loader that it can
-  if (q8 && a->dkernel && !b.restore && (dp_ok || b.dp.on)) b.load_k = kDma;
+  if (q8 && a->dkernel && !b.restore && (b.dp.on ? copy_dp_k : dp_ok && dp_k)) b.load_k = kDma;
   // (dP is formed again for every tile that reads it: for small ones)
   if ((a->dx || a->dkernel) && (b.make_dp || b.sums) && !a->dresidual && a->m * a->n <= 1 << 18) {
     Plan px, pk;

@@ -124,6 +124,16 @@ def test_what_dma_stages_lies_within_its_offsets(plan, dtype):
 
 
 @pytest.mark.parametrize('dtype', [BF16, F32])
+def test_wide_layers_are_staged_by_dma(plan, dtype):
+    """Free-contiguous operands are staged a step's rows at a time: theirs may be longer than a tile's rows."""
+    n = 16_000_003 // SIZE[dtype]
+    log = launches(plan, 'forward', forward(2048, 64, n, dtype))
+    assert check_products(log) == 1 and any(kind == 'pad' for kind, _ in log)
+    log = launches(plan, 'backward', backward(512, 64, n, dtype, 1))
+    assert check_products(log) == 1                      # the kernel's gradient, from dP in the workspace
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
 def test_column_sums_beside_a_join_leave_its_grid_in_bounds(plan, dtype):
     """A grid holds fewer than 2^32 threads, and 65,535 workgroups in y; a join of column sums by itself walks."""
     joined = 0

@@ -605,6 +605,24 @@ def test_rows_longer_than_dma_offsets(t, length):
     assert torch.equal(g.kernel, small.float().T @ dp) and torch.equal(g.bias, dp.sum(0))
 
 
+@pytest.mark.parametrize('t,n', [(BF16, 16_700_003), (F32, 8_300_000)], ids=str)
+def test_layers_as_wide_as_dma_offsets_allow(t, n):
+    """A step's 64 rows (32 in fp32) of a kernel or dP of n columns, up to 2^31 bytes.  Signs: sums are exact."""
+    from pet_posterior_distribution_amd import dense, dense_backward
+    m, k = 130, 72
+    x, w, dy, keep = signs((m, k), 1).to(t), signs((k, n), 2).to(t), signs((m, n), 3).to(t), signs((m, n), 4).to(t)
+    y = dense(x, w, out_dtype=F32)
+    g = dense_backward(dy, x, w, activation='relu', saved=keep, grad_dtype=F32)
+    gx = torch.zeros(m, k, device='cuda')
+    for i in range(0, n, 1 << 20):              # (the library's own product is wrong past 2^31 outputs)
+        c = slice(i, min(n, i + (1 << 20)))
+        wc, dp = w[:, c].float(), torch.where(keep[:, c] > 0, dy[:, c], torch.zeros_like(dy[:, c])).float()
+        assert torch.equal(y[:, c], x.float() @ wc), i
+        assert torch.equal(g.kernel[:, c], x.float().T @ dp) and torch.equal(g.bias[c], dp.sum(0)), i
+        gx += dp @ wc.T
+    assert torch.equal(g.x, gx.to(t))
+
+
 def test_one_row_of_more_columns_than_a_launch_has_threads():
     """2^27 columns: more than one launch of a kernel of 1024 threads for 32 columns could take.  Signs and whole
     numbers, so that every sum is exact in fp32 whatever its order."""
